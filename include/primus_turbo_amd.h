@@ -512,6 +512,75 @@ int pta_moe_unpermute(const void *permuted, int64_t num_permuted, int dtype, int
                       const float *permuted_probs, float *probs, int probs_stride,
                       pta_stream_t stream);
 
+/* ---- serving: paged key / value cache, attention over it, few-token experts --
+ * No reference counterpart.  A cache pool (keys or values) is
+ * [num_pages, Hkv, page_size, D], D a multiple of 16 in [16, 256], and for
+ * fp8 scale_inv [num_pages, Hkv, page_size] fp32 (value = fp8 * scale_inv).
+ * A slot is page * page_size + offset in the page.  pages * page_size * Hkv
+ * must stay below 2^31. */
+#define PTA_CACHE_16BIT 2 /* cache kind beside PTA_E4M3 / PTA_E5M2: elements of the queries' 16-bit type */
+
+/* Writes the keys and values of num_tokens tokens, [num_tokens, Hkv, D] with
+ * the given element strides (innermost 1), into the cache slots slots[t]
+ * (int32 or int64).  fp8 kinds quantize each (token, head) row as
+ * pta_quantize_fp8_rowwise does along the last axis and store its scale_inv;
+ * PTA_CACHE_16BIT copies.  A slot below 0 or past the pool is skipped.  Slots
+ * are distinct: what a slot named twice holds afterwards is not defined. */
+int pta_kv_cache_write(const void *k, const void *v, int in_dtype, int64_t num_tokens, int64_t Hkv, int64_t D,
+                       int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                       const void *slots, int slots_i64, void *k_cache, void *v_cache, int cache_kind,
+                       int64_t num_pages, int64_t page_size, float *k_scale_inv, float *v_scale_inv,
+                       pta_stream_t stream);
+
+/* Reads cache slots back: k_out, v_out [num_tokens, Hkv, D] contiguous =
+ * out_dtype(fp8 * scale_inv), or the 16-bit values as they are.  A slot below
+ * 0 or past the pool reads as zeros. */
+int pta_kv_cache_read(const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages,
+                      int64_t page_size, int64_t Hkv, int64_t D, const float *k_scale_inv,
+                      const float *v_scale_inv, const void *slots, int slots_i64, int64_t num_tokens,
+                      void *k_out, void *v_out, int out_dtype, pta_stream_t stream);
+
+/* Attention of the new tokens of num_seqs sequences over their cache pages.
+ * q [num_tokens, Hq, D] (bf16 / fp16, strides in elements, multiples of 8) holds
+ * sequence b's new tokens at rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1,
+ * n of them; seq_lens[b] = L counts the cached tokens, these n among them.
+ * Token i sits at position t = L - n + i and sees keys j <= t, with window_size
+ * > 0 only those with t - j < window_size or j < num_sinks.  Key j is in page
+ * page_table[b, j / page_size]; a page outside the pool reads as zeros.  Query
+ * head h belongs to cache head h / (Hq / Hkv).
+ *   out [num_tokens, Hq, D] = softmax(softmax_scale q.k) v
+ *   lse [num_tokens, Hq] fp32 (may be NULL) = ln sum exp(softmax_scale q.k)
+ * A token that sees no key gets zeros and -inf.  The lengths stay on the device;
+ * the workspace (pta_paged_attention_workspace_size bytes, often 0) depends on
+ * the sizes and the device's compute units alone and needs no clearing. */
+size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv,
+                                          int64_t D, int64_t max_pages, int64_t page_size);
+int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D,
+                        int64_t q_stride_t, int64_t q_stride_h, const void *k_cache, const void *v_cache,
+                        int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                        const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table,
+                        int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
+                        const int32_t *seq_lens, int64_t num_seqs, float softmax_scale, int64_t window_size,
+                        int64_t num_sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                        pta_stream_t stream);
+
+/* SwiGLU experts for the few tokens of a decoding step:
+ *   y[t] = sum_j topk_probs[t, j] * Wd_e (silu(Wg_e x[t]) * (Wu_e x[t])),  e = topk_idx[t, j]
+ * w_gate_up [E, 2 I, H] holds Wg's rows, then Wu's; w_down [E, H, I].  Weights
+ * are fp8 (weight_kind PTA_E4M3 / PTA_E5M2; granularity PTA_TENSORWISE: one
+ * scale_inv, PTA_ROWWISE: [E, rows], PTA_BLOCKWISE: [E, ceil(rows / 128),
+ * ceil(columns / 128)]) or of x's 16-bit type (PTA_CACHE_16BIT, granularity 0).
+ * An index outside [0, E) (int32 or int64) adds nothing: another rank's expert.
+ * H and I are multiples of 16, E <= 1024, topk <= 32.  Any number of tokens is
+ * right; the weights are read once for every 64.  Rounds silu(gate) * up * prob
+ * to x's type between the products. */
+size_t pta_moe_decode_workspace_size(int64_t num_tokens, int64_t num_experts, int64_t topk, int64_t I);
+int pta_moe_decode(const void *x, int x_dtype, int64_t num_tokens, int64_t H, int64_t x_stride,
+                   const void *w_gate_up, const void *w_down, int weight_kind, const float *gate_up_scale_inv,
+                   const float *down_scale_inv, int granularity, int64_t num_experts, int64_t I,
+                   const void *topk_idx, int idx_i64, const float *topk_probs, int64_t topk, void *y,
+                   void *workspace, size_t workspace_bytes, pta_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,110 @@
+// Attention of new tokens over a paged cache: the C entry, the choice between
+// the kernels and how far row tiles are split (paged_attention.h).
+#include "paged_attention.h"
+
+namespace pta {
+namespace {
+
+struct AttnPlan {
+    bool    wide;
+    int64_t slots, goal;
+    size_t  desc_bytes, ml_bytes, o_bytes;
+    size_t  bytes() const { return goal > 0 ? desc_bytes + ml_bytes + o_bytes : 0; }
+};
+
+// All of it goes by sizes that the host has: tokens, sequences, heads and the
+// page table's extent.  Lengths stay on the device.
+AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
+    AttnPlan      p    = {};
+    const int64_t G    = Hq / Hkv;
+    p.wide             = Tq * G > 32 * B;
+    const int64_t bq   = p.wide ? ATT_WIDE_ROWS : ATT_NARROW_ROWS, kt = p.wide ? ATT_WIDE_KEYS : ATT_NARROW_KEYS;
+    const int64_t most = Tq * G / bq + B; // row tiles of a head: sum of ceil(n G / bq)
+    const int64_t goal = cdiv(2 * device_cu_count(), Hkv);
+    // row tiles alone fill the chip, or no tile has keys for two chunks
+    p.goal  = most - B >= goal || max_pages * page <= kt ? 0 : goal;
+    p.slots = most + p.goal;
+    if (p.goal > 0) {
+        p.desc_bytes = static_cast<size_t>(cdiv(p.slots * 16, 256) * 256);
+        p.ml_bytes   = static_cast<size_t>(cdiv(p.slots * Hkv * bq * 8, 256) * 256);
+        p.o_bytes    = static_cast<size_t>(p.slots * Hkv * bq * D * 4);
+    }
+    return p;
+}
+
+} // namespace
+} // namespace pta
+
+using namespace pta;
+
+extern "C" size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv,
+                                                     int64_t D, int64_t max_pages, int64_t page_size) {
+    if (num_tokens <= 0 || num_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_pages < 0 || page_size <= 0) return 0;
+    return attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size).bytes();
+}
+
+extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D,
+                                   int64_t q_stride_t, int64_t q_stride_h, const void *k_cache, const void *v_cache,
+                                   int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                                   const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table,
+                                   int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
+                                   const int32_t *seq_lens, int64_t num_seqs, float softmax_scale, int64_t window_size,
+                                   int64_t num_sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                   pta_stream_t stream) {
+    clear_error();
+    PTA_CHECK_ARG(q_dtype == PTA_BF16 || q_dtype == PTA_F16, "queries must be bfloat16 or float16 (type %d)", q_dtype);
+    PTA_CHECK_ARG(cache_kind == PTA_E4M3 || cache_kind == PTA_E5M2 || cache_kind == PTA_CACHE_16BIT,
+                  "unknown cache kind %d", cache_kind);
+    PTA_CHECK_ARG(num_tokens >= 0 && num_seqs >= 0 && num_pages >= 0 && page_size > 0 && max_pages >= 0, "bad sizes");
+    PTA_CHECK_ARG(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "query heads (%lld) must be a multiple of cache heads (%lld)",
+                  static_cast<long long>(Hq), static_cast<long long>(Hkv));
+    PTA_CHECK_ARG(D >= 16 && D <= 256 && D % 16 == 0, "head_dim must be a multiple of 16 in [16, 256] (got %lld)",
+                  static_cast<long long>(D));
+    PTA_CHECK_ARG(page_size <= INT_MAX && num_pages <= INT_MAX / page_size && num_pages * page_size <= INT_MAX / Hkv,
+                  "the cache has 2^31 rows (pages * page_size * heads) or more");
+    PTA_CHECK_ARG(max_pages <= (INT_MAX - 1024) / page_size, "page_table spans 2^31 tokens or more");
+    PTA_CHECK_ARG(num_tokens <= (INT_MAX - 1024) / Hq && num_seqs < (1 << 24), "too many tokens or sequences");
+    PTA_CHECK_ARG(window_size >= 0 && num_sinks >= 0 && window_size <= INT_MAX / 2 && num_sinks <= INT_MAX / 2,
+                  "window_size and num_sinks must not be negative");
+    PTA_CHECK_ARG(softmax_scale == softmax_scale && softmax_scale - softmax_scale == 0.0f, "softmax_scale must be finite");
+    if (num_tokens == 0) return PTA_OK;
+    PTA_CHECK_ARG(num_seqs > 0, "tokens without a sequence");
+    PTA_CHECK_ARG(q && out && cu_seqlens_q && seq_lens, "null pointer");
+    PTA_CHECK_ARG(max_pages == 0 || page_table, "null page_table");
+    PTA_CHECK_ARG(aligned16(q) && aligned16(out) && q_stride_t % 8 == 0 && q_stride_h % 8 == 0,
+                  "queries and output must be 16-byte aligned, with strides of multiples of 8 elements");
+    if (num_pages > 0) {
+        PTA_CHECK_ARG(k_cache && v_cache, "null cache");
+        PTA_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "cache pools must be 16-byte aligned");
+        PTA_CHECK_ARG(cache_kind == PTA_CACHE_16BIT || (k_scale_inv && v_scale_inv), "an fp8 cache needs its scales");
+    }
+    const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
+    PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
+                  "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
+    PTA_CHECK_ARG(p.slots * Hkv <= INT_MAX / 4, "too many row tiles for one call");
+    AttnArgs a = {};
+    a.q = static_cast<const uint16_t *>(q);
+    a.q_st = q_stride_t; a.q_sh = q_stride_h;
+    a.kc = static_cast<const uint8_t *>(k_cache); a.vc = static_cast<const uint8_t *>(v_cache);
+    a.ks = k_scale_inv; a.vs = v_scale_inv;
+    a.table = page_table; a.table_st = table_stride;
+    a.cu = cu_seqlens_q; a.lens = seq_lens;
+    a.out = static_cast<uint16_t *>(out); a.lse = lse;
+    a.B = static_cast<int>(num_seqs); a.Tq = static_cast<int>(num_tokens);
+    a.Hq = static_cast<int>(Hq); a.Hkv = static_cast<int>(Hkv); a.G = static_cast<int>(Hq / Hkv); a.D = static_cast<int>(D);
+    a.num_pages = static_cast<int>(num_pages); a.page = static_cast<int>(page_size); a.max_pages = static_cast<int>(max_pages);
+    a.window = static_cast<int>(window_size); a.sinks = static_cast<int>(num_sinks);
+    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.slots = static_cast<int>(p.slots); a.split_goal = static_cast<int>(p.goal); a.min_chunk = 1;
+    if (p.goal > 0) {
+        uint8_t *ws = static_cast<uint8_t *>(workspace);
+        a.desc    = reinterpret_cast<int4 *>(ws);
+        a.part_ml = reinterpret_cast<float2 *>(ws + p.desc_bytes);
+        a.part_o  = reinterpret_cast<float *>(ws + p.desc_bytes + p.ml_bytes);
+    }
+    const hipStream_t st = as_stream(stream);
+    if (q_dtype == PTA_BF16) attn_launch<PTA_BF16>(a, cache_kind, p.wide, st);
+    else attn_launch<PTA_F16>(a, cache_kind, p.wide, st);
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
+}

@@ -25,6 +25,8 @@ MX_EXP_KMAJOR = 1
 SEGMENT_COL_TRANSPOSED = 1
 # expert_map kinds of pta_moe_permute_preprocess
 MOE_MAP_BOOL, MOE_MAP_I32, MOE_MAP_I64 = 0, 1, 2
+# cache kind of the paged cache entries beside PTA_E4M3 / PTA_E5M2
+CACHE_16BIT = 2
 
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 
@@ -105,6 +107,27 @@ SIGNATURES = {
         [_vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _vp],
     ),
     "pta_moe_unpermute": (_i32, [_vp, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp]),
+    "pta_kv_cache_write": (
+        _i32,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp, _vp,
+         _vp],
+    ),
+    "pta_kv_cache_read": (
+        _i32,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i32, _vp],
+    ),
+    "pta_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "pta_paged_attention": (
+        _i32,
+        [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
+         _vp, _i64, ctypes.c_float, _i64, _i64, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "pta_moe_decode_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "pta_moe_decode": (
+        _i32,
+        [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _vp, _sz,
+         _vp],
+    ),
 }
 
 _lib = None

@@ -8,4 +8,9 @@ from primus_turbo.pytorch.ops.quantization import (  # noqa: F401
     quantize_fp8,
     quantize_fp8_with_trans,
 )
-from primus_turbo.pytorch.ops.moe import moe_permute, moe_unpermute  # noqa: F401
+from primus_turbo.pytorch.ops.attention import (  # noqa: F401
+    kv_cache_read,
+    kv_cache_write,
+    paged_attention,
+)
+from primus_turbo.pytorch.ops.moe import moe_decode, moe_permute, moe_unpermute  # noqa: F401
