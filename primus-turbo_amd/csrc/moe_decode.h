@@ -10,11 +10,15 @@
 // and y moves beside them.
 //
 // The weights are the first operand of the matrix instructions (rows: output
-// features), the tokens the second (16 columns; up to 4 column tiles), so all
-// tokens of a step go along with one read of the weights.  fp8 converts exactly
-// to the tokens' 16-bit type; the scales are applied to fp32 sums.  The
-// contraction takes a step's elements in the order in which a lane has them in
-// one run of 32 bytes: a row's step is one 128-byte line.
+// features), the tokens that go to the expert the second (column tiles of 16, up
+// to 4), so all of them go along with one read of the weights.  fp8 converts
+// exactly to the tokens' 16-bit type; the scales are applied to fp32 sums.  A
+// step is 128 bytes of every row, two 16-byte pieces a lane with the 4 lanes of a
+// row side by side; the contraction takes the elements in that order.
+//
+// Loads are unconditional (rows, columns and pieces that do not exist read ones
+// that do, and their products are not stored or meet a zero), so that a ring of
+// register stages keeps several steps in flight.
 //
 // a is rounded to the tokens' type between the kernels, its probability
 // included, as a layer that runs its two products apart does.  Sums over an
@@ -38,7 +42,7 @@ struct MoeArgs {
     const void     *idx;     // [T, k] int32 or int64
     int             idx_i64;
     const float    *probs;   // [T, k]
-    uint16_t       *act;     // [groups, S, TG, I]
+    uint16_t       *act;     // [groups, S, TG, I]: an expert's tokens one after the other
     uint16_t       *y;       // [T, H]
     int             T, E, k, I, H, S, TG;
     int             by_entry; // slots are entries of the index rows (few tokens) instead of experts
@@ -51,45 +55,149 @@ __device__ __forceinline__ int moe_expert(const MoeArgs &a, int64_t at) {
     return e >= 0 && e < a.E ? static_cast<int>(e) : -1;
 }
 
-// 32 bytes of a lane's part of a weight row's step as operands
+// A step of one weight row: two pieces of 16 bytes
 template <int XT, int KIND> struct MoeFrag {
-    static constexpr int ES = KIND == PTA_CACHE_16BIT ? 2 : 1, EL = 32 / ES, NS = EL / 8, STEP = 4 * EL;
+    static constexpr int ES = KIND == PTA_CACHE_16BIT ? 2 : 1, EP = 16 / ES, NS = 2 * EP / 8, STEP = 8 * EP;
     uint4                w[2];
-    __device__ __forceinline__ void load(const uint8_t *row, int k, int K) { // row null: zeros
-        w[0] = w[1] = make_uint4(0, 0, 0, 0);
-        if (row != nullptr) {
-            if (k < K) w[0] = *reinterpret_cast<const uint4 *>(row + static_cast<int64_t>(k) * ES);
-            if (k + EL / 2 < K) w[1] = *reinterpret_cast<const uint4 *>(row + static_cast<int64_t>(k) * ES + 16);
+    __device__ __forceinline__ void load(const uint8_t *row, int k0, int qd, int K) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int k = k0 + p * 4 * EP + qd * EP;
+            w[p]        = *reinterpret_cast<const uint4 *>(row + static_cast<int64_t>(k < K ? k : 0) * ES);
         }
     }
     __device__ __forceinline__ uint4 get(int s) const {
         if constexpr (ES == 2) return w[s];
         else return s % 2 == 0 ? att_cvt8<XT, KIND>(w[s / 2].x, w[s / 2].y) : att_cvt8<XT, KIND>(w[s / 2].z, w[s / 2].w);
     }
+    // first element of operand s in the step, for quarter qd
+    static __device__ __forceinline__ int elem(int s, int qd) { return ES == 2 ? s * 32 + qd * 8 : (s / 2) * 64 + qd * 16 + (s % 2) * 8; }
 };
 
-template <int NS> struct MoeTok {
-    uint4 v[NS];
-    __device__ __forceinline__ void load(const uint16_t *row, int k, int K) { // row null: zeros
+// The same step of one token row.  Elements past K become zeros where they are
+// used: an instruction after the load would wait for it.
+template <class F> struct MoeTok {
+    uint4 v[F::NS];
+    __device__ __forceinline__ void load(const uint16_t *row, int k0, int qd, int K) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            v[s] = make_uint4(0, 0, 0, 0);
-            if (row != nullptr && k + 8 * s < K) v[s] = *reinterpret_cast<const uint4 *>(row + k + 8 * s);
+        for (int s = 0; s < F::NS; ++s) {
+            const int k = k0 + F::elem(s, qd);
+            v[s]        = *reinterpret_cast<const uint4 *>(row + (k < K ? k : 0));
         }
     }
+    __device__ __forceinline__ void cut(int k0, int qd, int K) {
+#pragma unroll
+        for (int s = 0; s < F::NS; ++s)
+            if (k0 + F::elem(s, qd) >= K) v[s] = make_uint4(0, 0, 0, 0);
+    }
 };
+
+template <class F, int RT, int NC> struct MoeStage {
+    F         w[RT];
+    MoeTok<F> x[NC];
+    float     sc[RT]; // block scales
+};
+
+__device__ __forceinline__ int moe_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---------------------------------------------------------------------------
 // gate and up products: workgroup = (32 features, slot, group of 64 tokens);
 // the waves take every fourth step
 // ---------------------------------------------------------------------------
-template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void moe_up_kernel(MoeArgs a) {
+struct MoeUpShared {
+    float    red[4 * 4 * 4 * 256]; // wave, column tile, row tile, 16 x 16
+    float    prob[MOE_TG];
+    int      tok[MOE_TG]; // the expert's tokens
+    int      n, expert;
+};
+
+// One pass over K: PR pairs of (gate, up) row tiles from pair p0 on, NC column tiles.
+template <int XT, int KIND, int PR, int NC, int RING>
+__device__ __forceinline__ void moe_up_pass(const MoeArgs &a, MoeUpShared &sh, int p0, int i0, int t0) {
     using F = MoeFrag<XT, KIND>;
-    __shared__ float    sred[4][NC][4][256]; // wave, column tile, row tile, 16 x 16
-    __shared__ float    sprob[MOE_TG];
-    __shared__ uint64_t smask;
-    __shared__ int      sexp;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int      lane = threadIdx.x & 63, wave = moe_uniform(threadIdx.x >> 6), c = lane & 15, qd = lane >> 4;
+    const int      e = moe_uniform(sh.expert);
+    const int      K = a.H, steps = (K + F::STEP - 1) / F::STEP;
+    const int64_t  rowb = static_cast<int64_t>(K) * F::ES;
+    const uint8_t *row[2 * PR]; // gate rows, then up rows
+#pragma unroll
+    for (int r = 0; r < 2 * PR; ++r) {
+        const int i = min(i0 + (p0 + r % PR) * 16 + c, a.I - 1);
+        row[r]      = a.w1 + (static_cast<int64_t>(e) * 2 * a.I + (r / PR) * a.I + i) * rowb;
+    }
+    const uint16_t *tok[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) tok[n] = a.x + (t0 + sh.tok[min(n * 16 + c, sh.n - 1)]) * a.x_st;
+    const bool block = a.scale == MOE_BLOCK;
+    const int  nkb = (K + 127) / 128, nrb = (2 * a.I + 127) / 128;
+    const float *bs[2 * PR]; // 16 rows lie in one block: I is a multiple of 16
+#pragma unroll
+    for (int r = 0; r < 2 * PR; ++r) {
+        const int i = min(i0 + (p0 + r % PR) * 16, a.I - 16) + (r / PR) * a.I;
+        bs[r]       = block ? a.s1 + (static_cast<int64_t>(e) * nrb + i / 128) * nkb : nullptr;
+    }
+    att_f4 acc[NC][2 * PR];
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int r = 0; r < 2 * PR; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
+    MoeStage<F, 2 * PR, NC> ring[RING];
+    auto fetch = [&](MoeStage<F, 2 * PR, NC> &g, int st) {
+#pragma unroll
+        for (int r = 0; r < 2 * PR; ++r) {
+            g.w[r].load(row[r], st * F::STEP, qd, K);
+            g.sc[r] = block ? bs[r][min(st, steps - 1)] : 1.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n) g.x[n].load(tok[n], st * F::STEP, qd, K);
+    };
+#pragma unroll
+    for (int u = 0; u < RING; ++u) fetch(ring[u], wave + 4 * u);
+    for (int st0 = wave; st0 < steps; st0 += 4 * RING) {
+#pragma unroll
+        for (int u = 0; u < RING; ++u) {
+            // steps past the last, too, whose tokens' operands are all cut to zeros: with a
+            // branch around them the loads in flight could not be counted, and every round
+            // would wait for all of them
+            const int st = st0 + 4 * u;
+            if ((st + 1) * F::STEP > K) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) ring[u].x[n].cut(st * F::STEP, qd, K);
+            }
+#pragma unroll
+            for (int r = 0; r < 2 * PR; ++r) {
+                att_f4 part[NC];
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < F::NS; ++s) {
+                    const uint4 wv = ring[u].w[r].get(s);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) part[n] = AttT<XT>::mfma16(wv, ring[u].x[n].v[s], part[n]);
+                }
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[n][r][j] = fmaf(part[n][j], ring[u].sc[r], acc[n][r][j]);
+            }
+            fetch(ring[u], st + 4 * RING);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int r = 0; r < 2 * PR; ++r) // [token][feature]: a lane's four features in a row
+            *reinterpret_cast<float4 *>(&sh.red[(((wave * 4 + n) * 4) + (r / PR) * 2 + p0 + r % PR) * 256 + c * 16 + 4 * qd]) =
+                make_float4(acc[n][r][0], acc[n][r][1], acc[n][r][2], acc[n][r][3]);
+}
+
+template <int XT, int KIND, bool MANY> __global__ __launch_bounds__(MOE_NT, 2) void moe_up_kernel(MoeArgs a) {
+    __shared__ __align__(16) MoeUpShared sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = moe_uniform(tid >> 6);
     const int slot = blockIdx.y, g = blockIdx.z, t0 = g * MOE_TG, tl = min(MOE_TG, a.T - t0);
 
     if (wave == 0) {
@@ -109,104 +217,34 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
         const uint64_t mask = __ballot(mine >= 0);
         // an expert that several entries name belongs to the first
         const int first = mask ? __shfl(mine, __ffsll(static_cast<unsigned long long>(mask)) - 1) : -1;
-        sprob[lane]     = p;
+        if (mine >= 0) {
+            const int at = __popcll(mask & ((1ull << lane) - 1));
+            sh.prob[at]  = p;
+            sh.tok[at]   = lane;
+        }
         if (lane == 0) {
-            smask = mask;
-            sexp  = mask && (!a.by_entry || first == slot) ? e : -1;
+            sh.n      = __popcll(mask);
+            sh.expert = mask && (!a.by_entry || first == slot) ? e : -1;
         }
     }
     __syncthreads();
-    const int      e    = sexp;
-    const uint64_t mask = smask;
+    const int e = moe_uniform(sh.expert), n_tok = moe_uniform(sh.n), i0 = blockIdx.x * 32;
     if (e < 0) return;
-
-    const int      c = lane & 15, qd = lane >> 4, i0 = blockIdx.x * 32;
-    const int      K = a.H, steps = (K + F::STEP - 1) / F::STEP;
-    const int64_t  rowb = static_cast<int64_t>(K) * F::ES;
-    const uint8_t *row[4]; // gate rows, then up rows
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = i0 + (r & 1) * 16 + c;
-        row[r]      = i < a.I ? a.w1 + (static_cast<int64_t>(e) * 2 * a.I + (r >> 1) * a.I + i) * rowb : nullptr;
+    if (!MANY || n_tok <= 16) {
+        moe_up_pass<XT, KIND, 2, 1, 3>(a, sh, 0, i0, t0);
+    } else if (n_tok <= 32) {
+        moe_up_pass<XT, KIND, 2, 2, 2>(a, sh, 0, i0, t0);
+    } else {
+        // a pair of row tiles at a time: the tokens' operands fill the registers
+        moe_up_pass<XT, KIND, 1, 4, 2>(a, sh, 0, i0, t0);
+        moe_up_pass<XT, KIND, 1, 4, 2>(a, sh, 1, i0, t0);
     }
-    const uint16_t *tok[NC];
-    bool            tile[NC]; // some token of the tile goes to this expert
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        tok[n]  = mask >> (n * 16 + c) & 1 ? a.x + (t0 + n * 16 + c) * a.x_st : nullptr;
-        tile[n] = (mask >> (n * 16) & 0xffff) != 0;
-    }
-    att_f4 acc[NC][4];
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
-
-    const bool     block = a.scale == MOE_BLOCK;
-    const int      nkb = (K + 127) / 128, nrb = (2 * a.I + 127) / 128;
-    const float   *bs = block ? a.s1 + static_cast<int64_t>(e) * nrb * nkb : nullptr;
-    F              wf[4], wn[4];
-    MoeTok<F::NS>  xf[NC], xn[NC];
-    auto           fetch = [&](int st, F(&w)[4], MoeTok<F::NS>(&x)[NC]) {
-        const int k = st * F::STEP + qd * F::EL;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[r].load(row[r], k, K);
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-            if (tile[n]) x[n].load(tok[n], k, K);
-    };
-    if (wave < steps) fetch(wave, wf, xf);
-    for (int st = wave; st < steps; st += 4) {
-        const bool more = st + 4 < steps;
-        if (more) fetch(st + 4, wn, xn);
-        att_f4 part[NC][4];
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[n][r][j] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < F::NS; ++s)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint4 wv = wf[r].get(s);
-#pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    if (tile[n]) part[n][r] = AttT<XT>::mfma16(wv, xf[n].v[s], part[n][r]);
-            }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            // 16 rows lie in one block: I is a multiple of 16
-            const int ib = i0 + (r & 1) * 16;
-            float     sc = 1.0f;
-            if (block && ib < a.I) sc = bs[static_cast<int64_t>(((r >> 1) * a.I + ib) / 128) * nkb + st];
-#pragma unroll
-            for (int n = 0; n < NC; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[n][r][j] = fmaf(part[n][r][j], sc, acc[n][r][j]);
-        }
-        if (more) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) wf[r] = wn[r];
-#pragma unroll
-            for (int n = 0; n < NC; ++n) xf[n] = xn[n];
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) // [token][feature]: a lane's four features in a row
-            *reinterpret_cast<float4 *>(&sred[wave][n][r][c * 16 + 4 * qd]) =
-                make_float4(acc[n][r][0], acc[n][r][1], acc[n][r][2], acc[n][r][3]);
     __syncthreads();
     // 8 features of one token a thread
-    for (int p = tid; p < NC * 16 * 4; p += MOE_NT) {
+    for (int p = tid; p < n_tok * 4; p += MOE_NT) {
         const int tt = p >> 2, f = (p & 3) * 8, n = tt >> 4; // token, first feature
         const int i = i0 + f;
-        if (!(mask >> tt & 1) || i >= a.I) continue;
+        if (i >= a.I) continue;
         const int at = (tt & 15) * 16 + (f & 15), u = f >> 4;
         float     v[8];
 #pragma unroll
@@ -214,8 +252,8 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
             float gate = 0.0f, up = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                gate += sred[w][n][u][at + j];
-                up += sred[w][n][2 + u][at + j];
+                gate += sh.red[((w * 4 + n) * 4 + u) * 256 + at + j];
+                up += sh.red[((w * 4 + n) * 4 + 2 + u) * 256 + at + j];
             }
             if (a.scale == MOE_TENSOR) {
                 gate *= a.s1[0];
@@ -224,7 +262,7 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
                 gate *= a.s1[static_cast<int64_t>(e) * 2 * a.I + i + j];
                 up *= a.s1[static_cast<int64_t>(e) * 2 * a.I + a.I + i + j];
             }
-            v[j] = gate / (1.0f + att_exp2(gate * -1.4426950408889634f)) * up * sprob[tt];
+            v[j] = gate / (1.0f + att_exp2(gate * -1.4426950408889634f)) * up * sh.prob[tt];
         }
         *reinterpret_cast<uint4 *>(a.act + ((static_cast<int64_t>(g) * a.S + slot) * a.TG + tt) * a.I + i) =
             make_uint4(AttT<XT>::pack(v[0], v[1]), AttT<XT>::pack(v[2], v[3]), AttT<XT>::pack(v[4], v[5]), AttT<XT>::pack(v[6], v[7]));
@@ -232,22 +270,27 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
 }
 
 // ---------------------------------------------------------------------------
-// down product and the sum over experts: workgroup = (32 features, group of 64
-// tokens); the waves take every fourth step of the list of all reached experts'
-// steps
+// down product and the sum over experts: workgroup = (16 RT features, group of
+// 64 tokens); the waves take every fourth step of the list of all reached
+// experts' steps.  Each wave sums into an LDS table of its own, [token][feature],
+// whenever it is done with an expert: the tokens of a column differ from expert
+// to expert.
 // ---------------------------------------------------------------------------
-template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void moe_down_kernel(MoeArgs a) {
+template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds__(MOE_NT, 2) void moe_down_kernel(MoeArgs a) {
     using F = MoeFrag<XT, KIND>;
-    __shared__ float              sred[4][NC][2][256];
-    __shared__ unsigned long long smask[MOE_MAX_E]; // tokens of a slot
+    constexpr int                 RS = RT * 16 + 4; // floats of a token's row
+    __shared__ __align__(16) float ssum[4][NC * 16][RS];
+    __shared__ unsigned long long smask[MOE_MAX_E];  // tokens of a slot
     __shared__ int                sfirst[MOE_MAX_E]; // by entry: an expert's slot; afterwards: list of reached slots
-    __shared__ int                sexp[MOE_MAX_E];   // expert of a listed slot
+    __shared__ short              sexp[MOE_MAX_E], scnt[MOE_MAX_E]; // expert of a listed slot, its tokens
+    __shared__ int                stok[4][NC * 16];  // a wave's tokens of the expert it sums
     __shared__ int                scount;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = moe_uniform(tid >> 6);
     const int g = blockIdx.y, t0 = g * MOE_TG, tl = min(MOE_TG, a.T - t0), n_ent = tl * a.k;
     const int64_t ent0 = static_cast<int64_t>(t0) * a.k;
 
     for (int i = tid; i < a.S; i += MOE_NT) smask[i] = 0;
+    for (int i = tid; i < 4 * NC * 16 * RS; i += MOE_NT) (&ssum[0][0][0])[i] = 0.0f;
     if (a.by_entry) {
         for (int i = tid; i < a.E; i += MOE_NT) sfirst[i] = INT_MAX;
         __syncthreads();
@@ -270,8 +313,9 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
             const uint64_t b  = __ballot(in);
             if (in) {
                 const int at = n + __popcll(b & ((1ull << lane) - 1));
-                sexp[at]     = a.by_entry ? moe_expert(a, ent0 + s) : s;
+                sexp[at]     = static_cast<short>(a.by_entry ? moe_expert(a, ent0 + s) : s);
                 sfirst[at]   = s;
+                scnt[at]     = static_cast<short>(__popcll(smask[s]));
             }
             n += __popcll(b);
         }
@@ -279,97 +323,113 @@ template <int XT, int KIND, int NC> __global__ __launch_bounds__(MOE_NT, 2) void
     }
     __syncthreads();
 
-    const int c = lane & 15, qd = lane >> 4, h0 = blockIdx.x * 32;
-    const int K = a.I, steps = (K + F::STEP - 1) / F::STEP, items = scount * steps;
+    const int c = lane & 15, qd = lane >> 4, h0 = blockIdx.x * (RT * 16);
+    const int K = a.I, steps = (K + F::STEP - 1) / F::STEP, items = moe_uniform(scount) * steps;
     const int nkb = (K + 127) / 128, nrb = (a.H + 127) / 128;
     const int64_t rowb = static_cast<int64_t>(K) * F::ES;
-    att_f4 acc[NC][2];
+    const bool    block = a.scale == MOE_BLOCK;
+    att_f4 acc[NC][RT];
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
-    F             wf[2], wn[2];
-    MoeTok<F::NS> xf[NC], xn[NC];
-    auto          fetch = [&](int it, F(&w)[2], MoeTok<F::NS>(&x)[NC]) {
-        const int      li = it / steps, st = it - li * steps, e = sexp[li], s = sfirst[li];
-        const uint64_t mask = smask[s];
-        const int      k    = st * F::STEP + qd * F::EL;
+    MoeStage<F, RT, NC> ring[RING];
+    float4              rs[RING][RT]; // row scales, of the stages that end an expert
+    int64_t             hoff[RT];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int h = h0 + r * 16 + c;
-            w[r].load(h < a.H ? a.w2 + (static_cast<int64_t>(e) * a.H + h) * rowb : nullptr, k, K);
-        }
+    for (int r = 0; r < RT; ++r) hoff[r] = min(h0 + r * 16 + c, a.H - 1) * rowb;
+    const float one = a.scale == MOE_TENSOR ? a.s2[0] : 1.0f;
+    auto fetch = [&](MoeStage<F, RT, NC> &q, float4(&qs)[RT], int it) {
+        // past the last: the last expert's tables, and a step past K
+        const int li = it < items ? it / steps : items / steps - 1, st = it < items ? it - li * steps : steps, k0 = st * F::STEP;
+        const int e = moe_uniform(sexp[li]), s = moe_uniform(sfirst[li]), n_tok = moe_uniform(scnt[li]);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int tt = n * 16 + c;
-            x[n].load(mask >> tt & 1 ? a.act + ((static_cast<int64_t>(g) * a.S + s) * a.TG + tt) * a.I : nullptr, k, K);
+        for (int r = 0; r < RT; ++r) {
+            q.w[r].load(a.w2 + static_cast<int64_t>(e) * a.H * rowb + hoff[r], k0, qd, K);
+            q.sc[r] = block ? a.s2[(static_cast<int64_t>(e) * nrb + min(h0 + r * 16, a.H - 16) / 128) * nkb + min(st, steps - 1)] : 1.0f;
         }
+        if (st + 4 >= steps) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                if (a.scale == MOE_ROW)
+                    qs[r] = *reinterpret_cast<const float4 *>(a.s2 + static_cast<int64_t>(e) * a.H + min(h0 + r * 16, a.H - 16) + 4 * qd);
+                else qs[r] = make_float4(one, one, one, one);
+        }
+        const uint16_t *act = a.act + (static_cast<int64_t>(g) * a.S + s) * a.TG * a.I;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+            if (n == 0 || n * 16 < n_tok) q.x[n].load(act + static_cast<int64_t>(min(n * 16 + c, n_tok - 1)) * a.I, k0, qd, K);
     };
-    if (wave < items) fetch(wave, wf, xf);
-    for (int it = wave; it < items; it += 4) {
-        const bool more = it + 4 < items;
-        if (more) fetch(it + 4, wn, xn);
-        const int      li = it / steps, st = it - li * steps, e = sexp[li];
-        const uint64_t mask = smask[sfirst[li]];
+    if (wave < items) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int hb = h0 + r * 16;
-            float     sc[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (a.scale == MOE_TENSOR) sc[0] = sc[1] = sc[2] = sc[3] = a.s2[0];
-            else if (a.scale == MOE_BLOCK) {
-                if (hb < a.H) sc[0] = sc[1] = sc[2] = sc[3] = a.s2[(static_cast<int64_t>(e) * nrb + hb / 128) * nkb + st];
-            } else if (a.scale == MOE_ROW) {
+        for (int u = 0; u < RING; ++u) fetch(ring[u], rs[u], wave + 4 * u);
+    }
+    for (int it0 = wave; it0 < items; it0 += 4 * RING) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (hb + 4 * qd + j < a.H) sc[j] = a.s2[static_cast<int64_t>(e) * a.H + hb + 4 * qd + j];
+        for (int u = 0; u < RING; ++u) {
+            const int it = it0 + 4 * u;
+            const int li = it < items ? it / steps : items / steps - 1, st = it < items ? it - li * steps : steps, n_tok = moe_uniform(scnt[li]);
+            if ((st + 1) * F::STEP > K) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) ring[u].x[n].cut(st * F::STEP, qd, K);
             }
-            att_f4 part[NC];
 #pragma unroll
-            for (int n = 0; n < NC; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < F::NS; ++s) {
-                const uint4 wv = wf[r].get(s);
+            for (int r = 0; r < RT; ++r) {
+                const float sc = ring[u].sc[r];
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
-                    if (mask >> (n * 16) & 0xffff) part[n] = AttT<XT>::mfma16(wv, xf[n].v[s], part[n]);
+                    if (n == 0 || n * 16 < n_tok) {
+                        att_f4 part;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) part[j] = 0.0f;
+#pragma unroll
+                        for (int s = 0; s < F::NS; ++s) part = AttT<XT>::mfma16(ring[u].w[r].get(s), ring[u].x[n].v[s], part);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[n][r][j] = fmaf(part[j], sc, acc[n][r][j]);
+                    }
             }
-            // a token that does not go to this expert has nothing of it, not even 0 * NaN
+            float4 s4[RT];
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const bool in = mask >> (n * 16 + c) & 1;
+            for (int r = 0; r < RT; ++r) s4[r] = rs[u][r];
+            fetch(ring[u], rs[u], it + 4 * RING);
+            if (st + 4 >= steps) { // the wave's last step of this expert
+                const uint64_t mask = smask[sfirst[li]];
+                if (mask >> lane & 1) stok[wave][__popcll(mask & ((1ull << lane) - 1))] = lane;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[n][r][j] = in ? fmaf(part[n][j], sc[j], acc[n][r][j]) : acc[n][r][j];
+                for (int n = 0; n < NC; ++n) {
+                    const bool in = n * 16 + c < n_tok;
+                    const int  tt = in ? stok[wave][n * 16 + c] : 0;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        if (in) {
+                            float4 *p = reinterpret_cast<float4 *>(&ssum[wave][tt][r * 16 + 4 * qd]);
+                            float4  v = *p;
+                            v.x = fmaf(acc[n][r][0], s4[r].x, v.x); v.y = fmaf(acc[n][r][1], s4[r].y, v.y);
+                            v.z = fmaf(acc[n][r][2], s4[r].z, v.z); v.w = fmaf(acc[n][r][3], s4[r].w, v.w);
+                            *p = v;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             }
-        }
-        if (more) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) wf[r] = wn[r];
-#pragma unroll
-            for (int n = 0; n < NC; ++n) xf[n] = xn[n];
         }
     }
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-            *reinterpret_cast<float4 *>(&sred[wave][n][r][c * 16 + 4 * qd]) =
-                make_float4(acc[n][r][0], acc[n][r][1], acc[n][r][2], acc[n][r][3]);
     __syncthreads();
-    for (int p = tid; p < NC * 16 * 4; p += MOE_NT) {
-        const int tt = p >> 2, f = (p & 3) * 8, n = tt >> 4;
-        if (tt >= tl || h0 + f >= a.H) continue;
-        const int at = (tt & 15) * 16 + (f & 15), r = f >> 4;
-        float     v[8];
+    for (int p = tid; p < tl * RT * 2; p += MOE_NT) {
+        const int tt = p / (RT * 2), f = (p % (RT * 2)) * 8;
+        if (h0 + f >= a.H) continue;
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) v[j] += sred[w][n][r][at + j];
-        }
+        for (int j = 0; j < 8; ++j) v[j] = ((ssum[0][tt][f + j] + ssum[1][tt][f + j]) + ssum[2][tt][f + j]) + ssum[3][tt][f + j];
         *reinterpret_cast<uint4 *>(a.y + static_cast<int64_t>(t0 + tt) * a.H + h0 + f) =
             make_uint4(AttT<XT>::pack(v[0], v[1]), AttT<XT>::pack(v[2], v[3]), AttT<XT>::pack(v[4], v[5]), AttT<XT>::pack(v[6], v[7]));
     }
