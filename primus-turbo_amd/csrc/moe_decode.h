@@ -144,7 +144,7 @@ __device__ __forceinline__ void moe_up_pass(const MoeArgs &a, MoeUpShared &sh, i
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
     MoeStage<F, 2 * PR, NC> ring[RING];
-    auto fetch = [&](MoeStage<F, 2 * PR, NC> &g, int st) {
+    auto fetch = [&](MoeStage<F, 2 * PR, NC> &g, int st) PTA_INLINE {
 #pragma unroll
         for (int r = 0; r < 2 * PR; ++r) {
             g.w[r].load(row[r], st * F::STEP, qd, K);
@@ -341,7 +341,7 @@ template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds
 #pragma unroll
     for (int r = 0; r < RT; ++r) hoff[r] = min(h0 + r * 16 + c, a.H - 1) * rowb;
     const float one = a.scale == MOE_TENSOR ? a.s2[0] : 1.0f;
-    auto fetch = [&](MoeStage<F, RT, NC> &q, float4(&qs)[RT], int it) {
+    auto fetch = [&](MoeStage<F, RT, NC> &q, float4(&qs)[RT], int it) PTA_INLINE {
         // past the last: the last expert's tables, and a step past K
         const int li = it < items ? it / steps : items / steps - 1, st = it < items ? it - li * steps : steps, k0 = st * F::STEP;
         const int e = moe_uniform(sexp[li]), s = moe_uniform(sfirst[li]), n_tok = moe_uniform(scnt[li]);

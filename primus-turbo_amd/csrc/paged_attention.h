@@ -26,17 +26,22 @@
 // comes from LDS through the transposing read in that order.
 //
 // Two kernels share this: the wide one (32 rows a wave, keys and values staged
-// in LDS for all waves) where there are many rows, the narrow one (16 rows,
-// keys straight into registers, every wave on keys of its own) where there are
+// in LDS for all waves) where a sequence has many rows, the narrow one (16
+// rows, keys straight into registers, every wave on keys of its own) where it has
 // few and the cache's bytes bound the call.  The keys of a row tile may be split
 // over several workgroups; a last kernel joins their parts.
 #pragma once
 
 #include <climits>
+#include <type_traits>
+#include <utility>
 
 #include "common.h"
 
 namespace pta {
+
+// on lambdas of a kernel: one that is called captures its arrays in memory
+#define PTA_INLINE __attribute__((always_inline))
 
 constexpr int ATT_NONE = INT_MIN; // desc of a slot without work
 
@@ -55,11 +60,12 @@ struct AttnArgs {
     int4           *desc;    // [slots]: sequence, row tile, chunk, chunks
     int             B, Tq, Hq, Hkv, G, D;
     int             num_pages, page, max_pages;
+    uint32_t        page_mul, page_shift; // j / page = mulhi(j, page_mul) >> page_shift for j < 2^31; page_mul 0: j >> page_shift
     int             window, sinks; // window 0: none
     float           scale_log2;
     int             slots;      // work items per key / value head that the grid holds
     int             split_goal; // 0: row tiles are never split
-    int             min_chunk;  // in key tiles
+    int             rows_min, rows_max; // sequences of this launch: rows_min < n G <= rows_max
 };
 
 typedef float    att_f4 __attribute__((ext_vector_type(4)));
@@ -85,6 +91,9 @@ template <> struct AttT<PTA_BF16> {
         r[1] = static_cast<__bf16>(y);
         return __builtin_bit_cast(uint32_t, r);
     }
+    static __device__ __forceinline__ float dot(uint32_t x, uint32_t y) { // of two pairs
+        return fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), __uint_as_float(x & 0xffff0000u) * __uint_as_float(y & 0xffff0000u));
+    }
     template <int KIND> static __device__ __forceinline__ uint2 from_fp8(uint32_t w) {
         if constexpr (KIND == PTA_E4M3)
             return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
@@ -107,6 +116,9 @@ template <> struct AttT<PTA_F16> {
         r[1] = static_cast<_Float16>(y);
         return __builtin_bit_cast(uint32_t, r);
     }
+    static __device__ __forceinline__ float dot(uint32_t x, uint32_t y) { // of two pairs
+        return fmaf(f16_bits_to_f32(x & 0xffffu), f16_bits_to_f32(y & 0xffffu), f16_bits_to_f32(x >> 16) * f16_bits_to_f32(y >> 16));
+    }
     template <int KIND> static __device__ __forceinline__ uint2 from_fp8(uint32_t w) {
         if constexpr (KIND == PTA_E4M3)
             return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
@@ -116,6 +128,14 @@ template <> struct AttT<PTA_F16> {
                               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, true)));
     }
 };
+
+// f(0), f(1), ..., f(N - 1) with constants: arrays indexed by them stay in registers
+template <class F, int... I> __device__ __forceinline__ void att_each(F &&f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F> __device__ __forceinline__ void att_each(F &&f) {
+    att_each(f, std::make_integer_sequence<int, N>{});
+}
 
 // 8 cache elements as 8 values of the queries' type
 template <int QT, int KIND> __device__ __forceinline__ uint4 att_cvt8(uint32_t lo, uint32_t hi) {
@@ -133,6 +153,13 @@ __device__ __forceinline__ uint2 att_tr16(const uint16_t *p) {
 
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float att_log2(float x) { return __builtin_amdgcn_logf(x); }
+
+// max(a, b, c), NaN dropped; the plain form quiets operands first
+__device__ __forceinline__ float att_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 // sum(v, v of lane ^ 16), sum(v, v of lane ^ 32): see max_xor16 / max_xor32
 __device__ __forceinline__ float add_xor16(float v) {
@@ -171,6 +198,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
     s.tok0        = min(max(a.cu[b], 0), a.Tq);
     const int end = min(max(a.cu[b + 1], s.tok0), a.Tq);
     s.n           = end - s.tok0;
+    const int64_t rows = static_cast<int64_t>(s.n) * a.G;
+    if (rows <= a.rows_min || rows > a.rows_max) s.n = 0; // another launch's
     s.len         = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)),
                                          static_cast<int64_t>(a.max_pages) * a.page));
     return s;
@@ -192,7 +221,7 @@ template <int KT> __device__ __forceinline__ int attn_tiles(const AttnArgs &a, c
 template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs &a, int slot, uint32_t *red) {
     constexpr int NW = NTHR / 64;
     const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    auto scan = [&](uint32_t v, uint32_t &total) -> uint32_t { // inclusive prefix sum over the workgroup
+    auto scan = [&](uint32_t v, uint32_t &total) PTA_INLINE -> uint32_t { // inclusive prefix sum over the workgroup
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(v, d);
@@ -231,8 +260,9 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         w = 0.0f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) w += __uint_as_float(red[8 + i]);
+        w = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(w)));
         // above the quotient by more than the sum's rounding: the grid holds all items
-        C = max(a.min_chunk, static_cast<int>(fminf(w * 1.001f / static_cast<float>(a.split_goal), 1e9f)) + 1);
+        C = static_cast<int>(fminf(w * 1.001f / static_cast<float>(a.split_goal), 1e9f)) + 1;
     }
     uint32_t seen = 0;
     for (int b0 = 0; b0 < a.B; b0 += NTHR) {
@@ -257,10 +287,11 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
                 red[2] = chunks;
             }
             __syncthreads();
-            it.b      = static_cast<int>(red[0]);
-            it.chunks = static_cast<int>(red[2]);
-            it.tile   = static_cast<int>(red[1]) / it.chunks;
-            it.chunk  = static_cast<int>(red[1]) - it.tile * it.chunks;
+            it.b      = __builtin_amdgcn_readfirstlane(red[0]);
+            it.chunks = __builtin_amdgcn_readfirstlane(red[2]);
+            const int at_b = __builtin_amdgcn_readfirstlane(red[1]);
+            it.tile   = at_b / it.chunks;
+            it.chunk  = at_b - it.tile * it.chunks;
             break;
         }
         seen += total;
@@ -283,6 +314,9 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
     const int64_t c0 = static_cast<int64_t>(it.chunk) * C;
     it.t0 = static_cast<int>(min(c0, static_cast<int64_t>(n)));
     it.t1 = it.chunk == it.chunks - 1 ? n : static_cast<int>(min(c0 + C, static_cast<int64_t>(n)));
+    // all of it is the workgroup's, but came through vector loads: into scalar registers
+    for (int *f : {&it.row0, &it.rows, &it.tok0, &it.pos0, &it.kend, &it.lo, &it.n_sink, &it.lo_tile, &it.t0, &it.t1})
+        *f = __builtin_amdgcn_readfirstlane(*f);
     return it;
 }
 
@@ -290,39 +324,118 @@ __device__ __forceinline__ int attn_key0(const AttnItem &it, int t, int KT) {
     return (t < it.n_sink ? t : it.lo_tile + t - it.n_sink) * KT;
 }
 
+__device__ __forceinline__ int attn_page_of(const AttnArgs &a, int j) {
+    const uint32_t u = static_cast<uint32_t>(j);
+    return static_cast<int>((a.page_mul ? __umulhi(u, a.page_mul) : u) >> a.page_shift);
+}
+// Page of key j, or -1 where there is none
+__device__ __forceinline__ int attn_key_page(const AttnArgs &a, const AttnItem &it, int j) {
+    if (j >= it.kend || (j < it.lo && j >= a.sinks)) return -1;
+    return a.table[it.b * a.table_st + attn_page_of(a, j)];
+}
+__device__ __forceinline__ int attn_page_row(const AttnArgs &a, int h, int j, int pg) {
+    if (pg < 0 || pg >= a.num_pages) return -1;
+    return (pg * a.Hkv + h) * a.page + (j - attn_page_of(a, j) * a.page);
+}
+
 // Pool row of key j for head h (row = (page * Hkv + h) * page_size + offset), or
 // -1 where there is none: past the keys, hidden from every row by the window, or
 // on a page outside the pool.
 __device__ __forceinline__ int attn_key_row(const AttnArgs &a, const AttnItem &it, int h, int j) {
-    if (j >= it.kend || (j < it.lo && j >= a.sinks)) return -1;
-    const uint32_t p  = static_cast<uint32_t>(j) / static_cast<uint32_t>(a.page);
-    const int      pg = a.table[it.b * a.table_st + p];
-    if (pg < 0 || pg >= a.num_pages) return -1;
-    return (pg * a.Hkv + h) * a.page + (j - static_cast<int>(p) * a.page);
+    const int pg = attn_key_page(a, it, j);
+    return attn_page_row(a, h, j, pg);
 }
 
 // ---------------------------------------------------------------------------
-// wide kernel: NW waves of 32 rows, key tiles of 64 in LDS
+// wide kernel: 4 waves of 32 rows, key tiles of 64 in LDS
 // ---------------------------------------------------------------------------
-template <int QT, int KIND, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void attn_wide_kernel(AttnArgs a) {
-    constexpr int  KT = 64, BQ = 32 * NW, NT = NW * 64;
+// Pipeline, one barrier an iteration.  Iteration t interleaves, one matrix
+// instruction a step, what the matrix pipe and the vector unit can do side by
+// side (a matrix instruction that has to wait for the pipe holds up the vector
+// instructions of both waves of the SIMD, so each is followed by about its own
+// length of others):
+//   S(t + 1) = K(t + 1) Q^T      beside three quarters of tile t's exponentials
+//   O += V(t)^T P(t)             beside the last quarter, the logits and maxima of
+//                                tile t + 1, and the staging of keys t + 2 and values t + 1
+// The loads of keys t + 3 and values t + 2 start at its end and stay in flight
+// over the barrier.  The softmax's reference m follows the running maximum only
+// when a tile exceeds it by 2^8: P then stays below 2^8 and most tiles rescale
+// nothing.
+constexpr float ATT_SLACK = 8.0f;
+
+// bits of a 16-bit type's infinity
+template <int QT> constexpr uint32_t att_inf16() { return QT == PTA_BF16 ? 0x7f80u : 0x7c00u; }
+
+// Operand of values with infinities and NaN taken out, and where they are: `plus`
+// is 1 for +inf and NaN, `minus` for -inf and NaN.
+template <int QT> __device__ __forceinline__ void att_split_special(uint4 v, uint4 &fin, uint4 &plus, uint4 &minus) {
+    constexpr uint32_t INF = att_inf16<QT>(), ONE = QT == PTA_BF16 ? 0x3f80u : 0x3c00u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t       f[4], p[4], m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = p[i] = m[i] = 0;
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+            const uint32_t e = w[i] >> h & 0xffffu, mag = e & 0x7fffu;
+            if (mag < INF) f[i] |= e << h;
+            if (mag > INF || e == INF) p[i] |= ONE << h;
+            if (mag > INF || e == (INF | 0x8000u)) m[i] |= ONE << h;
+        }
+    }
+    fin   = make_uint4(f[0], f[1], f[2], f[3]);
+    plus  = make_uint4(p[0], p[1], p[2], p[3]);
+    minus = make_uint4(m[0], m[1], m[2], m[3]);
+}
+
+// 1 where a probability of the operand is not zero
+template <int QT> __device__ __forceinline__ uint4 att_nonzero(uint4 v) {
+    constexpr uint32_t ONE = QT == PTA_BF16 ? 0x3f80u : 0x3c00u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t       r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = ((w[i] & 0xffffu) ? ONE : 0u) | ((w[i] >> 16) ? ONE << 16 : 0u);
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Whether a 16-byte piece of cache values holds infinities or NaN
+template <int QT, int KIND> __device__ __forceinline__ bool att_has_special(uint4 v) {
+    // exponents of all ones, and for e4m3 the NaN code: adding the distance to the
+    // sign bit carries into it
+    constexpr uint32_t MAG = KIND == PTA_CACHE_16BIT ? 0x7fff7fffu : 0x7f7f7f7fu;
+    constexpr uint32_t TOP = KIND == PTA_CACHE_16BIT ? 0x80008000u : 0x80808080u;
+    constexpr uint32_t ADD = KIND == PTA_CACHE_16BIT ? (QT == PTA_BF16 ? 0x00800080u : 0x04000400u)
+                                                     : (KIND == PTA_E4M3 ? 0x01010101u : 0x04040404u);
+    return ((((v.x & MAG) + ADD) | ((v.y & MAG) + ADD) | ((v.z & MAG) + ADD) | ((v.w & MAG) + ADD)) & TOP) != 0;
+}
+
+// Cache element i in fp32
+template <int QT, int KIND> __device__ __forceinline__ float att_value(const uint8_t *pool, int64_t i) {
+    if constexpr (KIND == PTA_CACHE_16BIT) return load_scalar<QT>(pool, i);
+    else if constexpr (KIND == PTA_E4M3) return __builtin_amdgcn_cvt_f32_fp8(pool[i], 0);
+    else return __builtin_amdgcn_cvt_f32_bf8(pool[i], 0);
+}
+
+template <int QT, int KIND, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a) {
+    constexpr int  KT = 64, BQ = 128, NT = 256;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;       // bytes of a cache element
     constexpr int  EC  = 16 / ES;           // elements of a 16-byte piece
     constexpr int  CPR = DP / EC;           // pieces of a row
     constexpr int  NP  = KT * CPR / NT;     // pieces of a thread and pool
-    constexpr int  KC  = DP / 8;            // 16-byte pieces of a staged row
-    constexpr int  VS  = DP + 32;           // elements of a staged value row: the transposed read's 8 rows
-                                            // of 64 bytes then fall into different banks
+    constexpr int  KS  = DP + 8;            // elements of a staged key row: 16 rows' equal pieces lie in different banks
+    constexpr int  VS  = DP + 32;           // of a value row: the transposed read's 8 rows of 64 bytes do
     static_assert(KT * CPR % NT == 0, "pieces");
-    __shared__ __align__(16) uint16_t sk[2][KT * DP];
+    __shared__ __align__(16) uint16_t sk[2][KT * KS];
     __shared__ __align__(16) uint16_t sv[2][KT * VS];
-    __shared__ __align__(16) float    ssc[FP8 ? 2 : 1][3][FP8 ? KT : 4];
-    __shared__ int                    srow[2][KT];
+    __shared__ __align__(16) float    ssc[FP8 ? 3 : 1][3][FP8 ? KT : 4]; // scale log2e ks, log2 vs, 1 / vs by tile % 3
+    __shared__ int                    srow[4][KT];
+    __shared__ int                    shole[4];   // by tile % 4: some key has no row
+    __shared__ int                    sspec[2][4]; // by tile % 2 and wave: values with infinities or NaN
     __shared__ uint32_t               red[16];
 
-    const int      tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int      h    = blockIdx.x % a.Hkv;
     const int      slot = blockIdx.x / a.Hkv;
     const AttnItem it   = attn_find<BQ, KT, NT>(a, slot, red);
@@ -330,202 +443,420 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void attn_wide_kernel(At
         a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
     if (it.b < 0) return;
 
-    const int  c = lane & 31, half = lane >> 5;
-    const int  r     = it.row0 + wave * 32 + c; // this lane's row
-    const bool rin   = r < it.row0 + it.rows;
-    const int  rtok  = rin ? r / a.G : 0;
-    const int  tok   = it.tok0 + rtok;
-    const int  hq    = h * a.G + (rin ? r - rtok * a.G : 0);
-    const int  pos   = rin ? it.pos0 + rtok : -1; // rows past the tile see nothing
-    const int  wlo   = a.window > 0 ? pos - a.window + 1 : INT_MIN;
-    // positions of the wave's rows, for whole tiles that need no mask
-    const int  wrow  = it.row0 + wave * 32;
-    const int  wend  = min(wrow + 32, it.row0 + it.rows);
-    const bool whole = wrow + 32 <= it.row0 + it.rows;
-    const int  wpmin = it.pos0 + wrow / a.G, wpmax = it.pos0 + (wend - 1) / a.G;
-    const bool wave_in = wrow < it.row0 + it.rows;
-
-    uint4 qf[DP / 16];
+    const int c = lane & 31, half = lane >> 5;
+    uint4     qf[DP / 16];
+    int       pos = -1; // of this lane's row; rows past the tile see nothing
+    {
+        const int  r  = it.row0 + wave * 32 + c;
+        const bool in = r < it.row0 + it.rows;
+        const int  rt = in ? r / a.G : 0, hq = h * a.G + (in ? r - rt * a.G : 0);
+        if (in) pos = it.pos0 + rt;
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        const int d = s * 16 + half * 8;
-        qf[s]       = rin && d < a.D ? *reinterpret_cast<const uint4 *>(a.q + tok * a.q_st + hq * a.q_sh + d)
-                                     : make_uint4(0, 0, 0, 0);
+        for (int s = 0; s < DP / 16; ++s) {
+            const int d = s * 16 + half * 8;
+            qf[s]       = in && d < a.D ? *reinterpret_cast<const uint4 *>(a.q + (it.tok0 + rt) * a.q_st + hq * a.q_sh + d)
+                                        : make_uint4(0, 0, 0, 0);
+        }
     }
+    // positions of the wave's rows
+    const int  wrow = it.row0 + wave * 32, wend = min(wrow + 32, it.row0 + it.rows);
+    const bool full = wrow + 32 <= it.row0 + it.rows;
+    const int  wpmin = it.pos0 + wrow / a.G, wpmax = it.pos0 + (wend - 1) / a.G;
+    // the wave's tiles: keys past its last row's are other waves'
+    int tend = it.t0;
+    if (wend > wrow && wpmax >= 0) {
+        const int last = wpmax / KT + 1; // key tiles up to its last key
+        tend = last <= it.n_sink ? last : last > it.lo_tile ? it.n_sink + last - it.lo_tile : it.n_sink;
+        tend = max(it.t0, min(tend, it.t1));
+    }
+    tend = __builtin_amdgcn_readfirstlane(tend);
+    // tiles in which not every row sees every key
+    const int  bpmin  = it.pos0 + it.row0 / a.G;
+    auto edge = [&](int t, int pmin, int pmax) PTA_INLINE {
+        const int key0 = attn_key0(it, t, KT);
+        return key0 + KT - 1 > pmin || (a.window > 0 && key0 < pmax - a.window + 1);
+    };
+
     att_f16 o[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f, mx = -INFINITY;
 
     uint4 kreg[NP], vreg[NP];
-    float scl[2] = {0.0f, 1.0f}; // key and value scale of key `tid`
-    auto  rows = [&](int t) { // pool rows of a key tile's keys
-        if (tid < KT) srow[t & 1][tid] = t < it.t1 ? attn_key_row(a, it, h, attn_key0(it, t, KT) + tid) : -1;
+    float kscl = 0.0f, vscl = 1.0f; // of key `tid`, as old as kreg
+    // pool rows of a key tile's keys, from their pages, which were fetched an
+    // iteration before
+    int  page_id = -1;
+    auto fetch_pages = [&](int t) PTA_INLINE {
+        if (wave == 0) page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
     };
-    auto load = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int p = i * NT + tid, key = p / CPR, e = (p % CPR) * EC;
-            const int row = srow[t & 1][key];
-            kreg[i] = vreg[i] = make_uint4(0, 0, 0, 0);
-            if (row >= 0 && e < a.D) {
-                const int64_t off = (static_cast<int64_t>(row) * a.D + e) * ES;
-                kreg[i]           = *reinterpret_cast<const uint4 *>(a.kc + off);
-                vreg[i]           = *reinterpret_cast<const uint4 *>(a.vc + off);
-            }
-        }
-        if constexpr (FP8) {
-            if (tid < KT) {
-                const int row = srow[t & 1][tid];
-                scl[0]        = row >= 0 ? a.ks[row] : 0.0f;
-                scl[1]        = row >= 0 ? a.vs[row] : 1.0f;
-            }
+    auto rows = [&](int t) PTA_INLINE {
+        if (wave == 0) {
+            const int row     = attn_page_row(a, h, attn_key0(it, t, KT) + lane, page_id);
+            srow[t & 3][lane] = row;
+            const uint64_t no = __ballot(row < 0);
+            if (lane == 0) shole[t & 3] = no != 0;
         }
     };
-    auto stage = [&](int t) {
-        uint16_t *K = sk[t & 1], *V = sv[t & 1];
+    // keys without a row read row 0 and become zeros when they are staged; the
+    // values of a tile are loaded an iteration after its keys, from the same rows
+    int  krow[NP], vrow[NP], khole = 0, vhole = 0;
+    auto piece = [&](const uint8_t *pool, int i, int row) PTA_INLINE {
+        const int e = ((i * NT + tid) % CPR) * EC;
+        return *reinterpret_cast<const uint4 *>(pool + (static_cast<int64_t>(max(row, 0)) * a.D + (e < a.D ? e : 0)) * ES);
+    };
+    auto load_v = [&]() PTA_INLINE { // of the tile whose keys were loaded last
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int p = i * NT + tid, key = p / CPR, e = (p % CPR) * EC;
-            // 16-byte pieces of a key row in an order of its own, so that equal
-            // pieces of consecutive keys lie in different banks
-            if constexpr (FP8) {
-                const int pc = e / 8;
-                *reinterpret_cast<uint4 *>(K + key * DP + ((pc ^ (key & (KC - 1))) * 8)) =
-                    att_cvt8<QT, KIND>(kreg[i].x, kreg[i].y);
-                *reinterpret_cast<uint4 *>(K + key * DP + (((pc + 1) ^ (key & (KC - 1))) * 8)) =
-                    att_cvt8<QT, KIND>(kreg[i].z, kreg[i].w);
-                *reinterpret_cast<uint4 *>(V + key * VS + e)     = att_cvt8<QT, KIND>(vreg[i].x, vreg[i].y);
-                *reinterpret_cast<uint4 *>(V + key * VS + e + 8) = att_cvt8<QT, KIND>(vreg[i].z, vreg[i].w);
-            } else {
-                *reinterpret_cast<uint4 *>(K + key * DP + (((e / 8) ^ (key & (KC - 1))) * 8)) = kreg[i];
-                *reinterpret_cast<uint4 *>(V + key * VS + e)                                  = vreg[i];
-            }
+            vrow[i] = krow[i];
+            vreg[i] = piece(a.vc, i, vrow[i]);
         }
+        vhole = khole;
+    };
+    auto load_k = [&](int t) PTA_INLINE {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) krow[i] = srow[t & 3][(i * NT + tid) / CPR];
+        khole = shole[t & 3];
+        int row = 0;
+        if constexpr (FP8) row = max(srow[t & 3][lane], 0);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) kreg[i] = piece(a.kc, i, krow[i]);
         if constexpr (FP8) {
-            if (tid < KT) {
-                // no scale of the writer is below 2^-49; one of zero stands for values of zero
-                const float vs = fmaxf(scl[1], 0x1p-100f);
-                ssc[t & 1][0][tid] = scl[0] * a.scale_log2;
-                ssc[t & 1][1][tid] = att_log2(vs);
-                ssc[t & 1][2][tid] = 1.0f / vs;
+            kscl = a.ks[row];
+            vscl = a.vs[row];
+        }
+    };
+    auto holes = [&](int hole, const int(&row)[NP], uint4(&r)[NP]) PTA_INLINE {
+        if (a.D != DP || __builtin_amdgcn_readfirstlane(hole)) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int e = ((i * NT + tid) % CPR) * EC;
+                if (row[i] < 0 || e >= a.D) r[i] = make_uint4(0, 0, 0, 0);
             }
         }
+    };
+    // what is rare about the keys of tile t + 2 and the values of tile t + 1, ahead of their staging
+    auto ready = [&](int t) PTA_INLINE {
+        holes(khole, krow, kreg);
+        holes(vhole, vrow, vreg);
+        if (t + 1 >= it.t0 && t + 1 < it.t1 && edge(t + 1, bpmin, it.kend - 1)) {
+            bool sp = false;
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+                if (att_has_special<QT, KIND>(vreg[i])) {
+                    sp      = true;
+                    vreg[i] = make_uint4(0, 0, 0, 0); // slow() reads the cache's
+                }
+            const uint64_t any = __ballot(sp);
+            if (lane == 0) sspec[(t + 1) & 1][wave] = any != 0;
+        }
+    };
+    auto put = [&](uint16_t *at, const uint4 &r) PTA_INLINE {
+        if constexpr (FP8) {
+            *reinterpret_cast<uint4 *>(at)     = att_cvt8<QT, KIND>(r.x, r.y);
+            *reinterpret_cast<uint4 *>(at + 8) = att_cvt8<QT, KIND>(r.z, r.w);
+        } else {
+            *reinterpret_cast<uint4 *>(at) = r;
+        }
+    };
+    // The registers are opaque where they are staged: their conversions would
+    // otherwise go to the iteration's begin, and the wait for the loads with them
+    auto here = [&](uint4 &r) PTA_INLINE { asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); };
+    auto stage_key = [&](int t, int i) PTA_INLINE {
+        const int p = i * NT + tid;
+        here(kreg[i]);
+        put(&sk[0][0] + (t & 1) * (KT * KS) + (p / CPR) * KS + (p % CPR) * EC, kreg[i]);
+    };
+    auto stage_value = [&](int t, int i) PTA_INLINE {
+        const int p = i * NT + tid;
+        here(vreg[i]);
+        put(&sv[0][0] + (t & 1) * (KT * VS) + (p / CPR) * VS + (p % CPR) * EC, vreg[i]);
+    };
+    auto stage_scale = [&](int t) PTA_INLINE { // the waves share the three tables
+        if constexpr (FP8) {
+            asm volatile("" : "+v"(kscl), "+v"(vscl));
+            const bool  no = srow[t & 3][lane] < 0;
+            const float vs = no ? 1.0f : fmaxf(vscl, 0x1p-100f); // a scale of zero: values of zero
+            const float w  = wave == 0 ? (no ? 0.0f : kscl) * a.scale_log2 : wave == 1 ? att_log2(vs) : 1.0f / vs;
+            ssc[(t + 3) % 3][min(wave, 2)][lane] = w; // the fourth writes what the third does
+        }
+    };
+    auto stage_keys = [&](int t) PTA_INLINE {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) stage_key(t, i);
+        stage_scale(t);
+    };
+    // a quarter of the staging of iteration t
+    auto stage = [&](int t, auto p_c) PTA_INLINE {
+        constexpr int p = decltype(p_c)::value;
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i)
+            if (i * 4 / (2 * NP) == p) {
+                if (i < NP) stage_value(t + 1, i);
+                else stage_key(t + 2, i - NP);
+            }
+        if (p == 3) stage_scale(t + 2);
+    };
+    auto stage_all = [&](int t) PTA_INLINE { att_each<4>([&](auto p) PTA_INLINE { stage(t, p); }); };
+    // operand of step i: of K(t + 1) (key block i / (DP / 16), k-step i % (DP / 16)), then of
+    // V(t) (keys 16 j .. + 15, columns 32 (i % (DP / 32)) .. + 31)
+    constexpr int   NQ = DP / 8; // steps of one product
+    const uint16_t *klane = &sk[0][0] + c * KS + half * 8;
+    const uint16_t *vlane = &sv[0][0] + (half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
+    auto key_op = [&](int t, int i) PTA_INLINE {
+        return *reinterpret_cast<const uint4 *>(klane + (t & 1) * (KT * KS) + i / (DP / 16) * 32 * KS + i % (DP / 16) * 16);
+    };
+    auto value_op = [&](int t, int i) PTA_INLINE {
+        const uint16_t *V = vlane + (t & 1) * (KT * VS) + i / (DP / 32) * 16 * VS + i % (DP / 32) * 32;
+        const uint2     v0 = att_tr16(V), v1 = att_tr16(V + 8 * VS);
+        return make_uint4(v0.x, v0.y, v1.x, v1.y);
+    };
+    // register 4 g + j of key block kb holds key kb * 32 + 8 g + 4 half + j; a chunk is one g
+    auto key_of = [&](int kb, int g) PTA_INLINE { return kb * 32 + 8 * g + 4 * half; };
+    auto scale_of = [&](int t, int which, int ch) PTA_INLINE { // of chunk ch's keys
+        if constexpr (FP8) return *reinterpret_cast<const float4 *>(&ssc[t % 3][which][key_of(ch / 4, ch % 4)]);
+        else return make_float4(1.f, 1.f, 1.f, 1.f);
     };
 
-    rows(it.t0);
-    __syncthreads();
-    if (it.t0 < it.t1) load(it.t0);
-    rows(it.t0 + 1);
-    for (int t = it.t0; t < it.t1; ++t) {
-        stage(t);
-        __syncthreads();
-        if (t + 1 < it.t1) load(t + 1);
-        const int key0 = attn_key0(it, t, KT);
-        if (wave_in && key0 <= wpmax) {
-            const uint16_t *K = sk[t & 1], *V = sv[t & 1];
-            att_f16 s[2];
+    att_f16  u[2];       // base-2 logits of the current tile
+    uint32_t pf[4][4];   // its probabilities, operands of the second product
+    // exponentials of registers 2 i, 2 i + 1
+    auto exps = [&](auto i_c, float base, float z0, float z1) PTA_INLINE {
+        constexpr int i = decltype(i_c)::value, kb = i / 8, j = i % 8 * 2;
+        const float e0 = att_exp2(u[kb][j] - base), e1 = att_exp2(u[kb][j + 1] - base);
+        if constexpr (FP8) l = fmaf(e1, z1, fmaf(e0, z0, l));
+        else l += e0 + e1;
+        uint32_t w = AttT<QT>::pack(e0, e1);
+        asm volatile("" : "+v"(w), "+v"(l)); // here, and not where the product uses it
+        pf[i / 4][i % 4] = w;
+    };
+    // chunk ch of the logits from the products s, with their maximum
+    auto logits = [&](auto ch_c, const att_f16(&s)[2], const float4 &x, const float4 &y) PTA_INLINE {
+        constexpr int ch = decltype(ch_c)::value, kb = ch / 4, g = ch % 4;
+        float         r[4];
+        if constexpr (FP8) {
+            r[0] = fmaf(s[kb][4 * g], x.x, y.x);
+            r[1] = fmaf(s[kb][4 * g + 1], x.y, y.y);
+            r[2] = fmaf(s[kb][4 * g + 2], x.z, y.z);
+            r[3] = fmaf(s[kb][4 * g + 3], x.w, y.w);
+        } else {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int j = 0; j < 4; ++j) r[j] = s[kb][4 * g + j] * a.scale_log2;
+        }
+        asm volatile("" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3])); // here, and not behind the tile
+        mx = att_max3(ch == 0 ? r[0] : mx, r[0], r[1]);
+        mx = att_max3(mx, r[2], r[3]);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
-                const int key = b * 32 + c;
+        for (int j = 0; j < 4; ++j) u[kb][4 * g + j] = r[j];
+    };
+    auto mask = [&](int t) PTA_INLINE {
+        const int key0 = attn_key0(it, t, KT), wlo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
+        mx             = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint4 kf =
-                        *reinterpret_cast<const uint4 *>(K + key * DP + (((k * 2 + half) ^ (key & (KC - 1))) * 8));
-                    s[b] = AttT<QT>::mfma32(kf, qf[k], s[b]);
-                }
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int  key = key0 + key_of(kb, j / 4) + j % 4;
+                const bool see = (key <= pos) & ((key >= wlo) | (key < a.sinks));
+                u[kb][j]       = see ? u[kb][j] : -INFINITY;
+                mx             = fmaxf(mx, u[kb][j]);
+                if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0); // or all comparisons come first, in SGPRs that spill
             }
-            // logits; register j of block b holds key b * 32 + 8 (j / 4) + 4 half + j % 4
-            float mx = m;
-            float iv[2][16];
+    };
+    // moves the reference where a tile's maximum has left it behind
+    auto rescale = [&]() PTA_INLINE {
+        mx             = max_xor32(mx);
+        const bool far = mx > m + ATT_SLACK || (m == -INFINITY && mx > m);
+        if (!__any(far)) return;
+        const float n     = fmaxf(m, mx);
+        const float alpha = n == -INFINITY ? 1.0f : att_exp2(m - n);
+        m                 = n;
+        l *= alpha;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+        for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int kk = b * 32 + 8 * g + 4 * half;
-                    if constexpr (FP8) {
-                        const float4 x = *reinterpret_cast<const float4 *>(&ssc[t & 1][0][kk]);
-                        const float4 y = *reinterpret_cast<const float4 *>(&ssc[t & 1][1][kk]);
-                        const float4 z = *reinterpret_cast<const float4 *>(&ssc[t & 1][2][kk]);
-                        s[b][4 * g]     = fmaf(s[b][4 * g], x.x, y.x);
-                        s[b][4 * g + 1] = fmaf(s[b][4 * g + 1], x.y, y.y);
-                        s[b][4 * g + 2] = fmaf(s[b][4 * g + 2], x.z, y.z);
-                        s[b][4 * g + 3] = fmaf(s[b][4 * g + 3], x.w, y.w);
-                        iv[b][4 * g] = z.x; iv[b][4 * g + 1] = z.y; iv[b][4 * g + 2] = z.z; iv[b][4 * g + 3] = z.w;
-                    } else {
+            for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
+    };
+    // Tile t key by key, for a tile in which some values are infinite or NaN and some
+    // rows do not see them: 0 * inf must not reach those.  The tile's logits become
+    // -inf, so that nothing of it is counted twice.
+    auto slow = [&](int t) PTA_INLINE {
+        const int key0 = attn_key0(it, t, KT), wlo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
+#pragma unroll 1
+        for (int j = 0; j < KT; ++j) {
+            const int       row = srow[t & 3][j], key = key0 + j;
+            const uint16_t *K   = &sk[0][0] + (t & 1) * (KT * KS) + j * KS + half * 8;
+            float           x   = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[b][4 * g + j] *= a.scale_log2;
-                    }
-                }
-            if (!whole || key0 + KT - 1 > wpmin || (a.window > 0 && key0 < wpmax - a.window + 1)) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int  key = key0 + b * 32 + 8 * (j / 4) + 4 * half + j % 4;
-                        const bool see = key <= pos && (key >= wlo || key < a.sinks);
-                        s[b][j]        = see ? s[b][j] : -INFINITY;
-                    }
+            for (int s = 0; s < DP / 16; ++s) {
+                const uint4 kw = *reinterpret_cast<const uint4 *>(K + s * 16), qw = qf[s];
+                x += AttT<QT>::dot(kw.x, qw.x) + AttT<QT>::dot(kw.y, qw.y) + AttT<QT>::dot(kw.z, qw.z) + AttT<QT>::dot(kw.w, qw.w);
             }
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
-            mx                = max_xor32(mx);
-            const float base  = mx == -INFINITY ? 0.0f : mx; // nothing seen yet
-            const float alpha = att_exp2(m - base);
-            m                 = mx;
-            l *= alpha;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    s[b][j] = att_exp2(s[b][j] - base);
-                    if constexpr (FP8) l = fmaf(s[b][j], iv[b][j], l);
-                    else l += s[b][j];
-                }
+            x        = add_xor32(x);
+            float iv = 1.0f;
+            if constexpr (FP8) {
+                x  = fmaf(x, ssc[t % 3][0][j], ssc[t % 3][1][j]);
+                iv = ssc[t % 3][2][j];
+            } else {
+                x *= a.scale_log2;
+            }
+            if (!(key <= pos && (key >= wlo || key < a.sinks))) continue;
+            const float n = fmaxf(m, x), base = n == -INFINITY ? 0.0f : n;
+            const float f = att_exp2(m - base), p = att_exp2(x - base);
+            m = n;
+            // each half of the wave sums its own keys: this one is the first half's
+            l = fmaf(half == 0 ? p : 0.0f, iv, l * f);
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const int   j0 = 8 * st;
-                    const uint4 pf = make_uint4(AttT<QT>::pack(s[b][j0], s[b][j0 + 1]), AttT<QT>::pack(s[b][j0 + 2], s[b][j0 + 3]),
-                                                AttT<QT>::pack(s[b][j0 + 4], s[b][j0 + 5]), AttT<QT>::pack(s[b][j0 + 6], s[b][j0 + 7]));
-                    const int   kr = b * 32 + st * 16 + half * 4 + (lane & 15) / 4;
-                    const int   dc = ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) {
-                        const uint2 v0 = att_tr16(V + kr * VS + i * 32 + dc), v1 = att_tr16(V + (kr + 8) * VS + i * 32 + dc);
-                        o[i] = AttT<QT>::mfma32(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, o[i]);
-                    }
+                for (int e = 0; e < 16; ++e) {
+                    const int d = i * 32 + 8 * (e / 4) + 4 * half + e % 4;
+                    float     v = 0.0f;
+                    if (row >= 0 && d < a.D) v = att_value<QT, KIND>(a.vc, static_cast<int64_t>(row) * a.D + d);
+                    o[i][e] = fmaf(p, v, o[i][e] * f);
                 }
         }
-        rows(t + 2);
+        mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) u[kb][j] = -INFINITY;
+    };
+    // Tile t's exponentials and second product, with the first product and the
+    // logits of tile t + 1 (behind the last tile: of what is in its place, for
+    // nothing) and the staging in between.  A scheduling barrier closes each step;
+    // operands and scales are read several steps ahead.
+    auto tile = [&](int t) PTA_INLINE {
+        att_f16 s[2];
+        uint4   op[4];
+        float4  z[2], x[2], y[2];
+        const float base = m == -INFINITY ? 0.0f : m; // nothing seen yet
+        z[0] = scale_of(t, 2, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) op[i] = key_op(t + 1, i);
+        z[1] = scale_of(t, 2, 1);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[kb][j] = 0.0f;
+        auto exp_pair = [&](auto i_c) PTA_INLINE { // pair i of 16, two a chunk
+            constexpr int i = decltype(i_c)::value, ch = i / 2;
+            const float4  w = z[ch & 1];
+            exps(i_c, base, i % 2 ? w.z : w.x, i % 2 ? w.w : w.y);
+            if (i % 2 && ch < 6) z[ch & 1] = scale_of(t, 2, ch + 2);
+        };
+        auto logit_chunk = [&](auto ch_c) PTA_INLINE {
+            constexpr int ch = decltype(ch_c)::value;
+            logits(ch_c, s, x[ch & 1], y[ch & 1]);
+            if (ch < 6) {
+                x[ch & 1] = scale_of(t + 1, 0, ch + 2);
+                y[ch & 1] = scale_of(t + 1, 1, ch + 2);
+            }
+        };
+        att_each<NQ>([&](auto i_c) PTA_INLINE {
+            constexpr int i = decltype(i_c)::value, kb = i / (DP / 16), k = i % (DP / 16);
+            s[kb] = AttT<QT>::mfma32(op[i & 3], qf[k], s[kb]);
+            op[i & 3] = i + 4 < NQ ? key_op(t + 1, i + 4) : value_op(t, i + 4 - NQ);
+            // pairs 0 .. 11 over the steps
+            att_each<(i + 1) * 12 / NQ - i * 12 / NQ>([&](auto q) PTA_INLINE {
+                exp_pair(std::integral_constant<int, i * 12 / NQ + decltype(q)::value>{});
+            });
+            if (i >= NQ - 2) {
+                x[i - NQ + 2 < 0 ? 0 : i - NQ + 2] = scale_of(t + 1, 0, i - NQ + 2);
+                y[i - NQ + 2 < 0 ? 0 : i - NQ + 2] = scale_of(t + 1, 1, i - NQ + 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        // the rest: pairs 12 .. 15 (E) before the last quarter of the product needs them,
+        // a chunk of logits (L) after its pairs are through, staging (S)
+        constexpr int E = 0, L = 1, S = 2;
+        constexpr int kind[16] = {E, L, S, E, L, L, E, S, L, E, L, S, L, L, S, L};
+        constexpr int which[16] = {12, 0, 0, 13, 1, 2, 14, 1, 3, 15, 4, 2, 5, 6, 3, 7};
+        att_each<NQ>([&](auto i_c) PTA_INLINE {
+            constexpr int i = decltype(i_c)::value, ks = i / (DP / 32), d = i % (DP / 32);
+            o[d] = AttT<QT>::mfma32(op[i & 3], make_uint4(pf[ks][0], pf[ks][1], pf[ks][2], pf[ks][3]), o[d]);
+            if (i + 4 < NQ) op[i & 3] = value_op(t, i + 4);
+            att_each<(i + 1) * 16 / NQ - i * 16 / NQ>([&](auto q) PTA_INLINE {
+                constexpr int w = i * 16 / NQ + decltype(q)::value;
+                using W = std::integral_constant<int, which[w]>;
+                if constexpr (kind[w] == E) exp_pair(W{});
+                else if constexpr (kind[w] == L) logit_chunk(W{});
+                else stage(t, W{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        fetch_pages(it.t0 + i);
+        rows(it.t0 + i);
     }
-    l = add_xor32(l);
-    if (!rin) return;
+    fetch_pages(it.t0 + 4);
+    __syncthreads();
+    if (it.t0 < it.t1) {
+        // tile t0 whole and the keys of t0 + 1 into LDS; then the state of an iteration's begin
+        const int t = it.t0;
+        load_k(t);
+        load_v();
+        holes(khole, krow, kreg);
+        stage_keys(t);
+        load_k(t + 1);
+        ready(t - 1);
+        stage_all(t - 1);
+        load_v();
+        load_k(t + 2);
+        __syncthreads();
+        if (t < tend) {
+            att_f16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[kb][j] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) s[kb] = AttT<QT>::mfma32(key_op(t, kb * (DP / 16) + k), qf[k], s[kb]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            att_each<8>([&](auto ch) PTA_INLINE { logits(ch, s, scale_of(t, 0, ch), scale_of(t, 1, ch)); });
+            if (!full || edge(t, wpmin, wpmax)) mask(t);
+        }
+    }
+    for (int t = it.t0; t < it.t1; ++t) {
+        ready(t);
+        if (t < tend) {
+            if (edge(t, bpmin, it.kend - 1) && (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3])) slow(t);
+            rescale();
+            tile(t);
+            if (!full || edge(t + 1, wpmin, wpmax)) mask(t + 1);
+        } else {
+            stage_all(t);
+        }
+        load_v();
+        load_k(t + 3);
+        rows(t + 4);
+        fetch_pages(t + 5);
+        // the loads stay in flight over the barrier
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    l           = add_xor32(l);
+    const int r = it.row0 + wave * 32 + c;
+    if (r >= it.row0 + it.rows) return;
     if (it.chunks == 1) {
         const float   inv = l > 0.0f || l != l ? 1.0f / l : 0.0f; // no key seen: zeros
-        const int64_t at  = (static_cast<int64_t>(tok) * a.Hq + hq) * a.D;
+        const int     rt  = r / a.G;
+        const int64_t row = static_cast<int64_t>(it.tok0 + rt) * a.Hq + h * a.G + (r - rt * a.G);
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = i * 32 + 8 * g + 4 * half;
                 if (d < a.D)
-                    *reinterpret_cast<uint2 *>(a.out + at + d) =
-                        make_uint2(AttT<QT>::pack(o[i][4 * g] * inv, o[i][4 * g + 1] * inv),
-                                   AttT<QT>::pack(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv));
+                    *reinterpret_cast<uint2 *>(a.out + row * a.D + d) = make_uint2(
+                        AttT<QT>::pack(o[i][4 * g] * inv, o[i][4 * g + 1] * inv), AttT<QT>::pack(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv));
             }
-        if (a.lse != nullptr && half == 0) a.lse[static_cast<int64_t>(tok) * a.Hq + hq] = (m + att_log2(l)) * 0.69314718055994531f;
+        if (a.lse != nullptr && half == 0) a.lse[row] = (m + att_log2(l)) * 0.69314718055994531f;
     } else {
         const int64_t at = (static_cast<int64_t>(slot) * a.Hkv + h) * BQ + wave * 32 + c;
 #pragma unroll
@@ -534,8 +865,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void attn_wide_kernel(At
             for (int g = 0; g < 4; ++g) {
                 const int d = i * 32 + 8 * g + 4 * half;
                 if (d < a.D)
-                    *reinterpret_cast<float4 *>(a.part_o + at * a.D + d) =
-                        make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+                    *reinterpret_cast<float4 *>(a.part_o + at * a.D + d) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
             }
         if (half == 0) a.part_ml[at] = make_float2(m, l);
     }
@@ -563,7 +893,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     __shared__ float2                sml[4][BQ];
     __shared__ uint32_t              red[16];
 
-    const int      tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int      h    = blockIdx.x % a.Hkv;
     const int      slot = blockIdx.x / a.Hkv;
     const AttnItem it   = attn_find<BQ, KT, 256>(a, slot, red);
@@ -579,6 +909,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     const int  hq   = h * a.G + (rin ? r - rtok * a.G : 0);
     const int  pos  = rin ? it.pos0 + rtok : -1;
     const int  wlo  = a.window > 0 ? pos - a.window + 1 : INT_MIN;
+    const bool mixed = a.window > 0 || it.row0 / a.G != (it.row0 + it.rows - 1) / a.G; // rows may see different keys
 
     // k-step s of the products over the head dimension takes elements
     // qd * DP / 4 + 8 s .. + 7 from quarter qd of the lanes: a lane's part of a
@@ -600,10 +931,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     uint16_t *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
     uint4     kreg[2][KP], vreg[VP];
     float     scl[2] = {0.0f, 1.0f};
-    auto      row_of = [&](int t) { // pool row of key lane % 32 of this wave's part
+    auto      row_of = [&](int t) PTA_INLINE { // pool row of key lane % 32 of this wave's part
         return t < it.t1 ? attn_key_row(a, it, h, attn_key0(it, t, KT) + wave * WK + (lane & 31)) : -1;
     };
-    auto load = [&](int row) {
+    auto load = [&](int row) PTA_INLINE {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int kr = __shfl(row, b * 16 + c);
@@ -632,6 +963,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     load(row_of(it.t0));
     int next = row_of(it.t0 + 1);
     for (int t = it.t0; t < it.t1; ++t) {
+        bool special = false;
+        if (mixed) {
+#pragma unroll
+            for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[i]);
+            special = __any(special);
+        }
         // this tile's values to LDS, its keys as operands; then the next tile's loads
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
@@ -698,7 +1035,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int  key = key0 + kk + j;
-                const bool see = key <= pos && (key >= wlo || key < a.sinks);
+                const bool see = (key <= pos) & ((key >= wlo) | (key < a.sinks));
                 s[b][j]        = see ? s[b][j] : -INFINITY;
                 mx             = fmaxf(mx, s[b][j]);
             }
@@ -724,7 +1061,23 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
             const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
-            o[i] = AttT<QT>::mfma16(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, o[i]);
+            const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+            if (!special) {
+                o[i] = AttT<QT>::mfma16(vf, pf, o[i]);
+            } else { // as in the wide kernel's values_special
+                uint4  fin, plus, minus;
+                att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
+                att_split_special<QT>(vf, fin, plus, minus);
+                const uint4 see = att_nonzero<QT>(pf);
+                o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
+                np   = AttT<QT>::mfma16(plus, see, np);
+                nm   = AttT<QT>::mfma16(minus, see, nm);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (np[j] > 0.0f) o[i][j] += INFINITY;
+                    if (nm[j] > 0.0f) o[i][j] -= INFINITY;
+                }
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -777,30 +1130,60 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
 }
 
 // ---------------------------------------------------------------------------
-// joins the chunks of a row tile: workgroup = (first slot of the tile, head)
+// joins the chunks of a row tile: workgroup = (first slot of the tile, head), a
+// part of the tile's rows; four threads share an element's chunks
 // ---------------------------------------------------------------------------
+constexpr int ATT_JOIN_PARTS = 8;
+
 template <int QT, int BQ> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int  h = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
     const int4 w = a.desc[slot]; // sequence, row tile, chunk, chunks
     if (w.x == ATT_NONE || w.z != 0 || w.w == 1) return;
     const AttnSeq s    = attn_seq(a, w.x);
     const int     row0 = w.y * BQ, rows = min(BQ, s.n * a.G - row0);
-    const int     tpr = a.D / 4; // threads of a row
-    for (int p = threadIdx.x; p < rows * tpr; p += 256) {
-        const int jr = p / tpr, d = (p - jr * tpr) * 4;
-        float     mm = -INFINITY;
-        for (int c = 0; c < w.w; ++c) mm = fmaxf(mm, a.part_ml[(static_cast<int64_t>(slot + c) * a.Hkv + h) * BQ + jr].x);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        float       ll = 0.0f;
-        float4      acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; c < w.w; ++c) {
-            const int64_t at = (static_cast<int64_t>(slot + c) * a.Hkv + h) * BQ + jr;
-            const float2  ml = a.part_ml[at];
-            const float   f  = att_exp2(ml.x - base);
-            const float4  x  = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
-            ll               = fmaf(ml.y, f, ll);
-            acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-            acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    const int     tpr = a.D / 4; // elements (of 4 values) of a row
+    const int     lane = threadIdx.x & 63, quarter = threadIdx.x >> 6;
+    __shared__ float4 sacc[4][64];
+    __shared__ float2 sml[4][64];
+    for (int p0 = blockIdx.y * 64; p0 < rows * tpr; p0 += ATT_JOIN_PARTS * 64) {
+        const int p = p0 + lane, jr = min(p / tpr, rows - 1), d = p < rows * tpr ? (p - jr * tpr) * 4 : 0;
+        float     mm = -INFINITY, ll = 0.0f;
+        float4    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c0 = quarter; c0 < w.w; c0 += 16) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = (static_cast<int64_t>(slot + min(c0 + 4 * u, w.w - 1)) * a.Hkv + h) * BQ + jr;
+                ml[u]            = a.part_ml[at];
+                x[u]             = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + 4 * u >= w.w) break;
+                const float n = fmaxf(mm, ml[u].x), base = n == -INFINITY ? 0.0f : n;
+                const float f = att_exp2(mm - base), g = att_exp2(ml[u].x - base);
+                mm    = n;
+                ll    = fmaf(ml[u].y, g, ll * f);
+                acc.x = fmaf(x[u].x, g, acc.x * f); acc.y = fmaf(x[u].y, g, acc.y * f);
+                acc.z = fmaf(x[u].z, g, acc.z * f); acc.w = fmaf(x[u].w, g, acc.w * f);
+            }
+        }
+        __syncthreads();
+        sacc[quarter][lane] = acc;
+        sml[quarter][lane]  = make_float2(mm, ll);
+        __syncthreads();
+        if (quarter != 0 || p >= rows * tpr) continue;
+#pragma unroll
+        for (int u = 1; u < 4; ++u) {
+            const float2 ml = sml[u][lane];
+            const float4 x  = sacc[u][lane];
+            const float  n = fmaxf(mm, ml.x), base = n == -INFINITY ? 0.0f : n;
+            const float  f = att_exp2(mm - base), g = att_exp2(ml.x - base);
+            mm    = n;
+            ll    = fmaf(ml.y, g, ll * f);
+            acc.x = fmaf(x.x, g, acc.x * f); acc.y = fmaf(x.y, g, acc.y * f);
+            acc.z = fmaf(x.z, g, acc.z * f); acc.w = fmaf(x.w, g, acc.w * f);
         }
         const int     rr = row0 + jr, rt = rr / a.G;
         const int64_t orow = static_cast<int64_t>(s.tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
@@ -811,11 +1194,11 @@ template <int QT, int BQ> __global__ __launch_bounds__(256) void attn_join_kerne
     }
 }
 
-// Launches the kernels of one type of queries (paged_attention_inst_*.hip).
-// wide: rows of the row tile are 128 (wide) or 16 (narrow).
-template <int QT> void attn_launch(const AttnArgs &a, int kind, bool wide, hipStream_t st);
-extern template void attn_launch<PTA_BF16>(const AttnArgs &, int, bool, hipStream_t);
-extern template void attn_launch<PTA_F16>(const AttnArgs &, int, bool, hipStream_t);
+// Launches one kernel, and the join if row tiles may be split, for one type of
+// queries (paged_attention_inst_*.hip).  rows: of a row tile, which says the kernel.
+template <int QT> void attn_launch(const AttnArgs &a, int kind, int rows, hipStream_t st);
+extern template void attn_launch<PTA_BF16>(const AttnArgs &, int, int, hipStream_t);
+extern template void attn_launch<PTA_F16>(const AttnArgs &, int, int, hipStream_t);
 
 constexpr int ATT_WIDE_ROWS = 128, ATT_WIDE_KEYS = 64, ATT_NARROW_ROWS = 16, ATT_NARROW_KEYS = 128;
 

@@ -1,34 +1,58 @@
 // Attention of new tokens over a paged cache: the C entry, the choice between
 // the kernels and how far row tiles are split (paged_attention.h).
+#include <algorithm>
+
 #include "paged_attention.h"
 
 namespace pta {
 namespace {
 
-struct AttnPlan {
-    bool    wide;
+// One kernel's share of a call
+struct AttnPart {
+    int     rows; // of a row tile; 0: not launched
+    int     rows_min, rows_max;
     int64_t slots, goal;
     size_t  desc_bytes, ml_bytes, o_bytes;
     size_t  bytes() const { return goal > 0 ? desc_bytes + ml_bytes + o_bytes : 0; }
 };
 
-// All of it goes by sizes that the host has: tokens, sequences, heads and the
-// page table's extent.  Lengths stay on the device.
-AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
-    AttnPlan      p    = {};
-    const int64_t G    = Hq / Hkv;
-    p.wide             = Tq * G > 32 * B;
-    const int64_t bq   = p.wide ? ATT_WIDE_ROWS : ATT_NARROW_ROWS, kt = p.wide ? ATT_WIDE_KEYS : ATT_NARROW_KEYS;
-    const int64_t most = Tq * G / bq + B; // row tiles of a head: sum of ceil(n G / bq)
-    const int64_t goal = cdiv(2 * device_cu_count(), Hkv);
+struct AttnPlan {
+    AttnPart part[2]; // narrow, wide
+    size_t   bytes() const { return part[0].bytes() + part[1].bytes(); }
+};
+
+// Rows of a sequence up to which the narrow kernel takes it where both run
+constexpr int ATT_NARROW_MOST = 64;
+
+AttnPart attn_part(int rows, int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t keys) {
+    AttnPart p = {};
+    p.rows     = rows;
+    p.rows_max = INT_MAX;
+    const int64_t kt   = rows == ATT_NARROW_ROWS ? ATT_NARROW_KEYS : ATT_WIDE_KEYS;
+    const int64_t most = Tq * G / rows + B; // row tiles of a head: sum of ceil(n G / rows)
+    const int64_t goal = cdiv((rows == ATT_NARROW_ROWS ? 2 : 1) * device_cu_count(), Hkv); // workgroups a CU
     // row tiles alone fill the chip, or no tile has keys for two chunks
-    p.goal  = most - B >= goal || max_pages * page <= kt ? 0 : goal;
+    p.goal  = most - B >= goal || keys <= kt ? 0 : goal;
     p.slots = most + p.goal;
     if (p.goal > 0) {
         p.desc_bytes = static_cast<size_t>(cdiv(p.slots * 16, 256) * 256);
-        p.ml_bytes   = static_cast<size_t>(cdiv(p.slots * Hkv * bq * 8, 256) * 256);
-        p.o_bytes    = static_cast<size_t>(p.slots * Hkv * bq * D * 4);
+        p.ml_bytes   = static_cast<size_t>(cdiv(p.slots * Hkv * rows * 8, 256) * 256);
+        p.o_bytes    = static_cast<size_t>(p.slots * Hkv * rows * D * 4);
     }
+    return p;
+}
+
+// All of it goes by sizes that the host has: tokens, sequences, heads and the
+// page table's extent.  Lengths stay on the device, so where sequences of few and
+// of many rows may be together both kernels run, each on its own.
+AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
+    AttnPlan      p = {};
+    const int64_t G = Hq / Hkv, keys = max_pages * page;
+    const bool    few = Tq * G <= 16 * B || Tq * G <= ATT_NARROW_MOST; // a row tile each on average, or no sequence has many
+    const bool    mix = !few && B > 1;
+    if (few || mix) p.part[0] = attn_part(ATT_NARROW_ROWS, mix ? std::min<int64_t>(Tq, B * ATT_NARROW_MOST) : Tq, B, Hkv, G, D, keys);
+    if (!few) p.part[1] = attn_part(ATT_WIDE_ROWS, Tq, B, Hkv, G, D, keys);
+    if (mix) p.part[0].rows_max = p.part[1].rows_min = ATT_NARROW_MOST;
     return p;
 }
 
@@ -81,7 +105,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
     PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
                   "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG(p.slots * Hkv <= INT_MAX / 4, "too many row tiles for one call");
+    PTA_CHECK_ARG((p.part[0].slots + p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
     AttnArgs a = {};
     a.q = static_cast<const uint16_t *>(q);
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
@@ -93,18 +117,31 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     a.B = static_cast<int>(num_seqs); a.Tq = static_cast<int>(num_tokens);
     a.Hq = static_cast<int>(Hq); a.Hkv = static_cast<int>(Hkv); a.G = static_cast<int>(Hq / Hkv); a.D = static_cast<int>(D);
     a.num_pages = static_cast<int>(num_pages); a.page = static_cast<int>(page_size); a.max_pages = static_cast<int>(max_pages);
+    // j / page for 0 <= j < 2^31: ceil(2^(32 + s) / page) with s = floor(log2(page)), exact there
+    while (page_size >> (a.page_shift + 1)) ++a.page_shift;
+    if (page_size & (page_size - 1)) a.page_mul = static_cast<uint32_t>(((1ull << (32 + a.page_shift)) + page_size - 1) / page_size);
     a.window = static_cast<int>(window_size); a.sinks = static_cast<int>(num_sinks);
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
-    a.slots = static_cast<int>(p.slots); a.split_goal = static_cast<int>(p.goal); a.min_chunk = 1;
-    if (p.goal > 0) {
-        uint8_t *ws = static_cast<uint8_t *>(workspace);
-        a.desc    = reinterpret_cast<int4 *>(ws);
-        a.part_ml = reinterpret_cast<float2 *>(ws + p.desc_bytes);
-        a.part_o  = reinterpret_cast<float *>(ws + p.desc_bytes + p.ml_bytes);
+    if (num_pages == 0) { // keys without a row read row 0 of something and drop it
+        a.kc = a.vc = static_cast<const uint8_t *>(q);
+        a.ks = a.vs = static_cast<const float *>(q);
     }
+    uint8_t          *ws = static_cast<uint8_t *>(workspace);
     const hipStream_t st = as_stream(stream);
-    if (q_dtype == PTA_BF16) attn_launch<PTA_BF16>(a, cache_kind, p.wide, st);
-    else attn_launch<PTA_F16>(a, cache_kind, p.wide, st);
+    for (const AttnPart &part : p.part) {
+        if (part.rows == 0) continue;
+        a.slots = static_cast<int>(part.slots); a.split_goal = static_cast<int>(part.goal);
+        a.rows_min = part.rows_min; a.rows_max = part.rows_max;
+        a.desc = nullptr; a.part_ml = nullptr; a.part_o = nullptr;
+        if (part.goal > 0) {
+            a.desc    = reinterpret_cast<int4 *>(ws);
+            a.part_ml = reinterpret_cast<float2 *>(ws + part.desc_bytes);
+            a.part_o  = reinterpret_cast<float *>(ws + part.desc_bytes + part.ml_bytes);
+            ws += part.bytes();
+        }
+        if (q_dtype == PTA_BF16) attn_launch<PTA_BF16>(a, cache_kind, part.rows, st);
+        else attn_launch<PTA_F16>(a, cache_kind, part.rows, st);
+    }
     PTA_CHECK_LAUNCH();
     return PTA_OK;
 }
