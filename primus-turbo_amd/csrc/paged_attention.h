@@ -55,16 +55,17 @@ struct AttnArgs {
     const int32_t  *cu, *lens;
     uint16_t       *out; // [Tq, Hq, D]
     float          *lse; // [Tq, Hq] or null
-    float          *part_o;  // [slots, Hkv, BQ, D]
-    float2         *part_ml; // [slots, Hkv, BQ]
-    int4           *desc;    // [slots]: sequence, row tile, chunk, chunks
+    float          *part_o;  // [slots, Hkv, BQ, D] (wide), [split, Tq, Hq, D] (narrow)
+    float2         *part_ml; // the same without D
+    int4           *desc;    // [slots]: sequence, row tile, chunk, chunks (wide)
     int             B, Tq, Hq, Hkv, G, D;
     int             num_pages, page, max_pages;
     uint32_t        page_mul, page_shift; // j / page = mulhi(j, page_mul) >> page_shift for j < 2^31; page_mul 0: j >> page_shift
     int             window, sinks; // window 0: none
     float           scale_log2;
-    int             slots;      // work items per key / value head that the grid holds
-    int             split_goal; // 0: row tiles are never split
+    int             slots;      // wide: work items per key / value head that the grid holds
+    int             split_goal; // wide; 0: row tiles are never split
+    int             split, tiles; // narrow: chunks of a sequence, row tiles of it side by side
     int             rows_min, rows_max; // sequences of this launch: rows_min < n G <= rows_max
 };
 
@@ -151,6 +152,13 @@ __device__ __forceinline__ uint2 att_tr16(const uint16_t *p) {
         (lds_s4 *)reinterpret_cast<att_s4 *>(const_cast<uint16_t *>(p))));
 }
 
+// the lane's number, opaque to the compiler
+__device__ __forceinline__ int att_lane() {
+    int r;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(r));
+    return r;
+}
+
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float att_log2(float x) { return __builtin_amdgcn_logf(x); }
 
@@ -212,6 +220,19 @@ template <int KT> __device__ __forceinline__ int attn_tiles(const AttnArgs &a, c
     const int64_t span = static_cast<int64_t>(a.window) + bq / a.G + 1;
     const int64_t win  = span / KT + 2 + (min(a.sinks, s.len) + KT - 1) / KT;
     return static_cast<int>(min(static_cast<int64_t>(full), win));
+}
+
+// The list of key tiles of an item whose rows and positions are set: its fields,
+// and its length.
+template <int KT> __device__ __forceinline__ int attn_keys(const AttnArgs &a, AttnItem &it, int len) {
+    const int pmin = it.pos0 + it.row0 / a.G, pmax = it.pos0 + (it.row0 + it.rows - 1) / a.G;
+    it.kend = max(0, min(pmax + 1, len));
+    it.lo   = min(a.window > 0 ? max(0, pmin - a.window + 1) : 0, it.kend);
+    // sink tiles that the window's tiles do not cover
+    const int first = it.lo / KT, last = (it.kend + KT - 1) / KT;
+    it.n_sink  = min(a.window > 0 ? (min(a.sinks, it.kend) + KT - 1) / KT : 0, first);
+    it.lo_tile = first;
+    return it.n_sink + max(0, last - first);
 }
 
 // Finds the item of slot `slot`; all threads of the workgroup call it (`red`:
@@ -302,15 +323,7 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
     it.pos0 = s.len - s.n; // below 0 where more tokens came than the length says: those see nothing
     it.row0 = it.tile * BQ;
     it.rows = min(BQ, s.n * a.G - it.row0);
-    const int pmin = it.pos0 + it.row0 / a.G, pmax = it.pos0 + (it.row0 + it.rows - 1) / a.G;
-    it.kend = max(0, min(pmax + 1, s.len));
-    it.lo   = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
-    it.lo   = min(it.lo, it.kend);
-    // sink tiles that the window's tiles do not cover
-    const int first = it.lo / KT, last = (it.kend + KT - 1) / KT;
-    it.n_sink  = min(a.window > 0 ? (min(a.sinks, it.kend) + KT - 1) / KT : 0, first);
-    it.lo_tile = first;
-    const int n = it.n_sink + max(0, last - first);
+    const int     n  = attn_keys<KT>(a, it, s.len);
     const int64_t c0 = static_cast<int64_t>(it.chunk) * C;
     it.t0 = static_cast<int>(min(c0, static_cast<int64_t>(n)));
     it.t1 = it.chunk == it.chunks - 1 ? n : static_cast<int>(min(c0 + C, static_cast<int64_t>(n)));
@@ -357,8 +370,8 @@ __device__ __forceinline__ int attn_key_row(const AttnArgs &a, const AttnItem &i
 //   S(t + 1) = K(t + 1) Q^T      beside three quarters of tile t's exponentials
 //   O += V(t)^T P(t)             beside the last quarter, the logits and maxima of
 //                                tile t + 1, and the staging of keys t + 2 and values t + 1
-// The loads of keys t + 3 and values t + 2 start at its end and stay in flight
-// over the barrier.  The softmax's reference m follows the running maximum only
+// Each register is loaded with keys t + 3 or values t + 2 once it is staged; the
+// loads stay in flight over the barrier.  The softmax's reference m follows the running maximum only
 // when a tile exceeds it by 2^8: P then stays below 2^8 and most tiles rescale
 // nothing.
 constexpr float ATT_SLACK = 8.0f;
@@ -409,11 +422,25 @@ template <int QT, int KIND> __device__ __forceinline__ bool att_has_special(uint
     return ((((v.x & MAG) + ADD) | ((v.y & MAG) + ADD) | ((v.z & MAG) + ADD) | ((v.w & MAG) + ADD)) & TOP) != 0;
 }
 
-// Cache element i in fp32
-template <int QT, int KIND> __device__ __forceinline__ float att_value(const uint8_t *pool, int64_t i) {
-    if constexpr (KIND == PTA_CACHE_16BIT) return load_scalar<QT>(pool, i);
-    else if constexpr (KIND == PTA_E4M3) return __builtin_amdgcn_cvt_f32_fp8(pool[i], 0);
-    else return __builtin_amdgcn_cvt_f32_bf8(pool[i], 0);
+// Cache elements i .. i + 3 in fp32
+template <int QT, int KIND> __device__ __forceinline__ void att_values4(const uint8_t *pool, int64_t i, float (&v)[4]) {
+    if constexpr (KIND == PTA_CACHE_16BIT) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(pool + 2 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t h = (j < 2 ? w.x : w.y) >> (16 * (j & 1)) & 0xffffu;
+            v[j]             = QT == PTA_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+        }
+    } else {
+        const int w = *reinterpret_cast<const int *>(pool + i);
+        if constexpr (KIND == PTA_E4M3) {
+            v[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0); v[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+            v[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2); v[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+        } else {
+            v[0] = __builtin_amdgcn_cvt_f32_bf8(w, 0); v[1] = __builtin_amdgcn_cvt_f32_bf8(w, 1);
+            v[2] = __builtin_amdgcn_cvt_f32_bf8(w, 2); v[3] = __builtin_amdgcn_cvt_f32_bf8(w, 3);
+        }
+    }
 }
 
 template <int QT, int KIND, int DP>
@@ -435,7 +462,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     __shared__ int                    sspec[2][4]; // by tile % 2 and wave: values with infinities or NaN
     __shared__ uint32_t               red[16];
 
-    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int            tid = threadIdx.x, lane = tid & 63;
+    const int      wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int      h    = blockIdx.x % a.Hkv;
     const int      slot = blockIdx.x / a.Hkv;
     const AttnItem it   = attn_find<BQ, KT, NT>(a, slot, red);
@@ -443,7 +471,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
     if (it.b < 0) return;
 
-    const int c = lane & 31, half = lane >> 5;
+    int c = lane & 31, half = lane >> 5;
     uint4     qf[DP / 16];
     int       pos = -1; // of this lane's row; rows past the tile see nothing
     {
@@ -500,47 +528,48 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
             if (lane == 0) shole[t & 3] = no != 0;
         }
     };
-    // keys without a row read row 0 and become zeros when they are staged; the
-    // values of a tile are loaded an iteration after its keys, from the same rows
-    int  krow[NP], vrow[NP], khole = 0, vhole = 0;
+    // Keys without a row read row 0 and become zeros when they are staged.  At an
+    // iteration's begin kreg, krow are of tile t + 2, vreg is of tile t + 1; each
+    // register is loaded again (t + 3, t + 2) as soon as it is staged, which leaves
+    // the loads a whole iteration.
+    int  krow[NP], nrow[NP], srow_n = 0, khole = 0, vhole = 0, nhole = 0;
     auto piece = [&](const uint8_t *pool, int i, int row) PTA_INLINE {
         const int e = ((i * NT + tid) % CPR) * EC;
         return *reinterpret_cast<const uint4 *>(pool + (static_cast<int64_t>(max(row, 0)) * a.D + (e < a.D ? e : 0)) * ES);
     };
-    auto load_v = [&]() PTA_INLINE { // of the tile whose keys were loaded last
+    auto next_rows = [&](int t) PTA_INLINE { // of the tile whose keys are loaded next
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            vrow[i] = krow[i];
-            vreg[i] = piece(a.vc, i, vrow[i]);
-        }
-        vhole = khole;
+        for (int i = 0; i < NP; ++i) nrow[i] = srow[t & 3][(i * NT + tid) / CPR];
+        nhole = shole[t & 3];
+        if constexpr (FP8) srow_n = srow[t & 3][lane];
     };
-    auto load_k = [&](int t) PTA_INLINE {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) krow[i] = srow[t & 3][(i * NT + tid) / CPR];
-        khole = shole[t & 3];
-        int row = 0;
-        if constexpr (FP8) row = max(srow[t & 3][lane], 0);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) kreg[i] = piece(a.kc, i, krow[i]);
+    auto load_key = [&](int i) PTA_INLINE { kreg[i] = piece(a.kc, i, nrow[i]); };
+    auto load_value = [&](int i) PTA_INLINE { vreg[i] = piece(a.vc, i, krow[i]); };
+    auto load_scale = [&]() PTA_INLINE {
         if constexpr (FP8) {
-            kscl = a.ks[row];
-            vscl = a.vs[row];
+            kscl = a.ks[max(srow_n, 0)];
+            vscl = a.vs[max(srow_n, 0)];
         }
     };
-    auto holes = [&](int hole, const int(&row)[NP], uint4(&r)[NP]) PTA_INLINE {
-        if (a.D != DP || __builtin_amdgcn_readfirstlane(hole)) {
+    auto shift_rows = [&]() PTA_INLINE {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) krow[i] = nrow[i];
+        vhole = khole;
+        khole = __builtin_amdgcn_readfirstlane(nhole);
+    };
+    auto holes = [&](int hole, int t, uint4(&r)[NP]) PTA_INLINE {
+        if (a.D != DP || hole) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int e = ((i * NT + tid) % CPR) * EC;
-                if (row[i] < 0 || e >= a.D) r[i] = make_uint4(0, 0, 0, 0);
+                if (srow[t & 3][(i * NT + tid) / CPR] < 0 || e >= a.D) r[i] = make_uint4(0, 0, 0, 0);
             }
         }
     };
     // what is rare about the keys of tile t + 2 and the values of tile t + 1, ahead of their staging
     auto ready = [&](int t) PTA_INLINE {
-        holes(khole, krow, kreg);
-        holes(vhole, vrow, vreg);
+        holes(khole, t + 2, kreg);
+        holes(vhole, t + 1, vreg);
         if (t + 1 >= it.t0 && t + 1 < it.t1 && edge(t + 1, bpmin, it.kend - 1)) {
             bool sp = false;
 #pragma unroll
@@ -594,21 +623,29 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 #pragma unroll
         for (int i = 0; i < 2 * NP; ++i)
             if (i * 4 / (2 * NP) == p) {
-                if (i < NP) stage_value(t + 1, i);
-                else stage_key(t + 2, i - NP);
+                if (i < NP) {
+                    stage_value(t + 1, i);
+                    load_value(i);
+                } else {
+                    stage_key(t + 2, i - NP);
+                    load_key(i - NP);
+                }
             }
-        if (p == 3) stage_scale(t + 2);
+        if (p == 3) {
+            stage_scale(t + 2);
+            load_scale();
+        }
     };
     auto stage_all = [&](int t) PTA_INLINE { att_each<4>([&](auto p) PTA_INLINE { stage(t, p); }); };
     // operand of step i: of K(t + 1) (key block i / (DP / 16), k-step i % (DP / 16)), then of
     // V(t) (keys 16 j .. + 15, columns 32 (i % (DP / 32)) .. + 31)
     constexpr int   NQ = DP / 8; // steps of one product
-    const uint16_t *klane = &sk[0][0] + c * KS + half * 8;
-    const uint16_t *vlane = &sv[0][0] + (half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
     auto key_op = [&](int t, int i) PTA_INLINE {
+        const uint16_t *klane = &sk[0][0] + c * KS + half * 8;
         return *reinterpret_cast<const uint4 *>(klane + (t & 1) * (KT * KS) + i / (DP / 16) * 32 * KS + i % (DP / 16) * 16);
     };
     auto value_op = [&](int t, int i) PTA_INLINE {
+        const uint16_t *vlane = &sv[0][0] + (half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
         const uint16_t *V = vlane + (t & 1) * (KT * VS) + i / (DP / 32) * 16 * VS + i % (DP / 32) * 32;
         const uint2     v0 = att_tr16(V), v1 = att_tr16(V + 8 * VS);
         return make_uint4(v0.x, v0.y, v1.x, v1.y);
@@ -686,7 +723,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         const int key0 = attn_key0(it, t, KT), wlo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
 #pragma unroll 1
         for (int j = 0; j < KT; ++j) {
-            const int       row = srow[t & 3][j], key = key0 + j;
+            const int       row = __builtin_amdgcn_readfirstlane(srow[t & 3][j]), key = key0 + j;
             const uint16_t *K   = &sk[0][0] + (t & 1) * (KT * KS) + j * KS + half * 8;
             float           x   = 0.0f;
 #pragma unroll
@@ -711,11 +748,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int d = i * 32 + 8 * (e / 4) + 4 * half + e % 4;
-                    float     v = 0.0f;
-                    if (row >= 0 && d < a.D) v = att_value<QT, KIND>(a.vc, static_cast<int64_t>(row) * a.D + d);
-                    o[i][e] = fmaf(p, v, o[i][e] * f);
+                for (int g = 0; g < 4; ++g) {
+                    // outputs past D are not stored: what is in bounds does
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (row >= 0) att_values4<QT, KIND>(a.vc, static_cast<int64_t>(row) * a.D + min(i * 32 + 8 * g + 4 * half, a.D - 4), v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][4 * g + e] = fmaf(p, v[e], o[i][4 * g + e] * f);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
         }
         mx = -INFINITY;
@@ -730,12 +769,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     // operands and scales are read several steps ahead.
     auto tile = [&](int t) PTA_INLINE {
         att_f16 s[2];
-        uint4   op[4];
-        float4  z[2], x[2], y[2];
+        constexpr int R = 3; // operands in flight
+        uint4   op[R];
+        float4  z[2], x, y;
         const float base = m == -INFINITY ? 0.0f : m; // nothing seen yet
         z[0] = scale_of(t, 2, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) op[i] = key_op(t + 1, i);
+        for (int i = 0; i < R; ++i) op[i] = key_op(t + 1, i);
         z[1] = scale_of(t, 2, 1);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -749,23 +789,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         };
         auto logit_chunk = [&](auto ch_c) PTA_INLINE {
             constexpr int ch = decltype(ch_c)::value;
-            logits(ch_c, s, x[ch & 1], y[ch & 1]);
-            if (ch < 6) {
-                x[ch & 1] = scale_of(t + 1, 0, ch + 2);
-                y[ch & 1] = scale_of(t + 1, 1, ch + 2);
+            logits(ch_c, s, x, y);
+            if (ch < 7) {
+                x = scale_of(t + 1, 0, ch + 1);
+                y = scale_of(t + 1, 1, ch + 1);
             }
         };
         att_each<NQ>([&](auto i_c) PTA_INLINE {
             constexpr int i = decltype(i_c)::value, kb = i / (DP / 16), k = i % (DP / 16);
-            s[kb] = AttT<QT>::mfma32(op[i & 3], qf[k], s[kb]);
-            op[i & 3] = i + 4 < NQ ? key_op(t + 1, i + 4) : value_op(t, i + 4 - NQ);
+            s[kb] = AttT<QT>::mfma32(op[i % R], qf[k], s[kb]);
+            op[i % R] = i + R < NQ ? key_op(t + 1, i + R) : value_op(t, i + R - NQ);
             // pairs 0 .. 11 over the steps
             att_each<(i + 1) * 12 / NQ - i * 12 / NQ>([&](auto q) PTA_INLINE {
                 exp_pair(std::integral_constant<int, i * 12 / NQ + decltype(q)::value>{});
             });
-            if (i >= NQ - 2) {
-                x[i - NQ + 2 < 0 ? 0 : i - NQ + 2] = scale_of(t + 1, 0, i - NQ + 2);
-                y[i - NQ + 2 < 0 ? 0 : i - NQ + 2] = scale_of(t + 1, 1, i - NQ + 2);
+            if (i == NQ - 2) {
+                x = scale_of(t + 1, 0, 0);
+                y = scale_of(t + 1, 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -776,8 +816,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         constexpr int which[16] = {12, 0, 0, 13, 1, 2, 14, 1, 3, 15, 4, 2, 5, 6, 3, 7};
         att_each<NQ>([&](auto i_c) PTA_INLINE {
             constexpr int i = decltype(i_c)::value, ks = i / (DP / 32), d = i % (DP / 32);
-            o[d] = AttT<QT>::mfma32(op[i & 3], make_uint4(pf[ks][0], pf[ks][1], pf[ks][2], pf[ks][3]), o[d]);
-            if (i + 4 < NQ) op[i & 3] = value_op(t, i + 4);
+            o[d] = AttT<QT>::mfma32(op[(i + NQ) % R], make_uint4(pf[ks][0], pf[ks][1], pf[ks][2], pf[ks][3]), o[d]);
+            if (i + R < NQ) op[(i + NQ) % R] = value_op(t, i + R);
             att_each<(i + 1) * 16 / NQ - i * 16 / NQ>([&](auto q) PTA_INLINE {
                 constexpr int w = i * 16 / NQ + decltype(q)::value;
                 using W = std::integral_constant<int, which[w]>;
@@ -799,15 +839,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     if (it.t0 < it.t1) {
         // tile t0 whole and the keys of t0 + 1 into LDS; then the state of an iteration's begin
         const int t = it.t0;
-        load_k(t);
-        load_v();
-        holes(khole, krow, kreg);
+        auto load_keys = [&](int tt) PTA_INLINE {
+            next_rows(tt);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) load_key(i);
+            load_scale();
+            shift_rows();
+        };
+        load_keys(t);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) load_value(i);
+        holes(khole, t, kreg);
         stage_keys(t);
-        load_k(t + 1);
+        load_keys(t + 1);
         ready(t - 1);
-        stage_all(t - 1);
-        load_v();
-        load_k(t + 2);
+        next_rows(t + 2);
+        stage_all(t - 1); // values t, keys t + 1; loads values t + 1, keys t + 2
+        shift_rows();
         __syncthreads();
         if (t < tend) {
             att_f16 s[2];
@@ -824,6 +872,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         }
     }
     for (int t = it.t0; t < it.t1; ++t) {
+        // the lane's number anew: what derives from it (addresses in LDS and of the
+        // pieces) is then made again in an iteration instead of kept in registers,
+        // which all have a use: a spilled one's reload would wait for every load in flight
+        lane = att_lane();
+        c    = lane & 31;
+        half = lane >> 5;
+        tid  = wave * 64 + lane;
+        next_rows(t + 3);
         ready(t);
         if (t < tend) {
             if (edge(t, bpmin, it.kend - 1) && (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3])) slow(t);
@@ -833,8 +889,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         } else {
             stage_all(t);
         }
-        load_v();
-        load_k(t + 3);
+        shift_rows();
         rows(t + 4);
         fetch_pages(t + 5);
         // the loads stay in flight over the barrier
@@ -874,12 +929,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 // ---------------------------------------------------------------------------
 // narrow kernel: 16 rows, four waves on 32 keys each of a key tile of 128
 // ---------------------------------------------------------------------------
+// Workgroup = (head, chunk, row tile, sequence), without a search: every sequence
+// has the same number of chunks, of a size of its own.  A wave keeps ST tiles of
+// keys and values in flight in registers.
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(AttnArgs a) {
     constexpr int  KT = 128, BQ = 16, WK = 32;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;
     constexpr int  EC  = 16 / ES;
+    constexpr int  ST  = DP * ES <= 128 ? 2 : 1;
     constexpr int  KP  = DP / 4 / EC;       // 16-byte pieces of a lane's quarter of a key row
     constexpr int  CPR = DP / EC;           // pieces of a value row
     constexpr int  VP  = WK * CPR / 64;     // value pieces of a lane
@@ -891,246 +950,352 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     __shared__ __align__(16) uint8_t smem[SV_BYTES > SO_BYTES ? SV_BYTES : SO_BYTES];
     __shared__ __align__(16) float   ssc[4][3][WK];
     __shared__ float2                sml[4][BQ];
-    __shared__ uint32_t              red[16];
 
-    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int      h    = blockIdx.x % a.Hkv;
-    const int      slot = blockIdx.x / a.Hkv;
-    const AttnItem it   = attn_find<BQ, KT, 256>(a, slot, red);
-    if (a.desc != nullptr && h == 0 && tid == 0)
-        a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
-    if (it.b < 0) return;
+    const int     tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int     h = blockIdx.x % a.Hkv, w0 = blockIdx.x / a.Hkv, chunk = w0 % a.split, w1 = w0 / a.split;
+    const int     b = w1 / a.tiles;
+    const AttnSeq sq   = attn_seq(a, b);
+    const int     n    = __builtin_amdgcn_readfirstlane(sq.n), len = __builtin_amdgcn_readfirstlane(sq.len);
+    const int     tok0 = __builtin_amdgcn_readfirstlane(sq.tok0);
+    const int     c = lane & 15, qd = lane >> 4;
+    uint16_t     *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
 
-    const int  c = lane & 15, qd = lane >> 4;
-    const int  r    = it.row0 + c;
-    const bool rin  = c < it.rows;
-    const int  rtok = rin ? r / a.G : 0;
-    const int  tok  = it.tok0 + rtok;
-    const int  hq   = h * a.G + (rin ? r - rtok * a.G : 0);
-    const int  pos  = rin ? it.pos0 + rtok : -1;
-    const int  wlo  = a.window > 0 ? pos - a.window + 1 : INT_MIN;
-    const bool mixed = a.window > 0 || it.row0 / a.G != (it.row0 + it.rows - 1) / a.G; // rows may see different keys
+    for (int tile = w1 % a.tiles; tile * BQ < n * a.G; tile += a.tiles) {
+        AttnItem it;
+        it.b    = b;
+        it.row0 = tile * BQ;
+        it.rows = min(BQ, n * a.G - it.row0);
+        it.pos0 = len - n;
+        const int total = attn_keys<KT>(a, it, len);
+        const int per   = (total + a.split - 1) / a.split;
+        it.t0           = min(chunk * per, total);
+        it.t1           = min(it.t0 + per, total);
 
-    // k-step s of the products over the head dimension takes elements
-    // qd * DP / 4 + 8 s .. + 7 from quarter qd of the lanes: a lane's part of a
-    // key row is one run of bytes
-    uint4 qf[DP / 32];
-#pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-        const int d = qd * (DP / 4) + s * 8;
-        qf[s]       = rin && d < a.D ? *reinterpret_cast<const uint4 *>(a.q + tok * a.q_st + hq * a.q_sh + d)
-                                     : make_uint4(0, 0, 0, 0);
-    }
-    att_f4 o[DP / 16];
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+        const int  r    = it.row0 + c;
+        const bool rin  = c < it.rows;
+        const int  rtok = rin ? r / a.G : 0;
+        const int  hq   = h * a.G + (rin ? r - rtok * a.G : 0);
+        const int  pos  = rin ? it.pos0 + rtok : -1;
+        const int  wlo  = a.window > 0 ? pos - a.window + 1 : INT_MIN;
+        const bool mixed = a.window > 0 || it.row0 / a.G != (it.row0 + it.rows - 1) / a.G; // rows may see different keys
 
-    uint16_t *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
-    uint4     kreg[2][KP], vreg[VP];
-    float     scl[2] = {0.0f, 1.0f};
-    auto      row_of = [&](int t) PTA_INLINE { // pool row of key lane % 32 of this wave's part
-        return t < it.t1 ? attn_key_row(a, it, h, attn_key0(it, t, KT) + wave * WK + (lane & 31)) : -1;
-    };
-    auto load = [&](int row) PTA_INLINE {
+        uint4    kreg[ST][2][KP], vreg[ST][VP];
+        float    scl[ST][2];
+        int      krow[ST], page_id = -1;
+        uint64_t hole[ST];
+        auto     key = [&](int t) PTA_INLINE { return attn_key0(it, t, KT) + wave * WK + (lane & 31); };
+        auto     fetch_page = [&](int t) PTA_INLINE { page_id = t < it.t1 ? attn_key_page(a, it, key(t)) : -1; };
+        // loads tile t, whose pages were fetched before; keys without a row read row 0
+        // and become zeros when they are used
+        auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no) PTA_INLINE {
+            row = t < it.t1 ? attn_page_row(a, h, key(t), page_id) : -1;
+            no  = __ballot(row < 0);
+            const int at = max(row, 0);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int kr = __shfl(row, b * 16 + c);
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t *p = a.kc + static_cast<int64_t>(__shfl(at, k * 16 + c)) * a.D * ES;
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const int e = qd * (DP / 4) + i * EC;
-                kreg[b][i]  = make_uint4(0, 0, 0, 0);
-                if (kr >= 0 && e < a.D)
-                    kreg[b][i] = *reinterpret_cast<const uint4 *>(a.kc + (static_cast<int64_t>(kr) * a.D + e) * ES);
+                for (int i = 0; i < KP; ++i) {
+                    const int e = qd * (DP / 4) + i * EC;
+                    kr[k][i]    = *reinterpret_cast<const uint4 *>(p + (e < a.D ? e : 0) * ES);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int p = i * 64 + lane, key = p / CPR, e = (p % CPR) * EC;
-            const int vr = __shfl(row, key);
-            vreg[i]      = make_uint4(0, 0, 0, 0);
-            if (vr >= 0 && e < a.D)
-                vreg[i] = *reinterpret_cast<const uint4 *>(a.vc + (static_cast<int64_t>(vr) * a.D + e) * ES);
-        }
-        if constexpr (FP8) {
-            scl[0] = row >= 0 ? a.ks[row] : 0.0f;
-            scl[1] = row >= 0 ? a.vs[row] : 1.0f;
-        }
-    };
-
-    load(row_of(it.t0));
-    int next = row_of(it.t0 + 1);
-    for (int t = it.t0; t < it.t1; ++t) {
-        bool special = false;
-        if (mixed) {
-#pragma unroll
-            for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[i]);
-            special = __any(special);
-        }
-        // this tile's values to LDS, its keys as operands; then the next tile's loads
-#pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int p = i * 64 + lane, key = p / CPR, e = (p % CPR) * EC;
+            for (int i = 0; i < VP; ++i) {
+                const int p = i * 64 + lane, e = (p % CPR) * EC;
+                vr[i]       = *reinterpret_cast<const uint4 *>(a.vc + (static_cast<int64_t>(__shfl(at, p / CPR)) * a.D + (e < a.D ? e : 0)) * ES);
+            }
             if constexpr (FP8) {
-                *reinterpret_cast<uint4 *>(V + key * VS + e)     = att_cvt8<QT, KIND>(vreg[i].x, vreg[i].y);
-                *reinterpret_cast<uint4 *>(V + key * VS + e + 8) = att_cvt8<QT, KIND>(vreg[i].z, vreg[i].w);
-            } else {
-                *reinterpret_cast<uint4 *>(V + key * VS + e) = vreg[i];
+                sc[0] = a.ks[at];
+                sc[1] = a.vs[at];
             }
-        }
-        if constexpr (FP8) {
-            if (lane < WK) {
-                const float vs        = fmaxf(scl[1], 0x1p-100f); // no scale of the writer is below 2^-49; one of zero stands for values of zero
-                ssc[wave][0][lane] = scl[0] * a.scale_log2;
-                ssc[wave][1][lane] = att_log2(vs);
-                ssc[wave][2][lane] = 1.0f / vs;
-            }
-        }
-        uint4 kf[2][DP / 32];
+        };
+        fetch_page(it.t0);
+        // k-step s of the products over the head dimension takes elements
+        // qd * DP / 4 + 8 s .. + 7 from quarter qd of the lanes: a lane's part of a
+        // key row is one run of bytes
+        uint4 qf[DP / 32];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int s = 0; s < DP / 32; ++s) {
+            const int d = qd * (DP / 4) + s * 8;
+            qf[s]       = rin && d < a.D ? *reinterpret_cast<const uint4 *>(a.q + (tok0 + rtok) * a.q_st + hq * a.q_sh + d)
+                                         : make_uint4(0, 0, 0, 0);
+        }
+        att_f4 o[DP / 16];
 #pragma unroll
-            for (int s = 0; s < DP / 32; ++s) {
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+
+        att_each<ST>([&](auto u_c) PTA_INLINE {
+            constexpr int u = decltype(u_c)::value;
+            load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u]);
+            fetch_page(it.t0 + u + 1);
+        });
+        for (int tt = it.t0; tt < it.t1; tt += ST)
+            att_each<ST>([&](auto u_c) PTA_INLINE {
+                constexpr int u = decltype(u_c)::value;
+                const int     t = tt + u;
+                if (u > 0 && t >= it.t1) return;
+                if (a.D != DP || hole[u] != 0) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const bool no = __shfl(krow[u], k * 16 + c) < 0;
+#pragma unroll
+                        for (int i = 0; i < KP; ++i)
+                            if (no || qd * (DP / 4) + i * EC >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VP; ++i) {
+                        const int p = i * 64 + lane;
+                        if (__shfl(krow[u], p / CPR) < 0 || (p % CPR) * EC >= a.D) vreg[u][i] = make_uint4(0, 0, 0, 0);
+                    }
+                    if (krow[u] < 0) {
+                        scl[u][0] = 0.0f;
+                        scl[u][1] = 1.0f;
+                    }
+                }
+                bool special = false;
+                if (mixed) {
+#pragma unroll
+                    for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[u][i]);
+                    special = __any(special);
+                }
+                // this tile's values to LDS, its keys as operands; then the loads of the tile after next
+#pragma unroll
+                for (int i = 0; i < VP; ++i) {
+                    const int p = i * 64 + lane, ky = p / CPR, e = (p % CPR) * EC;
+                    if constexpr (FP8) {
+                        *reinterpret_cast<uint4 *>(V + ky * VS + e)     = att_cvt8<QT, KIND>(vreg[u][i].x, vreg[u][i].y);
+                        *reinterpret_cast<uint4 *>(V + ky * VS + e + 8) = att_cvt8<QT, KIND>(vreg[u][i].z, vreg[u][i].w);
+                    } else {
+                        *reinterpret_cast<uint4 *>(V + ky * VS + e) = vreg[u][i];
+                    }
+                }
                 if constexpr (FP8) {
-                    const uint4 w = kreg[b][s / 2];
-                    kf[b][s] = s % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
-                } else {
-                    kf[b][s] = kreg[b][s];
+                    if (lane < WK) {
+                        const float vs        = fmaxf(scl[u][1], 0x1p-100f); // a scale of zero: values of zero
+                        ssc[wave][0][lane] = scl[u][0] * a.scale_log2;
+                        ssc[wave][1][lane] = att_log2(vs);
+                        ssc[wave][2][lane] = 1.0f / vs;
+                    }
                 }
+                uint4 kf[2][DP / 32];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int s = 0; s < DP / 32; ++s) {
+                        if constexpr (FP8) {
+                            const uint4 w = kreg[u][k][s / 2];
+                            kf[k][s] = s % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
+                        } else {
+                            kf[k][s] = kreg[u][k][s];
+                        }
+                    }
+                load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u]);
+                fetch_page(t + ST + 1);
+                att_f4 s[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[k][j] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) s[k] = AttT<QT>::mfma16(kf[k][i], qf[i], s[k]);
+                }
+                // the wave's own LDS writes are seen by its later reads once they are done
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                const int key0 = attn_key0(it, t, KT) + wave * WK;
+                float     mx = m, iv[2][4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int kk = k * 16 + 4 * qd;
+                    if constexpr (FP8) {
+                        const float4 x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
+                        const float4 y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
+                        const float4 z = *reinterpret_cast<const float4 *>(&ssc[wave][2][kk]);
+                        s[k][0] = fmaf(s[k][0], x.x, y.x); s[k][1] = fmaf(s[k][1], x.y, y.y);
+                        s[k][2] = fmaf(s[k][2], x.z, y.z); s[k][3] = fmaf(s[k][3], x.w, y.w);
+                        iv[k][0] = z.x; iv[k][1] = z.y; iv[k][2] = z.z; iv[k][3] = z.w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[k][j] *= a.scale_log2;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int  ky  = key0 + kk + j;
+                        const bool see = (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
+                        s[k][j]        = see ? s[k][j] : -INFINITY;
+                        mx             = fmaxf(mx, s[k][j]);
+                    }
+                }
+                mx                = max_xor32(max_xor16(mx));
+                const float base  = mx == -INFINITY ? 0.0f : mx;
+                const float alpha = att_exp2(m - base);
+                m                 = mx;
+                l *= alpha;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[k][j] = att_exp2(s[k][j] - base);
+                        if constexpr (FP8) l = fmaf(s[k][j], iv[k][j], l);
+                        else l += s[k][j];
+                    }
+                const uint4 pf = make_uint4(AttT<QT>::pack(s[0][0], s[0][1]), AttT<QT>::pack(s[0][2], s[0][3]),
+                                            AttT<QT>::pack(s[1][0], s[1][1]), AttT<QT>::pack(s[1][2], s[1][3]));
+                const int   kr = 4 * qd + c / 4, dc = 4 * (c & 3);
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+                    const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
+                    const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+                    if (!special) {
+                        o[i] = AttT<QT>::mfma16(vf, pf, o[i]);
+                    } else {
+                        // infinities and NaN that only some rows see: 0 * inf must not reach the
+                        // others.  Finite values go as ever; then a count of the special ones that
+                        // a row sees decides.
+                        uint4  fin, plus, minus;
+                        att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
+                        att_split_special<QT>(vf, fin, plus, minus);
+                        const uint4 seen = att_nonzero<QT>(pf);
+                        o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
+                        np   = AttT<QT>::mfma16(plus, seen, np);
+                        nm   = AttT<QT>::mfma16(minus, seen, nm);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (np[j] > 0.0f) o[i][j] += INFINITY;
+                            if (nm[j] > 0.0f) o[i][j] -= INFINITY;
+                        }
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            });
+        l = add_xor32(add_xor16(l));
+        // the four waves' parts join in LDS
+        __syncthreads(); // the values' LDS becomes the outputs'
+        float *so = reinterpret_cast<float *>(smem);
+        if (qd == 0) sml[wave][c] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+            *reinterpret_cast<float4 *>(so + (wave * BQ + c) * OS + i * 16 + 4 * qd) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        __syncthreads();
+        constexpr int TPR = 16, DPT = DP / TPR; // threads of a row, their elements
+        const int     jr = tid / TPR, jd = (tid % TPR) * DPT;
+        if (jr < it.rows) {
+            float mm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w][jr].x);
+            const float base = mm == -INFINITY ? 0.0f : mm;
+            float       ll = 0.0f, acc[DPT];
+#pragma unroll
+            for (int e = 0; e < DPT; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = att_exp2(sml[w][jr].x - base);
+                ll            = fmaf(sml[w][jr].y, f, ll);
+#pragma unroll
+                for (int e = 0; e < DPT; ++e) acc[e] = fmaf(so[(w * BQ + jr) * OS + jd + e], f, acc[e]);
             }
-        if (t + 1 < it.t1) {
-            load(next);
-            next = row_of(t + 2);
-        }
-        att_f4 s[2];
+            const int     rr = it.row0 + jr, rt = rr / a.G;
+            const int64_t orow = static_cast<int64_t>(tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
+            if (a.split == 1) {
+                const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f; // no key seen: zeros
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[b][j] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < DP / 32; ++k) s[b] = AttT<QT>::mfma16(kf[b][k], qf[k], s[b]);
-        }
-        // the wave's own LDS writes are seen by its later reads once they are done
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const int key0 = attn_key0(it, t, KT) + wave * WK;
-        float     mx = m, iv[2][4];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int kk = b * 16 + 4 * qd;
-            if constexpr (FP8) {
-                const float4 x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
-                const float4 y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
-                const float4 z = *reinterpret_cast<const float4 *>(&ssc[wave][2][kk]);
-                s[b][0] = fmaf(s[b][0], x.x, y.x); s[b][1] = fmaf(s[b][1], x.y, y.y);
-                s[b][2] = fmaf(s[b][2], x.z, y.z); s[b][3] = fmaf(s[b][3], x.w, y.w);
-                iv[b][0] = z.x; iv[b][1] = z.y; iv[b][2] = z.z; iv[b][3] = z.w;
+                for (int e = 0; e < DPT; e += 4)
+                    if (jd + e < a.D)
+                        *reinterpret_cast<uint2 *>(a.out + orow * a.D + jd + e) =
+                            make_uint2(AttT<QT>::pack(acc[e] * inv, acc[e + 1] * inv), AttT<QT>::pack(acc[e + 2] * inv, acc[e + 3] * inv));
+                if (a.lse != nullptr && jd == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;
             } else {
+                const int64_t at = static_cast<int64_t>(chunk) * a.Tq * a.Hq + orow;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[b][j] *= a.scale_log2;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int  key = key0 + kk + j;
-                const bool see = (key <= pos) & ((key >= wlo) | (key < a.sinks));
-                s[b][j]        = see ? s[b][j] : -INFINITY;
-                mx             = fmaxf(mx, s[b][j]);
+                for (int e = 0; e < DPT; e += 4)
+                    if (jd + e < a.D)
+                        *reinterpret_cast<float4 *>(a.part_o + at * a.D + jd + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+                if (jd == 0) a.part_ml[at] = make_float2(mm, ll);
             }
         }
-        mx                = max_xor32(max_xor16(mx));
-        const float base  = mx == -INFINITY ? 0.0f : mx;
-        const float alpha = att_exp2(m - base);
-        m                 = mx;
-        l *= alpha;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[b][j] = att_exp2(s[b][j] - base);
-                if constexpr (FP8) l = fmaf(s[b][j], iv[b][j], l);
-                else l += s[b][j];
-            }
-        const uint4 pf = make_uint4(AttT<QT>::pack(s[0][0], s[0][1]), AttT<QT>::pack(s[0][2], s[0][3]),
-                                    AttT<QT>::pack(s[1][0], s[1][1]), AttT<QT>::pack(s[1][2], s[1][3]));
-        const int   kr = 4 * qd + c / 4, dc = 4 * (c & 3);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
-            const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
-            const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
-            if (!special) {
-                o[i] = AttT<QT>::mfma16(vf, pf, o[i]);
-            } else { // as in the wide kernel's values_special
-                uint4  fin, plus, minus;
-                att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
-                att_split_special<QT>(vf, fin, plus, minus);
-                const uint4 see = att_nonzero<QT>(pf);
-                o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
-                np   = AttT<QT>::mfma16(plus, see, np);
-                nm   = AttT<QT>::mfma16(minus, see, nm);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (np[j] > 0.0f) o[i][j] += INFINITY;
-                    if (nm[j] > 0.0f) o[i][j] -= INFINITY;
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
-    l = add_xor32(add_xor16(l));
-    // the four waves' parts join in LDS
-    __syncthreads(); // the values' LDS becomes the outputs'
-    float *so = reinterpret_cast<float *>(smem);
-    if (qd == 0) sml[wave][c] = make_float2(m, l);
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-        *reinterpret_cast<float4 *>(so + (wave * BQ + c) * OS + i * 16 + 4 * qd) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-    __syncthreads();
-    constexpr int TPR = 16, DPT = DP / TPR; // threads of a row, their elements
-    const int     jr = tid / TPR, jd = (tid % TPR) * DPT;
-    if (jr >= it.rows) return;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w][jr].x);
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float       ll = 0.0f, acc[DPT];
-#pragma unroll
-    for (int e = 0; e < DPT; ++e) acc[e] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = att_exp2(sml[w][jr].x - base);
-        ll            = fmaf(sml[w][jr].y, f, ll);
-#pragma unroll
-        for (int e = 0; e < DPT; ++e) acc[e] = fmaf(so[(w * BQ + jr) * OS + jd + e], f, acc[e]);
-    }
-    if (it.chunks == 1) {
-        const int     rr = it.row0 + jr, rt = rr / a.G;
-        const int64_t orow = static_cast<int64_t>(it.tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
-        const float   inv  = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
-#pragma unroll
-        for (int e = 0; e < DPT; e += 4)
-            if (jd + e < a.D)
-                *reinterpret_cast<uint2 *>(a.out + orow * a.D + jd + e) =
-                    make_uint2(AttT<QT>::pack(acc[e] * inv, acc[e + 1] * inv), AttT<QT>::pack(acc[e + 2] * inv, acc[e + 3] * inv));
-        if (a.lse != nullptr && jd == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;
-    } else {
-        const int64_t at = (static_cast<int64_t>(slot) * a.Hkv + h) * BQ + jr;
-#pragma unroll
-        for (int e = 0; e < DPT; e += 4)
-            if (jd + e < a.D)
-                *reinterpret_cast<float4 *>(a.part_o + at * a.D + jd + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-        if (jd == 0) a.part_ml[at] = make_float2(mm, ll);
+        __syncthreads(); // the outputs' LDS becomes the values' of the next row tile
     }
 }
 
 // ---------------------------------------------------------------------------
-// joins the chunks of a row tile: workgroup = (first slot of the tile, head), a
+// joins the narrow kernel's chunks: 64 elements of 4 values a workgroup, four
+// threads share an element's chunks
+// ---------------------------------------------------------------------------
+template <int QT> __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
+    __shared__ float4 sacc[4][64];
+    __shared__ float2 sml[4][64];
+    const int     lane = threadIdx.x & 63, quarter = threadIdx.x >> 6, tpr = a.D / 4;
+    const int64_t rows = static_cast<int64_t>(a.Tq) * a.Hq, all = rows * tpr;
+    const int64_t p = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    const int64_t row = min(p / tpr, rows - 1);
+    const int     d = static_cast<int>(p - p / tpr * tpr) * 4;
+    bool          in = p < all;
+    if (a.rows_max != INT_MAX) { // rows of other sequences are the wide kernel's
+        const int tok = static_cast<int>(row / a.Hq);
+        int       lo = 0, hi = a.B; // the last sequence that begins at or before the token
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu[mid] <= tok) lo = mid;
+            else hi = mid;
+        }
+        const AttnSeq s = attn_seq(a, lo);
+        in              = in && tok >= s.tok0 && tok < s.tok0 + s.n;
+    }
+    float  mm = -INFINITY, ll = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in)
+        for (int c0 = quarter; c0 < a.split; c0 += 16) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = min(c0 + 4 * u, a.split - 1) * rows + row;
+                ml[u]            = a.part_ml[at];
+                x[u]             = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + 4 * u >= a.split) break;
+                const float n = fmaxf(mm, ml[u].x), base = n == -INFINITY ? 0.0f : n;
+                const float f = att_exp2(mm - base), g = att_exp2(ml[u].x - base);
+                mm    = n;
+                ll    = fmaf(ml[u].y, g, ll * f);
+                acc.x = fmaf(x[u].x, g, acc.x * f); acc.y = fmaf(x[u].y, g, acc.y * f);
+                acc.z = fmaf(x[u].z, g, acc.z * f); acc.w = fmaf(x[u].w, g, acc.w * f);
+            }
+        }
+    sacc[quarter][lane] = acc;
+    sml[quarter][lane]  = make_float2(mm, ll);
+    __syncthreads();
+    if (quarter != 0 || !in) return;
+#pragma unroll
+    for (int u = 1; u < 4; ++u) {
+        const float2 ml = sml[u][lane];
+        const float4 x  = sacc[u][lane];
+        const float  n = fmaxf(mm, ml.x), base = n == -INFINITY ? 0.0f : n;
+        const float  f = att_exp2(mm - base), g = att_exp2(ml.x - base);
+        mm    = n;
+        ll    = fmaf(ml.y, g, ll * f);
+        acc.x = fmaf(x.x, g, acc.x * f); acc.y = fmaf(x.y, g, acc.y * f);
+        acc.z = fmaf(x.z, g, acc.z * f); acc.w = fmaf(x.w, g, acc.w * f);
+    }
+    const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
+    *reinterpret_cast<uint2 *>(a.out + row * a.D + d) =
+        make_uint2(AttT<QT>::pack(acc.x * inv, acc.y * inv), AttT<QT>::pack(acc.z * inv, acc.w * inv));
+    if (a.lse != nullptr && d == 0) a.lse[row] = (mm + att_log2(ll)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------------------
+// joins the wide kernel's chunks of a row tile: workgroup = (first slot of the tile, head), a
 // part of the tile's rows; four threads share an element's chunks
 // ---------------------------------------------------------------------------
 constexpr int ATT_JOIN_PARTS = 8;

@@ -11,9 +11,10 @@ namespace {
 struct AttnPart {
     int     rows; // of a row tile; 0: not launched
     int     rows_min, rows_max;
-    int64_t slots, goal;
+    int64_t slots, goal;  // wide
+    int64_t split, tiles; // narrow
     size_t  desc_bytes, ml_bytes, o_bytes;
-    size_t  bytes() const { return goal > 0 ? desc_bytes + ml_bytes + o_bytes : 0; }
+    size_t  bytes() const { return desc_bytes + ml_bytes + o_bytes; }
 };
 
 struct AttnPlan {
@@ -21,23 +22,43 @@ struct AttnPlan {
     size_t   bytes() const { return part[0].bytes() + part[1].bytes(); }
 };
 
+size_t round256(int64_t n) { return static_cast<size_t>(cdiv(n, 256) * 256); }
+
 // Rows of a sequence up to which the narrow kernel takes it where both run
 constexpr int ATT_NARROW_MOST = 64;
 
-AttnPart attn_part(int rows, int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t keys) {
+// Every sequence gets the same number of chunks: two workgroups a CU from all of
+// them, four chunks where sequences may differ in length, no more than key tiles.
+AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool mix) {
+    AttnPart      p    = {};
+    const int64_t fill = cdiv(2 * device_cu_count(), B * Hkv);
+    p.rows     = ATT_NARROW_ROWS;
+    p.rows_max = mix ? ATT_NARROW_MOST : INT_MAX;
+    p.tiles    = mix ? ATT_NARROW_MOST / ATT_NARROW_ROWS : 1;
+    p.split    = std::max<int64_t>(1, std::min(std::max<int64_t>(fill, B > 1 ? 4 : 1), cdiv(keys, ATT_NARROW_KEYS)));
+    if (p.split > 1) {
+        p.ml_bytes = round256(p.split * Tq * Hq * 8);
+        p.o_bytes  = round256(p.split * Tq * Hq * D * 4);
+    }
+    return p;
+}
+
+// Row tiles are found on the device (their number goes by the lengths); they are
+// split where they do not give every CU one.
+AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t keys, bool mix) {
     AttnPart p = {};
-    p.rows     = rows;
+    p.rows     = ATT_WIDE_ROWS;
+    p.rows_min = mix ? ATT_NARROW_MOST : 0;
     p.rows_max = INT_MAX;
-    const int64_t kt   = rows == ATT_NARROW_ROWS ? ATT_NARROW_KEYS : ATT_WIDE_KEYS;
-    const int64_t most = Tq * G / rows + B; // row tiles of a head: sum of ceil(n G / rows)
-    const int64_t goal = cdiv((rows == ATT_NARROW_ROWS ? 2 : 1) * device_cu_count(), Hkv); // workgroups a CU
+    const int64_t most = Tq * G / ATT_WIDE_ROWS + B; // row tiles of a head: sum of ceil(n G / rows)
+    const int64_t goal = cdiv(device_cu_count(), Hkv);
     // row tiles alone fill the chip, or no tile has keys for two chunks
-    p.goal  = most - B >= goal || keys <= kt ? 0 : goal;
+    p.goal  = most - B >= goal || keys <= ATT_WIDE_KEYS ? 0 : goal;
     p.slots = most + p.goal;
     if (p.goal > 0) {
-        p.desc_bytes = static_cast<size_t>(cdiv(p.slots * 16, 256) * 256);
-        p.ml_bytes   = static_cast<size_t>(cdiv(p.slots * Hkv * rows * 8, 256) * 256);
-        p.o_bytes    = static_cast<size_t>(p.slots * Hkv * rows * D * 4);
+        p.desc_bytes = round256(p.slots * 16);
+        p.ml_bytes   = round256(p.slots * Hkv * ATT_WIDE_ROWS * 8);
+        p.o_bytes    = round256(p.slots * Hkv * ATT_WIDE_ROWS * D * 4);
     }
     return p;
 }
@@ -50,9 +71,8 @@ AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, in
     const int64_t G = Hq / Hkv, keys = max_pages * page;
     const bool    few = Tq * G <= 16 * B || Tq * G <= ATT_NARROW_MOST; // a row tile each on average, or no sequence has many
     const bool    mix = !few && B > 1;
-    if (few || mix) p.part[0] = attn_part(ATT_NARROW_ROWS, mix ? std::min<int64_t>(Tq, B * ATT_NARROW_MOST) : Tq, B, Hkv, G, D, keys);
-    if (!few) p.part[1] = attn_part(ATT_WIDE_ROWS, Tq, B, Hkv, G, D, keys);
-    if (mix) p.part[0].rows_max = p.part[1].rows_min = ATT_NARROW_MOST;
+    if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix);
+    if (!few) p.part[1] = attn_wide_part(Tq, B, Hkv, G, D, keys, mix);
     return p;
 }
 
@@ -105,7 +125,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
     PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
                   "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG((p.part[0].slots + p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
+    PTA_CHECK_ARG((p.part[0].split * p.part[0].tiles * num_seqs + p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
     AttnArgs a = {};
     a.q = static_cast<const uint16_t *>(q);
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
@@ -131,9 +151,10 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     for (const AttnPart &part : p.part) {
         if (part.rows == 0) continue;
         a.slots = static_cast<int>(part.slots); a.split_goal = static_cast<int>(part.goal);
+        a.split = static_cast<int>(part.split); a.tiles = static_cast<int>(part.tiles);
         a.rows_min = part.rows_min; a.rows_max = part.rows_max;
         a.desc = nullptr; a.part_ml = nullptr; a.part_o = nullptr;
-        if (part.goal > 0) {
+        if (part.bytes() > 0) {
             a.desc    = reinterpret_cast<int4 *>(ws);
             a.part_ml = reinterpret_cast<float2 *>(ws + part.desc_bytes);
             a.part_o  = reinterpret_cast<float *>(ws + part.desc_bytes + part.ml_bytes);

@@ -6,15 +6,15 @@
 namespace pta {
 
 template <int QT, int KIND, int DP> void attn_launch_d(const AttnArgs &a, int rows, hipStream_t st) {
-    const unsigned grid = static_cast<unsigned>(a.slots) * static_cast<unsigned>(a.Hkv);
-    const dim3     join(grid, ATT_JOIN_PARTS);
     if (rows == ATT_NARROW_ROWS) {
+        const unsigned grid = static_cast<unsigned>(a.B) * a.tiles * a.split * a.Hkv;
         attn_narrow_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(a);
-        if (a.split_goal > 0) attn_join_kernel<QT, ATT_NARROW_ROWS><<<join, 256, 0, st>>>(a);
-        return;
+        if (a.split > 1) attn_join_rows_kernel<QT><<<static_cast<unsigned>(cdiv(static_cast<int64_t>(a.Tq) * a.Hq * (a.D / 4), 64)), 256, 0, st>>>(a);
+    } else {
+        const unsigned grid = static_cast<unsigned>(a.slots) * static_cast<unsigned>(a.Hkv);
+        attn_wide_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(a);
+        if (a.split_goal > 0) attn_join_kernel<QT, ATT_WIDE_ROWS><<<dim3(grid, ATT_JOIN_PARTS), 256, 0, st>>>(a);
     }
-    attn_wide_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(a);
-    if (a.split_goal > 0) attn_join_kernel<QT, 128><<<join, 256, 0, st>>>(a);
 }
 
 template <int QT, int KIND> void attn_launch_k(const AttnArgs &a, int rows, hipStream_t st) {
