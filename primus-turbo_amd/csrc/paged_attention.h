@@ -452,13 +452,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     constexpr int  CPR = DP / EC;           // pieces of a row
     constexpr int  NP  = KT * CPR / NT;     // pieces of a thread and pool
     constexpr int  KS  = DP + 8;            // elements of a staged key row: 16 rows' equal pieces lie in different banks
-    constexpr int  VS  = DP + 32;           // of a value row: the transposed read's 8 rows of 64 bytes do
+    constexpr int  VS  = DP + 32;           // of a value row: the transposed read's 8 rows of 64 bytes do; odd keys have
+                                            // the halves of every 32 bytes exchanged, for the writes' sake
     static_assert(KT * CPR % NT == 0, "pieces");
     __shared__ __align__(16) uint16_t sk[2][KT * KS];
     __shared__ __align__(16) uint16_t sv[2][KT * VS];
     __shared__ __align__(16) float    ssc[FP8 ? 3 : 1][3][FP8 ? KT : 4]; // scale log2e ks, log2 vs, 1 / vs by tile % 3
-    __shared__ int                    srow[4][KT];
-    __shared__ int                    shole[4];   // by tile % 4: some key has no row
+    __shared__ int                    srow[8][KT];
+    __shared__ int                    shole[8];   // by tile % 8: some key has no row
     __shared__ int                    sspec[2][4]; // by tile % 2 and wave: values with infinities or NaN
     __shared__ uint32_t               red[16];
 
@@ -500,6 +501,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     tend = __builtin_amdgcn_readfirstlane(tend);
     // tiles in which not every row sees every key
     const int  bpmin  = it.pos0 + it.row0 / a.G;
+    const bool full_block = it.rows == BQ;
     auto edge = [&](int t, int pmin, int pmax) PTA_INLINE {
         const int key0 = attn_key0(it, t, KT);
         return key0 + KT - 1 > pmin || (a.window > 0 && key0 < pmax - a.window + 1);
@@ -514,19 +516,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 
     uint4 kreg[NP], vreg[NP];
     float kscl = 0.0f, vscl = 1.0f; // of key `tid`, as old as kreg
-    // pool rows of a key tile's keys, from their pages, which were fetched an
-    // iteration before
+    // Pool rows of four key tiles' keys, one tile a wave, every fourth iteration; from
+    // their pages, which were fetched four iterations before
     int  page_id = -1;
-    auto fetch_pages = [&](int t) PTA_INLINE {
-        if (wave == 0) page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
+    auto fetch_pages = [&](int t) PTA_INLINE { // t: the wave's tile
+        page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
     };
     auto rows = [&](int t) PTA_INLINE {
-        if (wave == 0) {
-            const int row     = attn_page_row(a, h, attn_key0(it, t, KT) + lane, page_id);
-            srow[t & 3][lane] = row;
-            const uint64_t no = __ballot(row < 0);
-            if (lane == 0) shole[t & 3] = no != 0;
-        }
+        const int row     = attn_page_row(a, h, attn_key0(it, t, KT) + lane, page_id);
+        srow[t & 7][lane] = row;
+        const uint64_t no = __ballot(row < 0);
+        if (lane == 0) shole[t & 7] = no != 0;
     };
     // Keys without a row read row 0 and become zeros when they are staged.  At an
     // iteration's begin kreg, krow are of tile t + 2, vreg is of tile t + 1; each
@@ -539,9 +539,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     };
     auto next_rows = [&](int t) PTA_INLINE { // of the tile whose keys are loaded next
 #pragma unroll
-        for (int i = 0; i < NP; ++i) nrow[i] = srow[t & 3][(i * NT + tid) / CPR];
-        nhole = shole[t & 3];
-        if constexpr (FP8) srow_n = srow[t & 3][lane];
+        for (int i = 0; i < NP; ++i) nrow[i] = srow[t & 7][(i * NT + tid) / CPR];
+        nhole = shole[t & 7];
+        if constexpr (FP8) srow_n = srow[t & 7][lane];
     };
     auto load_key = [&](int i) PTA_INLINE { kreg[i] = piece(a.kc, i, nrow[i]); };
     auto load_value = [&](int i) PTA_INLINE { vreg[i] = piece(a.vc, i, krow[i]); };
@@ -562,10 +562,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int e = ((i * NT + tid) % CPR) * EC;
-                if (srow[t & 3][(i * NT + tid) / CPR] < 0 || e >= a.D) r[i] = make_uint4(0, 0, 0, 0);
+                if (srow[t & 7][(i * NT + tid) / CPR] < 0 || e >= a.D) r[i] = make_uint4(0, 0, 0, 0);
             }
         }
     };
+    // tiles [calm0, calm1): every row sees every key
+    int calm0 = it.n_sink, calm1 = it.n_sink;
+    if (full_block) {
+        const int first = a.window > 0 ? max(0, it.kend - a.window + KT - 1) / KT : 0; // key0 >= the last row's window's begin
+        const int last  = (bpmin + 1) / KT;                                            // key0 + KT - 1 <= the first row's position
+        calm0           = it.n_sink + max(0, first - it.lo_tile);
+        calm1           = max(calm0, it.n_sink + last - it.lo_tile);
+    }
     // what is rare about the keys of tile t + 2 and the values of tile t + 1, ahead of their staging
     auto ready = [&](int t) PTA_INLINE {
         holes(khole, t + 2, kreg);
@@ -582,12 +590,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
             if (lane == 0) sspec[(t + 1) & 1][wave] = any != 0;
         }
     };
-    auto put = [&](uint16_t *at, const uint4 &r) PTA_INLINE {
+    auto put = [&](uint16_t *row, int e, int odd, const uint4 &r) PTA_INLINE { // odd: 8, or 0
         if constexpr (FP8) {
-            *reinterpret_cast<uint4 *>(at)     = att_cvt8<QT, KIND>(r.x, r.y);
-            *reinterpret_cast<uint4 *>(at + 8) = att_cvt8<QT, KIND>(r.z, r.w);
+            *reinterpret_cast<uint4 *>(row + (e ^ odd))       = att_cvt8<QT, KIND>(r.x, r.y);
+            *reinterpret_cast<uint4 *>(row + (e ^ 8 ^ odd)) = att_cvt8<QT, KIND>(r.z, r.w);
         } else {
-            *reinterpret_cast<uint4 *>(at) = r;
+            *reinterpret_cast<uint4 *>(row + (e ^ odd)) = r;
         }
     };
     // The registers are opaque where they are staged: their conversions would
@@ -596,19 +604,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     auto stage_key = [&](int t, int i) PTA_INLINE {
         const int p = i * NT + tid;
         here(kreg[i]);
-        put(&sk[0][0] + (t & 1) * (KT * KS) + (p / CPR) * KS + (p % CPR) * EC, kreg[i]);
+        put(&sk[0][0] + (t & 1) * (KT * KS) + (p / CPR) * KS, (p % CPR) * EC, 0, kreg[i]);
     };
     auto stage_value = [&](int t, int i) PTA_INLINE {
         const int p = i * NT + tid;
         here(vreg[i]);
-        put(&sv[0][0] + (t & 1) * (KT * VS) + (p / CPR) * VS + (p % CPR) * EC, vreg[i]);
+        put(&sv[0][0] + (t & 1) * (KT * VS) + (p / CPR) * VS, (p % CPR) * EC, (p / CPR & 1) * 8, vreg[i]);
     };
     auto stage_scale = [&](int t) PTA_INLINE { // the waves share the three tables
         if constexpr (FP8) {
             asm volatile("" : "+v"(kscl), "+v"(vscl));
-            const bool  no = srow[t & 3][lane] < 0;
+            const bool  no = srow[t & 7][lane] < 0;
             const float vs = no ? 1.0f : fmaxf(vscl, 0x1p-100f); // a scale of zero: values of zero
-            const float w  = wave == 0 ? (no ? 0.0f : kscl) * a.scale_log2 : wave == 1 ? att_log2(vs) : 1.0f / vs;
+            const float w  = wave == 0 ? (no ? 0.0f : kscl) * a.scale_log2 : wave == 1 ? att_log2(vs) : __builtin_amdgcn_rcpf(vs);
             ssc[(t + 3) % 3][min(wave, 2)][lane] = w; // the fourth writes what the third does
         }
     };
@@ -645,7 +653,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         return *reinterpret_cast<const uint4 *>(klane + (t & 1) * (KT * KS) + i / (DP / 16) * 32 * KS + i % (DP / 16) * 16);
     };
     auto value_op = [&](int t, int i) PTA_INLINE {
-        const uint16_t *vlane = &sv[0][0] + (half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
+        const uint16_t *vlane = &sv[0][0] + (half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + ((4 * (lane & 3)) ^ (8 * ((lane >> 2) & 1)));
         const uint16_t *V = vlane + (t & 1) * (KT * VS) + i / (DP / 32) * 16 * VS + i % (DP / 32) * 32;
         const uint2     v0 = att_tr16(V), v1 = att_tr16(V + 8 * VS);
         return make_uint4(v0.x, v0.y, v1.x, v1.y);
@@ -723,7 +731,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         const int key0 = attn_key0(it, t, KT), wlo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
 #pragma unroll 1
         for (int j = 0; j < KT; ++j) {
-            const int       row = __builtin_amdgcn_readfirstlane(srow[t & 3][j]), key = key0 + j;
+            const int       row = __builtin_amdgcn_readfirstlane(srow[t & 7][j]), key = key0 + j;
             const uint16_t *K   = &sk[0][0] + (t & 1) * (KT * KS) + j * KS + half * 8;
             float           x   = 0.0f;
 #pragma unroll
@@ -829,12 +837,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         });
     };
 
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        fetch_pages(it.t0 + i);
-        rows(it.t0 + i);
-    }
-    fetch_pages(it.t0 + 4);
+    fetch_pages(it.t0 + wave);
+    rows(it.t0 + wave);
+    fetch_pages(it.t0 + 4 + wave);
     __syncthreads();
     if (it.t0 < it.t1) {
         // tile t0 whole and the keys of t0 + 1 into LDS; then the state of an iteration's begin
@@ -880,18 +885,25 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         half = lane >> 5;
         tid  = wave * 64 + lane;
         next_rows(t + 3);
-        ready(t);
+        const bool calm = t >= calm0 && t + 1 < calm1 && (khole | vhole) == 0 && a.D == DP;
+        if (!calm) {
+            ready(t);
+            if (t < tend && edge(t, bpmin, it.kend - 1) &&
+                (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3]))
+                slow(t);
+        }
         if (t < tend) {
-            if (edge(t, bpmin, it.kend - 1) && (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3])) slow(t);
             rescale();
             tile(t);
-            if (!full || edge(t + 1, wpmin, wpmax)) mask(t + 1);
+            if (!calm && (!full || edge(t + 1, wpmin, wpmax))) mask(t + 1);
         } else {
             stage_all(t);
         }
         shift_rows();
-        rows(t + 4);
-        fetch_pages(t + 5);
+        if (((t - it.t0) & 3) == 0) { // tiles t + 4 .. t + 7; the slots of t - 4 .. t - 1
+            rows(t + 4 + wave);
+            fetch_pages(t + 8 + wave);
+        }
         // the loads stay in flight over the barrier
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
