@@ -43,6 +43,7 @@ namespace pta {
 // on lambdas of a kernel: one that is called captures its arrays in memory
 #define PTA_INLINE __attribute__((always_inline))
 
+constexpr int ATT_WIDE_ROWS = 128, ATT_WIDE_KEYS = 64, ATT_NARROW_ROWS = 16, ATT_NARROW_KEYS = 128;
 constexpr int ATT_NONE = INT_MIN; // desc of a slot without work
 
 struct AttnArgs {
@@ -237,8 +238,9 @@ template <int KT> __device__ __forceinline__ int attn_keys(const AttnArgs &a, At
 
 // Finds the item of slot `slot`; all threads of the workgroup call it (`red`:
 // 2 * 8 words of LDS).  Items are numbered sequence by sequence, row tile by row
-// tile, chunk by chunk; a chunk is `C` key tiles, C such that all items of a
-// head fit the grid: sum over the row tiles of ceil(k / C) <= sum(k) / C + tiles.
+// tile, chunk by chunk; a row tile's k key tiles make ceil(k / C) equal chunks, C
+// such that all items of a head fit the grid: sum over the row tiles of
+// ceil(k / C) <= sum(k) / C + tiles.
 template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs &a, int slot, uint32_t *red) {
     constexpr int NW = NTHR / 64;
     const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -261,7 +263,8 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         return v + before;
     };
     AttnItem it;
-    it.b    = -1;
+    it.b            = -1;
+    const AttnSeq s0 = tid < a.B ? attn_seq(a, tid) : AttnSeq{0, 0, 0};
     int   C = INT_MAX;
     if (a.split_goal > 0) {
         // sums past 32 bits only make C larger than needed: in floating point
@@ -269,7 +272,7 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         for (int b0 = 0; b0 < a.B; b0 += NTHR) {
             const int b = b0 + tid;
             if (b < a.B) {
-                const AttnSeq s = attn_seq(a, b);
+                const AttnSeq s = b0 == 0 ? s0 : attn_seq(a, b);
                 const float   r = static_cast<float>((static_cast<int64_t>(s.n) * a.G + BQ - 1) / BQ);
                 w += r * static_cast<float>(attn_tiles<KT>(a, s, BQ));
             }
@@ -291,7 +294,7 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         AttnSeq   s = {0, 0, 0};
         uint32_t  tiles = 0, chunks = 1;
         if (b < a.B) {
-            s      = attn_seq(a, b);
+            s      = b0 == 0 ? s0 : attn_seq(a, b);
             tiles  = static_cast<uint32_t>((static_cast<int64_t>(s.n) * a.G + BQ - 1) / BQ);
             const int k = attn_tiles<KT>(a, s, BQ);
             chunks      = k > C ? (k - 1) / C + 1 : 1;
@@ -306,6 +309,9 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
                 red[0] = b;
                 red[1] = at - (incl - mine);
                 red[2] = chunks;
+                red[3] = s.n;
+                red[4] = s.len;
+                red[5] = s.tok0;
             }
             __syncthreads();
             it.b      = __builtin_amdgcn_readfirstlane(red[0]);
@@ -318,15 +324,14 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         seen += total;
     }
     if (it.b < 0) return it;
-    const AttnSeq s = attn_seq(a, it.b);
-    it.tok0 = s.tok0;
-    it.pos0 = s.len - s.n; // below 0 where more tokens came than the length says: those see nothing
+    const int n = __builtin_amdgcn_readfirstlane(red[3]), len = __builtin_amdgcn_readfirstlane(red[4]);
+    it.tok0 = __builtin_amdgcn_readfirstlane(red[5]);
+    it.pos0 = len - n; // below 0 where more tokens came than the length says: those see nothing
     it.row0 = it.tile * BQ;
-    it.rows = min(BQ, s.n * a.G - it.row0);
-    const int     n  = attn_keys<KT>(a, it, s.len);
-    const int64_t c0 = static_cast<int64_t>(it.chunk) * C;
-    it.t0 = static_cast<int>(min(c0, static_cast<int64_t>(n)));
-    it.t1 = it.chunk == it.chunks - 1 ? n : static_cast<int>(min(c0 + C, static_cast<int64_t>(n)));
+    it.rows = min(BQ, n * a.G - it.row0);
+    const int64_t k = attn_keys<KT>(a, it, len);
+    it.t0 = static_cast<int>(k * it.chunk / it.chunks);
+    it.t1 = static_cast<int>(k * (it.chunk + 1) / it.chunks);
     // all of it is the workgroup's, but came through vector loads: into scalar registers
     for (int *f : {&it.row0, &it.rows, &it.tok0, &it.pos0, &it.kend, &it.lo, &it.n_sink, &it.lo_tile, &it.t0, &it.t1})
         *f = __builtin_amdgcn_readfirstlane(*f);
@@ -341,22 +346,17 @@ __device__ __forceinline__ int attn_page_of(const AttnArgs &a, int j) {
     const uint32_t u = static_cast<uint32_t>(j);
     return static_cast<int>((a.page_mul ? __umulhi(u, a.page_mul) : u) >> a.page_shift);
 }
-// Page of key j, or -1 where there is none
+// Page of key j, or -1 where there is none: past the keys, or hidden from every
+// row by the window
 __device__ __forceinline__ int attn_key_page(const AttnArgs &a, const AttnItem &it, int j) {
     if (j >= it.kend || (j < it.lo && j >= a.sinks)) return -1;
     return a.table[it.b * a.table_st + attn_page_of(a, j)];
 }
+// Pool row of key j for head h (row = (page * Hkv + h) * page_size + offset), or
+// -1 where its page is none of the pool's
 __device__ __forceinline__ int attn_page_row(const AttnArgs &a, int h, int j, int pg) {
     if (pg < 0 || pg >= a.num_pages) return -1;
     return (pg * a.Hkv + h) * a.page + (j - attn_page_of(a, j) * a.page);
-}
-
-// Pool row of key j for head h (row = (page * Hkv + h) * page_size + offset), or
-// -1 where there is none: past the keys, hidden from every row by the window, or
-// on a page outside the pool.
-__device__ __forceinline__ int attn_key_row(const AttnArgs &a, const AttnItem &it, int h, int j) {
-    const int pg = attn_key_page(a, it, j);
-    return attn_page_row(a, h, j, pg);
 }
 
 // ---------------------------------------------------------------------------
@@ -445,7 +445,7 @@ template <int QT, int KIND> __device__ __forceinline__ void att_values4(const ui
 
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a) {
-    constexpr int  KT = 64, BQ = 128, NT = 256;
+    constexpr int  KT = ATT_WIDE_KEYS, BQ = ATT_WIDE_ROWS, NT = 256;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;       // bytes of a cache element
     constexpr int  EC  = 16 / ES;           // elements of a 16-byte piece
@@ -472,6 +472,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
     if (it.b < 0) return;
 
+    int  page_id     = -1;
+    auto fetch_pages = [&](int t) PTA_INLINE { // t: the wave's tile
+        page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
+    };
+    fetch_pages(it.t0 + wave);
     int c = lane & 31, half = lane >> 5;
     uint4     qf[DP / 16];
     int       pos = -1; // of this lane's row; rows past the tile see nothing
@@ -518,10 +523,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
     float kscl = 0.0f, vscl = 1.0f; // of key `tid`, as old as kreg
     // Pool rows of four key tiles' keys, one tile a wave, every fourth iteration; from
     // their pages, which were fetched four iterations before
-    int  page_id = -1;
-    auto fetch_pages = [&](int t) PTA_INLINE { // t: the wave's tile
-        page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
-    };
     auto rows = [&](int t) PTA_INLINE {
         const int row     = attn_page_row(a, h, attn_key0(it, t, KT) + lane, page_id);
         srow[t & 7][lane] = row;
@@ -837,7 +838,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         });
     };
 
-    fetch_pages(it.t0 + wave);
     rows(it.t0 + wave);
     fetch_pages(it.t0 + 4 + wave);
     __syncthreads();
@@ -946,7 +946,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 // keys and values in flight in registers.
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(AttnArgs a) {
-    constexpr int  KT = 128, BQ = 16, WK = 32;
+    constexpr int  KT = ATT_NARROW_KEYS, BQ = ATT_NARROW_ROWS, WK = 32;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;
     constexpr int  EC  = 16 / ES;
@@ -1239,144 +1239,94 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
 }
 
 // ---------------------------------------------------------------------------
-// joins the narrow kernel's chunks: 64 elements of 4 values a workgroup, four
-// threads share an element's chunks
+// joins the chunks of both kernels: o = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c
 // ---------------------------------------------------------------------------
-template <int QT> __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
-    __shared__ float4 sacc[4][64];
-    __shared__ float2 sml[4][64];
-    const int     lane = threadIdx.x & 63, quarter = threadIdx.x >> 6, tpr = a.D / 4;
-    const int64_t rows = static_cast<int64_t>(a.Tq) * a.Hq, all = rows * tpr;
-    const int64_t p = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-    const int64_t row = min(p / tpr, rows - 1);
-    const int     d = static_cast<int>(p - p / tpr * tpr) * 4;
-    bool          in = p < all;
-    if (a.rows_max != INT_MAX) { // rows of other sequences are the wide kernel's
-        const int tok = static_cast<int>(row / a.Hq);
-        int       lo = 0, hi = a.B; // the last sequence that begins at or before the token
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.cu[mid] <= tok) lo = mid;
-            else hi = mid;
-        }
-        const AttnSeq s = attn_seq(a, lo);
-        in              = in && tok >= s.tok0 && tok < s.tok0 + s.n;
-    }
-    float  mm = -INFINITY, ll = 0.0f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (in)
-        for (int c0 = quarter; c0 < a.split; c0 += 16) {
-            float2 ml[4];
-            float4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t at = min(c0 + 4 * u, a.split - 1) * rows + row;
-                ml[u]            = a.part_ml[at];
-                x[u]             = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (c0 + 4 * u >= a.split) break;
-                const float n = fmaxf(mm, ml[u].x), base = n == -INFINITY ? 0.0f : n;
-                const float f = att_exp2(mm - base), g = att_exp2(ml[u].x - base);
-                mm    = n;
-                ll    = fmaf(ml[u].y, g, ll * f);
-                acc.x = fmaf(x[u].x, g, acc.x * f); acc.y = fmaf(x[u].y, g, acc.y * f);
-                acc.z = fmaf(x[u].z, g, acc.z * f); acc.w = fmaf(x[u].w, g, acc.w * f);
-            }
-        }
-    sacc[quarter][lane] = acc;
-    sml[quarter][lane]  = make_float2(mm, ll);
-    __syncthreads();
-    if (quarter != 0 || !in) return;
-#pragma unroll
-    for (int u = 1; u < 4; ++u) {
-        const float2 ml = sml[u][lane];
-        const float4 x  = sacc[u][lane];
-        const float  n = fmaxf(mm, ml.x), base = n == -INFINITY ? 0.0f : n;
-        const float  f = att_exp2(mm - base), g = att_exp2(ml.x - base);
-        mm    = n;
-        ll    = fmaf(ml.y, g, ll * f);
-        acc.x = fmaf(x.x, g, acc.x * f); acc.y = fmaf(x.y, g, acc.y * f);
-        acc.z = fmaf(x.z, g, acc.z * f); acc.w = fmaf(x.w, g, acc.w * f);
-    }
-    const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
-    *reinterpret_cast<uint2 *>(a.out + row * a.D + d) =
-        make_uint2(AttT<QT>::pack(acc.x * inv, acc.y * inv), AttT<QT>::pack(acc.z * inv, acc.w * inv));
-    if (a.lse != nullptr && d == 0) a.lse[row] = (mm + att_log2(ll)) * 0.69314718055994531f;
-}
-
-// ---------------------------------------------------------------------------
-// joins the wide kernel's chunks of a row tile: workgroup = (first slot of the tile, head), a
-// part of the tile's rows; four threads share an element's chunks
-// ---------------------------------------------------------------------------
-constexpr int ATT_JOIN_PARTS = 8;
-
-template <int QT, int BQ> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    const int  h = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
-    const int4 w = a.desc[slot]; // sequence, row tile, chunk, chunks
-    if (w.x == ATT_NONE || w.z != 0 || w.w == 1) return;
-    const AttnSeq s    = attn_seq(a, w.x);
-    const int     row0 = w.y * BQ, rows = min(BQ, s.n * a.G - row0);
-    const int     tpr = a.D / 4; // elements (of 4 values) of a row
-    const int     lane = threadIdx.x & 63, quarter = threadIdx.x >> 6;
-    __shared__ float4 sacc[4][64];
-    __shared__ float2 sml[4][64];
-    for (int p0 = blockIdx.y * 64; p0 < rows * tpr; p0 += ATT_JOIN_PARTS * 64) {
-        const int p = p0 + lane, jr = min(p / tpr, rows - 1), d = p < rows * tpr ? (p - jr * tpr) * 4 : 0;
-        float     mm = -INFINITY, ll = 0.0f;
-        float4    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c0 = quarter; c0 < w.w; c0 += 16) {
-            float2 ml[4];
-            float4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t at = (static_cast<int64_t>(slot + min(c0 + 4 * u, w.w - 1)) * a.Hkv + h) * BQ + jr;
-                ml[u]            = a.part_ml[at];
-                x[u]             = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (c0 + 4 * u >= w.w) break;
-                const float n = fmaxf(mm, ml[u].x), base = n == -INFINITY ? 0.0f : n;
-                const float f = att_exp2(mm - base), g = att_exp2(ml[u].x - base);
-                mm    = n;
-                ll    = fmaf(ml[u].y, g, ll * f);
-                acc.x = fmaf(x[u].x, g, acc.x * f); acc.y = fmaf(x[u].y, g, acc.y * f);
-                acc.z = fmaf(x[u].z, g, acc.z * f); acc.w = fmaf(x[u].w, g, acc.w * f);
-            }
-        }
-        __syncthreads();
-        sacc[quarter][lane] = acc;
-        sml[quarter][lane]  = make_float2(mm, ll);
-        __syncthreads();
-        if (quarter != 0 || p >= rows * tpr) continue;
-#pragma unroll
-        for (int u = 1; u < 4; ++u) {
-            const float2 ml = sml[u][lane];
-            const float4 x  = sacc[u][lane];
-            const float  n = fmaxf(mm, ml.x), base = n == -INFINITY ? 0.0f : n;
-            const float  f = att_exp2(mm - base), g = att_exp2(ml.x - base);
+// An element is 4 values of a row; Q threads share its chunks, four chunks of a
+// thread are in flight.
+template <int QT, int Q> __device__ __forceinline__ void attn_join(const AttnArgs &a, const AttnSeq &s, int h, int row0, int rows,
+                                                                   bool by_token, int64_t at0, int64_t stride, int count, int part, int parts) {
+    constexpr int N = 256 / Q; // elements of a workgroup at a time
+    __shared__ float4 sacc[Q][N];
+    __shared__ float2 sml[Q][N];
+    const int tpr = a.D / 4, lane = threadIdx.x % N, quarter = threadIdx.x / N;
+    for (int64_t p0 = part * N; p0 < static_cast<int64_t>(rows) * tpr; p0 += parts * N) {
+        const int64_t p = p0 + lane;
+        const bool    in = p < static_cast<int64_t>(rows) * tpr;
+        const int     jr = in ? static_cast<int>(p / tpr) : rows - 1, d = in ? static_cast<int>(p - static_cast<int64_t>(jr) * tpr) * 4 : 0;
+        const int     rr = row0 + jr, rt = rr / a.G;
+        const int64_t orow = static_cast<int64_t>(s.tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
+        const int64_t first = by_token ? orow : at0 + jr;
+        float         mm = -INFINITY, ll = 0.0f;
+        float4        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float2 &ml, const float4 &x) PTA_INLINE {
+            const float n = fmaxf(mm, ml.x), base = n == -INFINITY ? 0.0f : n;
+            const float f = att_exp2(mm - base), g = att_exp2(ml.x - base);
             mm    = n;
             ll    = fmaf(ml.y, g, ll * f);
             acc.x = fmaf(x.x, g, acc.x * f); acc.y = fmaf(x.y, g, acc.y * f);
             acc.z = fmaf(x.z, g, acc.z * f); acc.w = fmaf(x.w, g, acc.w * f);
+        };
+        for (int c0 = quarter; c0 < count; c0 += 4 * Q) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = min(c0 + Q * u, count - 1) * stride + first;
+                ml[u]            = a.part_ml[at];
+                x[u]             = *reinterpret_cast<const float4 *>(a.part_o + at * a.D + d);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + Q * u >= count) break;
+                add(ml[u], x[u]);
+            }
         }
-        const int     rr = row0 + jr, rt = rr / a.G;
-        const int64_t orow = static_cast<int64_t>(s.tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
-        const float   inv  = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
+        if constexpr (Q > 1) {
+            __syncthreads();
+            sacc[quarter][lane] = acc;
+            sml[quarter][lane]  = make_float2(mm, ll);
+            __syncthreads();
+        }
+        if (quarter != 0 || !in) continue;
+        if constexpr (Q > 1) {
+#pragma unroll
+            for (int u = 1; u < Q; ++u) add(sml[u][lane], sacc[u][lane]);
+        }
+        const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f; // no key seen: zeros
         *reinterpret_cast<uint2 *>(a.out + orow * a.D + d) =
             make_uint2(AttT<QT>::pack(acc.x * inv, acc.y * inv), AttT<QT>::pack(acc.z * inv, acc.w * inv));
         if (a.lse != nullptr && d == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;
     }
 }
 
-// Launches one kernel, and the join if row tiles may be split, for one type of
-// queries (paged_attention_inst_*.hip).  rows: of a row tile, which says the kernel.
-template <int QT> void attn_launch(const AttnArgs &a, int kind, int rows, hipStream_t st);
-extern template void attn_launch<PTA_BF16>(const AttnArgs &, int, int, hipStream_t);
-extern template void attn_launch<PTA_F16>(const AttnArgs &, int, int, hipStream_t);
+// Workgroups of the narrow kernel's sequences (head, part, sequence), then of the
+// wide kernel's slots (head, part, slot).
+constexpr int ATT_JOIN_PARTS = 8;
 
-constexpr int ATT_WIDE_ROWS = 128, ATT_WIDE_KEYS = 64, ATT_NARROW_ROWS = 16, ATT_NARROW_KEYS = 128;
+template <int QT, int QN> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs n, AttnArgs w, int n_blocks, int n_parts) {
+    if (static_cast<int>(blockIdx.x) < n_blocks) {
+        const int     h = blockIdx.x % n.Hkv, g = blockIdx.x / n.Hkv;
+        const AttnSeq s = attn_seq(n, g / n_parts);
+        attn_join<QT, QN>(n, s, h, 0, s.n * n.G, true, 0, static_cast<int64_t>(n.Tq) * n.Hq, n.split, g % n_parts, n_parts);
+    } else {
+        const int  x = blockIdx.x - n_blocks, h = x % w.Hkv, g = x / w.Hkv, slot = g / ATT_JOIN_PARTS;
+        const int4 d = w.desc[slot]; // sequence, row tile, chunk, chunks
+        if (d.x == ATT_NONE || d.z != 0 || d.w == 1) return;
+        const AttnSeq s    = attn_seq(w, d.x);
+        const int     row0 = d.y * ATT_WIDE_ROWS;
+        attn_join<QT, 1>(w, s, h, row0, min(ATT_WIDE_ROWS, s.n * w.G - row0), false, (static_cast<int64_t>(slot) * w.Hkv + h) * ATT_WIDE_ROWS,
+                      static_cast<int64_t>(w.Hkv) * ATT_WIDE_ROWS, d.w, g % ATT_JOIN_PARTS, ATT_JOIN_PARTS);
+    }
+}
+
+// One call's launches for one type of queries (paged_attention_inst_*.hip).
+struct AttnCall {
+    AttnArgs narrow, wide;
+    bool     has_narrow, has_wide;
+    int      narrow_join_parts; // workgroups of a sequence's head that join its chunks
+};
+template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st);
+extern template void attn_launch<PTA_BF16>(const AttnCall &, int, hipStream_t);
+extern template void attn_launch<PTA_F16>(const AttnCall &, int, hipStream_t);
 
 } // namespace pta

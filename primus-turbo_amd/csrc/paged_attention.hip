@@ -51,7 +51,7 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
     p.rows_min = mix ? ATT_NARROW_MOST : 0;
     p.rows_max = INT_MAX;
     const int64_t most = Tq * G / ATT_WIDE_ROWS + B; // row tiles of a head: sum of ceil(n G / rows)
-    const int64_t goal = cdiv(device_cu_count(), Hkv);
+    const int64_t goal = cdiv(2 * device_cu_count(), Hkv);
     // row tiles alone fill the chip, or no tile has keys for two chunks
     p.goal  = most - B >= goal || keys <= ATT_WIDE_KEYS ? 0 : goal;
     p.slots = most + p.goal;
@@ -125,7 +125,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
     PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
                   "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG((p.part[0].split * p.part[0].tiles * num_seqs + p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
+    PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split * p.part[0].tiles, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
     AttnArgs a = {};
     a.q = static_cast<const uint16_t *>(q);
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
@@ -146,23 +146,31 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
         a.kc = a.vc = static_cast<const uint8_t *>(q);
         a.ks = a.vs = static_cast<const float *>(q);
     }
-    uint8_t          *ws = static_cast<uint8_t *>(workspace);
-    const hipStream_t st = as_stream(stream);
-    for (const AttnPart &part : p.part) {
-        if (part.rows == 0) continue;
-        a.slots = static_cast<int>(part.slots); a.split_goal = static_cast<int>(part.goal);
-        a.split = static_cast<int>(part.split); a.tiles = static_cast<int>(part.tiles);
-        a.rows_min = part.rows_min; a.rows_max = part.rows_max;
-        a.desc = nullptr; a.part_ml = nullptr; a.part_o = nullptr;
-        if (part.bytes() > 0) {
-            a.desc    = reinterpret_cast<int4 *>(ws);
-            a.part_ml = reinterpret_cast<float2 *>(ws + part.desc_bytes);
-            a.part_o  = reinterpret_cast<float *>(ws + part.desc_bytes + part.ml_bytes);
-            ws += part.bytes();
-        }
-        if (q_dtype == PTA_BF16) attn_launch<PTA_BF16>(a, cache_kind, part.rows, st);
-        else attn_launch<PTA_F16>(a, cache_kind, part.rows, st);
+    AttnCall c = {};
+    c.has_narrow = p.part[0].rows > 0;
+    c.has_wide   = p.part[1].rows > 0;
+    // 64 elements of 4 values a workgroup, at the sequences' mean of rows
+    c.narrow_join_parts = static_cast<int>(std::min<int64_t>(ATT_JOIN_PARTS, cdiv(num_tokens * (Hq / Hkv) * (D / 4), 64 * num_seqs)));
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    for (int i = 0; i < 2; ++i) {
+        const AttnPart &part = p.part[i];
+        AttnArgs       &x    = i == 0 ? c.narrow : c.wide;
+        x            = a;
+        x.slots      = static_cast<int>(part.slots);
+        x.split_goal = static_cast<int>(part.goal);
+        x.split      = static_cast<int>(part.split);
+        x.tiles      = static_cast<int>(part.tiles);
+        x.rows_min   = part.rows_min;
+        x.rows_max   = part.rows_max;
+        if (part.bytes() == 0) continue;
+        x.desc    = reinterpret_cast<int4 *>(ws);
+        x.part_ml = reinterpret_cast<float2 *>(ws + part.desc_bytes);
+        x.part_o  = reinterpret_cast<float *>(ws + part.desc_bytes + part.ml_bytes);
+        ws += part.bytes();
     }
+    const hipStream_t st = as_stream(stream);
+    if (q_dtype == PTA_BF16) attn_launch<PTA_BF16>(c, cache_kind, st);
+    else attn_launch<PTA_F16>(c, cache_kind, st);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
 }

@@ -2,5 +2,5 @@
 #include "paged_attention_launch.h"
 
 namespace pta {
-template void attn_launch<PTA_F16>(const AttnArgs &, int, int, hipStream_t);
+template void attn_launch<PTA_F16>(const AttnCall &, int, hipStream_t);
 } // namespace pta

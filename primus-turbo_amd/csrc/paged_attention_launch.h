@@ -5,28 +5,34 @@
 
 namespace pta {
 
-template <int QT, int KIND, int DP> void attn_launch_d(const AttnArgs &a, int rows, hipStream_t st) {
-    if (rows == ATT_NARROW_ROWS) {
-        const unsigned grid = static_cast<unsigned>(a.B) * a.tiles * a.split * a.Hkv;
-        attn_narrow_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(a);
-        if (a.split > 1) attn_join_rows_kernel<QT><<<static_cast<unsigned>(cdiv(static_cast<int64_t>(a.Tq) * a.Hq * (a.D / 4), 64)), 256, 0, st>>>(a);
-    } else {
-        const unsigned grid = static_cast<unsigned>(a.slots) * static_cast<unsigned>(a.Hkv);
-        attn_wide_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(a);
-        if (a.split_goal > 0) attn_join_kernel<QT, ATT_WIDE_ROWS><<<dim3(grid, ATT_JOIN_PARTS), 256, 0, st>>>(a);
+template <int QT, int KIND, int DP> void attn_launch_d(const AttnCall &c, hipStream_t st) {
+    const AttnArgs &n = c.narrow, &w = c.wide;
+    if (c.has_narrow) {
+        const unsigned grid = static_cast<unsigned>(n.B) * n.tiles * n.split * n.Hkv;
+        attn_narrow_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(n);
+    }
+    if (c.has_wide) {
+        const unsigned grid = static_cast<unsigned>(w.slots) * static_cast<unsigned>(w.Hkv);
+        attn_wide_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(w);
     }
 }
 
-template <int QT, int KIND> void attn_launch_k(const AttnArgs &a, int rows, hipStream_t st) {
-    if (a.D <= 64) attn_launch_d<QT, KIND, 64>(a, rows, st);
-    else if (a.D <= 128) attn_launch_d<QT, KIND, 128>(a, rows, st);
-    else attn_launch_d<QT, KIND, 256>(a, rows, st);
+template <int QT, int KIND> void attn_launch_k(const AttnCall &c, int D, hipStream_t st) {
+    if (D <= 64) attn_launch_d<QT, KIND, 64>(c, st);
+    else if (D <= 128) attn_launch_d<QT, KIND, 128>(c, st);
+    else attn_launch_d<QT, KIND, 256>(c, st);
 }
 
-template <int QT> void attn_launch(const AttnArgs &a, int kind, int rows, hipStream_t st) {
-    if (kind == PTA_E4M3) attn_launch_k<QT, PTA_E4M3>(a, rows, st);
-    else if (kind == PTA_E5M2) attn_launch_k<QT, PTA_E5M2>(a, rows, st);
-    else attn_launch_k<QT, PTA_CACHE_16BIT>(a, rows, st);
+template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st) {
+    const int D = c.has_narrow ? c.narrow.D : c.wide.D;
+    if (kind == PTA_E4M3) attn_launch_k<QT, PTA_E4M3>(c, D, st);
+    else if (kind == PTA_E5M2) attn_launch_k<QT, PTA_E5M2>(c, D, st);
+    else attn_launch_k<QT, PTA_CACHE_16BIT>(c, D, st);
+    const int n = c.has_narrow && c.narrow.split > 1 ? c.narrow.B * c.narrow.Hkv * c.narrow_join_parts : 0;
+    const int w = c.has_wide && c.wide.split_goal > 0 ? c.wide.slots * c.wide.Hkv * ATT_JOIN_PARTS : 0;
+    if (n + w == 0) return;
+    auto join = c.narrow.split > 4 ? attn_join_kernel<QT, 4> : attn_join_kernel<QT, 1>;
+    join<<<static_cast<unsigned>(n + w), 256, 0, st>>>(c.narrow, c.wide, n, c.narrow_join_parts);
 }
 
 } // namespace pta
