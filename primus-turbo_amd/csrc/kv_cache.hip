@@ -23,6 +23,12 @@ namespace {
 
 constexpr int KV_NT = 256;
 
+// Rows of a thread in the read: with one, 131072 tokens of 8 heads of 128 took 217
+// us, with eight 158 (their loads are in flight together, and a workgroup uses more
+// of the scales' lines that it touches).  Eight once they give every CU four
+// workgroups: below, 1021 tokens of 4 heads of 64 want the chip's width.
+constexpr int KV_READ_ROWS = 8;
+
 struct KVArgs {
     const void    *x[2];        // keys, values of the tokens (write) or null
     void          *y[2];        // outputs of the read
@@ -102,24 +108,45 @@ __global__ __launch_bounds__(KV_NT) void kv_write_kernel(KVArgs a) {
     }
 }
 
-template <int KIND, int OUT_DT, int LPR> __global__ __launch_bounds__(KV_NT) void kv_read_kernel(KVArgs a) {
+// R rows of a thread, loaded together.
+template <int KIND, int OUT_DT, int LPR, int R> __global__ __launch_bounds__(KV_NT) void kv_read_kernel(KVArgs a) {
+    constexpr bool FP8   = KIND != PTA_CACHE_16BIT;
+    constexpr int  ROWS  = KV_NT / LPR;
     const int      which = blockIdx.y;
-    const uint32_t l     = threadIdx.x % LPR;
-    const uint32_t row   = blockIdx.x * (KV_NT / LPR) + threadIdx.x / LPR;
-    const uint32_t t     = row / a.heads, h = row - t * a.heads;
-    if (t >= a.tokens || l * 8 >= a.D) return;
-    const int64_t src = kv_row(a, t, h);
-    const int64_t dst = static_cast<int64_t>(row) * a.D + l * 8;
-    if constexpr (KIND == PTA_CACHE_16BIT) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (src >= 0) w = *reinterpret_cast<const uint4 *>(a.cache[which] + (src * a.D + l * 8) * 2);
-        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y[which]) + dst) = w;
-    } else {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (src >= 0) {
-            const uint2 w   = *reinterpret_cast<const uint2 *>(a.cache[which] + src * a.D + l * 8);
-            const float s   = a.scale[which][src];
-            const int   ws[2] = {static_cast<int>(w.x), static_cast<int>(w.y)};
+    const uint32_t l = threadIdx.x % LPR, row0 = blockIdx.x * (ROWS * R) + threadIdx.x / LPR, rows = a.tokens * a.heads;
+    if (l * 8 >= a.D) return;
+    int64_t src[R];
+    uint4   w[R];
+    float   s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t row = min(row0 + r * ROWS, rows - 1), t = row / a.heads;
+        src[r] = kv_row(a, t, row - t * a.heads);
+    }
+    if (a.nslots > 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t at = src[r] < 0 ? 0 : src[r];
+            if constexpr (FP8) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(a.cache[which] + at * a.D + l * 8);
+                w[r]          = make_uint4(x.x, x.y, 0, 0);
+                s[r]          = a.scale[which][at];
+            } else {
+                w[r] = *reinterpret_cast<const uint4 *>(a.cache[which] + (at * a.D + l * 8) * 2);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t row = row0 + r * ROWS;
+        if (row >= rows) return;
+        const int64_t dst = static_cast<int64_t>(row) * a.D + l * 8;
+        if constexpr (!FP8) {
+            if (src[r] < 0) w[r] = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y[which]) + dst) = w[r];
+        } else {
+            float     v[8];
+            const int ws[2] = {static_cast<int>(w[r].x), static_cast<int>(w[r].y)};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if constexpr (KIND == PTA_E4M3) {
@@ -131,17 +158,17 @@ template <int KIND, int OUT_DT, int LPR> __global__ __launch_bounds__(KV_NT) voi
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= s;
-        }
-        if constexpr (OUT_DT == PTA_F32) {
-            float4 *y = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y[which]) + dst);
-            y[0]      = make_float4(v[0], v[1], v[2], v[3]);
-            y[1]      = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t o[4];
+            for (int j = 0; j < 8; ++j) v[j] = src[r] < 0 ? 0.0f : v[j] * s[r];
+            if constexpr (OUT_DT == PTA_F32) {
+                float4 *y = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y[which]) + dst);
+                y[0]      = make_float4(v[0], v[1], v[2], v[3]);
+                y[1]      = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = pack_16(OUT_DT, v[2 * j], v[2 * j + 1]);
-            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y[which]) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+                for (int j = 0; j < 4; ++j) o[j] = pack_16(OUT_DT, v[2 * j], v[2 * j + 1]);
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.y[which]) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
         }
     }
 }
@@ -252,13 +279,20 @@ extern "C" int pta_kv_cache_read(const void *k_cache, const void *v_cache, int c
     a.D = static_cast<uint32_t>(D); a.page = static_cast<uint32_t>(page_size);
     a.nslots = static_cast<uint32_t>(num_pages * page_size);
     const int         lpr = kv_lpr(D);
-    const dim3        grid(static_cast<unsigned>(cdiv(num_tokens * Hkv, KV_NT / lpr)), 2);
+    const int64_t     blocks = cdiv(num_tokens * Hkv, KV_NT / lpr); // of one row a thread
+    const bool        many   = blocks * 2 >= KV_READ_ROWS * 4 * device_cu_count();
+    const dim3        grid(static_cast<unsigned>(many ? cdiv(blocks, KV_READ_ROWS) : blocks), 2);
     const hipStream_t st = as_stream(stream);
+#define PTA_KVR_R(KIND, DT, LPR)                                                                   \
+    do {                                                                                           \
+        if (many) kv_read_kernel<KIND, DT, LPR, KV_READ_ROWS><<<grid, KV_NT, 0, st>>>(a);          \
+        else kv_read_kernel<KIND, DT, LPR, 1><<<grid, KV_NT, 0, st>>>(a);                          \
+    } while (0)
 #define PTA_KVR(KIND, DT)                                                                          \
     do {                                                                                           \
-        if (lpr == 8) kv_read_kernel<KIND, DT, 8><<<grid, KV_NT, 0, st>>>(a);                      \
-        else if (lpr == 16) kv_read_kernel<KIND, DT, 16><<<grid, KV_NT, 0, st>>>(a);               \
-        else kv_read_kernel<KIND, DT, 32><<<grid, KV_NT, 0, st>>>(a);                              \
+        if (lpr == 8) PTA_KVR_R(KIND, DT, 8);                                                      \
+        else if (lpr == 16) PTA_KVR_R(KIND, DT, 16);                                               \
+        else PTA_KVR_R(KIND, DT, 32);                                                              \
     } while (0)
 #define PTA_KVR_O(KIND)                                                                            \
     do {                                                                                           \
@@ -271,6 +305,7 @@ extern "C" int pta_kv_cache_read(const void *k_cache, const void *v_cache, int c
     else PTA_KVR_O(PTA_E5M2);
 #undef PTA_KVR_O
 #undef PTA_KVR
+#undef PTA_KVR_R
     PTA_CHECK_LAUNCH();
     return PTA_OK;
 }
