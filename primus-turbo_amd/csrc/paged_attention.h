@@ -888,9 +888,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
         const bool calm = t >= calm0 && t + 1 < calm1 && (khole | vhole) == 0 && a.D == DP;
         if (!calm) {
             ready(t);
-            if (t < tend && edge(t, bpmin, it.kend - 1) &&
-                (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3]))
-                slow(t);
+            // the same for all waves
+            if (edge(t, bpmin, it.kend - 1) && (sspec[t & 1][0] | sspec[t & 1][1] | sspec[t & 1][2] | sspec[t & 1][3])) {
+                if (t < tend) slow(t);
+                // it reads the keys' LDS, which this iteration's staging overwrites
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
         }
         if (t < tend) {
             rescale();

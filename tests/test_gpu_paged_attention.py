@@ -143,6 +143,36 @@ def test_large_logits():
     check(case, scale=8.0)
 
 
+@pytest.mark.parametrize("cache,dtype", KINDS)
+@pytest.mark.parametrize("n,D,window,sinks", [(10, 64, None, 0), (10, 128, 30, 2), (150, 64, None, 0), (150, 128, 40, 3), (100, 256, None, 0)])
+def test_infinities_and_nan_reach_the_rows_that_see_them(cache, dtype, n, D, window, sinks):
+    """Values and a key that are NaN or infinite: rows that do not see the token keep
+    their finite results, the others get what the formula gives."""
+    L = 2 * n + 60
+    q, (kc, vc), (ks, vs), table, cu, lens = make([n, 1], [L, 5], 4, 2, D, 16, cache, dtype, seed=n)
+    inf = torch.tensor(float("-inf"))
+
+    def put(pool, j, d, x):
+        pool[int(table[0, j // 16]), :, j % 16, d] = x
+
+    nan = torch.tensor(float("nan")).to(cache)
+    put(vc, L - n // 2, 3, nan)
+    put(vc, L - n // 3, D - 1, nan if cache == E4 else inf.to(cache))
+    put(vc, L - n // 4, 8, nan if cache == E4 else (-inf).to(cache))
+    put(kc, L - 2, 9, nan)
+    put(vc, 1, 5, nan)  # seen as a sink, or until the window has passed it
+    dev = [t if t is None else t.cuda() for t in (q, kc, vc, table, cu, lens, ks, vs)]
+    got = _ops().paged_attention(*dev, window_size=window, num_sinks=sinks).cpu().double()
+    args = (table, cu, lens, D ** -0.5, window, sinks)
+    raw = attention(q, kc.double(), vc.double(), ks, vs, *args)[0]
+    zero = lambda c: torch.nan_to_num(c.double(), 0.0, 0.0, 0.0)  # noqa: E731
+    want, _, bound, _ = attention(q, zero(kc), zero(vc), *(s if s is None else torch.nan_to_num(s) for s in (ks, vs)), *args)
+    fin = torch.isfinite(raw)
+    assert bool((~fin).any()) and torch.equal(torch.isnan(got), torch.isnan(raw))
+    assert torch.equal(got[torch.isinf(raw)], raw[torch.isinf(raw)])
+    within(torch.where(fin, got, 0.0), torch.where(fin, want, 0.0), bound, "finite results")
+
+
 @pytest.mark.parametrize("cache", [E4, BF])
 @pytest.mark.parametrize("new,lens,Hq,Hkv", [([1] * 3, [9000, 20, 5000], 8, 1), ([100, 1], [6000, 300], 2, 1), ([17], [20000], 1, 1)])
 def test_long_contexts_split_over_workgroups(cache, new, lens, Hq, Hkv):
