@@ -70,12 +70,18 @@ template <int XT, int KIND> struct MoeFrag {
         if constexpr (ES == 2) return w[s];
         else return s % 2 == 0 ? att_cvt8<XT, KIND>(w[s / 2].x, w[s / 2].y) : att_cvt8<XT, KIND>(w[s / 2].z, w[s / 2].w);
     }
+    __device__ __forceinline__ void cut(int k0, int qd, int K) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            if (k0 + p * 4 * EP + qd * EP >= K) w[p] = make_uint4(0, 0, 0, 0);
+    }
     // first element of operand s in the step, for quarter qd
     static __device__ __forceinline__ int elem(int s, int qd) { return ES == 2 ? s * 32 + qd * 8 : (s / 2) * 64 + qd * 16 + (s % 2) * 8; }
 };
 
 // The same step of one token row.  Elements past K become zeros where they are
-// used: an instruction after the load would wait for it.
+// used (an instruction after the load would wait for it), of weights too: what
+// was read in their place may be infinite.
 template <class F> struct MoeTok {
     uint4 v[F::NS];
     __device__ __forceinline__ void load(const uint16_t *row, int k0, int qd, int K) {
@@ -96,6 +102,12 @@ template <class F, int RT, int NC> struct MoeStage {
     F         w[RT];
     MoeTok<F> x[NC];
     float     sc[RT]; // block scales
+    __device__ __forceinline__ void cut(int k0, int qd, int K) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) w[r].cut(k0, qd, K);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) x[n].cut(k0, qd, K);
+    }
 };
 
 __device__ __forceinline__ int moe_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -158,14 +170,11 @@ __device__ __forceinline__ void moe_up_pass(const MoeArgs &a, MoeUpShared &sh, i
     for (int st0 = wave; st0 < steps; st0 += 4 * RING) {
 #pragma unroll
         for (int u = 0; u < RING; ++u) {
-            // steps past the last, too, whose tokens' operands are all cut to zeros: with a
+            // steps past the last, too, whose operands are all cut to zeros: with a
             // branch around them the loads in flight could not be counted, and every round
             // would wait for all of them
             const int st = st0 + 4 * u;
-            if ((st + 1) * F::STEP > K) {
-#pragma unroll
-                for (int n = 0; n < NC; ++n) ring[u].x[n].cut(st * F::STEP, qd, K);
-            }
+            if ((st + 1) * F::STEP > K) ring[u].cut(st * F::STEP, qd, K);
 #pragma unroll
             for (int r = 0; r < 2 * PR; ++r) {
                 att_f4 part[NC];
@@ -272,35 +281,38 @@ template <int XT, int KIND, bool MANY> __global__ __launch_bounds__(MOE_NT, 2) v
 // ---------------------------------------------------------------------------
 // down product and the sum over experts: workgroup = (16 RT features, group of
 // 64 tokens); the waves take every fourth step of the list of all reached
-// experts' steps.  Each wave sums into an LDS table of its own, [token][feature],
-// whenever it is done with an expert: the tokens of a column differ from expert
-// to expert.
+// experts' steps.  An expert with more tokens than the NC column tiles hold is
+// listed again for the rest, its weights then come from the caches.  Each wave sums
+// into an LDS table of its own, [token][feature], whenever it is done with an entry:
+// the tokens of a column differ from expert to expert.
 // ---------------------------------------------------------------------------
-template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds__(MOE_NT, 2) void moe_down_kernel(MoeArgs a) {
+template <int XT, int KIND, bool ROW, int RT, int NC, int RING>
+__global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeArgs a) {
     using F = MoeFrag<XT, KIND>;
-    constexpr int                 RS = RT * 16 + 4; // floats of a token's row
-    __shared__ __align__(16) float ssum[4][NC * 16][RS];
+    constexpr int                 NT = MOE_NT, NW = NT / 64, RS = RT * 16 + 4; // floats of a token's row
+    constexpr int                 TOKS = NC == 1 ? 16 : MOE_TG, PART = NC * 16, LIST = MOE_MAX_E + MOE_TG * MOE_MAX_K / PART;
+    __shared__ __align__(16) float ssum[NW][TOKS][RS];
     __shared__ unsigned long long smask[MOE_MAX_E];  // tokens of a slot
-    __shared__ int                sfirst[MOE_MAX_E]; // by entry: an expert's slot; afterwards: list of reached slots
-    __shared__ short              sexp[MOE_MAX_E], scnt[MOE_MAX_E]; // expert of a listed slot, its tokens
-    __shared__ int                stok[4][NC * 16];  // a wave's tokens of the expert it sums
+    __shared__ int                sfirst[LIST]; // by entry: an expert's slot; afterwards: list of reached slots
+    __shared__ short              sexp[LIST], scnt[LIST], sfrom[LIST]; // of the list: expert, tokens, the first of them
+    __shared__ int                stok[NW][PART]; // a wave's tokens of the expert it sums
     __shared__ int                scount;
     const int tid = threadIdx.x, lane = tid & 63, wave = moe_uniform(tid >> 6);
     const int g = blockIdx.y, t0 = g * MOE_TG, tl = min(MOE_TG, a.T - t0), n_ent = tl * a.k;
     const int64_t ent0 = static_cast<int64_t>(t0) * a.k;
 
-    for (int i = tid; i < a.S; i += MOE_NT) smask[i] = 0;
-    for (int i = tid; i < 4 * NC * 16 * RS; i += MOE_NT) (&ssum[0][0][0])[i] = 0.0f;
+    for (int i = tid; i < a.S; i += NT) smask[i] = 0;
+    for (int i = tid; i < NW * TOKS * RS; i += NT) (&ssum[0][0][0])[i] = 0.0f;
     if (a.by_entry) {
-        for (int i = tid; i < a.E; i += MOE_NT) sfirst[i] = INT_MAX;
+        for (int i = tid; i < a.E; i += NT) sfirst[i] = INT_MAX;
         __syncthreads();
-        for (int i = tid; i < n_ent; i += MOE_NT) {
+        for (int i = tid; i < n_ent; i += NT) {
             const int e = moe_expert(a, ent0 + i);
             if (e >= 0) atomicMin(&sfirst[e], i);
         }
     }
     __syncthreads();
-    for (int i = tid; i < n_ent; i += MOE_NT) {
+    for (int i = tid; i < n_ent; i += NT) {
         const int e = moe_expert(a, ent0 + i);
         if (e >= 0) atomicOr(&smask[a.by_entry ? sfirst[e] : e], 1ull << (i / a.k));
     }
@@ -308,16 +320,23 @@ template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds
     if (wave == 0) {
         int n = 0;
         for (int s0 = 0; s0 < a.S; s0 += 64) {
-            const int      s  = s0 + lane;
-            const bool     in = s < a.S && smask[s] != 0;
-            const uint64_t b  = __ballot(in);
-            if (in) {
-                const int at = n + __popcll(b & ((1ull << lane) - 1));
-                sexp[at]     = static_cast<short>(a.by_entry ? moe_expert(a, ent0 + s) : s);
-                sfirst[at]   = s;
-                scnt[at]     = static_cast<short>(__popcll(smask[s]));
+            const int      s   = s0 + lane;
+            const int      cnt = s < a.S ? __popcll(smask[s]) : 0;
+            const uint64_t below = (1ull << lane) - 1;
+            int            at = n;
+#pragma unroll
+            for (int q = 0; q < TOKS; q += PART) at += __popcll(__ballot(cnt > q) & below);
+#pragma unroll
+            for (int q = 0; q < TOKS; q += PART) {
+                if (cnt > q) {
+                    sexp[at]   = static_cast<short>(a.by_entry ? moe_expert(a, ent0 + s) : s);
+                    sfirst[at] = s;
+                    sfrom[at]  = static_cast<short>(q);
+                    scnt[at]   = static_cast<short>(min(cnt - q, PART));
+                    ++at;
+                }
+                n += __popcll(__ballot(cnt > q));
             }
-            n += __popcll(b);
         }
         if (lane == 0) scount = n;
     }
@@ -336,7 +355,7 @@ template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[n][r][j] = 0.0f;
     MoeStage<F, RT, NC> ring[RING];
-    float4              rs[RING][RT]; // row scales, of the stages that end an expert
+    float4              rs[RING][RT]; // row scales
     int64_t             hoff[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) hoff[r] = min(h0 + r * 16 + c, a.H - 1) * rowb;
@@ -350,53 +369,47 @@ template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds
             q.w[r].load(a.w2 + static_cast<int64_t>(e) * a.H * rowb + hoff[r], k0, qd, K);
             q.sc[r] = block ? a.s2[(static_cast<int64_t>(e) * nrb + min(h0 + r * 16, a.H - 16) / 128) * nkb + min(st, steps - 1)] : 1.0f;
         }
-        if (st + 4 >= steps) {
+        if constexpr (ROW) { // in every step: a load in a branch would drain the ring
 #pragma unroll
             for (int r = 0; r < RT; ++r)
-                if (a.scale == MOE_ROW)
-                    qs[r] = *reinterpret_cast<const float4 *>(a.s2 + static_cast<int64_t>(e) * a.H + min(h0 + r * 16, a.H - 16) + 4 * qd);
-                else qs[r] = make_float4(one, one, one, one);
+                qs[r] = *reinterpret_cast<const float4 *>(a.s2 + static_cast<int64_t>(e) * a.H + min(h0 + r * 16, a.H - 16) + 4 * qd);
         }
-        const uint16_t *act = a.act + (static_cast<int64_t>(g) * a.S + s) * a.TG * a.I;
+        const uint16_t *act = a.act + ((static_cast<int64_t>(g) * a.S + s) * a.TG + moe_uniform(sfrom[li])) * a.I;
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
-            if (n == 0 || n * 16 < n_tok) q.x[n].load(act + static_cast<int64_t>(min(n * 16 + c, n_tok - 1)) * a.I, k0, qd, K);
+        for (int n = 0; n < NC; ++n) q.x[n].load(act + static_cast<int64_t>(min(n * 16 + c, n_tok - 1)) * a.I, k0, qd, K);
     };
     if (wave < items) {
 #pragma unroll
-        for (int u = 0; u < RING; ++u) fetch(ring[u], rs[u], wave + 4 * u);
+        for (int u = 0; u < RING; ++u) fetch(ring[u], rs[u], wave + NW * u);
     }
-    for (int it0 = wave; it0 < items; it0 += 4 * RING) {
+    for (int it0 = wave; it0 < items; it0 += NW * RING) {
 #pragma unroll
         for (int u = 0; u < RING; ++u) {
-            const int it = it0 + 4 * u;
+            const int it = it0 + NW * u;
             const int li = it < items ? it / steps : items / steps - 1, st = it < items ? it - li * steps : steps, n_tok = moe_uniform(scnt[li]);
-            if ((st + 1) * F::STEP > K) {
-#pragma unroll
-                for (int n = 0; n < NC; ++n) ring[u].x[n].cut(st * F::STEP, qd, K);
-            }
+            if ((st + 1) * F::STEP > K) ring[u].cut(st * F::STEP, qd, K);
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 const float sc = ring[u].sc[r];
 #pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    if (n == 0 || n * 16 < n_tok) {
-                        att_f4 part;
+                for (int n = 0; n < NC; ++n) {
+                    att_f4 part;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) part[j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) part[j] = 0.0f;
 #pragma unroll
-                        for (int s = 0; s < F::NS; ++s) part = AttT<XT>::mfma16(ring[u].w[r].get(s), ring[u].x[n].v[s], part);
+                    for (int s = 0; s < F::NS; ++s) part = AttT<XT>::mfma16(ring[u].w[r].get(s), ring[u].x[n].v[s], part);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[n][r][j] = fmaf(part[j], sc, acc[n][r][j]);
-                    }
+                    for (int j = 0; j < 4; ++j) acc[n][r][j] = fmaf(part[j], sc, acc[n][r][j]);
+                }
             }
             float4 s4[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) s4[r] = rs[u][r];
-            fetch(ring[u], rs[u], it + 4 * RING);
-            if (st + 4 >= steps) { // the wave's last step of this expert
+            for (int r = 0; r < RT; ++r) s4[r] = ROW ? rs[u][r] : make_float4(one, one, one, one);
+            fetch(ring[u], rs[u], it + NW * RING);
+            if (st + NW >= steps) { // the wave's last step of this expert
                 const uint64_t mask = smask[sfirst[li]];
-                if (mask >> lane & 1) stok[wave][__popcll(mask & ((1ull << lane) - 1))] = lane;
+                const int      nth  = __popcll(mask & ((1ull << lane) - 1)) - sfrom[li];
+                if ((mask >> lane & 1) && nth >= 0 && nth < n_tok) stok[wave][nth] = lane;
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -424,12 +437,16 @@ template <int XT, int KIND, int RT, int NC, int RING> __global__ __launch_bounds
         }
     }
     __syncthreads();
-    for (int p = tid; p < tl * RT * 2; p += MOE_NT) {
+    for (int p = tid; p < tl * RT * 2; p += NT) {
         const int tt = p / (RT * 2), f = (p % (RT * 2)) * 8;
         if (h0 + f >= a.H) continue;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = ((ssum[0][tt][f + j] + ssum[1][tt][f + j]) + ssum[2][tt][f + j]) + ssum[3][tt][f + j];
+        for (int j = 0; j < 8; ++j) {
+            v[j] = ssum[0][tt][f + j];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v[j] += ssum[w][tt][f + j];
+        }
         *reinterpret_cast<uint4 *>(a.y + static_cast<int64_t>(t0 + tt) * a.H + h0 + f) =
             make_uint4(AttT<XT>::pack(v[0], v[1]), AttT<XT>::pack(v[2], v[3]), AttT<XT>::pack(v[4], v[5]), AttT<XT>::pack(v[6], v[7]));
     }

@@ -19,17 +19,19 @@ MoePlan moe_plan(int64_t T, int64_t E, int64_t k) {
     return p;
 }
 
+template <int XT, int KIND, bool ROW> void moe_launch_down(const MoeArgs &a, unsigned groups, hipStream_t st) {
+    if (a.TG <= 16) moe_down_kernel<XT, KIND, ROW, 1, 1, 4><<<dim3(static_cast<unsigned>(cdiv(a.H, 16)), groups), MOE_NT, 0, st>>>(a);
+    else moe_down_kernel<XT, KIND, ROW, 2, 2, 4><<<dim3(static_cast<unsigned>(cdiv(a.H, 32)), groups), MOE_NT, 0, st>>>(a);
+}
+
 template <int XT, int KIND> void moe_launch_k(const MoeArgs &a, unsigned groups, hipStream_t st) {
     const dim3 up(static_cast<unsigned>(cdiv(a.I, 32)), static_cast<unsigned>(a.S), groups);
-    if (a.TG <= 16) {
-        moe_up_kernel<XT, KIND, false><<<up, MOE_NT, 0, st>>>(a);
-        moe_down_kernel<XT, KIND, 1, 1, 4><<<dim3(static_cast<unsigned>(cdiv(a.H, 16)), groups), MOE_NT, 0, st>>>(a);
-    } else {
-        moe_up_kernel<XT, KIND, true><<<up, MOE_NT, 0, st>>>(a);
-        const dim3 down(static_cast<unsigned>(cdiv(a.H, 32)), groups);
-        if (a.TG <= 32) moe_down_kernel<XT, KIND, 2, 2, 2><<<down, MOE_NT, 0, st>>>(a);
-        else moe_down_kernel<XT, KIND, 2, 4, 2><<<down, MOE_NT, 0, st>>>(a);
+    if (a.TG <= 16) moe_up_kernel<XT, KIND, false><<<up, MOE_NT, 0, st>>>(a);
+    else moe_up_kernel<XT, KIND, true><<<up, MOE_NT, 0, st>>>(a);
+    if constexpr (KIND != PTA_CACHE_16BIT) {
+        if (a.scale == MOE_ROW) return moe_launch_down<XT, KIND, true>(a, groups, st);
     }
+    moe_launch_down<XT, KIND, false>(a, groups, st);
 }
 
 template <int XT> void moe_launch(const MoeArgs &a, int kind, unsigned groups, hipStream_t st) {

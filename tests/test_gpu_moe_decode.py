@@ -104,6 +104,23 @@ def test_all_tokens_to_one_expert():
     check(tokens(64, 128, BF), w, idx, torch.rand(64, 1, generator=torch.Generator().manual_seed(0)).cuda())
 
 
+@pytest.mark.parametrize("gran,fmt", [("ROWWISE", E5), ("NONE", E4)])
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("which", ["up", "down"])
+def test_infinite_weights_give_infinite_outputs(gran, fmt, T, which):
+    """An infinity at the begin of rows that end inside a step of the contraction."""
+    E, k, I, H = 4, 2, 48, 80
+    w = weights(E, I, H, gran, fmt, BF, 7)
+    inf = torch.tensor(float("inf")).to(w[0].dtype).cuda()
+    w[0 if which == "up" else 1][1, I + 5 if which == "up" else 5, 0] = inf
+    x, (idx, probs) = tokens(T, H, BF), routing(T, E, k, T)
+    y = _ops().moe_decode(x, w[0], w[1], idx, probs, w[2], w[3]).cpu().double()
+    want = experts(x, w[0], w[1], idx, probs, w[2], w[3])[0]
+    assert bool(torch.isinf(want).any()) and not bool(torch.isnan(want).any())
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    assert torch.equal(y[torch.isinf(want)], want[torch.isinf(want)]) and bool(torch.isfinite(y[torch.isfinite(want)]).all())
+
+
 @pytest.mark.parametrize("T", [2, 40])
 def test_broken_experts_reach_their_tokens_alone(T):
     """NaN in one expert's weights stays with the tokens that go to it."""
