@@ -13,7 +13,9 @@
 //
 // Both kernels are HBM-bound: a row is read once and written once by D / 8
 // lanes (16 bytes of 16-bit data each), amax over the lanes by DPP; keys and
-// values go in one launch (blockIdx.y).
+// values go in one launch (blockIdx.y).  8192 tokens of 8 heads of 128, bf16 to
+// e4m3, are written in 11.5 us (4.4 TB/s), 131072 read back in 157 (5.2 TB/s; a
+// large copy reaches 4.9); a few tokens take 3 us of launch.
 #include <climits>
 
 #include "common.h"

@@ -6,7 +6,7 @@
 // with the weights as they were quantized once (e4m3 / e5m2 with one scale for
 // the tensor, for each row or for each 128 x 128 block) or in 16 bits.  What the
 // call cannot do without is every reached expert's weights once; at up to 64
-// tokens their read bounds it, so no weight is read twice and nothing but x, a
+// tokens their read bounds it, so no weight is read twice from memory and nothing but x, a
 // and y moves beside them.
 //
 // The weights are the first operand of the matrix instructions (rows: output
@@ -15,6 +15,12 @@
 // exactly to the tokens' 16-bit type; the scales are applied to fp32 sums.  A
 // step is 128 bytes of every row, two 16-byte pieces a lane with the 4 lanes of a
 // row side by side; the contraction takes the elements in that order.
+//
+// Measured, 32 experts of 2048 x 7168, top 8, e4m3: one token 79 us (352 MB, up 48 at
+// 4.8 TB/s, down 31 at 3.7), 64 tokens 346 (1.41 GB: up 217 at 4.3 TB/s, down 137 at
+// 3.4).  Up to 16 tokens the down product takes 16 rows a workgroup and a ring of
+// four (more workgroups where latency counts), beyond 32 rows, whose tokens' operands
+// are then used twice.
 //
 // Loads are unconditional (rows, columns and pieces that do not exist read ones
 // that do, and their products are not stored or meet a zero), so that a ring of

@@ -66,7 +66,7 @@ struct AttnArgs {
     float           scale_log2;
     int             slots;      // wide: work items per key / value head that the grid holds
     int             split_goal; // wide; 0: row tiles are never split
-    int             split, tiles; // narrow: chunks of a sequence, row tiles of it side by side
+    int             split;      // narrow: chunks of a sequence
     int             rows_min, rows_max; // sequences of this launch: rows_min < n G <= rows_max
 };
 
@@ -371,9 +371,17 @@ __device__ __forceinline__ int attn_page_row(const AttnArgs &a, int h, int j, in
 //   O += V(t)^T P(t)             beside the last quarter, the logits and maxima of
 //                                tile t + 1, and the staging of keys t + 2 and values t + 1
 // Each register is loaded with keys t + 3 or values t + 2 once it is staged; the
-// loads stay in flight over the barrier.  The softmax's reference m follows the running maximum only
-// when a tile exceeds it by 2^8: P then stays below 2^8 and most tiles rescale
-// nothing.
+// loads stay in flight over the barrier.  The softmax's reference m follows the
+// running maximum only when a tile exceeds it by 2^8: P then stays below 2^8 and
+// most tiles rescale nothing.
+//
+// Bound by what the vector unit has to do beside the matrix pipe: of the pipe's time
+// for a tile of 128 elements a head (4 waves x 64 instructions) the exponentials,
+// conversions, scales and staging take about as much again.  2048 new tokens over
+// 16384 of 32 / 8 heads of 128, e4m3: 655 us, 790 TFLOP/s, against 419 us at the
+// rate of a large library matrix product.  Keys and values go through LDS, converted
+// once for all four waves; a wave's registers hold O (64 of 256 a lane at 128
+// elements) and Q (32).  Two workgroups a CU hide some of each other's waits.
 constexpr float ATT_SLACK = 8.0f;
 
 // bits of a 16-bit type's infinity
@@ -944,9 +952,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 // ---------------------------------------------------------------------------
 // narrow kernel: 16 rows, four waves on 32 keys each of a key tile of 128
 // ---------------------------------------------------------------------------
-// Workgroup = (head, chunk, row tile, sequence), without a search: every sequence
-// has the same number of chunks, of a size of its own.  A wave keeps ST tiles of
+// Workgroup = (head, chunk, sequence), without a search: every sequence has the
+// same number of chunks, of a size of its own.  Its row tiles, mostly one, go one
+// after the other.  A wave keeps ST tiles of
 // keys and values in flight in registers.
+//
+// Bound by the cache's bytes: 64 sequences of up to 16384 tokens, 64 / 8 heads of
+// 128, e4m3, take 250 us at 4.9 TB/s, what a large copy reaches, and with the join
+// 259; the wide kernel takes 730 for them, since 120 of its 128 rows are empty.
+// With a search for the work item on the device (as in the wide kernel) and one
+// tile in flight instead of two that was 284.
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(AttnArgs a) {
     constexpr int  KT = ATT_NARROW_KEYS, BQ = ATT_NARROW_ROWS, WK = 32;
@@ -967,18 +982,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     __shared__ float2                sml[4][BQ];
 
     const int     tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int     h = blockIdx.x % a.Hkv, w0 = blockIdx.x / a.Hkv, chunk = w0 % a.split, w1 = w0 / a.split;
-    const int     b = w1 / a.tiles;
+    const int     h = blockIdx.x % a.Hkv, w0 = blockIdx.x / a.Hkv, chunk = w0 % a.split, b = w0 / a.split;
     const AttnSeq sq   = attn_seq(a, b);
     const int     n    = __builtin_amdgcn_readfirstlane(sq.n), len = __builtin_amdgcn_readfirstlane(sq.len);
     const int     tok0 = __builtin_amdgcn_readfirstlane(sq.tok0);
     const int     c = lane & 15, qd = lane >> 4;
     uint16_t     *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
 
-    for (int tile = w1 % a.tiles; tile * BQ < n * a.G; tile += a.tiles) {
+    for (int row0 = 0; row0 < n * a.G; row0 += BQ) {
         AttnItem it;
         it.b    = b;
-        it.row0 = tile * BQ;
+        it.row0 = row0;
         it.rows = min(BQ, n * a.G - it.row0);
         it.pos0 = len - n;
         const int total = attn_keys<KT>(a, it, len);
@@ -1245,7 +1259,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
 // joins the chunks of both kernels: o = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c
 // ---------------------------------------------------------------------------
 // An element is 4 values of a row; Q threads share its chunks, four chunks of a
-// thread are in flight.
+// thread are in flight.  Bound by the parts' bytes, 4 D + 8 a row and chunk: a batch
+// of chunks of up to 256 tokens, 32 heads of 128, takes 10 us.  One thread an
+// element where chunks are few (four threads: 17 us), four where a single row tile
+// is split over the chip.
 template <int QT, int Q> __device__ __forceinline__ void attn_join(const AttnArgs &a, const AttnSeq &s, int h, int row0, int rows,
                                                                    bool by_token, int64_t at0, int64_t stride, int count, int part, int parts) {
     constexpr int N = 256 / Q; // elements of a workgroup at a time

@@ -12,7 +12,7 @@ struct AttnPart {
     int     rows; // of a row tile; 0: not launched
     int     rows_min, rows_max;
     int64_t slots, goal;  // wide
-    int64_t split, tiles; // narrow
+    int64_t split;        // narrow
     size_t  desc_bytes, ml_bytes, o_bytes;
     size_t  bytes() const { return desc_bytes + ml_bytes + o_bytes; }
 };
@@ -24,17 +24,21 @@ struct AttnPlan {
 
 size_t round256(int64_t n) { return static_cast<size_t>(cdiv(n, 256) * 256); }
 
-// Rows of a sequence up to which the narrow kernel takes it where both run
-constexpr int ATT_NARROW_MOST = 64;
+// Rows of a sequence up to which the narrow kernel takes it where both run (16
+// sequences of up to 512 new tokens, 16 heads of 64: 103 us with 16, 108 with 64, 115
+// with 256; 4 of up to 256 under a window, 32 / 8 heads of 128: 46, 50 and 55), and up
+// to which it takes a call's only rows (8 tokens of 32 / 8 heads of 128 over 8192, 32
+// rows: 28.7 us, wide 27.3; over 1000: 15.6 and 16.5; 16 tokens, 64 rows: 51.8 and 32.7).
+constexpr int ATT_NARROW_MOST = 16, ATT_NARROW_ALONE = 32;
 
 // Every sequence gets the same number of chunks: two workgroups a CU from all of
-// them, four chunks where sequences may differ in length, no more than key tiles.
+// them, four chunks where sequences may differ in length (64 of up to 16384 tokens:
+// 260 us, 281 with one or two chunks), no more than key tiles.
 AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool mix) {
     AttnPart      p    = {};
     const int64_t fill = cdiv(2 * device_cu_count(), B * Hkv);
     p.rows     = ATT_NARROW_ROWS;
     p.rows_max = mix ? ATT_NARROW_MOST : INT_MAX;
-    p.tiles    = mix ? ATT_NARROW_MOST / ATT_NARROW_ROWS : 1;
     p.split    = std::max<int64_t>(1, std::min(std::max<int64_t>(fill, B > 1 ? 4 : 1), cdiv(keys, ATT_NARROW_KEYS)));
     if (p.split > 1) {
         p.ml_bytes = round256(p.split * Tq * Hq * 8);
@@ -44,7 +48,9 @@ AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_
 }
 
 // Row tiles are found on the device (their number goes by the lengths); they are
-// split where they do not give every CU one.
+// split where they do not give every CU two (chunks of up to 512 tokens over 4096,
+// 16 heads of 64: 145 us split for one a CU, 129 for two; of 256 over a window of
+// 1024, 32 / 8 heads of 128: 72 and 66).
 AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t keys, bool mix) {
     AttnPart p = {};
     p.rows     = ATT_WIDE_ROWS;
@@ -65,11 +71,14 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
 
 // All of it goes by sizes that the host has: tokens, sequences, heads and the
 // page table's extent.  Lengths stay on the device, so where sequences of few and
-// of many rows may be together both kernels run, each on its own.
+// of many rows may be together both kernels run, each on its own.  The wide kernel
+// alone would save the second launch (a mixed batch of 16 sequences: 109 us instead
+// of 129 at the time), but single tokens beside one chunk would cost three times as
+// much (64 sequences of 16384 tokens: 743 us instead of 259).
 AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
     AttnPlan      p = {};
     const int64_t G = Hq / Hkv, keys = max_pages * page;
-    const bool    few = Tq * G <= 16 * B || Tq * G <= ATT_NARROW_MOST; // a row tile each on average, or no sequence has many
+    const bool    few = Tq <= B || Tq * G <= ATT_NARROW_ALONE; // single tokens, or a few rows
     const bool    mix = !few && B > 1;
     if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix);
     if (!few) p.part[1] = attn_wide_part(Tq, B, Hkv, G, D, keys, mix);
@@ -125,7 +134,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
     PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
                   "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split * p.part[0].tiles, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
+    PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
     AttnArgs a = {};
     a.q = static_cast<const uint16_t *>(q);
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
@@ -159,7 +168,6 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
         x.slots      = static_cast<int>(part.slots);
         x.split_goal = static_cast<int>(part.goal);
         x.split      = static_cast<int>(part.split);
-        x.tiles      = static_cast<int>(part.tiles);
         x.rows_min   = part.rows_min;
         x.rows_max   = part.rows_max;
         if (part.bytes() == 0) continue;

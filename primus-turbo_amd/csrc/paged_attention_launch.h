@@ -8,7 +8,7 @@ namespace pta {
 template <int QT, int KIND, int DP> void attn_launch_d(const AttnCall &c, hipStream_t st) {
     const AttnArgs &n = c.narrow, &w = c.wide;
     if (c.has_narrow) {
-        const unsigned grid = static_cast<unsigned>(n.B) * n.tiles * n.split * n.Hkv;
+        const unsigned grid = static_cast<unsigned>(n.B) * n.split * n.Hkv;
         attn_narrow_kernel<QT, KIND, DP><<<grid, 256, 0, st>>>(n);
     }
     if (c.has_wide) {

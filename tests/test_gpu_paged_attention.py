@@ -144,7 +144,7 @@ def test_large_logits():
 
 
 @pytest.mark.parametrize("cache,dtype", KINDS)
-@pytest.mark.parametrize("n,D,window,sinks", [(10, 64, None, 0), (10, 128, 30, 2), (150, 64, None, 0), (150, 128, 40, 3), (100, 256, None, 0)])
+@pytest.mark.parametrize("n,D,window,sinks", [(8, 64, None, 0), (8, 128, 30, 2), (10, 64, None, 0), (10, 128, 30, 2), (150, 64, None, 0), (150, 128, 40, 3), (100, 256, None, 0)])
 def test_infinities_and_nan_reach_the_rows_that_see_them(cache, dtype, n, D, window, sinks):
     """Values and a key that are NaN or infinite: rows that do not see the token keep
     their finite results, the others get what the formula gives."""
