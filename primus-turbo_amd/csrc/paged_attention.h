@@ -25,11 +25,11 @@
 // contraction runs over the keys in the order in which S^T holds them, and V
 // comes from LDS through the transposing read in that order.
 //
-// Two kernels share this: the wide one (32 rows a wave, keys and values staged
-// in LDS for all waves) where a sequence has many rows, the narrow one (16
-// rows, keys straight into registers, every wave on keys of its own) where it has
-// few and the cache's bytes bound the call.  The keys of a row tile may be split
-// over several workgroups; a last kernel joins their parts.
+// Two forms share this: the wide one (32 rows a wave, keys and values staged in LDS
+// for all waves) where a sequence has many rows, the narrow one (16 rows, keys
+// straight into registers, every wave on keys of its own) where it has few and the
+// cache's bytes bound the call.  The keys of a row tile may be split over several
+// workgroups; a last kernel joins their parts.
 #pragma once
 
 #include <climits>
@@ -451,30 +451,38 @@ template <int QT, int KIND> __device__ __forceinline__ void att_values4(const ui
     }
 }
 
+template <int KIND, int DP> struct AttnWideLds {
+    static constexpr int KT = ATT_WIDE_KEYS;
+    static constexpr int KS = DP + 8;  // elements of a staged key row: 16 rows' equal pieces lie in different banks
+    static constexpr int VS = DP + 32; // of a value row: the transposed read's 8 rows of 64 bytes do; odd keys have
+                                       // the halves of every 32 bytes exchanged, for the writes' sake
+    static constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
+    alignas(16) uint16_t sk[2][KT * KS];
+    alignas(16) uint16_t sv[2][KT * VS];
+    alignas(16) float ssc[FP8 ? 3 : 1][3][FP8 ? KT : 4]; // scale log2e ks, log2 vs, 1 / vs by tile % 3
+    int      srow[8][KT];
+    int      shole[8];    // by tile % 8: some key has no row
+    int      sspec[2][4]; // by tile % 2 and wave: values with infinities or NaN
+    uint32_t red[16];
+};
+
 template <int QT, int KIND, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWideLds<KIND, DP> &lds) {
     constexpr int  KT = ATT_WIDE_KEYS, BQ = ATT_WIDE_ROWS, NT = 256;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;       // bytes of a cache element
     constexpr int  EC  = 16 / ES;           // elements of a 16-byte piece
     constexpr int  CPR = DP / EC;           // pieces of a row
     constexpr int  NP  = KT * CPR / NT;     // pieces of a thread and pool
-    constexpr int  KS  = DP + 8;            // elements of a staged key row: 16 rows' equal pieces lie in different banks
-    constexpr int  VS  = DP + 32;           // of a value row: the transposed read's 8 rows of 64 bytes do; odd keys have
-                                            // the halves of every 32 bytes exchanged, for the writes' sake
+    constexpr int  KS = AttnWideLds<KIND, DP>::KS, VS = AttnWideLds<KIND, DP>::VS;
     static_assert(KT * CPR % NT == 0, "pieces");
-    __shared__ __align__(16) uint16_t sk[2][KT * KS];
-    __shared__ __align__(16) uint16_t sv[2][KT * VS];
-    __shared__ __align__(16) float    ssc[FP8 ? 3 : 1][3][FP8 ? KT : 4]; // scale log2e ks, log2 vs, 1 / vs by tile % 3
-    __shared__ int                    srow[8][KT];
-    __shared__ int                    shole[8];   // by tile % 8: some key has no row
-    __shared__ int                    sspec[2][4]; // by tile % 2 and wave: values with infinities or NaN
-    __shared__ uint32_t               red[16];
+    auto &sk = lds.sk; auto &sv = lds.sv; auto &ssc = lds.ssc; auto &srow = lds.srow;
+    auto &shole = lds.shole; auto &sspec = lds.sspec; auto &red = lds.red;
 
     int            tid = threadIdx.x, lane = tid & 63;
     const int      wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int      h    = blockIdx.x % a.Hkv;
-    const int      slot = blockIdx.x / a.Hkv;
+    const int      h    = block % a.Hkv;
+    const int      slot = block / a.Hkv;
     const AttnItem it   = attn_find<BQ, KT, NT>(a, slot, red);
     if (a.desc != nullptr && h == 0 && tid == 0)
         a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
@@ -962,8 +970,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnA
 // 259; the wide kernel takes 730 for them, since 120 of its 128 rows are empty.
 // With a search for the work item on the device (as in the wide kernel) and one
 // tile in flight instead of two that was 284.
+template <int DP> struct AttnNarrowLds {
+    static constexpr int WK = 32, BQ = ATT_NARROW_ROWS;
+    static constexpr int VS = DP + 16; // elements of a staged value row: the transposed read's 16 rows
+                                       // of 32 bytes then fall into different banks
+    static constexpr int OS = DP + 4;  // floats of a row of the waves' joined output
+    static constexpr int SV_BYTES = 4 * WK * VS * 2, SO_BYTES = 4 * BQ * OS * 4;
+    alignas(16) uint8_t smem[SV_BYTES > SO_BYTES ? SV_BYTES : SO_BYTES];
+    alignas(16) float ssc[4][3][WK];
+    float2 sml[4][BQ];
+};
+
 template <int QT, int KIND, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNarrowLds<DP> &lds) {
     constexpr int  KT = ATT_NARROW_KEYS, BQ = ATT_NARROW_ROWS, WK = 32;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;
@@ -972,17 +991,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
     constexpr int  KP  = DP / 4 / EC;       // 16-byte pieces of a lane's quarter of a key row
     constexpr int  CPR = DP / EC;           // pieces of a value row
     constexpr int  VP  = WK * CPR / 64;     // value pieces of a lane
-    constexpr int  VS  = DP + 16;           // elements of a staged value row: the transposed read's 16 rows
-                                            // of 32 bytes then fall into different banks
-    constexpr int  OS  = DP + 4;            // floats of a row of the waves' joined output
-    constexpr int  SV_BYTES = 4 * WK * VS * 2, SO_BYTES = 4 * BQ * OS * 4;
+    constexpr int  VS = AttnNarrowLds<DP>::VS, OS = AttnNarrowLds<DP>::OS;
     static_assert(KP >= 1, "a quarter row is a piece at least");
-    __shared__ __align__(16) uint8_t smem[SV_BYTES > SO_BYTES ? SV_BYTES : SO_BYTES];
-    __shared__ __align__(16) float   ssc[4][3][WK];
-    __shared__ float2                sml[4][BQ];
+    auto &smem = lds.smem; auto &ssc = lds.ssc; auto &sml = lds.sml;
 
     const int     tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int     h = blockIdx.x % a.Hkv, w0 = blockIdx.x / a.Hkv, chunk = w0 % a.split, b = w0 / a.split;
+    const int     h = block % a.Hkv, w0 = block / a.Hkv, chunk = w0 % a.split, b = w0 / a.split;
     const AttnSeq sq   = attn_seq(a, b);
     const int     n    = __builtin_amdgcn_readfirstlane(sq.n), len = __builtin_amdgcn_readfirstlane(sq.len);
     const int     tok0 = __builtin_amdgcn_readfirstlane(sq.tok0);
@@ -1253,6 +1267,29 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_narrow_kernel(Attn
         }
         __syncthreads(); // the outputs' LDS becomes the values' of the next row tile
     }
+}
+
+// ---------------------------------------------------------------------------
+// the kernels: one form alone, or in one launch the wide form's workgroups, which
+// take longest, and behind them the narrow form's
+// ---------------------------------------------------------------------------
+template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a) {
+    __shared__ AttnWideLds<KIND, DP> lds;
+    attn_wide<QT, KIND, DP>(a, blockIdx.x, lds);
+}
+template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_narrow_kernel(AttnArgs a) {
+    __shared__ AttnNarrowLds<DP> lds;
+    attn_narrow<QT, KIND, DP>(a, blockIdx.x, lds);
+}
+template <int QT, int KIND, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnArgs w, AttnArgs n, int w_blocks) {
+    __shared__ union Lds {
+        AttnWideLds<KIND, DP> w;
+        AttnNarrowLds<DP>     n;
+        __device__ Lds() {}
+    } lds;
+    if (static_cast<int>(blockIdx.x) < w_blocks) attn_wide<QT, KIND, DP>(w, blockIdx.x, lds.w);
+    else attn_narrow<QT, KIND, DP>(n, blockIdx.x - w_blocks, lds.n);
 }
 
 // ---------------------------------------------------------------------------

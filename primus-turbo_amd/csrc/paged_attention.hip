@@ -71,10 +71,11 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
 
 // All of it goes by sizes that the host has: tokens, sequences, heads and the
 // page table's extent.  Lengths stay on the device, so where sequences of few and
-// of many rows may be together both kernels run, each on its own.  The wide kernel
-// alone would save the second launch (a mixed batch of 16 sequences: 109 us instead
-// of 129 at the time), but single tokens beside one chunk would cost three times as
-// much (64 sequences of 16384 tokens: 743 us instead of 259).
+// of many rows may be together both forms run, each on its own, in one launch
+// (chunks of up to 512 tokens over 4096, 16 heads of 64: 82 us, 103 as two launches;
+// of 256 over a window of 1024, 32 / 8 heads of 128: 42 and 46).  The wide form alone
+// would make single tokens beside one chunk three times as slow (64 sequences of
+// 16384 tokens: 743 us, narrow 259).
 AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
     AttnPlan      p = {};
     const int64_t G = Hq / Hkv, keys = max_pages * page;
