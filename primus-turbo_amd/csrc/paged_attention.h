@@ -891,6 +891,8 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
             att_each<8>([&](auto ch) PTA_INLINE { logits(ch, s, scale_of(t, 0, ch), scale_of(t, 1, ch)); });
             if (!full || edge(t, wpmin, wpmax)) mask(t);
         }
+        // the first iteration overwrites these keys: a wave without rows begins at once
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     for (int t = it.t0; t < it.t1; ++t) {
         // the lane's number anew: what derives from it (addresses in LDS and of the

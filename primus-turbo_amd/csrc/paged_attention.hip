@@ -24,16 +24,16 @@ struct AttnPlan {
 
 size_t round256(int64_t n) { return static_cast<size_t>(cdiv(n, 256) * 256); }
 
-// Rows of a sequence up to which the narrow kernel takes it where both run (16
-// sequences of up to 512 new tokens, 16 heads of 64: 103 us with 16, 108 with 64, 115
-// with 256; 4 of up to 256 under a window, 32 / 8 heads of 128: 46, 50 and 55), and up
+// Rows of a sequence up to which the narrow kernel takes it where both run (4 chunks
+// of up to 256 tokens under a window of 1024, 32 / 8 heads of 128: 42 us with 16 and 32,
+// 47 with 64; 16 of up to 512, 16 heads of 64: 81 to 82 with each), and up
 // to which it takes a call's only rows (8 tokens of 32 / 8 heads of 128 over 8192, 32
 // rows: 28.7 us, wide 27.3; over 1000: 15.6 and 16.5; 16 tokens, 64 rows: 51.8 and 32.7).
 constexpr int ATT_NARROW_MOST = 16, ATT_NARROW_ALONE = 32;
 
 // Every sequence gets the same number of chunks: two workgroups a CU from all of
 // them, four chunks where sequences may differ in length (64 of up to 16384 tokens:
-// 260 us, 281 with one or two chunks), no more than key tiles.
+// 260 us, 281 with one or two), no more than key tiles.
 AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool mix) {
     AttnPart      p    = {};
     const int64_t fill = cdiv(2 * device_cu_count(), B * Hkv);
@@ -48,9 +48,9 @@ AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_
 }
 
 // Row tiles are found on the device (their number goes by the lengths); they are
-// split where they do not give every CU two (chunks of up to 512 tokens over 4096,
-// 16 heads of 64: 145 us split for one a CU, 129 for two; of 256 over a window of
-// 1024, 32 / 8 heads of 128: 72 and 66).
+// split where they do not give every CU two (16 chunks of up to 512 tokens over 4096,
+// 16 heads of 64: 93 us split for one a CU, 82 for two, 81 for three; 4 of 256 over a
+// window of 1024, 32 / 8 heads of 128: 42, 42 and 51, more parts to join).
 AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t keys, bool mix) {
     AttnPart p = {};
     p.rows     = ATT_WIDE_ROWS;

@@ -180,6 +180,18 @@ def test_long_contexts_split_over_workgroups(cache, new, lens, Hq, Hkv):
     check(make(new, lens, Hq, Hkv, 128, 64, cache, BF), 4096, 4)
 
 
+@pytest.mark.parametrize("cache", [E4, BF])
+def test_row_tiles_with_waves_that_have_no_rows(cache):
+    """Row tiles of 8, 40 and 72 rows of 128: waves without rows run ahead of the
+    others, which must not change what those read, in this call or in the next."""
+    case = make([121, 17, 37, 181], [1183, 700, 900, 1435], 32, 4, 128, 128, cache, BF)
+    out, _ = check(case)
+    q, pools, scales, table, cu, lens = case
+    dev = [None if t is None else t.cuda() for t in (q, *pools, table, cu, lens, *scales)]
+    for _ in range(20):
+        assert torch.equal(_ops().paged_attention(*dev), out)
+
+
 def test_many_sequences():
     """More sequences than a workgroup has threads, some without tokens or keys."""
     g = torch.Generator().manual_seed(5)
