@@ -163,6 +163,13 @@ __device__ __forceinline__ int att_lane() {
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float att_log2(float x) { return __builtin_amdgcn_logf(x); }
 
+// The two values of a value scale: a scale of zero (values of zero) counts as 2^-100.
+// A NaN stays in the logits, where a row that does not see the key replaces it, and
+// not in the factor of the row's sum, which multiplies that row's zero.
+constexpr float ATT_LEAST_SCALE = 0x1p-100f;
+__device__ __forceinline__ float att_clamp_scale(float vs) { return fmaxf(vs, ATT_LEAST_SCALE); }
+__device__ __forceinline__ float att_log2_scale(float vs) { return att_log2(vs < ATT_LEAST_SCALE ? ATT_LEAST_SCALE : vs); }
+
 // max(a, b, c), NaN dropped; the plain form quiets operands first
 __device__ __forceinline__ float att_max3(float a, float b, float c) {
     float r;
@@ -632,8 +639,8 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
         if constexpr (FP8) {
             asm volatile("" : "+v"(kscl), "+v"(vscl));
             const bool  no = srow[t & 7][lane] < 0;
-            const float vs = no ? 1.0f : fmaxf(vscl, 0x1p-100f); // a scale of zero: values of zero
-            const float w  = wave == 0 ? (no ? 0.0f : kscl) * a.scale_log2 : wave == 1 ? att_log2(vs) : __builtin_amdgcn_rcpf(vs);
+            const float vs = no ? 1.0f : vscl;
+            const float w  = wave == 0 ? (no ? 0.0f : kscl) * a.scale_log2 : wave == 1 ? att_log2_scale(vs) : __builtin_amdgcn_rcpf(att_clamp_scale(vs));
             ssc[(t + 3) % 3][min(wave, 2)][lane] = w; // the fourth writes what the third does
         }
     };
@@ -1120,10 +1127,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
                 }
                 if constexpr (FP8) {
                     if (lane < WK) {
-                        const float vs        = fmaxf(scl[u][1], 0x1p-100f); // a scale of zero: values of zero
                         ssc[wave][0][lane] = scl[u][0] * a.scale_log2;
-                        ssc[wave][1][lane] = att_log2(vs);
-                        ssc[wave][2][lane] = 1.0f / vs;
+                        ssc[wave][1][lane] = att_log2_scale(scl[u][1]);
+                        ssc[wave][2][lane] = 1.0f / att_clamp_scale(scl[u][1]);
                     }
                 }
                 uint4 kf[2][DP / 32];

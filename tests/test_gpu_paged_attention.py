@@ -287,3 +287,28 @@ def test_written_tokens_are_attended():
     want, _, bound, _ = attention(q, *c, *s, table, torch.tensor([0, T]), torch.tensor([T]), D ** -0.5, None, 0)
     for o in outs:
         within(o, want, bound, "chunks")
+
+
+@pytest.mark.parametrize("cache,dtype", [(E4, BF), (E5, FH)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("n,L,j,window,sinks", [(1, 300, 7, None, 0), (8, 76, 72, None, 0), (8, 76, 70, 30, 2), (150, 360, 3, None, 0),
+                                                (150, 360, 285, None, 0), (150, 360, 285, 40, 3), (150, 360, 1, 40, 3)])
+def test_broken_value_scales_reach_the_rows_that_see_them(cache, dtype, bad, n, L, j, window, sinks):
+    """A value scale that is NaN (or infinite, beside elements of 0): NaN for the rows
+    that see its token, as fp8 * scale_inv gives it, and finite results for the others."""
+    q, (kc, vc), (ks, vs), table, cu, lens = make([n, 1], [L, 5], 4, 2, 64, 16, cache, dtype, seed=n)
+    clean = vs.clone()
+    page = int(table[0, j // 16])
+    vs[page, :, j % 16] = bad
+    vc.view(torch.uint8)[page, :, j % 16] = 0
+    dev = [t.cuda() for t in (q, kc, vc, table, cu, lens, ks, vs)]
+    got, lse = (x.cpu().double() for x in _ops().paged_attention(*dev, window_size=window, num_sinks=sinks, return_lse=True))
+    args = (table, cu, lens, 64 ** -0.5, window, sinks)
+    zero = lambda c: torch.nan_to_num(c.double(), 0.0, 0.0, 0.0)  # noqa: E731
+    raw = attention(q, zero(kc), zero(vc), torch.nan_to_num(ks), vs, *args)[0]
+    want, wlse, bound, b_lse = attention(q, zero(kc), zero(vc), *(torch.nan_to_num(s) for s in (ks, clean)), *args)
+    nan = torch.isnan(raw)
+    assert bool(nan.any()) and not bool(nan.all()) and torch.equal(torch.isnan(got), nan)
+    within(torch.where(nan, 0.0, got), torch.where(nan, 0.0, want), bound, "rows that do not see it")
+    seen = nan.any(2)
+    within(torch.where(seen, 0.0, lse), torch.where(seen, 0.0, wlse), b_lse, "their lse")
