@@ -170,6 +170,10 @@ constexpr float ATT_LEAST_SCALE = 0x1p-100f;
 __device__ __forceinline__ float att_clamp_scale(float vs) { return fmaxf(vs, ATT_LEAST_SCALE); }
 __device__ __forceinline__ float att_log2_scale(float vs) { return att_log2(vs < ATT_LEAST_SCALE ? ATT_LEAST_SCALE : vs); }
 
+// 1 / l of the row at position pos: below 0 it sees no key and becomes zeros, from 0
+// on its own at least.  Logits of -inf alone give l = 0 and 0 / 0, as the formula does.
+__device__ __forceinline__ float att_inverse(float l, int pos) { return pos < 0 ? 0.0f : 1.0f / l; }
+
 // max(a, b, c), NaN dropped; the plain form quiets operands first
 __device__ __forceinline__ float att_max3(float a, float b, float c) {
     float r;
@@ -939,7 +943,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
     const int r = it.row0 + wave * 32 + c;
     if (r >= it.row0 + it.rows) return;
     if (it.chunks == 1) {
-        const float   inv = l > 0.0f || l != l ? 1.0f / l : 0.0f; // no key seen: zeros
+        const float   inv = att_inverse(l, pos);
         const int     rt  = r / a.G;
         const int64_t row = static_cast<int64_t>(it.tok0 + rt) * a.Hq + h * a.G + (r - rt * a.G);
 #pragma unroll
@@ -1257,7 +1261,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
             const int     rr = it.row0 + jr, rt = rr / a.G;
             const int64_t orow = static_cast<int64_t>(tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
             if (a.split == 1) {
-                const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f; // no key seen: zeros
+                const float inv = att_inverse(ll, it.pos0 + rt);
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
@@ -1357,7 +1361,7 @@ template <int QT, int Q> __device__ __forceinline__ void attn_join(const AttnArg
 #pragma unroll
             for (int u = 1; u < Q; ++u) add(sml[u][lane], sacc[u][lane]);
         }
-        const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f; // no key seen: zeros
+        const float inv = att_inverse(ll, s.len - s.n + rt);
         *reinterpret_cast<uint2 *>(a.out + orow * a.D + d) =
             make_uint2(AttT<QT>::pack(acc.x * inv, acc.y * inv), AttT<QT>::pack(acc.z * inv, acc.w * inv));
         if (a.lse != nullptr && d == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;

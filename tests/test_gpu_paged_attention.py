@@ -312,3 +312,33 @@ def test_broken_value_scales_reach_the_rows_that_see_them(cache, dtype, bad, n, 
     within(torch.where(nan, 0.0, got), torch.where(nan, 0.0, want), bound, "rows that do not see it")
     seen = nan.any(2)
     within(torch.where(seen, 0.0, lse), torch.where(seen, 0.0, wlse), b_lse, "their lse")
+
+
+@pytest.mark.parametrize("cache,dtype", [(E5, BF), (E5, FH), (BF, BF), (FH, FH)])
+@pytest.mark.parametrize("n,L,count", [(1, 1, 1), (1, 40, 40), (1, 9000, 9000), (1, 300, 299), (8, 8, 5), (150, 150, 70), (150, 400, 330), (17, 5000, 5000)])
+def test_rows_whose_visible_logits_are_all_minus_infinity(cache, dtype, n, L, count):
+    """The first `count` keys give logits of -inf: a row that sees no other gets what the
+    formula gives, 0 / 0 and -inf, unlike a row that sees no key; the rest ignore them."""
+    q, (kc, vc), scales, table, cu, lens = make([n, 1], [L, 0], 4, 2, 64, 16, cache, dtype, seed=L)
+    q[..., 9] = q[..., 9].abs() + 1
+    low = kc.clone()
+    # logits below -250 in place of -inf have a weight of 0 beside the others, in 64 bits too
+    for pool, x in ((kc, float("-inf")), (low, -2000.0)):
+        for j in range(count):
+            pool[int(table[0, j // 16]), :, j % 16, 9] = torch.tensor(x).to(cache)
+    dev = [None if t is None else t.cuda() for t in (q, kc, vc, table, cu, lens, *scales)]
+    got, lse = (x.cpu().double() for x in _ops().paged_attention(*dev, return_lse=True))
+    if cache in FP8_MAX:
+        scales[0][:] = torch.nan_to_num(scales[0])
+        scales[1][:] = torch.nan_to_num(scales[1])
+        low = low.double() * scales[0][..., None]
+        for j in range(count):
+            low[int(table[0, j // 16]), :, j % 16, 9] = -2000.0
+    zero = lambda c: torch.nan_to_num(c.double(), 0.0, 0.0, 0.0)  # noqa: E731
+    want, wlse, bound, b_lse = attention(q, zero(low), zero(vc), None, scales[1], table, cu, lens, 64 ** -0.5, None, 0)
+    pos = torch.arange(n) + L - n
+    none = torch.cat([pos < count, torch.tensor([False])])[:, None].expand(n + 1, 4)  # the last token sees no key
+    assert torch.equal(torch.isnan(got).all(2), none) and torch.equal(torch.isnan(got).any(2), none)
+    assert bool((lse[none] == float("-inf")).all())
+    within(torch.where(none[..., None], 0.0, got), torch.where(none[..., None], 0.0, want), bound, "out")
+    within(torch.where(none, 0.0, lse), torch.where(none, 0.0, wlse), b_lse, "lse")
