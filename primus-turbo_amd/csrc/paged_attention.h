@@ -170,9 +170,14 @@ constexpr float ATT_LEAST_SCALE = 0x1p-100f;
 __device__ __forceinline__ float att_clamp_scale(float vs) { return fmaxf(vs, ATT_LEAST_SCALE); }
 __device__ __forceinline__ float att_log2_scale(float vs) { return att_log2(vs < ATT_LEAST_SCALE ? ATT_LEAST_SCALE : vs); }
 
-// 1 / l of the row at position pos: below 0 it sees no key and becomes zeros, from 0
-// on its own at least.  Logits of -inf alone give l = 0 and 0 / 0, as the formula does.
-__device__ __forceinline__ float att_inverse(float l, int pos) { return pos < 0 ? 0.0f : 1.0f / l; }
+// 1 / l of a row; one that sees no key (its position is below 0) becomes zeros.
+// Logits of -inf alone give l = 0 and 0 / 0, as the formula does.
+__device__ __forceinline__ float att_inverse(float l, bool none) { return none ? 0.0f : 1.0f / l; }
+// Among parts that are joined, such a row has m = 0 and l = 0, the others m = -inf
+// where they have seen nothing yet.  The join could read the lengths instead, but then
+// takes 81 scalar registers for 80, and 8.4 us for 6.8 (64 sequences, 64 heads of 128,
+// four chunks).
+__device__ __forceinline__ float att_part_max(float m, bool none) { return none ? 0.0f : m; }
 
 // max(a, b, c), NaN dropped; the plain form quiets operands first
 __device__ __forceinline__ float att_max3(float a, float b, float c) {
@@ -943,7 +948,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
     const int r = it.row0 + wave * 32 + c;
     if (r >= it.row0 + it.rows) return;
     if (it.chunks == 1) {
-        const float   inv = att_inverse(l, pos);
+        const float   inv = att_inverse(l, pos < 0);
         const int     rt  = r / a.G;
         const int64_t row = static_cast<int64_t>(it.tok0 + rt) * a.Hq + h * a.G + (r - rt * a.G);
 #pragma unroll
@@ -966,7 +971,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
                 if (d < a.D)
                     *reinterpret_cast<float4 *>(a.part_o + at * a.D + d) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
             }
-        if (half == 0) a.part_ml[at] = make_float2(m, l);
+        if (half == 0) a.part_ml[at] = make_float2(att_part_max(m, pos < 0), l);
     }
 }
 
@@ -1261,7 +1266,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
             const int     rr = it.row0 + jr, rt = rr / a.G;
             const int64_t orow = static_cast<int64_t>(tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
             if (a.split == 1) {
-                const float inv = att_inverse(ll, it.pos0 + rt);
+                const float inv = att_inverse(ll, it.pos0 + rt < 0);
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
@@ -1274,7 +1279,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
                         *reinterpret_cast<float4 *>(a.part_o + at * a.D + jd + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                if (jd == 0) a.part_ml[at] = make_float2(mm, ll);
+                if (jd == 0) a.part_ml[at] = make_float2(att_part_max(mm, it.pos0 + rt < 0), ll);
             }
         }
         __syncthreads(); // the outputs' LDS becomes the values' of the next row tile
@@ -1361,7 +1366,7 @@ template <int QT, int Q> __device__ __forceinline__ void attn_join(const AttnArg
 #pragma unroll
             for (int u = 1; u < Q; ++u) add(sml[u][lane], sacc[u][lane]);
         }
-        const float inv = att_inverse(ll, s.len - s.n + rt);
+        const float inv = att_inverse(ll, ll == 0.0f && mm > -INFINITY);
         *reinterpret_cast<uint2 *>(a.out + orow * a.D + d) =
             make_uint2(AttT<QT>::pack(acc.x * inv, acc.y * inv), AttT<QT>::pack(acc.z * inv, acc.w * inv));
         if (a.lse != nullptr && d == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;
