@@ -550,7 +550,8 @@ int pta_kv_cache_read(const void *k_cache, const void *v_cache, int cache_kind, 
  * head h belongs to cache head h / (Hq / Hkv).
  *   out [num_tokens, Hq, D] = softmax(softmax_scale q.k) v
  *   lse [num_tokens, Hq] fp32 (may be NULL) = ln sum exp(softmax_scale q.k)
- * A token that sees no key gets zeros and -inf, one that sees only keys with
+ * A token that sees no key or belongs to no sequence (ahead of cu_seqlens_q[0], from
+ * cu_seqlens_q[num_seqs] on) gets zeros and -inf, one that sees only keys with
  * logits of -inf NaN and -inf.  Value scales are not negative;
  * one that is NaN or infinite makes out and lse NaN for the tokens that see its
  * key.  The lengths stay on the device;

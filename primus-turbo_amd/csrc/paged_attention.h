@@ -1290,23 +1290,46 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
 // the kernels: one form alone, or in one launch the wide form's workgroups, which
 // take longest, and behind them the narrow form's
 // ---------------------------------------------------------------------------
-template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a) {
-    __shared__ AttnWideLds<KIND, DP> lds;
-    attn_wide<QT, KIND, DP>(a, blockIdx.x, lds);
+// Their last `pads` workgroups take the tokens that no sequence owns, ahead of the
+// first and behind the last: zeros and -inf, like tokens that see no key.
+__device__ __forceinline__ void attn_pad(const AttnArgs &a, int part, int parts) {
+    const int     first = min(max(a.cu[0], 0), a.Tq), last = min(max(a.cu[a.B], first), a.Tq);
+    const int     per = a.Hq * (a.D / 8); // 16-byte pieces of a token
+    const int64_t tokens = a.Tq - (last - first);
+    for (int64_t p = part * 256 + threadIdx.x; p < tokens * per; p += parts * 256) {
+        const int64_t t = p / per, row = t < first ? t : t - first + last;
+        reinterpret_cast<uint4 *>(a.out)[row * per + (p - t * per)] = make_uint4(0, 0, 0, 0);
+    }
+    if (a.lse == nullptr) return;
+    for (int64_t p = part * 256 + threadIdx.x; p < tokens * a.Hq; p += parts * 256) {
+        const int64_t t = p / a.Hq, row = t < first ? t : t - first + last;
+        a.lse[row * a.Hq + (p - t * a.Hq)] = -INFINITY;
+    }
 }
-template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_narrow_kernel(AttnArgs a) {
+
+template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a, int pads) {
+    __shared__ AttnWideLds<KIND, DP> lds;
+    const int block = blockIdx.x, work = gridDim.x - pads;
+    if (block < work) attn_wide<QT, KIND, DP>(a, block, lds);
+    else attn_pad(a, block - work, pads);
+}
+template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_narrow_kernel(AttnArgs a, int pads) {
     __shared__ AttnNarrowLds<DP> lds;
-    attn_narrow<QT, KIND, DP>(a, blockIdx.x, lds);
+    const int block = blockIdx.x, work = gridDim.x - pads;
+    if (block < work) attn_narrow<QT, KIND, DP>(a, block, lds);
+    else attn_pad(a, block - work, pads);
 }
 template <int QT, int KIND, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnArgs w, AttnArgs n, int w_blocks) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnArgs w, AttnArgs n, int w_blocks, int pads) {
     __shared__ union Lds {
         AttnWideLds<KIND, DP> w;
         AttnNarrowLds<DP>     n;
         __device__ Lds() {}
     } lds;
-    if (static_cast<int>(blockIdx.x) < w_blocks) attn_wide<QT, KIND, DP>(w, blockIdx.x, lds.w);
-    else attn_narrow<QT, KIND, DP>(n, blockIdx.x - w_blocks, lds.n);
+    const int block = blockIdx.x, work = gridDim.x - pads;
+    if (block < w_blocks) attn_wide<QT, KIND, DP>(w, block, lds.w);
+    else if (block < work) attn_narrow<QT, KIND, DP>(n, block - w_blocks, lds.n);
+    else attn_pad(n, block - work, pads);
 }
 
 // ---------------------------------------------------------------------------
@@ -1398,6 +1421,7 @@ struct AttnCall {
     AttnArgs narrow, wide;
     bool     has_narrow, has_wide;
     int      narrow_join_parts; // workgroups of a sequence's head that join its chunks
+    int      pads;              // workgroups for the tokens of no sequence
 };
 template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st);
 extern template void attn_launch<PTA_BF16>(const AttnCall &, int, hipStream_t);

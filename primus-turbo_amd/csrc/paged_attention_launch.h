@@ -8,9 +8,10 @@ namespace pta {
 template <int QT, int KIND, int DP> void attn_launch_d(const AttnCall &c, hipStream_t st) {
     const AttnArgs &n = c.narrow, &w = c.wide;
     const unsigned  n_blocks = static_cast<unsigned>(n.B) * n.split * n.Hkv, w_blocks = static_cast<unsigned>(w.slots) * w.Hkv;
-    if (c.has_narrow && c.has_wide) attn_both_kernel<QT, KIND, DP><<<w_blocks + n_blocks, 256, 0, st>>>(w, n, w_blocks);
-    else if (c.has_wide) attn_wide_kernel<QT, KIND, DP><<<w_blocks, 256, 0, st>>>(w);
-    else attn_narrow_kernel<QT, KIND, DP><<<n_blocks, 256, 0, st>>>(n);
+    const unsigned  pads = static_cast<unsigned>(c.pads);
+    if (c.has_narrow && c.has_wide) attn_both_kernel<QT, KIND, DP><<<w_blocks + n_blocks + pads, 256, 0, st>>>(w, n, w_blocks, c.pads);
+    else if (c.has_wide) attn_wide_kernel<QT, KIND, DP><<<w_blocks + pads, 256, 0, st>>>(w, c.pads);
+    else attn_narrow_kernel<QT, KIND, DP><<<n_blocks + pads, 256, 0, st>>>(n, c.pads);
 }
 
 template <int QT, int KIND> void attn_launch_k(const AttnCall &c, int D, hipStream_t st) {

@@ -100,9 +100,11 @@ def paged_attention(
 
     Returns [T, Hq, D] of q's type and, with ``return_lse``, the fp32 [T, Hq]
     logarithms of the softmax's sums.  A token that sees no key (a length of
-    zero, or shorter than its new tokens) gets zeros and -inf; one that sees only
-    keys with logits of -inf gets NaN and -inf.  A value scale that is NaN or
-    infinite makes NaN of the rows that see its token, of their sums too.
+    zero, or shorter than its new tokens) gets zeros and -inf, and so do rows that
+    no sequence owns, ahead of ``cu_seqlens_q[0]`` and from ``cu_seqlens_q[B]`` on
+    (a batch padded to a fixed size); one that sees only keys with logits of -inf
+    gets NaN and -inf.  A value scale that is NaN or infinite makes NaN of the
+    rows that see its token, of their sums too.
     Inference only: there is no backward pass.
     """
     out, lse = paged_attention_impl(q, k_cache, v_cache, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv,

@@ -342,3 +342,43 @@ def test_rows_whose_visible_logits_are_all_minus_infinity(cache, dtype, n, L, co
     assert bool((lse[none] == float("-inf")).all())
     within(torch.where(none[..., None], 0.0, got), torch.where(none[..., None], 0.0, want), bound, "out")
     within(torch.where(none, 0.0, lse), torch.where(none, 0.0, wlse), b_lse, "lse")
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv", [([1, 1, 1], [70, 300, 5], 4, 2), ([150], [400], 4, 2), ([150, 1, 0, 3], [400, 90, 7, 3], 4, 2),
+                                             ([40, 1], [90, 5000], 20, 1), ([0, 0], [9, 0], 4, 2)])
+def test_tokens_of_no_sequence(new, lens, Hq, Hkv):
+    """Rows ahead of the first sequence and behind the last (a batch padded to a fixed
+    size) become zeros and -inf, in a replayed graph too, whatever was there before."""
+    front, back = 3, 70
+    q, pools, scales, table, cu, ln = make(new, lens, Hq, Hkv, 64, 16, E4, BF)
+    q = torch.randn(front + len(q) + back, Hq, 64, generator=torch.Generator().manual_seed(1)).to(BF)
+    cu += front
+    junk = [torch.full(q.shape, float("nan"), dtype=BF, device="cuda"), torch.full(q.shape[:2], float("nan"), device="cuda")]
+    del junk  # its memory is the outputs' now
+    out, lse = check((q, pools, scales, table, cu, ln))
+    own = slice(front, front + sum(new))
+    for x, y in ((out, 0.0), (lse, float("-inf"))):
+        x[own] = y
+        assert bool((x == y).all())
+    dev = [t.cuda() for t in (q, *pools, table, cu, ln, *scales)]
+    ops = _ops()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.paged_attention(*dev, return_lse=True)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = ops.paged_attention(*dev, return_lse=True)
+    for i in range(4):  # a different first row, and the first sequence shorter
+        fewer = torch.tensor([max(0, new[0] - i), *new[1:]])
+        dev[4][0] = i
+        dev[4][1:] = i + fewer.cumsum(0)
+        want, wlse = ops.paged_attention(*dev, return_lse=True)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, wlse), f"replay {i}"
+        end = i + int(fewer.sum())
+        for a, b in ((0, i), (end, len(q))):
+            assert not bool(out[a:b].any()) and bool((lse[a:b] == float("-inf")).all()), f"replay {i}"
