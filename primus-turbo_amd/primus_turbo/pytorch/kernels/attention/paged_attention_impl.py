@@ -9,6 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from primus_turbo.pytorch import _C
+from primus_turbo.pytorch.core.inference import check_devices
 from primus_turbo.pytorch.core.low_precision import float8_e4m3, float8_e5m2
 
 _SIXTEEN = (torch.bfloat16, torch.float16)
@@ -18,17 +19,6 @@ _IN = {torch.bfloat16: _C.PTA_BF16, torch.float16: _C.PTA_F16, torch.float32: _C
 
 def _no_grad(what: str) -> None:
     assert not torch.is_grad_enabled(), f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors"
-
-
-def _check_devices(*tensors: Optional[torch.Tensor]) -> None:
-    """All on the first one's device.  These calls are made token by token: each check is
-    kept to what it costs."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            first = tensors[0].device
-            assert all(x is None or x.device == first for x in tensors), f"all tensors must be on {first}"
-            return
 
 
 def _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv):
@@ -78,7 +68,7 @@ def kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
     T = shape[0]
     n = _check_slots(slots)
     assert n == T, f"one slot for each of the {T} tokens, got {n}"
-    _check_devices(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
+    check_devices(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
     if k.requires_grad or v.requires_grad:
         _no_grad("kv_cache_write")
     if T == 0:
@@ -101,7 +91,7 @@ def kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
 def kv_cache_read_impl(k_cache, v_cache, slots, k_scale_inv, v_scale_inv, out_dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     kind, (P, Hkv, page, D) = _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv)
     T = _check_slots(slots)
-    _check_devices(k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
+    check_devices(k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
     dt = _IN.get(out_dtype)
     if dt is None:
         raise TypeError(f"unsupported output type {out_dtype}")
@@ -152,7 +142,7 @@ def paged_attention_impl(
     else:
         scale = float(softmax_scale)
         assert math.isfinite(scale), "softmax_scale must be finite"
-    _check_devices(q, k_cache, v_cache, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv)
+    check_devices(q, k_cache, v_cache, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv)
     if q.requires_grad:
         _no_grad("paged_attention")
     qs = q.stride()

@@ -8,6 +8,7 @@ from typing import Optional, Tuple
 import torch
 
 from primus_turbo.pytorch import _C
+from primus_turbo.pytorch.core.inference import check_devices
 from primus_turbo.pytorch.core.low_precision import ScalingGranularity, float8_e4m3, float8_e5m2
 from primus_turbo.pytorch.core.quantized_tensor import QuantizedTensor
 
@@ -77,10 +78,7 @@ def moe_decode_impl(x, w_gate_up, w_down, topk_idx, topk_probs, gate_up_scale_in
     k = idx_shape[1]
     assert 0 < k <= 32, f"1 to 32 experts a token, got {k}"
     assert topk_probs.shape == idx_shape and topk_probs.dtype == torch.float32, "topk_probs must be float32 like topk_idx"
-    at = x.get_device()
-    for t in (w1, w2, s1, s2, topk_idx, topk_probs):
-        if t is not None and (t.get_device() != at or at < 0):
-            assert t.device == x.device, f"all tensors must be on {x.device}"
+    check_devices(x, w1, w2, s1, s2, topk_idx, topk_probs)
     if x.requires_grad or topk_probs.requires_grad:
         assert not torch.is_grad_enabled(), (
             "moe_decode has no backward pass: call it under torch.no_grad() or on detached tensors"

@@ -188,3 +188,19 @@ def test_workspace_sizes():
     assert q(1, 1, 8, 8, 64, 1, 16) == 0              # one key tile: nothing to split
     assert q(1, 1, 8, 8, 64, 1000, 16) > 0            # few rows, many keys
     assert q(1 << 16, 1, 64, 8, 64, 1000, 16) == 0    # rows alone fill the chip
+
+
+def test_cpu_tensors_are_refused_beside_a_gpu(monkeypatch):
+    """Where a GPU is there, tensors in host memory must not reach a kernel."""
+    from primus_turbo.pytorch import _C
+
+    def launch(name, *args):
+        raise RuntimeError(f"{name} was launched on host memory")
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(_C, "stream", lambda device=None: 0)
+    monkeypatch.setattr(_C, "call", launch)
+    read = {n: x for n, x in cache_args().items() if n not in ("k", "v")}
+    for fn, args in ((_ops().kv_cache_write, cache_args()), (_ops().kv_cache_read, read), (_ops().paged_attention, attn_args()),
+                     (_ops().moe_decode, moe_args())):
+        refused(fn, args, "must be GPU tensors")
