@@ -56,7 +56,7 @@ struct AttnArgs {
     const int32_t  *cu, *lens;
     uint16_t       *out; // [Tq, Hq, D]
     float          *lse; // [Tq, Hq] or null
-    float          *part_o;  // [slots, Hkv, BQ, D] (wide), [split, Tq, Hq, D] (narrow)
+    float          *part_o;  // [slots, Hkv, BQ, D] (wide), [split, Tq, Hq, D] or [split, B, Hkv, 16, D] (narrow)
     float2         *part_ml; // the same without D
     int4           *desc;    // [slots]: sequence, row tile, chunk, chunks (wide)
     int             B, Tq, Hq, Hkv, G, D;
@@ -67,6 +67,7 @@ struct AttnArgs {
     int             slots;      // wide: work items per key / value head that the grid holds
     int             split_goal; // wide; 0: row tiles are never split
     int             split;      // narrow: chunks of a sequence
+    int             part_seq, part_step; // narrow: parts go by sequence, not by token; rows of a chunk's parts
     int             rows_min, rows_max; // sequences of this launch: rows_min < n G <= rows_max
 };
 
@@ -1274,7 +1275,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
                             make_uint2(AttT<QT>::pack(acc[e] * inv, acc[e + 1] * inv), AttT<QT>::pack(acc[e + 2] * inv, acc[e + 3] * inv));
                 if (a.lse != nullptr && jd == 0) a.lse[orow] = (mm + att_log2(ll)) * 0.69314718055994531f;
             } else {
-                const int64_t at = static_cast<int64_t>(chunk) * a.Tq * a.Hq + orow;
+                const int64_t at = static_cast<int64_t>(chunk) * a.part_step + (a.part_seq ? (b * a.Hkv + h) * BQ + rr : orow);
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
@@ -1404,7 +1405,8 @@ template <int QT, int QN> __global__ __launch_bounds__(256) void attn_join_kerne
     if (static_cast<int>(blockIdx.x) < n_blocks) {
         const int     h = blockIdx.x % n.Hkv, g = blockIdx.x / n.Hkv;
         const AttnSeq s = attn_seq(n, g / n_parts);
-        attn_join<QT, QN>(n, s, h, 0, s.n * n.G, true, 0, static_cast<int64_t>(n.Tq) * n.Hq, n.split, g % n_parts, n_parts);
+        attn_join<QT, QN>(n, s, h, 0, s.n * n.G, !n.part_seq, (static_cast<int64_t>(g / n_parts) * n.Hkv + h) * ATT_NARROW_ROWS, n.part_step,
+                          n.split, g % n_parts, n_parts);
     } else {
         const int  x = blockIdx.x - n_blocks, h = x % w.Hkv, g = x / w.Hkv, slot = g / ATT_JOIN_PARTS;
         const int4 d = w.desc[slot]; // sequence, row tile, chunk, chunks

@@ -12,7 +12,8 @@ struct AttnPart {
     int     rows; // of a row tile; 0: not launched
     int     rows_min, rows_max;
     int64_t slots, goal;  // wide
-    int64_t split;        // narrow
+    int64_t split, part_step; // narrow
+    bool    part_seq;
     size_t  desc_bytes, ml_bytes, o_bytes;
     size_t  bytes() const { return desc_bytes + ml_bytes + o_bytes; }
 };
@@ -30,6 +31,7 @@ size_t round256(int64_t n) { return static_cast<size_t>(cdiv(n, 256) * 256); }
 // to which it takes a call's only rows (8 tokens of 32 / 8 heads of 128 over 8192, 32
 // rows: 28.7 us, wide 27.3; over 1000: 15.6 and 16.5; 16 tokens, 64 rows: 51.8 and 32.7).
 constexpr int ATT_NARROW_MOST = 16, ATT_NARROW_ALONE = 32;
+static_assert(ATT_NARROW_MOST <= ATT_NARROW_ROWS, "parts by sequence hold one row tile");
 
 // Workgroups at most that fill the tokens of no sequence.  Where there are none they
 // cost nothing that shows: 1 token over 1000 16.0 us without and 15.9 with, 64 tokens
@@ -46,8 +48,12 @@ AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_
     p.rows_max = mix ? ATT_NARROW_MOST : INT_MAX;
     p.split    = std::max<int64_t>(1, std::min(std::max<int64_t>(fill, B > 1 ? 4 : 1), cdiv(keys, ATT_NARROW_KEYS)));
     if (p.split > 1) {
-        p.ml_bytes = round256(p.split * Tq * Hq * 8);
-        p.o_bytes  = round256(p.split * Tq * Hq * D * 4);
+        // a mixed call's tokens are mostly the wide form's: parts for the rows that a
+        // sequence can have here, unless the tokens are fewer
+        p.part_seq  = mix && B * Hkv * ATT_NARROW_ROWS < Tq * Hq;
+        p.part_step = p.part_seq ? B * Hkv * ATT_NARROW_ROWS : Tq * Hq;
+        p.ml_bytes  = round256(p.split * p.part_step * 8);
+        p.o_bytes   = round256(p.split * p.part_step * D * 4);
     }
     return p;
 }
@@ -177,6 +183,8 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
         x.slots      = static_cast<int>(part.slots);
         x.split_goal = static_cast<int>(part.goal);
         x.split      = static_cast<int>(part.split);
+        x.part_seq   = part.part_seq;
+        x.part_step  = static_cast<int>(part.part_step);
         x.rows_min   = part.rows_min;
         x.rows_max   = part.rows_max;
         if (part.bytes() == 0) continue;

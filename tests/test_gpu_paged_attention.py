@@ -382,3 +382,11 @@ def test_tokens_of_no_sequence(new, lens, Hq, Hkv):
         end = i + int(fewer.sum())
         for a, b in ((0, i), (end, len(q))):
             assert not bool(out[a:b].any()) and bool((lse[a:b] == float("-inf")).all()), f"replay {i}"
+
+
+@pytest.mark.parametrize("cache,dtype", [(E4, BF), (FH, FH)])
+@pytest.mark.parametrize("new,lens,Hq,Hkv", [([300, 2, 1, 5], [300, 9000, 7000, 40], 12, 4), ([200, 1], [5000, 6000], 16, 1),
+                                             ([30, 1, 1, 2, 16], [700, 3000, 5, 900, 2000], 2, 2)])
+def test_few_rows_beside_prompts_over_long_contexts(cache, dtype, new, lens, Hq, Hkv):
+    """Sequences of up to 16 rows whose keys are split, in a batch with longer chunks."""
+    check(make(new, lens, Hq, Hkv, 64, 64, cache, dtype, seed=Hq))

@@ -204,3 +204,14 @@ def test_cpu_tensors_are_refused_beside_a_gpu(monkeypatch):
     for fn, args in ((_ops().kv_cache_write, cache_args()), (_ops().kv_cache_read, read), (_ops().paged_attention, attn_args()),
                      (_ops().moe_decode, moe_args())):
         refused(fn, args, "must be GPU tensors")
+
+
+@pytest.mark.parametrize("T,B,Hq,Hkv,D,keys", [(8193, 2, 64, 8, 128, 8192), (16384, 2, 64, 8, 128, 16384), (8193, 2, 64, 1, 128, 32768),
+                                               (32769, 2, 8, 1, 128, 32768), (2049, 2, 32, 8, 128, 16384)])
+def test_workspace_of_prompts_beside_single_tokens(T, B, Hq, Hkv, D, keys):
+    """Long prompts in a batch of several sequences: their rows have no parts among the
+    few rows' ones."""
+    from primus_turbo.pytorch import _C
+
+    size = _C.query("pta_paged_attention_workspace_size", T, B, Hq, Hkv, D, keys // 64, 64)
+    assert size <= max(16 << 20, 2 * T * Hq * D)
