@@ -91,7 +91,7 @@ AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, in
     AttnPlan      p = {};
     const int64_t G = Hq / Hkv, keys = max_pages * page;
     const bool    few = Tq <= B || Tq * G <= ATT_NARROW_ALONE; // single tokens, or a few rows
-    const bool    mix = !few && B > 1;
+    const bool    mix = !few && B > 1 && G <= ATT_NARROW_MOST; // more rows to a token: none is the narrow form's
     if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix);
     if (!few) p.part[1] = attn_wide_part(Tq, B, Hkv, G, D, keys, mix);
     return p;

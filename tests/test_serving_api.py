@@ -215,3 +215,13 @@ def test_workspace_of_prompts_beside_single_tokens(T, B, Hq, Hkv, D, keys):
 
     size = _C.query("pta_paged_attention_workspace_size", T, B, Hq, Hkv, D, keys // 64, 64)
     assert size <= max(16 << 20, 2 * T * Hq * D)
+
+
+def test_workspace_without_few_rows():
+    """Beyond 16 query heads to a cache head no token has few rows: its form has no parts."""
+    from primus_turbo.pytorch import _C
+
+    q = lambda *a: _C.query("pta_paged_attention_workspace_size", *a)  # noqa: E731
+    assert q(8193, 2, 64, 1, 128, 512, 64) == 0   # row tiles alone fill the chip
+    assert q(8193, 2, 136, 8, 64, 512, 64) == 0
+    assert q(8193, 2, 128, 8, 64, 512, 64) > 0    # 16 heads: a single token is 16 rows
