@@ -550,13 +550,15 @@ int pta_kv_cache_read(const void *k_cache, const void *v_cache, int cache_kind, 
  * head h belongs to cache head h / (Hq / Hkv).
  *   out [num_tokens, Hq, D] = softmax(softmax_scale q.k) v
  *   lse [num_tokens, Hq] fp32 (may be NULL) = ln sum exp(softmax_scale q.k)
- * A token that sees no key or belongs to no sequence (ahead of cu_seqlens_q[0], from
- * cu_seqlens_q[num_seqs] on) gets zeros and -inf, one that sees only keys with
- * logits of -inf NaN and -inf.  Value scales are not negative;
- * one that is NaN or infinite makes out and lse NaN for the tokens that see its
- * key.  The lengths stay on the device;
- * the workspace (pta_paged_attention_workspace_size bytes, often 0) depends on
- * the sizes and the device's compute units alone and needs no clearing. */
+ * A token that sees no key or belongs to no sequence (ahead of cu_seqlens_q[0],
+ * from cu_seqlens_q[num_seqs] on) gets zeros and -inf, one that sees only keys
+ * with logits of -inf NaN and -inf.  Value scales are not negative; one that is
+ * NaN or infinite makes out and lse NaN for the tokens that see its key.  The
+ * lengths stay on the device; the workspace depends on the sizes and the device's
+ * compute units alone and needs no clearing: 4 D + 8 bytes a row of the parts that
+ * are joined.  It is 0 where no keys are split (one key tile, or one sequence whose
+ * rows fill the chip), elsewhere at most about 256 rows for each CU of row tiles,
+ * and of few rows four times or what fills the CUs twice. */
 size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv,
                                           int64_t D, int64_t max_pages, int64_t page_size);
 int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D,

@@ -44,7 +44,6 @@ namespace pta {
 #define PTA_INLINE __attribute__((always_inline))
 
 constexpr int ATT_WIDE_ROWS = 128, ATT_WIDE_KEYS = 64, ATT_NARROW_ROWS = 16, ATT_NARROW_KEYS = 128;
-constexpr int ATT_NONE = INT_MIN; // desc of a slot without work
 
 struct AttnArgs {
     const uint16_t *q;
@@ -56,9 +55,9 @@ struct AttnArgs {
     const int32_t  *cu, *lens;
     uint16_t       *out; // [Tq, Hq, D]
     float          *lse; // [Tq, Hq] or null
-    float          *part_o;  // [slots, Hkv, BQ, D] (wide), [split, Tq, Hq, D] or [split, B, Hkv, 16, D] (narrow)
+    float          *part_o;  // [parts, Hkv, BQ, D] (wide), [split, Tq, Hq, D] or [split, B, Hkv, 16, D] (narrow)
     float2         *part_ml; // the same without D
-    int4           *desc;    // [slots]: sequence, row tile, chunk, chunks (wide)
+    int4           *desc;    // [slots]: sequence, row tile, its first part (-1: none, or another chunk's), chunks (wide)
     int             B, Tq, Hq, Hkv, G, D;
     int             num_pages, page, max_pages;
     uint32_t        page_mul, page_shift; // j / page = mulhi(j, page_mul) >> page_shift for j < 2^31; page_mul 0: j >> page_shift
@@ -205,6 +204,7 @@ __device__ __forceinline__ float add_xor32(float v) {
 // tile: key tiles [0, n_sink), then those from lo_tile on.
 struct AttnItem {
     int b, tile, chunk, chunks; // b < 0: no work
+    int part;                   // number of the chunk among those of split row tiles
     int row0, rows;             // rows [row0, row0 + rows) of the sequence
     int tok0;                   // first new token of the sequence in q
     int pos0;                   // position of the sequence's token 0
@@ -254,30 +254,41 @@ template <int KT> __device__ __forceinline__ int attn_keys(const AttnArgs &a, At
 }
 
 // Finds the item of slot `slot`; all threads of the workgroup call it (`red`:
-// 2 * 8 words of LDS).  Items are numbered sequence by sequence, row tile by row
+// 16 words of LDS).  Items are numbered sequence by sequence, row tile by row
 // tile, chunk by chunk; a row tile's k key tiles make ceil(k / C) equal chunks, C
 // such that all items of a head fit the grid: sum over the row tiles of
-// ceil(k / C) <= sum(k) / C + tiles.
+// ceil(k / C) <= sum(k) / C + tiles.  A tile is split where k > C, into less than
+// 2 k / C chunks: less than twice the split goal in all have parts.
 template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs &a, int slot, uint32_t *red) {
     constexpr int NW = NTHR / 64;
     const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    auto scan = [&](uint32_t v, uint32_t &total) PTA_INLINE -> uint32_t { // inclusive prefix sum over the workgroup
+    // inclusive prefix sums over the workgroup, two side by side
+    auto scan = [&](uint32_t(&v)[2], uint32_t(&total)[2]) PTA_INLINE {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(v, d);
-            if (lane >= d) v += o;
+            const uint32_t o0 = __shfl_up(v[0], d), o1 = __shfl_up(v[1], d);
+            if (lane >= d) {
+                v[0] += o0;
+                v[1] += o1;
+            }
         }
         __syncthreads();
-        if (lane == 63) red[wave] = v;
+        if (lane == 63) {
+            red[wave]      = v[0];
+            red[12 + wave] = v[1];
+        }
         __syncthreads();
-        uint32_t before = 0;
-        total           = 0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            if (w < wave) before += red[w];
-            total += red[w];
+        for (int i = 0; i < 2; ++i) {
+            uint32_t before = 0;
+            total[i]        = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                if (w < wave) before += red[12 * i + w];
+                total[i] += red[12 * i + w];
+            }
+            v[i] += before;
         }
-        return v + before;
     };
     AttnItem it;
     it.b            = -1;
@@ -285,15 +296,20 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
     int   C = INT_MAX;
     if (a.split_goal > 0) {
         // sums past 32 bits only make C larger than needed: in floating point
-        float w = 0.0f;
+        float w = 0.0f, some = 0.0f; // `some`: of up to 256 sequences, so that few roundings add up
         for (int b0 = 0; b0 < a.B; b0 += NTHR) {
             const int b = b0 + tid;
             if (b < a.B) {
                 const AttnSeq s = b0 == 0 ? s0 : attn_seq(a, b);
                 const float   r = static_cast<float>((static_cast<int64_t>(s.n) * a.G + BQ - 1) / BQ);
-                w += r * static_cast<float>(attn_tiles<KT>(a, s, BQ));
+                some += r * static_cast<float>(attn_tiles<KT>(a, s, BQ));
+            }
+            if (b0 / NTHR % 256 == 255) {
+                w += some;
+                some = 0.0f;
             }
         }
+        w += some;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) w += __shfl_xor(w, d);
         if (lane == 0) red[8 + wave] = __float_as_uint(w);
@@ -305,7 +321,7 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
         // above the quotient by more than the sum's rounding: the grid holds all items
         C = static_cast<int>(fminf(w * 1.001f / static_cast<float>(a.split_goal), 1e9f)) + 1;
     }
-    uint32_t seen = 0;
+    uint32_t seen = 0, split = 0; // items of the sequences before, those among them that have parts
     for (int b0 = 0; b0 < a.B; b0 += NTHR) {
         const int b = b0 + tid;
         AttnSeq   s = {0, 0, 0};
@@ -316,15 +332,18 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
             const int k = attn_tiles<KT>(a, s, BQ);
             chunks      = k > C ? (k - 1) / C + 1 : 1;
         }
-        uint32_t       total;
+        uint32_t       incl[2], total[2];
         const uint32_t mine = tiles * chunks;
-        const uint32_t incl = scan(mine, total);
-        if (static_cast<uint32_t>(slot) < seen + total) {
+        incl[0] = mine;
+        incl[1] = chunks > 1 ? mine : 0;
+        scan(incl, total);
+        if (static_cast<uint32_t>(slot) < seen + total[0]) {
             const uint32_t at = static_cast<uint32_t>(slot) - seen;
             __syncthreads();
-            if (at < incl && at >= incl - mine) {
+            if (at < incl[0] && at >= incl[0] - mine) {
                 red[0] = b;
-                red[1] = at - (incl - mine);
+                red[1] = at - (incl[0] - mine);
+                red[6] = split + incl[1] - mine; // the sequence's first, if it is split
                 red[2] = chunks;
                 red[3] = s.n;
                 red[4] = s.len;
@@ -336,9 +355,11 @@ template <int BQ, int KT, int NTHR> __device__ AttnItem attn_find(const AttnArgs
             const int at_b = __builtin_amdgcn_readfirstlane(red[1]);
             it.tile   = at_b / it.chunks;
             it.chunk  = at_b - it.tile * it.chunks;
+            it.part   = __builtin_amdgcn_readfirstlane(red[6]) + at_b;
             break;
         }
-        seen += total;
+        seen += total[0];
+        split += total[1];
     }
     if (it.b < 0) return it;
     const int n = __builtin_amdgcn_readfirstlane(red[3]), len = __builtin_amdgcn_readfirstlane(red[4]);
@@ -502,7 +523,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
     const int      slot = block / a.Hkv;
     const AttnItem it   = attn_find<BQ, KT, NT>(a, slot, red);
     if (a.desc != nullptr && h == 0 && tid == 0)
-        a.desc[slot] = it.b < 0 ? make_int4(ATT_NONE, 0, 0, 0) : make_int4(it.b, it.tile, it.chunk, it.chunks);
+        a.desc[slot] = it.b < 0 || it.chunks == 1 || it.chunk > 0 ? make_int4(0, 0, -1, 0) : make_int4(it.b, it.tile, it.part, it.chunks);
     if (it.b < 0) return;
 
     int  page_id     = -1;
@@ -963,7 +984,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
             }
         if (a.lse != nullptr && half == 0) a.lse[row] = (m + att_log2(l)) * 0.69314718055994531f;
     } else {
-        const int64_t at = (static_cast<int64_t>(slot) * a.Hkv + h) * BQ + wave * 32 + c;
+        const int64_t at = (static_cast<int64_t>(it.part) * a.Hkv + h) * BQ + wave * 32 + c;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -1409,11 +1430,11 @@ template <int QT, int QN> __global__ __launch_bounds__(256) void attn_join_kerne
                           n.split, g % n_parts, n_parts);
     } else {
         const int  x = blockIdx.x - n_blocks, h = x % w.Hkv, g = x / w.Hkv, slot = g / ATT_JOIN_PARTS;
-        const int4 d = w.desc[slot]; // sequence, row tile, chunk, chunks
-        if (d.x == ATT_NONE || d.z != 0 || d.w == 1) return;
+        const int4 d = w.desc[slot]; // sequence, row tile, first part, chunks
+        if (d.z < 0) return;
         const AttnSeq s    = attn_seq(w, d.x);
         const int     row0 = d.y * ATT_WIDE_ROWS;
-        attn_join<QT, 1>(w, s, h, row0, min(ATT_WIDE_ROWS, s.n * w.G - row0), false, (static_cast<int64_t>(slot) * w.Hkv + h) * ATT_WIDE_ROWS,
+        attn_join<QT, 1>(w, s, h, row0, min(ATT_WIDE_ROWS, s.n * w.G - row0), false, (static_cast<int64_t>(d.z) * w.Hkv + h) * ATT_WIDE_ROWS,
                       static_cast<int64_t>(w.Hkv) * ATT_WIDE_ROWS, d.w, g % ATT_JOIN_PARTS, ATT_JOIN_PARTS);
     }
 }

@@ -67,15 +67,17 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
     p.rows     = ATT_WIDE_ROWS;
     p.rows_min = mix ? ATT_NARROW_MOST : 0;
     p.rows_max = INT_MAX;
-    const int64_t most = Tq * G / ATT_WIDE_ROWS + B; // row tiles of a head: sum of ceil(n G / rows)
+    // row tiles of a head, sum of ceil(n G / rows), over the sequences that come here
+    const int64_t full = Tq * G / ATT_WIDE_ROWS, most = full + std::min(B, Tq * G / (p.rows_min + 1));
     const int64_t goal = cdiv(2 * device_cu_count(), Hkv);
     // row tiles alone fill the chip, or no tile has keys for two chunks
-    p.goal  = most - B >= goal || keys <= ATT_WIDE_KEYS ? 0 : goal;
+    p.goal  = full >= goal || keys <= ATT_WIDE_KEYS ? 0 : goal;
     p.slots = most + p.goal;
     if (p.goal > 0) {
+        const int64_t parts = std::min(p.slots, 2 * p.goal); // chunks of split row tiles
         p.desc_bytes = round256(p.slots * 16);
-        p.ml_bytes   = round256(p.slots * Hkv * ATT_WIDE_ROWS * 8);
-        p.o_bytes    = round256(p.slots * Hkv * ATT_WIDE_ROWS * D * 4);
+        p.ml_bytes   = round256(parts * Hkv * ATT_WIDE_ROWS * 8);
+        p.o_bytes    = round256(parts * Hkv * ATT_WIDE_ROWS * D * 4);
     }
     return p;
 }

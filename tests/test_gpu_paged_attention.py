@@ -390,3 +390,13 @@ def test_tokens_of_no_sequence(new, lens, Hq, Hkv):
 def test_few_rows_beside_prompts_over_long_contexts(cache, dtype, new, lens, Hq, Hkv):
     """Sequences of up to 16 rows whose keys are split, in a batch with longer chunks."""
     check(make(new, lens, Hq, Hkv, 64, 64, cache, dtype, seed=Hq))
+
+
+@pytest.mark.parametrize("cache,dtype", [(E4, BF), (FH, FH)])
+def test_split_row_tiles_of_many_sequences(cache, dtype):
+    """More sequences than a workgroup has threads, with split row tiles among the first
+    256, the next and the last, one sequence of two tiles, one that is not split."""
+    new, lens = [1] * 600, [3 + i % 90 for i in range(600)]
+    for i, n, L in ((5, 40, 3000), (6, 9, 20), (255, 20, 1500), (256, 33, 2000), (300, 100, 2500), (599, 17, 700)):
+        new[i], lens[i] = n, L
+    check(make(new, lens, 4, 2, 32, 64, cache, dtype))

@@ -225,3 +225,15 @@ def test_workspace_without_few_rows():
     assert q(8193, 2, 64, 1, 128, 512, 64) == 0   # row tiles alone fill the chip
     assert q(8193, 2, 136, 8, 64, 512, 64) == 0
     assert q(8193, 2, 128, 8, 64, 512, 64) > 0    # 16 heads: a single token is 16 rows
+
+
+@pytest.mark.parametrize("T,B,Hq,Hkv,D,keys", [(1001, 1000, 16, 16, 256, 4096), (1500, 1000, 16, 16, 256, 4096), (192, 64, 64, 8, 128, 16384),
+                                               (3000, 170, 8, 8, 128, 32768), (40, 1, 8, 2, 256, 32768), (300, 16, 16, 16, 64, 4096)])
+def test_workspace_of_many_sequences(T, B, Hq, Hkv, D, keys):
+    """Parts of 4 D + 8 bytes a row: row tiles of 128 for less than twice the chunks that fill
+    256 CUs twice, and at least four of few rows, no more than tokens and what fills the CUs."""
+    from primus_turbo.pytorch import _C
+
+    size = _C.query("pta_paged_attention_workspace_size", T, B, Hq, Hkv, D, keys // 64, 64)
+    rows = 2 * (512 + Hkv) * 128 + 4 * T * Hq + 512 * max(16, Hq // Hkv) + T * Hq
+    assert size <= rows * (4 * D + 8) + 16 * (T * Hq // Hkv // 128 + B + 512) + 1024
