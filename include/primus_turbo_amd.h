@@ -557,7 +557,7 @@ int pta_kv_cache_read(const void *k_cache, const void *v_cache, int cache_kind, 
  * lengths stay on the device; the workspace depends on the sizes and the device's
  * compute units alone and needs no clearing: 4 D + 8 bytes a row of the parts that
  * are joined.  It is 0 where no keys are split (one key tile, or one sequence whose
- * rows fill the chip), elsewhere at most about 256 rows for each CU of row tiles,
+ * rows fill the chip), elsewhere at most about 512 rows for each CU of row tiles,
  * and of few rows four times or what fills the CUs twice. */
 size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv,
                                           int64_t D, int64_t max_pages, int64_t page_size);

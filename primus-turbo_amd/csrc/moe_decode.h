@@ -48,10 +48,12 @@ struct MoeArgs {
     const void     *idx;     // [T, k] int32 or int64
     int             idx_i64;
     const float    *probs;   // [T, k]
-    uint16_t       *act;     // [groups, S, TG, I]: an expert's tokens one after the other
+    uint16_t       *act;     // [groups, rows, I]: an expert's tokens one after the other
     uint16_t       *y;       // [T, H]
     int             T, E, k, I, H, S, TG;
     int             by_entry; // slots are entries of the index rows (few tokens) instead of experts
+    int             rows;     // of a group in act
+    int             packed;   // an expert's rows begin behind the entries of those before; else at slot * TG
     int             scale;    // MoeScale
 };
 
@@ -126,7 +128,7 @@ struct MoeUpShared {
     float    red[4 * 4 * 4 * 256]; // wave, column tile, row tile, 16 x 16
     float    prob[MOE_TG];
     int      tok[MOE_TG]; // the expert's tokens
-    int      n, expert;
+    int      n, expert, row0; // row0: its first row in act
 };
 
 // One pass over K: PR pairs of (gate, up) row tiles from pair p0 on, NC column tiles.
@@ -220,10 +222,13 @@ template <int XT, int KIND, bool MANY> __global__ __launch_bounds__(MOE_NT, 2) v
         if (a.by_entry) e = slot < tl * a.k ? moe_expert(a, static_cast<int64_t>(t0) * a.k + slot) : -1;
         float p    = 0.0f;
         int   mine = -1; // the token's first entry for this expert
+        int   below = 0; // entries for experts before it
         if (lane < tl && e >= 0) {
             for (int j = a.k - 1; j >= 0; --j) {
                 const int64_t at = static_cast<int64_t>(t0 + lane) * a.k + j;
-                if (moe_expert(a, at) == e) {
+                const int     ej = moe_expert(a, at);
+                if (a.packed) below += __popcll(__ballot(static_cast<unsigned>(ej) < static_cast<unsigned>(e)));
+                if (ej == e) {
                     mine = lane * a.k + j;
                     p += a.probs[at];
                 }
@@ -240,6 +245,7 @@ template <int XT, int KIND, bool MANY> __global__ __launch_bounds__(MOE_NT, 2) v
         if (lane == 0) {
             sh.n      = __popcll(mask);
             sh.expert = mask && (!a.by_entry || first == slot) ? e : -1;
+            sh.row0   = a.packed ? below : slot * a.TG;
         }
     }
     __syncthreads();
@@ -279,7 +285,7 @@ template <int XT, int KIND, bool MANY> __global__ __launch_bounds__(MOE_NT, 2) v
             }
             v[j] = gate / (1.0f + att_exp2(gate * -1.4426950408889634f)) * up * sh.prob[tt];
         }
-        *reinterpret_cast<uint4 *>(a.act + ((static_cast<int64_t>(g) * a.S + slot) * a.TG + tt) * a.I + i) =
+        *reinterpret_cast<uint4 *>(a.act + (static_cast<int64_t>(g) * a.rows + sh.row0 + tt) * a.I + i) =
             make_uint4(AttT<XT>::pack(v[0], v[1]), AttT<XT>::pack(v[2], v[3]), AttT<XT>::pack(v[4], v[5]), AttT<XT>::pack(v[6], v[7]));
     }
 }
@@ -301,6 +307,8 @@ __global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeAr
     __shared__ unsigned long long smask[MOE_MAX_E];  // tokens of a slot
     __shared__ int                sfirst[LIST]; // by entry: an expert's slot; afterwards: list of reached slots
     __shared__ short              sexp[LIST], scnt[LIST], sfrom[LIST]; // of the list: expert, tokens, the first of them
+    __shared__ int                srow[LIST];        // of the list: first row in act
+    __shared__ int                sbefore[MOE_MAX_E]; // packed: an expert's entries, then those of the experts before it
     __shared__ int                stok[NW][PART]; // a wave's tokens of the expert it sums
     __shared__ int                scount;
     const int tid = threadIdx.x, lane = tid & 63, wave = moe_uniform(tid >> 6);
@@ -308,6 +316,8 @@ __global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeAr
     const int64_t ent0 = static_cast<int64_t>(t0) * a.k;
 
     for (int i = tid; i < a.S; i += NT) smask[i] = 0;
+    if (a.packed)
+        for (int i = tid; i < a.E; i += NT) sbefore[i] = 0;
     for (int i = tid; i < NW * TOKS * RS; i += NT) (&ssum[0][0][0])[i] = 0.0f;
     if (a.by_entry) {
         for (int i = tid; i < a.E; i += NT) sfirst[i] = INT_MAX;
@@ -321,21 +331,44 @@ __global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeAr
     for (int i = tid; i < n_ent; i += NT) {
         const int e = moe_expert(a, ent0 + i);
         if (e >= 0) atomicOr(&smask[a.by_entry ? sfirst[e] : e], 1ull << (i / a.k));
+        if (e >= 0 && a.packed) atomicAdd(&sbefore[e], 1);
     }
     __syncthreads();
     if (wave == 0) {
         int n = 0;
+        if (a.packed) {
+            int before = 0;
+            for (int e0 = 0; e0 < a.E; e0 += 64) {
+                const int mine = e0 + lane < a.E ? sbefore[e0 + lane] : 0;
+                int       sum  = mine;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int o = __shfl_up(sum, d);
+                    if (lane >= d) sum += o;
+                }
+                if (e0 + lane < a.E) sbefore[e0 + lane] = before + sum - mine;
+                before += __shfl(sum, 63);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
         for (int s0 = 0; s0 < a.S; s0 += 64) {
             const int      s   = s0 + lane;
             const int      cnt = s < a.S ? __popcll(smask[s]) : 0;
             const uint64_t below = (1ull << lane) - 1;
-            int            at = n;
+            int            at = n, e = s, row0 = s * a.TG;
+            if (cnt > 0) {
+                if (a.by_entry) e = moe_expert(a, ent0 + s);
+                if (a.packed) row0 = sbefore[e];
+            }
 #pragma unroll
             for (int q = 0; q < TOKS; q += PART) at += __popcll(__ballot(cnt > q) & below);
 #pragma unroll
             for (int q = 0; q < TOKS; q += PART) {
                 if (cnt > q) {
-                    sexp[at]   = static_cast<short>(a.by_entry ? moe_expert(a, ent0 + s) : s);
+                    sexp[at]   = static_cast<short>(e);
+                    srow[at]   = row0 + q;
                     sfirst[at] = s;
                     sfrom[at]  = static_cast<short>(q);
                     scnt[at]   = static_cast<short>(min(cnt - q, PART));
@@ -369,7 +402,7 @@ __global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeAr
     auto fetch = [&](MoeStage<F, RT, NC> &q, float4(&qs)[RT], int it) PTA_INLINE {
         // past the last: the last expert's tables, and a step past K
         const int li = it < items ? it / steps : items / steps - 1, st = it < items ? it - li * steps : steps, k0 = st * F::STEP;
-        const int e = moe_uniform(sexp[li]), s = moe_uniform(sfirst[li]), n_tok = moe_uniform(scnt[li]);
+        const int e = moe_uniform(sexp[li]), n_tok = moe_uniform(scnt[li]);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             q.w[r].load(a.w2 + static_cast<int64_t>(e) * a.H * rowb + hoff[r], k0, qd, K);
@@ -380,7 +413,7 @@ __global__ __launch_bounds__(MOE_NT, NC == 1 ? 2 : 1) void moe_down_kernel(MoeAr
             for (int r = 0; r < RT; ++r)
                 qs[r] = *reinterpret_cast<const float4 *>(a.s2 + static_cast<int64_t>(e) * a.H + min(h0 + r * 16, a.H - 16) + 4 * qd);
         }
-        const uint16_t *act = a.act + ((static_cast<int64_t>(g) * a.S + s) * a.TG + moe_uniform(sfrom[li])) * a.I;
+        const uint16_t *act = a.act + (static_cast<int64_t>(g) * a.rows + moe_uniform(srow[li])) * a.I;
 #pragma unroll
         for (int n = 0; n < NC; ++n) q.x[n].load(act + static_cast<int64_t>(min(n * 16 + c, n_tok - 1)) * a.I, k0, qd, K);
     };

@@ -6,8 +6,9 @@ namespace {
 
 struct MoePlan {
     int64_t groups, TG, S;
-    bool    by_entry;
-    size_t  bytes(int64_t I) const { return static_cast<size_t>(groups * S * TG * I * 2); }
+    bool    by_entry, packed;
+    int64_t rows, all; // of act: a group's, the call's
+    size_t  bytes(int64_t I) const { return static_cast<size_t>(all * I * 2); }
 };
 
 MoePlan moe_plan(int64_t T, int64_t E, int64_t k) {
@@ -16,6 +17,12 @@ MoePlan moe_plan(int64_t T, int64_t E, int64_t k) {
     p.TG       = T < MOE_TG ? T : MOE_TG;
     p.by_entry = p.TG * k <= E;
     p.S        = p.by_entry ? p.TG * k : E;
+    // Room for every token in every slot needs no counting, but grows with T E: calls of
+    // several groups have a row for each entry (4096 tokens, top 8 of 256, I = 2048: 134 MB
+    // for 4.29 GB)
+    p.packed = p.groups > 1;
+    p.rows   = p.packed ? p.TG * k : p.S * p.TG;
+    p.all    = p.packed ? T * k : p.rows;
     return p;
 }
 
@@ -88,6 +95,7 @@ extern "C" int pta_moe_decode(const void *x, int x_dtype, int64_t num_tokens, in
     a.T = static_cast<int>(num_tokens); a.E = static_cast<int>(num_experts); a.k = static_cast<int>(topk);
     a.I = static_cast<int>(I); a.H = static_cast<int>(H); a.S = static_cast<int>(p.S); a.TG = static_cast<int>(p.TG);
     a.by_entry = p.by_entry ? 1 : 0;
+    a.rows = static_cast<int>(p.rows); a.packed = p.packed ? 1 : 0;
     a.scale    = granularity; // PTA_TENSORWISE / ROWWISE / BLOCKWISE are MoeScale's values
     const unsigned    groups = static_cast<unsigned>(p.groups);
     const hipStream_t st     = as_stream(stream);

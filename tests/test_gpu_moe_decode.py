@@ -199,3 +199,15 @@ def test_graph_replay_with_new_routing():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want), f"replay {i}"
+
+
+@pytest.mark.parametrize("T,E,k", [(65, 256, 3), (130, 6, 4), (200, 1024, 2), (129, 300, 8), (1000, 16, 2)])
+def test_several_groups_of_tokens(T, E, k):
+    """More tokens than a pass takes, whose rows between the products lie close together:
+    experts that nobody reaches, entries of other ranks, an expert named twice by a token."""
+    idx, probs = routing(T, E, k, T, away=E // 5)
+    idx[1, k - 1] = idx[1, 0]
+    idx[T - 1, 0] = idx[T - 1, 1]
+    idx[64:, :][idx[64:, :] == E // 2] = -1
+    idx[5] = -1
+    check(tokens(T, 48, BF, T), weights(E, 32, 48, "ROWWISE", E4, BF, E), idx, probs)

@@ -237,3 +237,11 @@ def test_workspace_of_many_sequences(T, B, Hq, Hkv, D, keys):
     size = _C.query("pta_paged_attention_workspace_size", T, B, Hq, Hkv, D, keys // 64, 64)
     rows = 2 * (512 + Hkv) * 128 + 4 * T * Hq + 512 * max(16, Hq // Hkv) + T * Hq
     assert size <= rows * (4 * D + 8) + 16 * (T * Hq // Hkv // 128 + B + 512) + 1024
+
+
+@pytest.mark.parametrize("T,E,k,I", [(4096, 256, 8, 2048), (512, 256, 8, 2048), (65, 1024, 1, 64), (1000, 8, 2, 1024)])
+def test_expert_workspace_of_many_tokens(T, E, k, I):
+    """A row of 16 bit for each entry of topk_idx, whatever the number of experts."""
+    from primus_turbo.pytorch import _C
+
+    assert _C.query("pta_moe_decode_workspace_size", T, E, k, I) <= T * k * I * 2
