@@ -9,16 +9,12 @@ from typing import Optional, Tuple
 import torch
 
 from primus_turbo.pytorch import _C
-from primus_turbo.pytorch.core.inference import check_devices
+from primus_turbo.pytorch.core.inference import check_tensors
 from primus_turbo.pytorch.core.low_precision import float8_e4m3, float8_e5m2
 
 _SIXTEEN = (torch.bfloat16, torch.float16)
 _KIND = {float8_e4m3: _C.PTA_E4M3, float8_e5m2: _C.PTA_E5M2, torch.bfloat16: _C.CACHE_16BIT, torch.float16: _C.CACHE_16BIT}
 _IN = {torch.bfloat16: _C.PTA_BF16, torch.float16: _C.PTA_F16, torch.float32: _C.PTA_F32}
-
-
-def _no_grad(what: str) -> None:
-    assert not torch.is_grad_enabled(), f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors"
 
 
 def _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv):
@@ -68,9 +64,7 @@ def kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
     T = shape[0]
     n = _check_slots(slots)
     assert n == T, f"one slot for each of the {T} tokens, got {n}"
-    check_devices(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
-    if k.requires_grad or v.requires_grad:
-        _no_grad("kv_cache_write")
+    check_tensors("kv_cache_write", (k, v, k_cache, v_cache, k_scale_inv, v_scale_inv), slots)
     if T == 0:
         return
     ks, vs = k.stride(), v.stride()
@@ -91,12 +85,12 @@ def kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
 def kv_cache_read_impl(k_cache, v_cache, slots, k_scale_inv, v_scale_inv, out_dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     kind, (P, Hkv, page, D) = _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv)
     T = _check_slots(slots)
-    check_devices(k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
     dt = _IN.get(out_dtype)
     if dt is None:
         raise TypeError(f"unsupported output type {out_dtype}")
     fp8 = kind != _C.CACHE_16BIT
     assert fp8 or out_dtype == k_cache.dtype, f"a {k_cache.dtype} cache is read back as it is"
+    check_tensors("kv_cache_read", (k_cache, v_cache, k_scale_inv, v_scale_inv), slots)
     dev = k_cache.device
     k = torch.empty((T, Hkv, D), dtype=out_dtype, device=dev)
     v = torch.empty_like(k)
@@ -142,9 +136,7 @@ def paged_attention_impl(
     else:
         scale = float(softmax_scale)
         assert math.isfinite(scale), "softmax_scale must be finite"
-    check_devices(q, k_cache, v_cache, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv)
-    if q.requires_grad:
-        _no_grad("paged_attention")
+    check_tensors("paged_attention", (q, k_cache, v_cache, k_scale_inv, v_scale_inv), page_table, cu_seqlens_q, seq_lens)
     qs = q.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)

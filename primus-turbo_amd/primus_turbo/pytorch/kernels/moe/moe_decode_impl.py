@@ -8,7 +8,7 @@ from typing import Optional, Tuple
 import torch
 
 from primus_turbo.pytorch import _C
-from primus_turbo.pytorch.core.inference import check_devices
+from primus_turbo.pytorch.core.inference import check_tensors, refuse_gradients
 from primus_turbo.pytorch.core.low_precision import ScalingGranularity, float8_e4m3, float8_e5m2
 from primus_turbo.pytorch.core.quantized_tensor import QuantizedTensor
 
@@ -21,6 +21,8 @@ def _weight(w, scale, name: str) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     if not isinstance(w, QuantizedTensor):
         return w, scale
     assert scale is None, f"{name} is a QuantizedTensor: it brings its scale_inv"
+    if w.requires_grad:
+        refuse_gradients("moe_decode", w)
     g = w.granularity
     assert g != ScalingGranularity.MX_BLOCKWISE, "moe_decode: MX_BLOCKWISE weights are not supported"
     if g == ScalingGranularity.ROWWISE:
@@ -78,11 +80,7 @@ def moe_decode_impl(x, w_gate_up, w_down, topk_idx, topk_probs, gate_up_scale_in
     k = idx_shape[1]
     assert 0 < k <= 32, f"1 to 32 experts a token, got {k}"
     assert topk_probs.shape == idx_shape and topk_probs.dtype == torch.float32, "topk_probs must be float32 like topk_idx"
-    check_devices(x, w1, w2, s1, s2, topk_idx, topk_probs)
-    if x.requires_grad or topk_probs.requires_grad:
-        assert not torch.is_grad_enabled(), (
-            "moe_decode has no backward pass: call it under torch.no_grad() or on detached tensors"
-        )
+    check_tensors("moe_decode", (x, topk_probs, w1, w2, s1, s2), topk_idx)
     dev = x.device
     y = torch.empty(xshape, dtype=dtype, device=dev)
     if T == 0:

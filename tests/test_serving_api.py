@@ -245,3 +245,50 @@ def test_expert_workspace_of_many_tokens(T, E, k, I):
     from primus_turbo.pytorch import _C
 
     assert _C.query("pta_moe_decode_workspace_size", T, E, k, I) <= T * k * I * 2
+
+
+def _calls_with_floats():
+    """(entry, arguments, name of one floating tensor) for every one of the four calls."""
+    h = dict(k_cache=z(4, 2, 8, 32), v_cache=z(4, 2, 8, 32), k_scale_inv=None, v_scale_inv=None)
+    w = dict(w_gate_up=z(4, 96, 64), w_down=z(4, 64, 48), gate_up_scale_inv=None, down_scale_inv=None)
+    read = {n: x for n, x in cache_args(**h).items() if n not in ("k", "v")}
+    ops = _ops()
+    out = [(ops.kv_cache_write, cache_args(**h), n) for n in ("k", "v", "k_cache", "v_cache")]
+    out += [(ops.kv_cache_read, read, n) for n in ("k_cache", "v_cache")]
+    out += [(ops.paged_attention, attn_args(**h), n) for n in ("q", "k_cache", "v_cache")]
+    out += [(ops.moe_decode, moe_args(**w), n) for n in ("x", "topk_probs", "w_gate_up", "w_down")]
+    out += [(ops.kv_cache_write, cache_args(), "k_scale_inv"), (ops.paged_attention, attn_args(), "v_scale_inv"),
+            (ops.moe_decode, moe_args(), "down_scale_inv")]
+    return out
+
+
+def test_gradients_are_refused_not_dropped():
+    """16-bit caches and weights that need gradients, as queries and tokens that do."""
+    for fn, args, name in _calls_with_floats():
+        args = args | {name: args[name].detach().clone().requires_grad_()}
+        refused(fn, args, "no backward")
+        with torch.no_grad():  # refused for another reason, or not at all
+            if not torch.cuda.is_available():
+                refused(fn, args, "need a ROCm GPU", RuntimeError)
+
+
+def test_forward_mode_tangents_are_refused_not_dropped():
+    import torch.autograd.forward_ad as fwad
+
+    for fn, args, name in _calls_with_floats():
+        with fwad.dual_level(), torch.no_grad():
+            t = args[name]
+            refused(fn, args | {name: fwad.make_dual(t, torch.ones_like(t))}, "no forward-mode derivative")
+
+
+def test_quantized_weights_that_need_gradients_are_refused():
+    from primus_turbo.pytorch.core.low_precision import ScalingGranularity
+    from primus_turbo.pytorch.core.quantized_tensor import QuantizedTensor
+
+    def make(N, K, grad):
+        return QuantizedTensor(z(4, N, K, dtype=E4), z(4, N, 1, dtype=torch.float32), shape=(4, N, K), orig_dtype=BF, dest_dtype=E4,
+                               granularity=ScalingGranularity.ROWWISE, quantized_axis=2, requires_grad=grad)
+
+    none = dict(gate_up_scale_inv=None, down_scale_inv=None)
+    refused(_ops().moe_decode, moe_args(w_gate_up=make(96, 64, False), w_down=make(64, 48, True), **none), "no backward")
+    no_gpu(_ops().moe_decode, moe_args(w_gate_up=make(96, 64, False), w_down=make(64, 48, False), **none))
