@@ -7,6 +7,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from primus_turbo.pytorch import _C
 from primus_turbo.pytorch.core.inference import check_tensors
@@ -80,6 +81,8 @@ def kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
         slots.dtype == torch.int64, k_cache.data_ptr(), v_cache.data_ptr(), kind, P, page,
         k_scale_inv.data_ptr() if fp8 else None, v_scale_inv.data_ptr() if fp8 else None, _C.stream(k.device),
     )
+    # torch's count of a tensor's changes, which autograd compares with what it has saved
+    increment_version((k_cache, v_cache, k_scale_inv, v_scale_inv) if fp8 else (k_cache, v_cache))
 
 
 def kv_cache_read_impl(k_cache, v_cache, slots, k_scale_inv, v_scale_inv, out_dtype) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -292,3 +292,27 @@ def test_quantized_weights_that_need_gradients_are_refused():
     none = dict(gate_up_scale_inv=None, down_scale_inv=None)
     refused(_ops().moe_decode, moe_args(w_gate_up=make(96, 64, False), w_down=make(64, 48, True), **none), "no backward")
     no_gpu(_ops().moe_decode, moe_args(w_gate_up=make(96, 64, False), w_down=make(64, 48, False), **none))
+
+
+def test_a_written_cache_counts_as_changed(monkeypatch):
+    """What autograd has saved of a pool is not used after the pool was written."""
+    from primus_turbo.pytorch import _C
+
+    done = []
+    monkeypatch.setattr(_C, "stream", lambda device=None: 0)
+    monkeypatch.setattr(_C, "call", lambda name, *args: done.append(name))
+    a = cache_args()
+    pools = [a[n] for n in ("k_cache", "v_cache", "k_scale_inv", "v_scale_inv")]
+    before = [p._version for p in pools]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    _ops().kv_cache_write(**a)
+    assert done == ["pta_kv_cache_write"] and all(p._version > b for p, b in zip(pools, before))
+    c = z(4, 2, 8, 32)
+    w = torch.ones(32, dtype=BF, requires_grad=True)
+    y = (w * c).sum()
+    _ops().kv_cache_write(**cache_args(k_cache=c, v_cache=z(4, 2, 8, 32), k_scale_inv=None, v_scale_inv=None))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        i = cache_args(**{n: x.clone() for n, x in a.items() if n in ("k_cache", "v_cache", "k_scale_inv", "v_scale_inv")})
+    _ops().kv_cache_write(**i)  # inference tensors have no version
