@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 from torch.autograd import forward_ad
 
 __all__ = ["check_tensors", "refuse_gradients"]
@@ -28,6 +29,8 @@ def check_tensors(what: str, floats: Sequence[Optional[torch.Tensor]], *others: 
     on); all tensors are on one device, and that a GPU: kernels get raw pointers.
     These calls are made token by token: one look at each tensor where all is well."""
     dev = floats[0].get_device()
+    # one is enough: they do not go together with tensors that have memory
+    assert not isinstance(floats[0], FakeTensor), f"{what} runs on memory: fake tensors have none"
     if dev >= 0 and forward_ad._current_level < 0:
         for t in floats:
             if t is not None and (t.requires_grad or t.get_device() != dev):

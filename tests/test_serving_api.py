@@ -316,3 +316,20 @@ def test_a_written_cache_counts_as_changed(monkeypatch):
     with torch.inference_mode():
         i = cache_args(**{n: x.clone() for n, x in a.items() if n in ("k_cache", "v_cache", "k_scale_inv", "v_scale_inv")})
     _ops().kv_cache_write(**i)  # inference tensors have no version
+
+
+def test_fake_tensors_are_refused(monkeypatch):
+    """Fake tensors have no memory, and views of them addresses that are not null."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from primus_turbo.pytorch import _C
+
+    done = []
+    monkeypatch.setattr(_C, "stream", lambda device=None: 0)
+    monkeypatch.setattr(_C, "call", lambda name, *args: done.append(name))
+    read = {n: x for n, x in cache_args().items() if n not in ("k", "v")}
+    for fn, args in ((_ops().kv_cache_write, cache_args()), (_ops().kv_cache_read, read), (_ops().paged_attention, attn_args()),
+                     (_ops().moe_decode, moe_args())):
+        with FakeTensorMode() as mode:
+            refused(fn, {n: mode.from_tensor(x) for n, x in args.items()}, "fake tensors")
+    assert not done
