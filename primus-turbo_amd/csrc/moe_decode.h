@@ -17,8 +17,8 @@
 // row side by side; the contraction takes the elements in that order.
 //
 // Measured, 32 experts of 2048 x 7168, top 8, e4m3: one token 79 us (352 MB, up 48 at
-// 4.8 TB/s, down 31 at 3.7), 64 tokens 346 (1.41 GB: up 217 at 4.3 TB/s, down 137 at
-// 3.4).  Up to 16 tokens the down product takes 16 rows a workgroup and a ring of
+// 4.8 TB/s, down 31 at 3.7), 64 tokens 347 (1.41 GB: up 217 at 4.3 TB/s, down 137 at
+// 3.4); a linear read reaches 6.9.  Up to 16 tokens the down product takes 16 rows a workgroup and a ring of
 // four (more workgroups where latency counts), beyond 32 rows, whose tokens' operands
 // are then used twice.
 //

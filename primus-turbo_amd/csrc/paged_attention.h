@@ -13,9 +13,10 @@
 //   u_j = (q.k8_j) * (scale * log2(e) * ks_j) + log2(vs_j),   m = max_j u_j,
 //   p_j = 2^(u_j - m):   l = sum_j p_j / vs_j,   O = sum_j p_j v8_j,   o = O / l
 //
-// P stays in [0, 1] however large or small the scales are, which fp16 needs,
-// and is rounded once, to the 16 bits that the matrix instructions take;
-// logits, m, l and O are fp32.
+// P stays in [0, 1], in the wide form, whose m may lag behind the maximum, below
+// 2^8, however large or small the scales are, which fp16 needs.  It is rounded
+// once, to the 16 bits that the matrix instructions take; logits, m, l and O are
+// fp32.
 //
 // The query heads of one key / value head are rows of one matrix, r = i * G + g
 // (G = Hq / Hkv), so a key is read once for all of them.  Both products are
@@ -1005,9 +1006,10 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
 // after the other.  A wave keeps ST tiles of
 // keys and values in flight in registers.
 //
-// Bound by the cache's bytes: 64 sequences of up to 16384 tokens, 64 / 8 heads of
-// 128, e4m3, take 250 us at 4.9 TB/s, what a large copy reaches, and with the join
-// 259; the wide kernel takes 730 for them, since 120 of its 128 rows are empty.
+// Bound by the cache's reads in flight: 64 sequences of up to 16384 tokens, 64 / 8
+// heads of 128, e4m3, take 251 to 256 us, 4.9 TB/s, what a large copy reaches (a linear
+// read 6.9), and with the join 261; the wide kernel takes 730 for them, since 120 of
+// its 128 rows are empty.
 // With a search for the work item on the device (as in the wide kernel) and one
 // tile in flight instead of two that was 284.
 template <int DP> struct AttnNarrowLds {
@@ -1357,11 +1359,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnA
 // ---------------------------------------------------------------------------
 // joins the chunks of both kernels: o = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c
 // ---------------------------------------------------------------------------
-// An element is 4 values of a row; Q threads share its chunks, four chunks of a
-// thread are in flight.  Bound by the parts' bytes, 4 D + 8 a row and chunk: a batch
-// of chunks of up to 256 tokens, 32 heads of 128, takes 10 us.  One thread an
-// element where chunks are few (four threads: 17 us), four where a single row tile
-// is split over the chip.
+// An element is 4 values of a row; Q threads share its chunks, which a thread adds
+// one after the other.  Bound by that chain of reads and the parts' bytes, 4 D + 8 a
+// row and chunk: a batch of chunks of up to 256 tokens, 32 heads of 128, takes 10 us.
+// The narrow form's parts have one thread an element where chunks are few (four
+// threads: 17 us), four beyond four chunks; the wide form's always one, which a row
+// tile of a hundred chunks pays for (35 tokens over 21119, 8 / 2 heads: 103 us a call).
 template <int QT, int Q> __device__ __forceinline__ void attn_join(const AttnArgs &a, const AttnSeq &s, int h, int row0, int rows,
                                                                    bool by_token, int64_t at0, int64_t stride, int count, int part, int parts) {
     constexpr int N = 256 / Q; // elements of a workgroup at a time

@@ -27,7 +27,9 @@ size_t round256(int64_t n) { return static_cast<size_t>(cdiv(n, 256) * 256); }
 
 // Rows of a sequence up to which the narrow kernel takes it where both run (4 chunks
 // of up to 256 tokens under a window of 1024, 32 / 8 heads of 128: 42 us with 16 and 32,
-// 47 with 64; 16 of up to 512, 16 heads of 64: 81 to 82 with each), and up
+// 47 with 64; 16 of up to 512, 16 heads of 64: 81 to 82 with each; a few tokens of each
+// of many long sequences were not among them: 64 of 1 to 3 tokens over 8192, 64 / 8
+// heads, where 24 rows go to the wide kernel, take 194), and up
 // to which it takes a call's only rows (8 tokens of 32 / 8 heads of 128 over 8192, 32
 // rows: 28.7 us, wide 27.3; over 1000: 15.6 and 16.5; 16 tokens, 64 rows: 51.8 and 32.7).
 constexpr int ATT_NARROW_MOST = 16, ATT_NARROW_ALONE = 32;
@@ -88,11 +90,13 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
 // (chunks of up to 512 tokens over 4096, 16 heads of 64: 82 us, 103 as two launches;
 // of 256 over a window of 1024, 32 / 8 heads of 128: 42 and 46).  The wide form alone
 // would make single tokens beside one chunk three times as slow (64 sequences of
-// 16384 tokens: 743 us, narrow 259).
+// 16384 tokens: 743 us, narrow 261).
 AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
     AttnPlan      p = {};
     const int64_t G = Hq / Hkv, keys = max_pages * page;
-    const bool    few = Tq <= B || Tq * G <= ATT_NARROW_ALONE; // single tokens, or a few rows
+    // single tokens, or a few rows; no more tokens than sequences may also be one chunk
+    // beside empty ones, which is right here, row tile by row tile, but slow
+    const bool    few = Tq <= B || Tq * G <= ATT_NARROW_ALONE;
     const bool    mix = !few && B > 1 && G <= ATT_NARROW_MOST; // more rows to a token: none is the narrow form's
     if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix);
     if (!few) p.part[1] = attn_wide_part(Tq, B, Hkv, G, D, keys, mix);

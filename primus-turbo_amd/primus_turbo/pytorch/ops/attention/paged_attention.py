@@ -10,7 +10,10 @@ A cache is four tensors that the caller allocates and keeps:
 D is a multiple of 16 up to 256; page_size is free.  A slot, page * page_size +
 offset, names the place of one token.  Lengths, slots and page tables stay on
 the device; nothing here synchronizes, so the calls can be captured in a HIP
-graph and replayed with new lengths, slots and pages written in place.
+graph and replayed with new lengths, slots and pages written in place.  Under
+torch.compile they run between its graphs (fullgraph=True, export and fake
+tensors are refused).  A tensor that needs gradients is refused outside
+torch.no_grad(), caches and scales too.
 """
 
 from __future__ import annotations
@@ -41,10 +44,11 @@ def kv_cache_write(
     """Write the keys and values of new tokens, [T, Hkv, D], into their cache slots, in place.
 
     ``slots``: [T] int32 / int64; a token whose slot is below 0 or past the pool
-    is skipped (padding).  An fp8 cache gets each (token, head) row quantized as
-    ``quantize_fp8(..., ScalingGranularity.ROWWISE, axis=-1)`` does, byte for
-    byte, with its ``scale_inv``; a 16-bit cache gets copies.  ``k`` and ``v``
-    may be slices of a larger tensor (their last dimension is contiguous).
+    is skipped (padding), and no slot may be named twice.  An fp8 cache gets each
+    (token, head) row quantized as ``quantize_fp8(..., ScalingGranularity.ROWWISE,
+    axis=-1)`` does, byte for byte, with its ``scale_inv``; a 16-bit cache gets
+    copies.  ``k`` and ``v`` may be slices of a larger tensor (their last dimension
+    is contiguous).
     """
     kv_cache_write_impl(k, v, k_cache, v_cache, slots, k_scale_inv, v_scale_inv)
 
@@ -105,7 +109,10 @@ def paged_attention(
     (a batch padded to a fixed size); one that sees only keys with logits of -inf
     gets NaN and -inf.  A value scale that is NaN or infinite makes NaN of the
     rows that see its token, of their sums too.
-    Inference only: there is no backward pass.
+
+    The probabilities are rounded to q's type before they multiply the values, and
+    the result once more; everything else is fp32.  Inference only: there is no
+    backward pass.
     """
     out, lse = paged_attention_impl(q, k_cache, v_cache, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv,
                                     softmax_scale, window_size, num_sinks, return_lse)

@@ -42,6 +42,8 @@ def moe_decode(
     quantized; silu(gate) * up * prob is rounded to x's type between the two
     products, everything else is summed in fp32.  Each reached expert's weights
     are read once for every 64 tokens, which makes this the path for small T;
-    for many tokens use moe_permute and grouped_gemm_fp8.  Inference only.
+    for many tokens use moe_permute and grouped_gemm_fp8.  Inference only: a
+    tensor that needs gradients, a weight too, is refused outside torch.no_grad().
+    Under torch.compile the call runs between its graphs.
     """
     return moe_decode_impl(x, w_gate_up, w_down, topk_idx, topk_probs, gate_up_scale_inv, down_scale_inv)
