@@ -570,6 +570,117 @@ int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t 
                         int64_t num_sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
                         pta_stream_t stream);
 
+/* Norms of queries and keys for each head and the rotation by their positions, in
+ * one pass.  A row x (a token's head, D elements):
+ *   n = x * (sum x^2 / D + eps)^(-1/2) * weight     (n = x without a weight: NULL)
+ *   y = n with the pairs (a, b) of its first rot_dim elements turned:
+ *       (a cos - b sin, a sin + b cos), cos and sin [num_positions, rot_dim / 2]
+ *       fp32 at row positions[t]; pairs (i, i + rot_dim / 2), interleaved (2 i, 2 i + 1)
+ * q, k, strides in elements, of one type; outputs [num_tokens, H, D] contiguous.
+ * Weights [D] of any type code.  A token whose position lies outside the tables gets
+ * zeros.  D and rot_dim are even, D <= 256. */
+int pta_qk_norm_rope(const void *q, const void *k, int dtype, int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D,
+                     int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, const float *cos,
+                     const float *sin, int64_t num_positions, int64_t rot_dim, const void *positions, int positions_i64,
+                     const void *q_weight, int q_weight_dtype, const void *k_weight, int k_weight_dtype, float eps,
+                     int interleaved, void *q_out, void *k_out, pta_stream_t stream);
+
+/* Its gradients: q_grad, k_grad [num_tokens, H, D] contiguous, and where they are not
+ * NULL the weights' (of the weights' types; sums over all tokens and heads in fp32, in
+ * an order that the sizes give: no atomics).  Hq or Hkv may be 0.  q, k are not read
+ * where their weight is NULL.  Tokens outside the tables get zeros and add nothing. */
+size_t pta_qk_norm_rope_backward_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D);
+int pta_qk_norm_rope_backward(const void *q_grad_out, const void *k_grad_out, int64_t gq_stride_t, int64_t gq_stride_h,
+                              int64_t gk_stride_t, int64_t gk_stride_h, const void *q, const void *k, int dtype,
+                              int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_stride_t,
+                              int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, const float *cos,
+                              const float *sin, int64_t num_positions, int64_t rot_dim, const void *positions,
+                              int positions_i64, const void *q_weight, int q_weight_dtype, const void *k_weight,
+                              int k_weight_dtype, float eps, int interleaved, void *q_grad, void *k_grad,
+                              void *q_weight_grad, void *k_weight_grad, void *workspace, size_t workspace_bytes,
+                              pta_stream_t stream);
+
+/* The same for new tokens, whose keys and values go into their cache slots as
+ * pta_kv_cache_write puts them there; an fp8 row is quantized from the fp32 key, without
+ * a rounding to dtype between.  dtype: PTA_F16 or PTA_BF16.  A token without a slot gets
+ * its query all the same. */
+int pta_qk_norm_rope_cache_write(const void *q, const void *k, const void *v, int dtype, int64_t num_tokens, int64_t Hq,
+                                 int64_t Hkv, int64_t D, int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t,
+                                 int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, const float *cos,
+                                 const float *sin, int64_t num_positions, int64_t rot_dim, const void *positions,
+                                 int positions_i64, const void *q_weight, int q_weight_dtype, const void *k_weight,
+                                 int k_weight_dtype, float eps, int interleaved, const void *slots, int slots_i64,
+                                 void *k_cache, void *v_cache, int cache_kind, int64_t num_pages, int64_t page_size,
+                                 float *k_scale_inv, float *v_scale_inv, void *q_out, pta_stream_t stream);
+
+/* Copies pages: page dst_pages[i] becomes page src_pages[i] (int32 or int64), in all
+ * num_layers layers of pools [num_layers, num_pages, Hkv, page_size, D], of their scales
+ * and, where it is not NULL, of key_ranges [num_layers, num_pages, Hkv, 2, D] bf16.  A
+ * pair with a page outside the pool is skipped.  Destinations are distinct and none of
+ * them a source of another pair: what such a page holds afterwards is not defined. */
+int pta_kv_cache_copy(void *k_cache, void *v_cache, int cache_kind, int64_t num_layers, int64_t num_pages, int64_t Hkv,
+                      int64_t page_size, int64_t D, float *k_scale_inv, float *v_scale_inv, void *key_ranges,
+                      const void *src_pages, const void *dst_pages, int pages_i64, int64_t num_pairs,
+                      pta_stream_t stream);
+
+/* New sequences that go on from others.  New sequence i has the tokens of sequence
+ * parents[i] (NULL: of sequence i).  Pages that it fills are shared.  A last page that
+ * is partly filled belongs to the first new sequence that ends in it (to none if another
+ * one fills it); the others get copies.  Every new sequence gets pages for `reserve`
+ * further tokens, as far as max_pages reach.  Copies and fresh pages are the lowest
+ * pages that no new sequence has, taken in the sequences' order; where they run out a
+ * sequence gets length -1 and no pages.  Other sequences' pages are free afterwards,
+ * and so are pages past a sequence's length.  compact: the new sequences' pages, n of
+ * them, move to pages below n.
+ *   new_page_table [num_new_seqs, max_pages], -1 behind a sequence's pages
+ *   new_seq_lens   [num_new_seqs]: its parent's; 0 for a parent that does not exist
+ * Entries of page_table outside the pool stay as they are.  The old table is left as it
+ * is; the new ones must not overlap it. */
+size_t pta_kv_cache_fork_workspace_size(int64_t num_new_seqs, int64_t max_pages, int64_t num_pages, int compact);
+int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, int64_t num_layers, int64_t num_pages, int64_t Hkv,
+                      int64_t page_size, int64_t D, float *k_scale_inv, float *v_scale_inv, void *key_ranges,
+                      const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *seq_lens,
+                      int64_t num_seqs, const void *parents, int parents_i64, int64_t num_new_seqs, int64_t reserve,
+                      int compact, int32_t *new_page_table, int32_t *new_seq_lens, void *workspace,
+                      size_t workspace_bytes, pta_stream_t stream);
+
+/* Ranges of the pages in which new tokens lie: key_ranges [num_pages, Hkv, 2, D] bf16 =
+ * each channel's smallest and largest key (fp32: fp8 * scale_inv) among the page's tokens
+ * below the sequence's length, rounded outward; NaN where a key is.  Other pages' ranges
+ * stay.  The arguments are pta_paged_attention's; is_f16: a 16-bit cache is fp16. */
+int pta_kv_page_ranges(const void *k_cache, int cache_kind, int is_f16, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                       int64_t D, const float *k_scale_inv, const int32_t *page_table, int64_t table_stride,
+                       int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs,
+                       void *key_ranges, pta_stream_t stream);
+
+/* The pages through which each token attends, for each cache head: of the pages that it
+ * sees the first num_first, the last num_last (1 at least) and, up to num_selected in
+ * all, those with the largest
+ *   score = sum_d max(0, q_d) hi_d + min(0, q_d) lo_d    summed over the head's queries
+ * (64 bits; NaN counts as +inf; ties to the lower page).
+ *   selected      [num_tokens, Hkv, min(num_selected, max_pages)]: pages of the pool in
+ *                 the sequence's order, -1 behind the last
+ *   selected_lens [num_tokens]: keys of them at or before the token (0: it sees none) */
+size_t pta_select_pages_workspace_size(int64_t num_tokens, int64_t Hkv, int64_t max_pages);
+int pta_select_pages(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t,
+                     int64_t q_stride_h, const void *key_ranges, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                     const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
+                     const int32_t *seq_lens, int64_t num_seqs, int64_t num_selected, int64_t num_first,
+                     int64_t num_last, int32_t *selected, int32_t *selected_lens, void *workspace,
+                     size_t workspace_bytes, pta_stream_t stream);
+
+/* pta_paged_attention over the pages that pta_select_pages takes, without a window. */
+size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
+                                                 int64_t page_size, int64_t num_selected);
+int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t,
+                               int64_t q_stride_h, const void *k_cache, const void *v_cache, int cache_kind,
+                               int64_t num_pages, int64_t page_size, int64_t Hkv, const float *k_scale_inv,
+                               const float *v_scale_inv, const void *key_ranges, const int32_t *page_table,
+                               int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
+                               const int32_t *seq_lens, int64_t num_seqs, int64_t num_selected, int64_t num_first,
+                               int64_t num_last, float softmax_scale, void *out, float *lse, void *workspace,
+                               size_t workspace_bytes, pta_stream_t stream);
+
 /* SwiGLU experts for the few tokens of a decoding step:
  *   y[t] = sum_j topk_probs[t, j] * Wd_e (silu(Wg_e x[t]) * (Wu_e x[t])),  e = topk_idx[t, j]
  * w_gate_up [E, 2 I, H] holds Wg's rows, then Wu's; w_down [E, H, I].  Weights

@@ -1,0 +1,375 @@
+// Pages of a paged key / value cache as wholes: copied, and their books kept on the
+// device: sequences that go on from others share full pages, get copies of the
+// partly filled last one and fresh pages for what comes, the pages of sequences that
+// nobody goes on from are free, and pages in use can be moved to the front.
+//
+// A page is up to five runs of bytes: keys, values, their scales and the keys'
+// ranges, in each of the layers.  Copies are bound by memory: a workgroup moves 16 KB
+// of one run, 4 x 16 bytes a thread in flight.
+#include <algorithm>
+#include <climits>
+
+#include "common.h"
+
+namespace pta {
+namespace {
+
+constexpr int KP_NT = 256, KP_DEPTH = 4, KP_RUNS = 5;
+constexpr int KP_CHUNK = KP_NT * KP_DEPTH * 16; // bytes of a workgroup
+
+struct KPPool {
+    uint8_t *p[KP_RUNS];
+    int64_t  bytes[KP_RUNS];  // of a page
+    int64_t  layer[KP_RUNS];  // to the next layer
+    int      first[KP_RUNS];  // number of its first chunk
+    int      wide[KP_RUNS];   // 16-byte pieces, else 4-byte ones
+    int      runs, chunks, layers;
+    int64_t  pages;
+};
+
+// Chunk c (of layer and run) of page `to` becomes that of page `from`
+__device__ __forceinline__ void kp_copy(const KPPool &a, int64_t from, int64_t to, int layer, int c) {
+    int r = 0;
+#pragma unroll
+    for (int i = 1; i < KP_RUNS; ++i)
+        if (i < a.runs && c >= a.first[i]) r = i;
+    const int64_t at = static_cast<int64_t>(c - a.first[r]) * KP_CHUNK;
+    const int64_t n  = min(a.bytes[r] - at, static_cast<int64_t>(KP_CHUNK));
+    const uint8_t *src = a.p[r] + layer * a.layer[r] + from * a.bytes[r] + at;
+    uint8_t       *dst = a.p[r] + layer * a.layer[r] + to * a.bytes[r] + at;
+    if (a.wide[r]) {
+        uint4 v[KP_DEPTH];
+#pragma unroll
+        for (int i = 0; i < KP_DEPTH; ++i) {
+            const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
+            if (o < n) v[i] = *reinterpret_cast<const uint4 *>(src + o);
+        }
+#pragma unroll
+        for (int i = 0; i < KP_DEPTH; ++i) {
+            const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
+            if (o < n) *reinterpret_cast<uint4 *>(dst + o) = v[i];
+        }
+    } else {
+        for (int64_t o = threadIdx.x * 4; o < n; o += KP_NT * 4)
+            *reinterpret_cast<uint32_t *>(dst + o) = *reinterpret_cast<const uint32_t *>(src + o);
+    }
+}
+
+__device__ __forceinline__ int64_t kp_index(const void *p, int i64, int64_t i) {
+    return i64 ? reinterpret_cast<const int64_t *>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t *>(p)[i]);
+}
+
+__global__ __launch_bounds__(KP_NT) void kp_copy_kernel(KPPool a, const void *src, const void *dst, int i64, int64_t total) {
+    const int per = a.chunks * a.layers;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int64_t pair = w / per;
+        const int     rest = static_cast<int>(w - pair * per), layer = rest / a.chunks;
+        const int64_t s = kp_index(src, i64, pair), d = kp_index(dst, i64, pair);
+        if (s < 0 || s >= a.pages || d < 0 || d >= a.pages || s == d) continue;
+        kp_copy(a, s, d, layer, rest - layer * a.chunks);
+    }
+}
+
+// ---- the books -------------------------------------------------------------------
+struct KFArgs {
+    const int32_t *table;
+    int64_t        table_st;
+    const int32_t *lens;
+    const void    *parents; // null: every sequence goes on from itself
+    int            parents_i64;
+    int            B, N, M, page, P;
+    int64_t        reserve;
+    int            compact;
+    int32_t       *new_table, *new_lens; // [N, M], [N]
+    // workspace
+    int32_t *owner;      // [P] who has the page: N nobody, -1 everybody (it is full), else the sequence whose last page it is
+    int32_t *free_pages; // [P] in rising order, as many as are taken
+    int32_t *moved;      // [P] where pages at or past `bound` go (compact)
+    int32_t *seq;        // [N] place of its first fresh page among the free ones; -1: it came too late
+    int2    *pairs;      // copies: from, to
+    int32_t *count;      // pairs; bound
+};
+
+struct KFSeq {
+    int parent, full, part, has, want; // full pages, 1 for a partly filled one, their sum, pages afterwards
+    int last;                          // page that is partly filled, -1: none of the pool's
+};
+
+__device__ __forceinline__ KFSeq kf_seq(const KFArgs &a, int i) {
+    KFSeq         s = {-1, 0, 0, 0, 0, -1};
+    const int64_t p = a.parents ? kp_index(a.parents, a.parents_i64, i) : i;
+    if (p < 0 || p >= a.B) return s;
+    s.parent        = static_cast<int>(p);
+    const int64_t most = static_cast<int64_t>(a.M) * a.page;
+    const int64_t len  = min(static_cast<int64_t>(max(a.lens[p], 0)), most);
+    s.full = static_cast<int>(len / a.page);
+    s.part = len - static_cast<int64_t>(s.full) * a.page > 0;
+    s.has  = s.full + s.part;
+    s.want = static_cast<int>(min((len + a.reserve + a.page - 1) / a.page, static_cast<int64_t>(a.M)));
+    if (s.part) {
+        const int u = a.table[s.parent * a.table_st + s.full];
+        s.last      = u >= 0 && u < a.P ? u : -1;
+    }
+    return s;
+}
+
+__global__ __launch_bounds__(KP_NT) void kf_init_kernel(KFArgs a) {
+    for (int u = blockIdx.x * KP_NT + threadIdx.x; u < a.P; u += gridDim.x * KP_NT) a.owner[u] = a.N;
+}
+
+__global__ __launch_bounds__(KP_NT) void kf_mark_kernel(KFArgs a) {
+    const int   i = blockIdx.x;
+    const KFSeq s = kf_seq(a, i);
+    for (int j = threadIdx.x; j < s.has; j += KP_NT) {
+        const int u = a.table[s.parent * a.table_st + j];
+        if (u >= 0 && u < a.P) atomicMin(&a.owner[u], j < s.full ? -1 : i);
+    }
+}
+
+constexpr int KF_NT = 1024;
+
+// exclusive sums over the workgroup's threads, and the totals
+__device__ __forceinline__ int2 kf_scan(int2 v, int2 *tmp, int2 &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int2      x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int ax = __shfl_up(x.x, o), ay = __shfl_up(x.y, o);
+        if (lane >= o) {
+            x.x += ax;
+            x.y += ay;
+        }
+    }
+    __syncthreads();
+    if (lane == 63) tmp[wave] = x;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
+    total       = make_int2(0, 0);
+    for (int w = 0; w < KF_NT / 64; ++w) {
+        if (w < wave) {
+            before.x += tmp[w].x;
+            before.y += tmp[w].y;
+        }
+        total.x += tmp[w].x;
+        total.y += tmp[w].y;
+    }
+    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+}
+
+// Fresh pages of a sequence (x), and whether one of them is a copy (y)
+__device__ __forceinline__ int2 kf_fresh(const KFArgs &a, int i, const KFSeq &s) {
+    const int copy = s.last >= 0 && a.owner[s.last] != i;
+    return make_int2(s.want - s.has + copy, copy);
+}
+
+// One workgroup: a thread has a run of pages, and of sequences
+__global__ __launch_bounds__(KF_NT) void kf_plan_kernel(KFArgs a) {
+    __shared__ int2 tmp[KF_NT / 64];
+    const int tid = threadIdx.x;
+    const int pr = (a.P + KF_NT - 1) / KF_NT, p0 = min(tid * pr, a.P), p1 = min(p0 + pr, a.P);
+    const int nr = (a.N + KF_NT - 1) / KF_NT, n0 = min(tid * nr, a.N), n1 = min(n0 + nr, a.N);
+    int2      v = make_int2(0, 0), used, fresh, total;
+    for (int u = p0; u < p1; ++u) v.x += a.owner[u] < a.N;
+    kf_scan(v, tmp, used);
+    v = make_int2(0, 0);
+    for (int i = n0; i < n1; ++i) {
+        const int2 f = kf_fresh(a, i, kf_seq(a, i));
+        v.x += f.x;
+        v.y += f.y;
+    }
+    int2      at    = kf_scan(v, tmp, fresh);
+    const int nfree = a.P - used.x;
+    // pages at or past `bound` move to the first free ones
+    const int bound = a.compact ? used.x + min(fresh.x, nfree) : a.P;
+    v               = make_int2(0, 0);
+    for (int u = p0; u < p1; ++u) {
+        if (a.owner[u] >= a.N) ++v.x;
+        else if (u >= bound) ++v.y;
+    }
+    const int2 rank = kf_scan(v, tmp, total);
+    const int  moves = total.y, taken = moves + min(fresh.x, nfree);
+    for (int u = p0, f = rank.x; u < p1 && f < taken; ++u)
+        if (a.owner[u] >= a.N) a.free_pages[f++] = u;
+    __syncthreads(); // the free pages are in place
+    if (moves > 0)
+        for (int u = max(p0, bound), m = rank.y; u < p1; ++u)
+            if (a.owner[u] < a.N) {
+                const int to = a.free_pages[m];
+                a.moved[u]   = to;
+                a.pairs[m++] = make_int2(u, to);
+            }
+    for (int i = n0; i < n1; ++i) {
+        const KFSeq s = kf_seq(a, i);
+        const int2  f = kf_fresh(a, i, s);
+        // sequences take their pages in order; those that come too late get none
+        const bool none = f.x > 0 && at.x + f.x > nfree;
+        a.seq[i]        = none ? -1 : moves + at.x;
+        if (f.y) a.pairs[moves + at.y] = none ? make_int2(-1, -1) : make_int2(s.last, a.free_pages[moves + at.x]);
+        at.x += f.x;
+        at.y += f.y;
+    }
+    if (tid == 0) {
+        a.count[0] = moves + fresh.y;
+        a.count[1] = bound;
+    }
+}
+
+// The first N workgroups write the sequences' rows, the others copy pages
+__global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) {
+    const int i = blockIdx.x;
+    if (i < a.N) {
+        const KFSeq s = kf_seq(a, i);
+        const int   place = a.seq[i], bound = a.count[1];
+        const int   copy = s.last >= 0 && a.owner[s.last] != i;
+        for (int j = threadIdx.x; j < a.M; j += KP_NT) {
+            int u = -1;
+            if (place >= 0 && j < s.want) {
+                if (j < s.has - copy) {
+                    u = a.table[s.parent * a.table_st + j];
+                    if (u >= bound && u < a.P) u = a.moved[u];
+                } else {
+                    u = a.free_pages[place + j - (s.has - copy)];
+                }
+            }
+            a.new_table[static_cast<int64_t>(i) * a.M + j] = u;
+        }
+        if (threadIdx.x == 0) a.new_lens[i] = place < 0 ? -1 : s.parent < 0 ? 0 : a.lens[s.parent];
+        return;
+    }
+    const int     per   = pool.chunks * pool.layers;
+    const int64_t total = static_cast<int64_t>(a.count[0]) * per;
+    for (int64_t w = i - a.N; w < total; w += gridDim.x - a.N) {
+        const int64_t pair = w / per;
+        const int     rest = static_cast<int>(w - pair * per), layer = rest / pool.chunks;
+        const int2    p = a.pairs[pair];
+        if (p.x >= 0) kp_copy(pool, p.x, p.y, layer, rest - layer * pool.chunks);
+    }
+}
+
+int kp_pool(KPPool &a, void *k_cache, void *v_cache, int kind, int64_t layers, int64_t num_pages, int64_t Hkv, int64_t page_size, int64_t D,
+            float *k_scale, float *v_scale, void *ranges) {
+    PTA_CHECK_ARG(kind == PTA_E4M3 || kind == PTA_E5M2 || kind == PTA_CACHE_16BIT, "unknown cache kind %d", kind);
+    PTA_CHECK_ARG(layers >= 0 && num_pages >= 0 && page_size > 0 && Hkv > 0, "bad cache sizes");
+    PTA_CHECK_ARG(D >= 16 && D <= 256 && D % 16 == 0, "head_dim must be a multiple of 16 in [16, 256] (got %lld)", static_cast<long long>(D));
+    PTA_CHECK_ARG(page_size <= INT_MAX && Hkv <= INT_MAX && num_pages <= INT_MAX / page_size && num_pages * page_size <= INT_MAX / Hkv,
+                  "the cache has 2^31 rows (pages * page_size * heads) or more");
+    a.layers = static_cast<int>(std::min<int64_t>(layers, INT_MAX));
+    a.pages  = num_pages;
+    if (layers == 0 || num_pages == 0) return PTA_OK;
+    PTA_CHECK_ARG(k_cache && v_cache, "null cache");
+    PTA_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) && aligned16(ranges), "cache pools must be 16-byte aligned");
+    PTA_CHECK_ARG(kind == PTA_CACHE_16BIT || (k_scale && v_scale), "an fp8 cache needs its scales");
+    const bool    fp8 = kind != PTA_CACHE_16BIT;
+    const int64_t data = Hkv * page_size * D * (fp8 ? 1 : 2), scale = Hkv * page_size * 4;
+    void   *const p[KP_RUNS] = {k_cache, v_cache, fp8 ? k_scale : nullptr, fp8 ? v_scale : nullptr, ranges};
+    const int64_t bytes[KP_RUNS] = {data, data, scale, scale, Hkv * D * 4};
+    int64_t       chunks = 0;
+    for (int i = 0; i < KP_RUNS; ++i) {
+        if (p[i] == nullptr) continue;
+        const int r = a.runs++;
+        a.p[r] = static_cast<uint8_t *>(p[i]);
+        a.bytes[r] = bytes[i];
+        a.layer[r] = bytes[i] * num_pages;
+        a.first[r] = static_cast<int>(chunks);
+        a.wide[r]  = aligned16(p[i]) && bytes[i] % 16 == 0;
+        chunks += cdiv(bytes[i], KP_CHUNK);
+    }
+    PTA_CHECK_ARG(layers <= INT_MAX / chunks, "too many layers");
+    a.chunks = static_cast<int>(chunks);
+    return PTA_OK;
+}
+
+// Workgroups of a copy: a CU's share of work many times over, so that they end together
+unsigned kp_blocks(int64_t total) { return static_cast<unsigned>(std::min<int64_t>(total, 64ll * device_cu_count())); }
+
+struct KFPlan {
+    int64_t pairs;
+    size_t  owner, free_pages, moved, seq, count, pair_bytes;
+    size_t  bytes() const { return owner + free_pages + moved + seq + count + pair_bytes; }
+};
+size_t kf_round(int64_t n) { return static_cast<size_t>(cdiv(n, 16) * 16); }
+KFPlan kf_plan(int64_t N, int64_t M, int64_t P, int compact) {
+    KFPlan p     = {};
+    p.pairs      = N + (compact ? std::min(P, N * M) : 0);
+    p.owner      = kf_round(P * 4);
+    p.free_pages = kf_round(P * 4);
+    p.moved      = compact ? kf_round(P * 4) : 0;
+    p.seq        = kf_round(N * 4);
+    p.count      = 16;
+    p.pair_bytes = kf_round(p.pairs * 8);
+    return p;
+}
+
+} // namespace
+} // namespace pta
+
+using namespace pta;
+
+extern "C" int pta_kv_cache_copy(void *k_cache, void *v_cache, int cache_kind, int64_t num_layers, int64_t num_pages, int64_t Hkv,
+                                 int64_t page_size, int64_t D, float *k_scale_inv, float *v_scale_inv, void *key_ranges,
+                                 const void *src_pages, const void *dst_pages, int pages_i64, int64_t num_pairs, pta_stream_t stream) {
+    clear_error();
+    KPPool a = {};
+    if (int rc = kp_pool(a, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    PTA_CHECK_ARG(num_pairs >= 0 && num_pairs <= INT_MAX, "bad number of pages");
+    if (num_pairs == 0 || num_layers == 0 || num_pages == 0) return PTA_OK;
+    PTA_CHECK_ARG(src_pages && dst_pages, "null page list");
+    const int64_t total = num_pairs * a.chunks * a.layers;
+    kp_copy_kernel<<<kp_blocks(total), KP_NT, 0, as_stream(stream)>>>(a, src_pages, dst_pages, pages_i64, total);
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
+}
+
+extern "C" size_t pta_kv_cache_fork_workspace_size(int64_t num_new_seqs, int64_t max_pages, int64_t num_pages, int compact) {
+    if (num_new_seqs <= 0 || max_pages < 0 || num_pages < 0) return 0;
+    return kf_plan(num_new_seqs, max_pages, num_pages, compact).bytes();
+}
+
+extern "C" int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, int64_t num_layers, int64_t num_pages, int64_t Hkv,
+                                 int64_t page_size, int64_t D, float *k_scale_inv, float *v_scale_inv, void *key_ranges,
+                                 const int32_t *page_table, int64_t table_stride, int64_t max_pages, const int32_t *seq_lens,
+                                 int64_t num_seqs, const void *parents, int parents_i64, int64_t num_new_seqs, int64_t reserve, int compact,
+                                 int32_t *new_page_table, int32_t *new_seq_lens, void *workspace, size_t workspace_bytes,
+                                 pta_stream_t stream) {
+    clear_error();
+    KPPool pool = {};
+    if (int rc = kp_pool(pool, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    PTA_CHECK_ARG(num_seqs >= 0 && num_new_seqs >= 0 && max_pages >= 0 && reserve >= 0, "bad sizes");
+    PTA_CHECK_ARG(num_seqs < (1 << 24) && num_new_seqs < (1 << 24) && max_pages <= (INT_MAX - 1024) / page_size &&
+                      max_pages <= INT_MAX / 2 / std::max<int64_t>(1, num_new_seqs) - 1,
+                  "page_table has too many entries");
+    PTA_CHECK_ARG(parents || num_new_seqs == num_seqs, "without parents there are as many new sequences as old ones");
+    if (num_new_seqs == 0) return PTA_OK;
+    PTA_CHECK_ARG(new_seq_lens && (max_pages == 0 || new_page_table) && (num_seqs == 0 || (seq_lens && (max_pages == 0 || page_table))),
+                  "null pointer");
+    const KFPlan p = kf_plan(num_new_seqs, max_pages, num_pages, compact);
+    PTA_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= p.bytes(), "workspace too small: %zu bytes needed, %zu given",
+                  p.bytes(), workspace_bytes);
+    KFArgs a = {};
+    a.table = page_table; a.table_st = table_stride; a.lens = seq_lens;
+    a.parents = parents; a.parents_i64 = parents_i64;
+    a.B = static_cast<int>(num_seqs); a.N = static_cast<int>(num_new_seqs); a.M = static_cast<int>(max_pages);
+    a.page = static_cast<int>(page_size); a.P = static_cast<int>(num_pages);
+    a.reserve = std::min<int64_t>(reserve, INT_MAX); a.compact = compact != 0;
+    a.new_table = new_page_table; a.new_lens = new_seq_lens;
+    uint8_t *w = static_cast<uint8_t *>(workspace);
+    a.owner      = reinterpret_cast<int32_t *>(w);
+    a.free_pages = reinterpret_cast<int32_t *>(w += p.owner);
+    a.moved      = reinterpret_cast<int32_t *>(w += p.free_pages);
+    a.seq        = reinterpret_cast<int32_t *>(w += p.moved);
+    a.count      = reinterpret_cast<int32_t *>(w += p.seq);
+    a.pairs      = reinterpret_cast<int2 *>(w += p.count);
+    const hipStream_t st = as_stream(stream);
+    if (num_pages > 0) {
+        kf_init_kernel<<<static_cast<unsigned>(std::min<int64_t>(cdiv(num_pages, KP_NT), 4 * device_cu_count())), KP_NT, 0, st>>>(a);
+        PTA_CHECK_LAUNCH();
+    }
+    kf_mark_kernel<<<static_cast<unsigned>(a.N), KP_NT, 0, st>>>(a);
+    PTA_CHECK_LAUNCH();
+    kf_plan_kernel<<<1, KF_NT, 0, st>>>(a);
+    PTA_CHECK_LAUNCH();
+    const int64_t total = num_pages > 0 ? p.pairs * pool.chunks * pool.layers : 0;
+    kf_apply_kernel<<<static_cast<unsigned>(a.N) + kp_blocks(total), KP_NT, 0, st>>>(a, pool);
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
+}

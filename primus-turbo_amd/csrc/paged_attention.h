@@ -52,7 +52,7 @@ struct AttnArgs {
     const uint8_t  *kc, *vc;
     const float    *ks, *vs;
     const int32_t  *table;
-    int64_t         table_st;
+    int64_t         table_st, table_sh; // sequence, cache head (narrow; 0: one row for all heads)
     const int32_t  *cu, *lens;
     uint16_t       *out; // [Tq, Hq, D]
     float          *lse; // [Tq, Hq] or null
@@ -387,9 +387,9 @@ __device__ __forceinline__ int attn_page_of(const AttnArgs &a, int j) {
 }
 // Page of key j, or -1 where there is none: past the keys, or hidden from every
 // row by the window
-__device__ __forceinline__ int attn_key_page(const AttnArgs &a, const AttnItem &it, int j) {
+__device__ __forceinline__ int attn_key_page(const AttnArgs &a, const AttnItem &it, const int32_t *pages, int j) {
     if (j >= it.kend || (j < it.lo && j >= a.sinks)) return -1;
-    return a.table[it.b * a.table_st + attn_page_of(a, j)];
+    return pages[attn_page_of(a, j)];
 }
 // Pool row of key j for head h (row = (page * Hkv + h) * page_size + offset), or
 // -1 where its page is none of the pool's
@@ -529,7 +529,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs &a, int block, AttnWide
 
     int  page_id     = -1;
     auto fetch_pages = [&](int t) PTA_INLINE { // t: the wave's tile
-        page_id = t < it.t1 ? attn_key_page(a, it, attn_key0(it, t, KT) + lane) : -1;
+        page_id = t < it.t1 ? attn_key_page(a, it, a.table + it.b * a.table_st, attn_key0(it, t, KT) + lane) : -1;
     };
     fetch_pages(it.t0 + wave);
     int c = lane & 31, half = lane >> 5;
@@ -1044,6 +1044,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
     const int     tok0 = __builtin_amdgcn_readfirstlane(sq.tok0);
     const int     c = lane & 15, qd = lane >> 4;
     uint16_t     *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
+    const int32_t *pages = a.table + b * a.table_st + h * a.table_sh;
 
     for (int row0 = 0; row0 < n * a.G; row0 += BQ) {
         AttnItem it;
@@ -1069,7 +1070,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
         int      krow[ST], page_id = -1;
         uint64_t hole[ST];
         auto     key = [&](int t) PTA_INLINE { return attn_key0(it, t, KT) + wave * WK + (lane & 31); };
-        auto     fetch_page = [&](int t) PTA_INLINE { page_id = t < it.t1 ? attn_key_page(a, it, key(t)) : -1; };
+        auto     fetch_page = [&](int t) PTA_INLINE { page_id = t < it.t1 ? attn_key_page(a, it, pages, key(t)) : -1; };
         // loads tile t, whose pages were fetched before; keys without a row read row 0
         // and become zeros when they are used
         auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no) PTA_INLINE {

@@ -2,6 +2,7 @@
 // the kernels and how far row tiles are split (paged_attention.h).
 #include <algorithm>
 
+#include "page_select.h"
 #include "paged_attention.h"
 
 namespace pta {
@@ -43,12 +44,13 @@ constexpr int ATT_PADS = 64;
 // Every sequence gets the same number of chunks: two workgroups a CU from all of
 // them, four chunks where sequences may differ in length (64 of up to 16384 tokens:
 // 260 us, 281 with one or two), no more than key tiles.
-AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool mix) {
+// `even`: all are about as long.
+AttnPart attn_narrow_part(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool mix, bool even) {
     AttnPart      p    = {};
     const int64_t fill = cdiv(2 * device_cu_count(), B * Hkv);
     p.rows     = ATT_NARROW_ROWS;
     p.rows_max = mix ? ATT_NARROW_MOST : INT_MAX;
-    p.split    = std::max<int64_t>(1, std::min(std::max<int64_t>(fill, B > 1 ? 4 : 1), cdiv(keys, ATT_NARROW_KEYS)));
+    p.split    = std::max<int64_t>(1, std::min(std::max<int64_t>(fill, B > 1 && !even ? 4 : 1), cdiv(keys, ATT_NARROW_KEYS)));
     if (p.split > 1) {
         // a mixed call's tokens are mostly the wide form's: parts for the rows that a
         // sequence can have here, unless the tokens are fewer
@@ -91,14 +93,14 @@ AttnPart attn_wide_part(int64_t Tq, int64_t B, int64_t Hkv, int64_t G, int64_t D
 // of 256 over a window of 1024, 32 / 8 heads of 128: 42 and 46).  The wide form alone
 // would make single tokens beside one chunk three times as slow (64 sequences of
 // 16384 tokens: 743 us, narrow 261).
-AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page) {
+AttnPlan attn_plan(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page, bool even = false) {
     AttnPlan      p = {};
     const int64_t G = Hq / Hkv, keys = max_pages * page;
     // single tokens, or a few rows; no more tokens than sequences may also be one chunk
     // beside empty ones, which is right here, row tile by row tile, but slow
     const bool    few = Tq <= B || Tq * G <= ATT_NARROW_ALONE;
     const bool    mix = !few && B > 1 && G <= ATT_NARROW_MOST; // more rows to a token: none is the narrow form's
-    if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix);
+    if (few || mix) p.part[0] = attn_narrow_part(Tq, B, Hq, Hkv, D, keys, mix, even);
     if (!few) p.part[1] = attn_wide_part(Tq, B, Hkv, G, D, keys, mix);
     return p;
 }
@@ -114,15 +116,14 @@ extern "C" size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t
     return attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size).bytes();
 }
 
-extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D,
-                                   int64_t q_stride_t, int64_t q_stride_h, const void *k_cache, const void *v_cache,
-                                   int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
-                                   const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table,
-                                   int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
-                                   const int32_t *seq_lens, int64_t num_seqs, float softmax_scale, int64_t window_size,
-                                   int64_t num_sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
-                                   pta_stream_t stream) {
-    clear_error();
+// table_stride_h: of a page table with a row for each cache head, whose sequences are single
+// tokens (so that the narrow form alone runs) of about the same length; 0: one row for all
+static int attn_call(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
+                     const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                     const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table, int64_t table_stride,
+                     int64_t table_stride_h, int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs,
+                     float softmax_scale, int64_t window_size, int64_t num_sinks, void *out, float *lse, void *workspace,
+                     size_t workspace_bytes, pta_stream_t stream) {
     PTA_CHECK_ARG(q_dtype == PTA_BF16 || q_dtype == PTA_F16, "queries must be bfloat16 or float16 (type %d)", q_dtype);
     PTA_CHECK_ARG(cache_kind == PTA_E4M3 || cache_kind == PTA_E5M2 || cache_kind == PTA_CACHE_16BIT,
                   "unknown cache kind %d", cache_kind);
@@ -149,7 +150,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
         PTA_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "cache pools must be 16-byte aligned");
         PTA_CHECK_ARG(cache_kind == PTA_CACHE_16BIT || (k_scale_inv && v_scale_inv), "an fp8 cache needs its scales");
     }
-    const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size);
+    const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, table_stride_h != 0);
     PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
                   "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
     PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
@@ -158,7 +159,7 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
     a.kc = static_cast<const uint8_t *>(k_cache); a.vc = static_cast<const uint8_t *>(v_cache);
     a.ks = k_scale_inv; a.vs = v_scale_inv;
-    a.table = page_table; a.table_st = table_stride;
+    a.table = page_table; a.table_st = table_stride; a.table_sh = table_stride_h;
     a.cu = cu_seqlens_q; a.lens = seq_lens;
     a.out = static_cast<uint16_t *>(out); a.lse = lse;
     a.B = static_cast<int>(num_seqs); a.Tq = static_cast<int>(num_tokens);
@@ -204,4 +205,71 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
     else attn_launch<PTA_F16>(c, cache_kind, st);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
+}
+
+extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D,
+                                   int64_t q_stride_t, int64_t q_stride_h, const void *k_cache, const void *v_cache,
+                                   int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                                   const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table,
+                                   int64_t table_stride, int64_t max_pages, const int32_t *cu_seqlens_q,
+                                   const int32_t *seq_lens, int64_t num_seqs, float softmax_scale, int64_t window_size,
+                                   int64_t num_sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                   pta_stream_t stream) {
+    clear_error();
+    return attn_call(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size, Hkv,
+                     k_scale_inv, v_scale_inv, page_table, table_stride, 0, max_pages, cu_seqlens_q, seq_lens, num_seqs, softmax_scale,
+                     window_size, num_sinks, out, lse, workspace, workspace_bytes, stream);
+}
+
+// The workspace of attention through selected pages: their numbers, how many keys of them
+// each token sees, 0, 1, 2, ... for its tokens as sequences, then what the choice and
+// (over the same bytes: it begins when the choice has ended) the attention need.
+namespace {
+struct SparsePlan {
+    int64_t K;
+    size_t  sel, lens, cu, rest;
+    size_t  bytes() const { return sel + lens + cu + rest; }
+};
+SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page, int64_t take) {
+    SparsePlan p = {};
+    p.K    = std::min(take, max_pages);
+    p.sel  = round256(T * Hkv * p.K * 4);
+    p.lens = round256(T * 4);
+    p.cu   = round256((T + 1) * 4);
+    p.rest = std::max(pta::ps_workspace(T, Hkv, max_pages), attn_plan(T, T, Hq, Hkv, D, p.K, page, true).bytes());
+    return p;
+}
+} // namespace
+
+extern "C" size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
+                                                            int64_t page_size, int64_t num_selected) {
+    if (num_tokens <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_pages < 0 || page_size <= 0 || num_selected <= 0) return 0;
+    return sparse_plan(num_tokens, Hq, Hkv, D, max_pages, page_size, num_selected).bytes();
+}
+
+extern "C" int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t,
+                                          int64_t q_stride_h, const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages,
+                                          int64_t page_size, int64_t Hkv, const float *k_scale_inv, const float *v_scale_inv,
+                                          const void *key_ranges, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                                          const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs, int64_t num_selected,
+                                          int64_t num_first, int64_t num_last, float softmax_scale, void *out, float *lse,
+                                          void *workspace, size_t workspace_bytes, pta_stream_t stream) {
+    clear_error();
+    if (int rc = ps_check(num_tokens, num_seqs, Hq, Hkv, D, num_pages, page_size, max_pages, num_selected, num_first, num_last)) return rc;
+    PTA_CHECK_ARG(softmax_scale > 0.0f && softmax_scale - softmax_scale == 0.0f, "softmax_scale must be positive and finite");
+    if (num_tokens == 0) return PTA_OK;
+    const SparsePlan p = sparse_plan(num_tokens, Hq, Hkv, D, max_pages, page_size, num_selected);
+    PTA_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= p.bytes(), "workspace too small: %zu bytes needed, %zu given",
+                  p.bytes(), workspace_bytes);
+    uint8_t *w    = static_cast<uint8_t *>(workspace);
+    int32_t *sel  = reinterpret_cast<int32_t *>(w), *lens = reinterpret_cast<int32_t *>(w + p.sel);
+    int32_t *cu   = reinterpret_cast<int32_t *>(w + p.sel + p.lens);
+    uint8_t *rest = w + p.sel + p.lens + p.cu;
+    if (int rc = ps_select(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, key_ranges, num_pages, page_size, Hkv, page_table,
+                           table_stride, max_pages, cu_seqlens_q, seq_lens, num_seqs, num_selected, num_first, num_last, sel, lens, cu,
+                           rest, as_stream(stream)))
+        return rc;
+    return attn_call(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size, Hkv,
+                     k_scale_inv, v_scale_inv, sel, Hkv * p.K, std::max<int64_t>(p.K, 1), p.K, cu, lens, num_tokens, softmax_scale, 0, 0,
+                     out, lse, rest, p.rest, stream);
 }

@@ -1,0 +1,754 @@
+// Norms of queries and keys for each head and the rotation by their positions,
+// in one pass; its backward pass; and the form that puts new tokens' keys and
+// values into the paged cache at once.
+//
+// A row x is the D values of one token and head, w its head's weights, p the
+// token's position:
+//
+//   r = (sum x^2 / D + eps)^(-1/2),   n = x r w       (without weights: n = x)
+//   y_a = n_a cos - n_b sin,  y_b = n_a sin + n_b cos  for the pairs (a, b) of the
+//         first R elements, cos and sin of row p of the tables; y = n beyond
+//
+// and with the gradient g of y, h = x r, g' = g turned by -angle:
+//
+//   dw = sum over rows g' h,   dx = r (g' w - h sum(g' w h) / D)
+//
+// A group of LPR lanes has a row; a lane has both elements of its pairs, so the
+// rotation stays in the lane and the sums take log2(LPR) DPP steps.  Where the
+// sizes allow, that is 8 elements of either half, 16 bytes each.  A lane takes HU
+// heads of one token: their loads are in flight together, and the token's angles
+// and the weights are read once for them.
+//
+// All of it is fp32 between the loads and the one rounding of what is stored.
+#include <algorithm>
+#include <climits>
+
+#include "common.h"
+
+namespace pta {
+namespace {
+
+constexpr int QR_NT = 256;
+
+struct QRArgs {
+    const void    *x[3];         // queries, keys, values (cache write)
+    int64_t        xt[3], xh[3]; // element strides: token, head
+    const void    *g[2];         // gradients of the outputs
+    int64_t        gt[2], gh[2];
+    void          *y[2];         // outputs, or gradients of the inputs: [T, H, D]
+    const void    *w[2];         // weights or null
+    int            w_dt[2];
+    float         *part[2];      // backward: [blocks, D] sums for the weights' gradients, or null
+    int            H[3], chunks[3]; // heads; groups of HU heads
+    const float   *cos, *sin;    // [positions, half]
+    const void    *pos;
+    int            pos_i64;
+    int64_t        positions;
+    uint32_t       T;
+    int            D, half, interleaved;
+    float          eps, inv_d;
+    uint32_t       blocks[2];    // backward: workgroups of the queries, of the keys
+    uint8_t       *cache[2];
+    float         *scale[2];
+    const void    *slots;
+    int            slots_i64;
+    uint32_t       page, nslots;
+};
+
+// ---- V elements of a type ----------------------------------------------------
+template <int DT> constexpr int qr_bytes() { return InTraits<DT>::bytes; }
+
+template <int DT, int V> struct QRRaw {
+    alignas(V * qr_bytes<DT>() < 16 ? V * qr_bytes<DT>() : 16) uint8_t b[V * qr_bytes<DT>()];
+};
+template <int DT, int V> __device__ __forceinline__ QRRaw<DT, V> qr_load(const void *base, int64_t i) {
+    return *reinterpret_cast<const QRRaw<DT, V> *>(reinterpret_cast<const uint8_t *>(base) + i * qr_bytes<DT>());
+}
+template <int DT, int V> __device__ __forceinline__ void qr_values(const QRRaw<DT, V> &r, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (DT == PTA_F32) {
+            __builtin_memcpy(&v[i], r.b + 4 * i, 4);
+        } else {
+            uint16_t s;
+            __builtin_memcpy(&s, r.b + 2 * i, 2);
+            v[i] = DT == PTA_BF16 ? bf16_bits_to_f32(s) : f16_bits_to_f32(s);
+        }
+    }
+}
+template <int DT, int V> __device__ __forceinline__ QRRaw<DT, V> qr_round(const float (&v)[V]) {
+    QRRaw<DT, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (DT == PTA_F32) {
+            __builtin_memcpy(r.b + 4 * i, &v[i], 4);
+        } else if constexpr (DT == PTA_BF16) {
+            const __bf16 s = static_cast<__bf16>(v[i]);
+            __builtin_memcpy(r.b + 2 * i, &s, 2);
+        } else {
+            const _Float16 s = static_cast<_Float16>(v[i]);
+            __builtin_memcpy(r.b + 2 * i, &s, 2);
+        }
+    }
+    return r;
+}
+template <int DT, int V> __device__ __forceinline__ void qr_store(void *base, int64_t i, const float (&v)[V]) {
+    *reinterpret_cast<QRRaw<DT, V> *>(reinterpret_cast<uint8_t *>(base) + i * qr_bytes<DT>()) = qr_round<DT, V>(v);
+}
+
+// sum and max over groups of LPR lanes (4, 8 or 16)
+template <int LPR> __device__ __forceinline__ float qr_sum(float v) {
+    v += dpp_f<PTA_DPP_QUAD_XOR1>(v);
+    v += dpp_f<PTA_DPP_QUAD_XOR2>(v);
+    if constexpr (LPR >= 8) v += dpp_f<PTA_DPP_ROW_HALF_MIRROR>(v);
+    if constexpr (LPR >= 16) v += dpp_f<PTA_DPP_ROW_MIRROR>(v);
+    return v;
+}
+template <int LPR> __device__ __forceinline__ float qr_max(float v) {
+    v = fmaxf(v, dpp_f<PTA_DPP_QUAD_XOR1>(v));
+    v = fmaxf(v, dpp_f<PTA_DPP_QUAD_XOR2>(v));
+    if constexpr (LPR >= 8) v = fmaxf(v, dpp_f<PTA_DPP_ROW_HALF_MIRROR>(v));
+    if constexpr (LPR >= 16) v = fmaxf(v, dpp_f<PTA_DPP_ROW_MIRROR>(v));
+    return v;
+}
+
+// ---- a lane's part of a row ----------------------------------------------------
+// P pieces of two runs of V elements at `at`: both halves' (pairs (i, i + half)), or
+// two neighbouring runs (pairs (2 i, 2 i + 1)); beyond the rotated elements any two.
+template <int V, int P> struct QRLane {
+    int   at[P][2];
+    bool  in[P];
+    float c[P][V], s[P][V]; // of pair j; (1, 0) beyond the rotated elements
+};
+
+template <int V, int LPR> constexpr int qr_pieces() { return V == 8 ? 1 : 128 / (V * LPR); }
+
+template <int V, int LPR>
+__device__ __forceinline__ QRLane<V, qr_pieces<V, LPR>()> qr_lane(const QRArgs &a, int l) {
+    constexpr int P = qr_pieces<V, LPR>();
+    QRLane<V, P>  k;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int e = (p * LPR + l) * V; // number of its first pair
+        k.in[p]     = 2 * e < a.D;
+        if (a.interleaved) {
+            k.at[p][0] = 2 * e;
+            k.at[p][1] = 2 * e + V;
+        } else {
+            k.at[p][0] = e < a.half ? e : a.half + e;
+            k.at[p][1] = e < a.half ? e + a.half : a.D / 2 + e;
+        }
+    }
+    return k;
+}
+
+// Angles of a token; false where its position has none.
+template <int V, int LPR, int P> __device__ __forceinline__ bool qr_angles(const QRArgs &a, uint32_t t, int l, QRLane<V, P> &k) {
+    const int64_t pos = a.pos_i64 ? reinterpret_cast<const int64_t *>(a.pos)[t]
+                                  : static_cast<int64_t>(reinterpret_cast<const int32_t *>(a.pos)[t]);
+    const bool    in  = pos >= 0 && pos < a.positions;
+    const float  *c = a.cos + (in ? pos : 0) * a.half, *s = a.sin + (in ? pos : 0) * a.half;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int e = (p * LPR + l) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            k.c[p][j] = 1.0f;
+            k.s[p][j] = 0.0f;
+        }
+        if (!in) continue;
+        if (e + V <= a.half) {
+            typedef float vec __attribute__((ext_vector_type(4)));
+            if constexpr (V % 4 == 0) {
+                // V = 4, 8: half and the tables' alignment allow 16-byte loads
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    const vec x = *reinterpret_cast<const vec *>(c + e + j), y = *reinterpret_cast<const vec *>(s + e + j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        k.c[p][j + i] = x[i];
+                        k.s[p][j + i] = y[i];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    k.c[p][j] = c[e + j];
+                    k.s[p][j] = s[e + j];
+                }
+            }
+        }
+    }
+    return in;
+}
+
+// Turns the lane's pairs by the angles, BACK: by their negatives.  The products are fused
+// here and not left to the compiler, so that every form of the kernels gives the same bits.
+template <bool BACK, int V, int P> __device__ __forceinline__ void qr_turn(const QRArgs &a, const QRLane<V, P> &k, float (&v)[P][2][V]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        if (V > 1 && a.interleaved) {
+            // the 2 V elements are V pairs of neighbours
+            constexpr int W = V > 1 ? V : 2; // V / 2 pairs in each run
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int j = 0; j + 1 < W; j += 2) {
+                    const float c = k.c[p][r * (W / 2) + j / 2], s = BACK ? -k.s[p][r * (W / 2) + j / 2] : k.s[p][r * (W / 2) + j / 2];
+                    const float x = v[p][r][j], y = v[p][r][j + 1];
+                    v[p][r][j]     = fmaf(x, c, -(y * s));
+                    v[p][r][j + 1] = fmaf(x, s, y * c);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float c = k.c[p][j], s = BACK ? -k.s[p][j] : k.s[p][j];
+                const float x = v[p][0][j], y = v[p][1][j];
+                v[p][0][j] = fmaf(x, c, -(y * s));
+                v[p][1][j] = fmaf(x, s, y * c);
+            }
+        }
+    }
+}
+
+template <int V, int P> __device__ __forceinline__ void qr_weights(const QRArgs &a, int which, const QRLane<V, P> &k, float (&w)[P][2][V]) {
+    const void *b = a.w[which];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[p][r][j] = 0.0f;
+            if (b == nullptr || !k.in[p]) continue;
+            // a handful of elements for HU rows; the alignment of a weight is no one's concern
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int e = k.at[p][r] + j;
+                w[p][r][j]  = a.w_dt[which] == PTA_F32    ? load_scalar<PTA_F32>(b, e)
+                              : a.w_dt[which] == PTA_BF16 ? load_scalar<PTA_BF16>(b, e)
+                                                          : load_scalar<PTA_F16>(b, e);
+            }
+        }
+}
+
+template <int DT, int V, int P>
+__device__ __forceinline__ void qr_load_row(const void *x, int64_t at, const QRLane<V, P> &k, QRRaw<DT, V> (&raw)[P][2]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+            if (k.in[p]) raw[p][r] = qr_load<DT, V>(x, at + k.at[p][r]);
+}
+template <int DT, int V, int P>
+__device__ __forceinline__ void qr_row(const QRLane<V, P> &k, const QRRaw<DT, V> (&raw)[P][2], float (&v)[P][2][V]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            qr_values<DT, V>(raw[p][r], v[p][r]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[p][r][j] = k.in[p] ? v[p][r][j] : 0.0f;
+        }
+}
+
+// 1 / rms of a row
+template <int LPR, int V, int P> __device__ __forceinline__ float qr_rsqrt(const QRArgs &a, const float (&v)[P][2][V]) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) ss = fmaf(v[p][r][j], v[p][r][j], ss);
+    return rsqrtf(fmaf(qr_sum<LPR>(ss), a.inv_d, a.eps));
+}
+
+// ---- forward, and cache write ------------------------------------------------
+// KIND: -1 queries and keys to y; a cache kind: queries to y, keys and values to their slots
+template <int KIND, int DT, int V, int P, int LPR>
+__device__ __forceinline__ void qr_put(const QRArgs &a, int which, int64_t row, int l, const QRLane<V, P> &k, const float (&v)[P][2][V]) {
+    if constexpr (KIND == PTA_CACHE_16BIT) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (k.in[p] && row >= 0) qr_store<DT, V>(a.cache[which], row * a.D + k.at[p][r], v[p][r]);
+    } else {
+        // ROWWISE quantization of the fp32 values, as kv_cache_write's of the rounded ones
+        float m = 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(__builtin_canonicalizef(v[p][r][j])));
+        const float sc = scale_from_amax<KIND>(qr_max<LPR>(m), 1e-12f);
+        if (row < 0) return;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (!k.in[p]) continue;
+                uint8_t *y = a.cache[which] + row * a.D + k.at[p][r];
+                if constexpr (V % 4 == 0) {
+#pragma unroll
+                    for (int j = 0; j < V; j += 8) {
+                        if constexpr (V == 8) *reinterpret_cast<uint2 *>(y) = make_uint2(quant4<KIND>(&v[p][r][0], sc), quant4<KIND>(&v[p][r][4], sc));
+                        else *reinterpret_cast<uint32_t *>(y) = quant4<KIND>(&v[p][r][0], sc);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[j] = cvt1_fp8<KIND>(qclamp<KIND>(v[p][r][j], sc));
+                }
+            }
+        if (l == 0) a.scale[which][row] = 1.0f / sc;
+    }
+}
+
+template <int KIND, int DT, int V, int LPR, int HU> __global__ __launch_bounds__(QR_NT) void qr_forward_kernel(QRArgs a) {
+    constexpr int  P    = qr_pieces<V, LPR>();
+    const int      l    = threadIdx.x % LPR;
+    const uint32_t item = blockIdx.x * (QR_NT / LPR) + threadIdx.x / LPR;
+    const uint32_t per  = a.chunks[0] + a.chunks[1] + (KIND >= 0 ? a.chunks[2] : 0);
+    const uint32_t t    = item / per;
+    if (t >= a.T) return;
+    int which = 0, c = static_cast<int>(item - t * per);
+    if (c >= a.chunks[0]) {
+        c -= a.chunks[0];
+        which = 1;
+        if (KIND >= 0 && c >= a.chunks[1]) {
+            c -= a.chunks[1];
+            which = 2;
+        }
+    }
+    const int     h0 = c * HU, H = a.H[which];
+    QRLane<V, P>  k = qr_lane<V, LPR>(a, l);
+    QRRaw<DT, V>  raw[HU][P][2];
+#pragma unroll
+    for (int u = 0; u < HU; ++u)
+        qr_load_row<DT, V, P>(a.x[which], static_cast<int64_t>(t) * a.xt[which] + min(h0 + u, H - 1) * a.xh[which], k, raw[u]);
+    int64_t row0 = 0, row_step = 0; // pool row of head 0 and of the next head
+    if (KIND >= 0 && which > 0) {
+        const int64_t s = a.slots_i64 ? reinterpret_cast<const int64_t *>(a.slots)[t]
+                                      : static_cast<int64_t>(reinterpret_cast<const int32_t *>(a.slots)[t]);
+        if (s < 0 || s >= a.nslots) return; // all lanes of the group
+        const uint32_t pg = static_cast<uint32_t>(s) / a.page;
+        row0     = static_cast<int64_t>(pg) * H * a.page + (static_cast<uint32_t>(s) - pg * a.page);
+        row_step = a.page;
+    }
+    if (KIND >= 0 && which == 2) {
+#pragma unroll
+        for (int u = 0; u < HU; ++u) {
+            if (h0 + u >= H) break;
+            float v[P][2][V];
+            qr_row<DT, V, P>(k, raw[u], v);
+            qr_put<KIND, DT, V, P, LPR>(a, 1, row0 + (h0 + u) * row_step, l, k, v);
+        }
+        return;
+    }
+    float      w[P][2][V];
+    const bool in = qr_angles<V, LPR, P>(a, t, l, k), norm = a.w[which] != nullptr;
+    qr_weights<V, P>(a, which, k, w);
+#pragma unroll
+    for (int u = 0; u < HU; ++u) {
+        if (h0 + u >= H) break;
+        float v[P][2][V];
+        qr_row<DT, V, P>(k, raw[u], v);
+        if (norm) {
+            const float r = qr_rsqrt<LPR, V, P>(a, v);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[p][i][j] = v[p][i][j] * r * w[p][i][j];
+        }
+        qr_turn<false, V, P>(a, k, v);
+        if (!in) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[p][i][j] = 0.0f;
+        }
+        if (KIND >= 0 && which == 1) {
+            qr_put<KIND < 0 ? 0 : KIND, DT, V, P, LPR>(a, 0, row0 + (h0 + u) * row_step, l, k, v);
+        } else {
+            const int64_t at = (static_cast<int64_t>(t) * H + h0 + u) * a.D;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (k.in[p]) qr_store<DT, V>(a.y[which], at + k.at[p][i], v[p][i]);
+        }
+    }
+}
+
+// ---- backward ------------------------------------------------------------------
+// The first blocks[0] workgroups take the queries, the others the keys, each every
+// blocks[]-th run of items, so that the weights' gradients are sums in registers,
+// then in LDS, then one row of `part` a workgroup: no atomics, the same bits every time.
+template <int DT, int V, int LPR, int HU> __global__ __launch_bounds__(QR_NT) void qr_backward_kernel(QRArgs a) {
+    constexpr int  P = qr_pieces<V, LPR>(), GROUPS = QR_NT / LPR, DMAX = 2 * V * P * LPR;
+    __shared__ float sums[GROUPS * DMAX];
+    const int      which = blockIdx.x >= a.blocks[0], grp = threadIdx.x / LPR, l = threadIdx.x % LPR;
+    const uint32_t block = which ? blockIdx.x - a.blocks[0] : blockIdx.x;
+    const uint32_t items = a.T * a.chunks[which], step = a.blocks[which] * GROUPS;
+    const int      H = a.H[which];
+    const bool     norm = a.w[which] != nullptr;
+    QRLane<V, P>   k = qr_lane<V, LPR>(a, l);
+    float          w[P][2][V], dw[P][2][V];
+    qr_weights<V, P>(a, which, k, w);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) dw[p][i][j] = 0.0f;
+    for (uint32_t item = block * GROUPS + grp; item < items; item += step) {
+        const uint32_t t  = item / a.chunks[which];
+        const int      h0 = static_cast<int>(item - t * a.chunks[which]) * HU;
+        QRRaw<DT, V>   rx[HU][P][2], rg[HU][P][2];
+#pragma unroll
+        for (int u = 0; u < HU; ++u) {
+            const int h = min(h0 + u, H - 1);
+            qr_load_row<DT, V, P>(a.g[which], static_cast<int64_t>(t) * a.gt[which] + h * a.gh[which], k, rg[u]);
+            if (norm) qr_load_row<DT, V, P>(a.x[which], static_cast<int64_t>(t) * a.xt[which] + h * a.xh[which], k, rx[u]);
+        }
+        const bool in = qr_angles<V, LPR, P>(a, t, l, k);
+#pragma unroll
+        for (int u = 0; u < HU; ++u) {
+            if (h0 + u >= H) break;
+            float g[P][2][V];
+            qr_row<DT, V, P>(k, rg[u], g);
+            qr_turn<true, V, P>(a, k, g);
+            if (norm) {
+                float v[P][2][V], dot = 0.0f;
+                qr_row<DT, V, P>(k, rx[u], v);
+                const float r = qr_rsqrt<LPR, V, P>(a, v);
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            v[p][i][j] *= r;
+                            if (in) dw[p][i][j] = fmaf(g[p][i][j], v[p][i][j], dw[p][i][j]);
+                            g[p][i][j] *= w[p][i][j];
+                            dot = fmaf(g[p][i][j], v[p][i][j], dot);
+                        }
+                dot = qr_sum<LPR>(dot) * a.inv_d;
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[p][i][j] = r * (g[p][i][j] - v[p][i][j] * dot);
+            }
+            const int64_t at = (static_cast<int64_t>(t) * H + h0 + u) * a.D;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) g[p][i][j] = in ? g[p][i][j] : 0.0f;
+                    if (k.in[p]) qr_store<DT, V>(a.y[which], at + k.at[p][i], g[p][i]);
+                }
+        }
+    }
+    if (a.part[which] == nullptr) return;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (k.in[p])
+#pragma unroll
+                for (int j = 0; j < V; ++j) sums[grp * DMAX + k.at[p][i] + j] = dw[p][i][j];
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += QR_NT) {
+        float s = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < GROUPS; ++i) s += sums[i * DMAX + d];
+        a.part[which][static_cast<int64_t>(block) * a.D + d] = s;
+    }
+}
+
+// Sums the workgroups' rows: 32 columns by 32 runs of rows a workgroup.
+struct QRSums {
+    const float *part[2];
+    void        *dw[2];
+    int          dt[2];
+    int          rows[2], D;
+};
+__global__ __launch_bounds__(1024) void qr_sums_kernel(QRSums a) {
+    __shared__ float s[32][33];
+    const int which = blockIdx.y, c = threadIdx.x % 32, run = threadIdx.x / 32, d = blockIdx.x * 32 + c;
+    if (a.dw[which] == nullptr) return;
+    float acc = 0.0f;
+    if (d < a.D) {
+#pragma unroll 8
+        for (int i = run; i < a.rows[which]; i += 32) acc += a.part[which][static_cast<int64_t>(i) * a.D + d];
+    }
+    s[run][c] = acc;
+    __syncthreads();
+    if (run != 0 || d >= a.D) return;
+    for (int i = 1; i < 32; ++i) acc += s[i][c];
+    if (a.dt[which] == PTA_F32) reinterpret_cast<float *>(a.dw[which])[d] = acc;
+    else reinterpret_cast<uint16_t *>(a.dw[which])[d] = a.dt[which] == PTA_BF16 ? f32_to_bf16_bits(acc) : f32_to_f16_bits(acc);
+}
+
+// ---- host ----------------------------------------------------------------------
+// Heads of a lane where there are enough rows to fill the chip without
+constexpr int QR_HEADS = 4, QR_HEADS_BACK = 2;
+
+struct QRShape {
+    int V, lpr; // run of elements, lanes of a row
+};
+
+bool qr_fits(const void *p, int64_t st, int64_t sh, int V, int bytes) {
+    return reinterpret_cast<uintptr_t>(p) % std::min(V * bytes, 16) == 0 && st * bytes % std::min(V * bytes, 16) == 0 &&
+           sh * bytes % std::min(V * bytes, 16) == 0;
+}
+
+int qr_check(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot, int64_t positions, float eps) {
+    PTA_CHECK_ARG(dtype == PTA_F32 || dtype == PTA_F16 || dtype == PTA_BF16, "unknown type %d", dtype);
+    PTA_CHECK_ARG(T >= 0 && Hq >= 0 && Hkv >= 0 && positions >= 0, "bad sizes");
+    PTA_CHECK_ARG(D >= 2 && D <= 256 && D % 2 == 0, "head_dim must be even and at most 256 (got %lld)", static_cast<long long>(D));
+    PTA_CHECK_ARG(rot >= 2 && rot <= D && rot % 2 == 0, "rotated elements must be even and at most head_dim (got %lld)",
+                  static_cast<long long>(rot));
+    PTA_CHECK_ARG(Hq <= INT_MAX / 4 && Hkv <= INT_MAX / 4 && T <= (INT_MAX - 1024) / std::max<int64_t>(1, Hq + 2 * Hkv),
+                  "too many rows for one call");
+    PTA_CHECK_ARG(eps >= 0.0f && eps - eps == 0.0f, "eps must be finite and not negative");
+    return PTA_OK;
+}
+
+// Longest run that the sizes and every tensor's alignment allow
+template <class Ok> QRShape qr_shape(int64_t D, int64_t half, const float *cos, const float *sin, Ok ok) {
+    for (int V : {8, 4, 2}) {
+        if (D % (2 * V) || half % V || !ok(V)) continue;
+        if (V >= 4 && (half % 4 || !aligned16(cos) || !aligned16(sin))) continue;
+        return {V, V < 8 ? 16 : D <= 64 ? 4 : D <= 128 ? 8 : 16};
+    }
+    return {1, 16};
+}
+
+void qr_fill(QRArgs &a, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, const float *cos, const float *sin, int64_t positions,
+             int64_t rot, const void *pos, int pos_i64, const void *wq, int wq_dt, const void *wk, int wk_dt, float eps, int interleaved) {
+    a.T = static_cast<uint32_t>(T);
+    a.H[0] = static_cast<int>(Hq); a.H[1] = a.H[2] = static_cast<int>(Hkv);
+    a.D = static_cast<int>(D); a.half = static_cast<int>(rot / 2); a.interleaved = interleaved;
+    a.cos = cos; a.sin = sin; a.positions = positions; a.pos = pos; a.pos_i64 = pos_i64;
+    a.w[0] = wq; a.w[1] = wk; a.w_dt[0] = wq_dt; a.w_dt[1] = wk_dt;
+    a.eps = eps; a.inv_d = 1.0f / static_cast<float>(D);
+}
+
+bool qr_weight_type(const void *w, int dt) { return w == nullptr || dt == PTA_F32 || dt == PTA_F16 || dt == PTA_BF16; }
+
+#define PTA_QR_SHAPE(S, F)                                                                         \
+    do {                                                                                           \
+        if (S.V == 8 && S.lpr == 4) F(8, 4);                                                       \
+        else if (S.V == 8 && S.lpr == 8) F(8, 8);                                                  \
+        else if (S.V == 8) F(8, 16);                                                               \
+        else if (S.V == 4) F(4, 16);                                                               \
+        else if (S.V == 2) F(2, 16);                                                               \
+        else F(1, 16);                                                                             \
+    } while (0)
+
+template <int KIND, int DT> void qr_forward(QRArgs &a, QRShape s, hipStream_t st) {
+    // QR_HEADS heads a lane once that leaves four workgroups a CU
+    const int64_t rows = static_cast<int64_t>(a.T) * (a.H[0] + a.H[1] + (KIND >= 0 ? a.H[2] : 0));
+    const int     HU   = rows >= static_cast<int64_t>(QR_HEADS) * 4 * device_cu_count() * (QR_NT / s.lpr) && s.V == 8 ? QR_HEADS : 1;
+    for (int i = 0; i < 3; ++i) a.chunks[i] = static_cast<int>(cdiv(a.H[i], HU));
+    const int64_t  items = static_cast<int64_t>(a.T) * (a.chunks[0] + a.chunks[1] + (KIND >= 0 ? a.chunks[2] : 0));
+    const unsigned grid  = static_cast<unsigned>(cdiv(items, QR_NT / s.lpr));
+    if (grid == 0) return;
+#define PTA_QRF(V, LPR)                                                                            \
+    do {                                                                                           \
+        if constexpr (V == 8) {                                                                    \
+            if (HU > 1) qr_forward_kernel<KIND, DT, V, LPR, QR_HEADS><<<grid, QR_NT, 0, st>>>(a);  \
+            else qr_forward_kernel<KIND, DT, V, LPR, 1><<<grid, QR_NT, 0, st>>>(a);                \
+        } else {                                                                                   \
+            qr_forward_kernel<KIND, DT, V, LPR, 1><<<grid, QR_NT, 0, st>>>(a);                     \
+        }                                                                                          \
+    } while (0)
+    PTA_QR_SHAPE(s, PTA_QRF);
+#undef PTA_QRF
+}
+
+// Workgroups of the backward pass for the queries and the keys: at most eight a CU
+// of both, each the same number of runs of items.
+void qr_back_blocks(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t (&blocks)[2]) {
+    const int64_t H[2] = {Hq, Hkv}, most = 8 * device_cu_count();
+    for (int i = 0; i < 2; ++i) {
+        // of the smallest workgroup's rows: the shape goes by alignment, which the size query does not know
+        const int64_t items = T * cdiv(H[i], QR_HEADS_BACK), runs = cdiv(items, QR_NT / 16);
+        const int64_t share = std::max<int64_t>(1, most * H[i] / std::max<int64_t>(1, Hq + Hkv));
+        blocks[i]           = runs == 0 ? 0 : cdiv(runs, cdiv(runs, share));
+    }
+}
+
+template <int DT> void qr_backward(QRArgs &a, QRShape s, hipStream_t st) {
+    const int HU = s.V == 8 ? QR_HEADS_BACK : 1;
+    for (int i = 0; i < 2; ++i) a.chunks[i] = static_cast<int>(cdiv(a.H[i], HU));
+    const unsigned grid = a.blocks[0] + a.blocks[1];
+    if (grid == 0) return;
+#define PTA_QRB(V, LPR) qr_backward_kernel<DT, V, LPR, V == 8 ? QR_HEADS_BACK : 1><<<grid, QR_NT, 0, st>>>(a)
+    PTA_QR_SHAPE(s, PTA_QRB);
+#undef PTA_QRB
+}
+
+} // namespace
+} // namespace pta
+
+using namespace pta;
+
+extern "C" int pta_qk_norm_rope(const void *q, const void *k, int dtype, int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, const float *cos,
+                                const float *sin, int64_t num_positions, int64_t rot_dim, const void *positions, int positions_i64,
+                                const void *q_weight, int q_weight_dtype, const void *k_weight, int k_weight_dtype, float eps,
+                                int interleaved, void *q_out, void *k_out, pta_stream_t stream) {
+    clear_error();
+    if (int rc = qr_check(dtype, num_tokens, Hq, Hkv, D, rot_dim, num_positions, eps)) return rc;
+    PTA_CHECK_ARG(qr_weight_type(q_weight, q_weight_dtype) && qr_weight_type(k_weight, k_weight_dtype), "unknown weight type");
+    if (num_tokens == 0 || Hq + Hkv == 0) return PTA_OK;
+    PTA_CHECK_ARG((Hq == 0 || (q && q_out)) && (Hkv == 0 || (k && k_out)) && positions && (num_positions == 0 || (cos && sin)), "null pointer");
+    PTA_CHECK_ARG(aligned16(q_out) && aligned16(k_out), "outputs must be 16-byte aligned");
+    QRArgs a = {};
+    qr_fill(a, num_tokens, Hq, Hkv, D, cos, sin, num_positions, rot_dim, positions, positions_i64, q_weight, q_weight_dtype, k_weight,
+            k_weight_dtype, eps, interleaved);
+    a.x[0] = q; a.x[1] = k;
+    a.xt[0] = q_stride_t; a.xt[1] = k_stride_t;
+    a.xh[0] = q_stride_h; a.xh[1] = k_stride_h;
+    a.y[0] = q_out; a.y[1] = k_out;
+    const int     b = dtype == PTA_F32 ? 4 : 2;
+    const QRShape s = qr_shape(D, rot_dim / 2, cos, sin, [&](int V) {
+        return qr_fits(q, q_stride_t, q_stride_h, V, b) && qr_fits(k, k_stride_t, k_stride_h, V, b);
+    });
+    const hipStream_t st = as_stream(stream);
+    if (dtype == PTA_BF16) qr_forward<-1, PTA_BF16>(a, s, st);
+    else if (dtype == PTA_F16) qr_forward<-1, PTA_F16>(a, s, st);
+    else qr_forward<-1, PTA_F32>(a, s, st);
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
+}
+
+extern "C" size_t pta_qk_norm_rope_backward_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D) {
+    if (num_tokens <= 0 || Hq < 0 || Hkv < 0 || D <= 0) return 0;
+    int64_t blocks[2];
+    qr_back_blocks(num_tokens, Hq, Hkv, D, blocks);
+    return static_cast<size_t>((blocks[0] + blocks[1]) * D * 4);
+}
+
+extern "C" int pta_qk_norm_rope_backward(const void *q_grad_out, const void *k_grad_out, int64_t gq_stride_t, int64_t gq_stride_h,
+                                         int64_t gk_stride_t, int64_t gk_stride_h, const void *q, const void *k, int dtype,
+                                         int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
+                                         int64_t k_stride_t, int64_t k_stride_h, const float *cos, const float *sin,
+                                         int64_t num_positions, int64_t rot_dim, const void *positions, int positions_i64,
+                                         const void *q_weight, int q_weight_dtype, const void *k_weight, int k_weight_dtype, float eps,
+                                         int interleaved, void *q_grad, void *k_grad, void *q_weight_grad, void *k_weight_grad,
+                                         void *workspace, size_t workspace_bytes, pta_stream_t stream) {
+    clear_error();
+    if (int rc = qr_check(dtype, num_tokens, Hq, Hkv, D, rot_dim, num_positions, eps)) return rc;
+    PTA_CHECK_ARG(qr_weight_type(q_weight, q_weight_dtype) && qr_weight_type(k_weight, k_weight_dtype), "unknown weight type");
+    PTA_CHECK_ARG((q_weight || !q_weight_grad) && (k_weight || !k_weight_grad), "a weight's gradient without the weight");
+    const bool rows = num_tokens > 0 && Hq + Hkv > 0;
+    PTA_CHECK_ARG(!rows || ((Hq == 0 || (q_grad_out && q_grad && (q || !q_weight))) &&
+                            (Hkv == 0 || (k_grad_out && k_grad && (k || !k_weight))) && positions && (num_positions == 0 || (cos && sin))),
+                  "null pointer");
+    PTA_CHECK_ARG(aligned16(q_grad) && aligned16(k_grad), "outputs must be 16-byte aligned");
+    QRArgs a = {};
+    qr_fill(a, num_tokens, Hq, Hkv, D, cos, sin, num_positions, rot_dim, positions, positions_i64, q_weight, q_weight_dtype, k_weight,
+            k_weight_dtype, eps, interleaved);
+    a.x[0] = q; a.x[1] = k;
+    a.xt[0] = q_stride_t; a.xt[1] = k_stride_t;
+    a.xh[0] = q_stride_h; a.xh[1] = k_stride_h;
+    a.g[0] = q_grad_out; a.g[1] = k_grad_out;
+    a.gt[0] = gq_stride_t; a.gt[1] = gk_stride_t;
+    a.gh[0] = gq_stride_h; a.gh[1] = gk_stride_h;
+    a.y[0] = q_grad; a.y[1] = k_grad;
+    int64_t blocks[2] = {0, 0};
+    if (rows) qr_back_blocks(num_tokens, Hq, Hkv, D, blocks);
+    a.blocks[0] = static_cast<uint32_t>(blocks[0]); a.blocks[1] = static_cast<uint32_t>(blocks[1]);
+    const size_t need = static_cast<size_t>((blocks[0] + blocks[1]) * D * 4);
+    const bool   sums = q_weight_grad || k_weight_grad;
+    PTA_CHECK_ARG(!sums || need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+                  "workspace too small: %zu bytes needed, %zu given", need, workspace_bytes);
+    float *part = static_cast<float *>(workspace);
+    if (q_weight_grad) a.part[0] = part;
+    if (k_weight_grad) a.part[1] = part + blocks[0] * D;
+    const int     b = dtype == PTA_F32 ? 4 : 2;
+    const QRShape s = qr_shape(D, rot_dim / 2, cos, sin, [&](int V) {
+        return (q_weight == nullptr || qr_fits(q, q_stride_t, q_stride_h, V, b)) && (k_weight == nullptr || qr_fits(k, k_stride_t, k_stride_h, V, b)) &&
+               qr_fits(q_grad_out, gq_stride_t, gq_stride_h, V, b) && qr_fits(k_grad_out, gk_stride_t, gk_stride_h, V, b);
+    });
+    const hipStream_t st = as_stream(stream);
+    if (dtype == PTA_BF16) qr_backward<PTA_BF16>(a, s, st);
+    else if (dtype == PTA_F16) qr_backward<PTA_F16>(a, s, st);
+    else qr_backward<PTA_F32>(a, s, st);
+    PTA_CHECK_LAUNCH();
+    if (sums) {
+        QRSums r = {};
+        r.part[0] = a.part[0]; r.part[1] = a.part[1];
+        r.dw[0] = q_weight_grad; r.dw[1] = k_weight_grad;
+        r.dt[0] = q_weight_dtype; r.dt[1] = k_weight_dtype;
+        r.rows[0] = static_cast<int>(blocks[0]); r.rows[1] = static_cast<int>(blocks[1]);
+        r.D = static_cast<int>(D);
+        qr_sums_kernel<<<dim3(static_cast<unsigned>(cdiv(D, 32)), 2), 1024, 0, st>>>(r);
+        PTA_CHECK_LAUNCH();
+    }
+    return PTA_OK;
+}
+
+extern "C" int pta_qk_norm_rope_cache_write(const void *q, const void *k, const void *v, int dtype, int64_t num_tokens, int64_t Hq,
+                                            int64_t Hkv, int64_t D, int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t,
+                                            int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, const float *cos, const float *sin,
+                                            int64_t num_positions, int64_t rot_dim, const void *positions, int positions_i64,
+                                            const void *q_weight, int q_weight_dtype, const void *k_weight, int k_weight_dtype, float eps,
+                                            int interleaved, const void *slots, int slots_i64, void *k_cache, void *v_cache, int cache_kind,
+                                            int64_t num_pages, int64_t page_size, float *k_scale_inv, float *v_scale_inv, void *q_out,
+                                            pta_stream_t stream) {
+    clear_error();
+    PTA_CHECK_ARG(dtype == PTA_F16 || dtype == PTA_BF16, "queries, keys and values must be bfloat16 or float16 (type %d)", dtype);
+    if (int rc = qr_check(dtype, num_tokens, Hq, Hkv, D, rot_dim, num_positions, eps)) return rc;
+    PTA_CHECK_ARG(qr_weight_type(q_weight, q_weight_dtype) && qr_weight_type(k_weight, k_weight_dtype), "unknown weight type");
+    PTA_CHECK_ARG(cache_kind == PTA_E4M3 || cache_kind == PTA_E5M2 || cache_kind == PTA_CACHE_16BIT, "unknown cache kind %d", cache_kind);
+    PTA_CHECK_ARG(D % 16 == 0, "a cache's head_dim must be a multiple of 16 (got %lld)", static_cast<long long>(D));
+    PTA_CHECK_ARG(num_pages >= 0 && page_size > 0 && Hkv > 0 && page_size <= INT_MAX && num_pages <= INT_MAX / page_size &&
+                      num_pages * page_size <= INT_MAX / Hkv,
+                  "the cache has 2^31 rows (pages * page_size * heads) or more");
+    if (num_tokens == 0) return PTA_OK;
+    PTA_CHECK_ARG((Hq == 0 || (q && q_out)) && k && v && slots && positions && (num_positions == 0 || (cos && sin)), "null pointer");
+    PTA_CHECK_ARG(aligned16(q_out), "the output must be 16-byte aligned");
+    if (num_pages > 0) {
+        PTA_CHECK_ARG(k_cache && v_cache, "null cache");
+        PTA_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "cache pools must be 16-byte aligned");
+        PTA_CHECK_ARG(cache_kind == PTA_CACHE_16BIT || (k_scale_inv && v_scale_inv), "an fp8 cache needs its scales");
+    }
+    QRArgs a = {};
+    qr_fill(a, num_tokens, Hq, Hkv, D, cos, sin, num_positions, rot_dim, positions, positions_i64, q_weight, q_weight_dtype, k_weight,
+            k_weight_dtype, eps, interleaved);
+    a.x[0] = q; a.x[1] = k; a.x[2] = v;
+    a.xt[0] = q_stride_t; a.xt[1] = k_stride_t; a.xt[2] = v_stride_t;
+    a.xh[0] = q_stride_h; a.xh[1] = k_stride_h; a.xh[2] = v_stride_h;
+    a.y[0] = q_out;
+    a.cache[0] = static_cast<uint8_t *>(k_cache); a.cache[1] = static_cast<uint8_t *>(v_cache);
+    a.scale[0] = k_scale_inv; a.scale[1] = v_scale_inv;
+    a.slots = slots; a.slots_i64 = slots_i64;
+    a.page = static_cast<uint32_t>(page_size); a.nslots = static_cast<uint32_t>(num_pages * page_size);
+    const QRShape s = qr_shape(D, rot_dim / 2, cos, sin, [&](int V) {
+        return qr_fits(q, q_stride_t, q_stride_h, V, 2) && qr_fits(k, k_stride_t, k_stride_h, V, 2) && qr_fits(v, v_stride_t, v_stride_h, V, 2);
+    });
+    const hipStream_t st = as_stream(stream);
+#define PTA_QRW(KIND)                                                                              \
+    do {                                                                                           \
+        if (dtype == PTA_BF16) qr_forward<KIND, PTA_BF16>(a, s, st);                               \
+        else qr_forward<KIND, PTA_F16>(a, s, st);                                                  \
+    } while (0)
+    if (cache_kind == PTA_E4M3) PTA_QRW(PTA_E4M3);
+    else if (cache_kind == PTA_E5M2) PTA_QRW(PTA_E5M2);
+    else PTA_QRW(PTA_CACHE_16BIT);
+#undef PTA_QRW
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
+}

@@ -28,7 +28,7 @@ MOE_MAP_BOOL, MOE_MAP_I32, MOE_MAP_I64 = 0, 1, 2
 # cache kind of the paged cache entries beside PTA_E4M3 / PTA_E5M2
 CACHE_16BIT = 2
 
-_vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+_vp, _i64, _i32, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/primus_turbo_amd.h
 SIGNATURES = {
@@ -122,6 +122,48 @@ SIGNATURES = {
         [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
          _vp, _i64, ctypes.c_float, _i64, _i64, _vp, _vp, _vp, _sz, _vp],
     ),
+    "pta_qk_norm_rope": (
+        _i32,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i32,
+         _vp, _i32, _f32, _i32, _vp, _vp, _vp],
+    ),
+    "pta_qk_norm_rope_backward_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "pta_qk_norm_rope_backward": (
+        _i32,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
+         _i64, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "pta_qk_norm_rope_cache_write": (
+        _i32,
+        [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
+         _i32, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp],
+    ),
+    "pta_kv_cache_copy": (
+        _i32,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp],
+    ),
+    "pta_kv_cache_fork_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
+    "pta_kv_cache_fork": (
+        _i32,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _i64,
+         _i64, _i32, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "pta_kv_page_ranges": (
+        _i32,
+        [_vp, _i32, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp],
+    ),
+    "pta_select_pages_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "pta_select_pages": (
+        _i32,
+        [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
+         _i64, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "pta_sparse_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "pta_sparse_paged_attention": (
+        _i32,
+        [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64,
+         _vp, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _sz, _vp],
+    ),
     "pta_moe_decode_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "pta_moe_decode": (
         _i32,
@@ -176,6 +218,15 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = load().pta_last_error().decode("utf-8", "replace")
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(device, name: str, *args) -> None:
+    """``call`` with the tensors' device as the current one: kernels are launched there."""
+    if device.type != "cuda" or device.index == _cur_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 # Debug mode (PRIMUS_TURBO_CHECK_WAITS=1): after each call that launched a
