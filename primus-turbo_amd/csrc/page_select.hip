@@ -75,6 +75,10 @@ struct PRArgs {
     int            B, Hkv, D, M, P, page, parts;
 };
 
+// The smaller and the larger of two, NaN if one is
+__device__ __forceinline__ float pr_less(float x, float y) { return x < y || x != x ? x : y; }
+__device__ __forceinline__ float pr_more(float x, float y) { return x > y || x != x ? x : y; }
+
 __device__ __forceinline__ uint16_t pr_outward(float x, bool up) {
     const uint32_t u = __float_as_uint(x);
     if (x != x) return 0x7fc0;
@@ -82,68 +86,68 @@ __device__ __forceinline__ uint16_t pr_outward(float x, bool up) {
     return static_cast<uint16_t>((u >> 16) + away);
 }
 
-// Workgroup = (head, part, sequence), for every parts-th page that holds new tokens: the
-// page's keys, 16 bytes a thread, NL threads a key.
+// Workgroup = (head, part, sequence), for every parts-th page that holds new tokens.  A
+// thread has 4 channels of every GROUPS-th key, NL threads a key.
 template <int KIND, int NL> __global__ __launch_bounds__(PS_NT) void pr_ranges_kernel(PRArgs a) {
-    constexpr int EC = KIND == PTA_E4M3 || KIND == PTA_E5M2 ? 16 : 8, GROUPS = PS_NT / NL;
-    __shared__ float red[2][GROUPS][NL * EC + 1];
-    const int        h = blockIdx.x % a.Hkv, w = blockIdx.x / a.Hkv, part = w % a.parts, b = w / a.parts;
-    const int64_t    fresh = static_cast<int64_t>(a.cu[b + 1]) - a.cu[b];
-    const int        len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), static_cast<int64_t>(a.M) * a.page));
+    constexpr int     GROUPS = PS_NT / NL;
+    constexpr bool    FP8    = KIND == PTA_E4M3 || KIND == PTA_E5M2;
+    __shared__ float4 red[2][GROUPS][NL];
+    const int         h = blockIdx.x % a.Hkv, w = blockIdx.x / a.Hkv, part = w % a.parts, b = w / a.parts;
+    const int64_t     fresh = static_cast<int64_t>(a.cu[b + 1]) - a.cu[b];
+    const int         len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), static_cast<int64_t>(a.M) * a.page));
     if (fresh <= 0 || len == 0) return;
-    const int first = static_cast<int>(max(static_cast<int64_t>(0), len - fresh)) / a.page, l = threadIdx.x % NL, g = threadIdx.x / NL;
+    const int  first = static_cast<int>(max(static_cast<int64_t>(0), len - fresh)) / a.page, l = threadIdx.x % NL, g = threadIdx.x / NL;
+    const bool in = l * 4 < a.D;
     for (int pg = first + part; pg * static_cast<int64_t>(a.page) < len; pg += a.parts) {
         const int u = a.table[b * a.table_st + pg];
         if (u < 0 || u >= a.P) continue;
         const int     n = min(a.page, len - pg * a.page);
         const int64_t row0 = (static_cast<int64_t>(u) * a.Hkv + h) * a.page;
-        float         lo[EC], hi[EC];
+        float         lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < EC; ++e) {
+        for (int e = 0; e < 4; ++e) {
             lo[e] = INFINITY;
             hi[e] = -INFINITY;
         }
-        if (l * EC < a.D)
-#pragma unroll 2
+        if (in)
+#pragma unroll 8
             for (int j = g; j < n; j += GROUPS) {
-                float v[EC];
-                if constexpr (KIND == PTA_E4M3 || KIND == PTA_E5M2) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(a.kc + (row0 + j) * a.D + l * EC);
+                float         v[4];
+                const int64_t at = (row0 + j) * a.D + l * 4;
+                if constexpr (FP8) {
+                    const int   x = *reinterpret_cast<const int *>(a.kc + at);
                     const float sc = a.ks[row0 + j];
-                    const int   ws[4] = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w)};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (KIND == PTA_E4M3) {
-                            v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(ws[i], 0) * sc; v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(ws[i], 1) * sc;
-                            v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(ws[i], 2) * sc; v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(ws[i], 3) * sc;
-                        } else {
-                            v[4 * i] = __builtin_amdgcn_cvt_f32_bf8(ws[i], 0) * sc; v[4 * i + 1] = __builtin_amdgcn_cvt_f32_bf8(ws[i], 1) * sc;
-                            v[4 * i + 2] = __builtin_amdgcn_cvt_f32_bf8(ws[i], 2) * sc; v[4 * i + 3] = __builtin_amdgcn_cvt_f32_bf8(ws[i], 3) * sc;
-                        }
+                    if constexpr (KIND == PTA_E4M3) {
+                        v[0] = __builtin_amdgcn_cvt_f32_fp8(x, 0) * sc; v[1] = __builtin_amdgcn_cvt_f32_fp8(x, 1) * sc;
+                        v[2] = __builtin_amdgcn_cvt_f32_fp8(x, 2) * sc; v[3] = __builtin_amdgcn_cvt_f32_fp8(x, 3) * sc;
+                    } else {
+                        v[0] = __builtin_amdgcn_cvt_f32_bf8(x, 0) * sc; v[1] = __builtin_amdgcn_cvt_f32_bf8(x, 1) * sc;
+                        v[2] = __builtin_amdgcn_cvt_f32_bf8(x, 2) * sc; v[3] = __builtin_amdgcn_cvt_f32_bf8(x, 3) * sc;
                     }
                 } else {
-                    load8<KIND == PTA_CACHE_16BIT ? PTA_BF16 : PTA_F16>(a.kc, (row0 + j) * a.D + l * EC, v);
+                    const uint2 x = *reinterpret_cast<const uint2 *>(a.kc + 2 * at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t y = (e < 2 ? x.x : x.y) >> (16 * (e & 1)) & 0xffffu;
+                        v[e] = KIND == PTA_CACHE_16BIT ? bf16_bits_to_f32(y) : f16_bits_to_f32(y);
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < EC; ++e) {
-                    lo[e] = v[e] < lo[e] || v[e] != v[e] ? v[e] : lo[e];
-                    hi[e] = v[e] > hi[e] || v[e] != v[e] ? v[e] : hi[e];
+                for (int e = 0; e < 4; ++e) {
+                    lo[e] = pr_less(v[e], lo[e]);
+                    hi[e] = pr_more(v[e], hi[e]);
                 }
             }
-#pragma unroll
-        for (int e = 0; e < EC; ++e) {
-            red[0][g][l * EC + e] = lo[e];
-            red[1][g][l * EC + e] = hi[e];
-        }
+        red[0][g][l] = make_float4(lo[0], lo[1], lo[2], lo[3]);
+        red[1][g][l] = make_float4(hi[0], hi[1], hi[2], hi[3]);
         __syncthreads();
         for (int d = threadIdx.x; d < 2 * a.D; d += PS_NT) {
-            const int  c = d < a.D ? d : d - a.D;
-            const bool up = d >= a.D;
-            float      x = red[up][0][c];
-            for (int i = 1; i < GROUPS; ++i) {
-                const float y = red[up][i][c];
-                x = (up ? y > x : y < x) || y != y ? y : x;
-            }
+            const bool   up = d >= a.D;
+            const int    c = up ? d - a.D : d;
+            const float *p = reinterpret_cast<const float *>(&red[up][0][0]) + c;
+            float        x = p[0];
+#pragma unroll 8
+            for (int i = 1; i < GROUPS; ++i) x = up ? pr_more(p[i * NL * 4], x) : pr_less(p[i * NL * 4], x);
             a.ranges[((static_cast<int64_t>(u) * a.Hkv + h) * 2 + up) * a.D + c] = pr_outward(x, up);
         }
         __syncthreads(); // the next page's values come to the same place
@@ -176,7 +180,7 @@ __device__ __forceinline__ uint64_t ps_key(double s) {
 
 // Pages [c per, (c + 1) per) of token t for head h; 8 channels a lane
 template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_kernel(PSArgs a, int per, int parts) {
-    constexpr int  GROUPS = PS_NT / LPR;
+    constexpr int  GROUPS = PS_NT / LPR, PAGES = 4;
     const uint32_t w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, ti = w1 / parts;
     const int      t = a.t0 + static_cast<int>(ti);
     const PSToken  s = ps_token(a.cu, a.lens, a.B, a.T, t, static_cast<int64_t>(a.M) * a.page);
@@ -199,20 +203,36 @@ template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_ker
                 down[e] += v[e] < 0.0f || v[e] != v[e] ? v[e] : 0.0f;
             }
         }
-    uint64_t *out = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
-    for (int j = j0 + g; j < j1; j += GROUPS) {
-        const int u = a.table[s.b * a.table_st + j];
-        double    x = 0.0;
-        if (in && u >= 0 && u < a.P) { // a page outside the pool holds zeros
-            const uint16_t *r = a.ranges + (static_cast<int64_t>(u) * a.Hkv + h) * 2 * a.D + d;
-            float           lo[8], hi[8];
-            load8<PTA_BF16>(r, 0, lo);
-            load8<PTA_BF16>(r + a.D, 0, hi);
+    uint64_t      *out = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
+    const int32_t *row = a.table + s.b * a.table_st;
+    for (int p0 = j0 + g; p0 < j1; p0 += GROUPS * PAGES) {
+        uint4 lo[PAGES], hi[PAGES];
+        bool  there[PAGES];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x = fma(up[e], static_cast<double>(hi[e]), fma(down[e], static_cast<double>(lo[e]), x));
+        for (int i = 0; i < PAGES; ++i) {
+            const int j = p0 + i * GROUPS, u = j < j1 ? row[j] : -1;
+            there[i]    = in && u >= 0 && u < a.P; // a page outside the pool holds zeros
+            const uint16_t *r = a.ranges + (static_cast<int64_t>(there[i] ? u : 0) * a.Hkv + h) * 2 * a.D + (in ? d : 0);
+            lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+            if (there[i]) {
+                lo[i] = *reinterpret_cast<const uint4 *>(r);
+                hi[i] = *reinterpret_cast<const uint4 *>(r + a.D);
+            }
         }
-        x = ps_sum<LPR>(x);
-        if (l == 0) out[j] = j < a.first || own - j < a.last ? ~0ull : ps_key(x);
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i) {
+            const int      j = p0 + i * GROUPS;
+            const uint32_t wl[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, wh[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+            double         x = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t bl = e % 2 ? wl[e / 2] & 0xffff0000u : wl[e / 2] << 16, bh = e % 2 ? wh[e / 2] & 0xffff0000u : wh[e / 2] << 16;
+                x = fma(up[e], static_cast<double>(__uint_as_float(bh)), fma(down[e], static_cast<double>(__uint_as_float(bl)), x));
+            }
+            if (!there[i]) x = 0.0; // also where a query is not finite
+            x = ps_sum<LPR>(x);
+            if (l == 0 && j < j1) out[j] = j < a.first || own - j < a.last ? ~0ull : ps_key(x);
+        }
     }
 }
 
@@ -287,6 +307,7 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
         int total, none, b0, b1;
         all(c, 0, total, none, b0, b1);
         if (total >= take) least = cand;
+        if (total == take) break; // all of these and no others
     }
     // all above the least, and of those equal to it the first ones
     int above = 0, equal = 0, sa, se, ba, be;
@@ -376,9 +397,9 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
             PTA_CHECK_LAUNCH();
         }
         const unsigned grid = static_cast<unsigned>(a.n) * a.Hkv;
-        if (a.M <= 256) ps_choose_kernel<1, 4><<<grid, 64, 0, st>>>(a);
-        else if (a.M <= 1024) ps_choose_kernel<4, 4><<<grid, 256, 0, st>>>(a);
-        else ps_choose_kernel<16, 4><<<grid, 1024, 0, st>>>(a);
+        if (a.M <= 512) ps_choose_kernel<1, 8><<<grid, 64, 0, st>>>(a);
+        else if (a.M <= 2048) ps_choose_kernel<4, 8><<<grid, 256, 0, st>>>(a);
+        else ps_choose_kernel<16, 8><<<grid, 1024, 0, st>>>(a);
         PTA_CHECK_LAUNCH();
     }
     return PTA_OK;
@@ -410,13 +431,11 @@ extern "C" int pta_kv_page_ranges(const void *k_cache, int cache_kind, int is_f1
     a.parts = static_cast<int>(std::min<int64_t>(max_pages, cdiv(4 * device_cu_count(), num_seqs * Hkv)));
     const unsigned    grid = static_cast<unsigned>(num_seqs * Hkv * a.parts);
     const hipStream_t st = as_stream(stream);
-    const int64_t     pieces = cache_kind == PTA_CACHE_16BIT ? D / 8 : D / 16;
 #define PTA_PR(KIND)                                                                               \
     do {                                                                                           \
-        if (pieces <= 4) pr_ranges_kernel<KIND, 4><<<grid, PS_NT, 0, st>>>(a);                     \
-        else if (pieces <= 8) pr_ranges_kernel<KIND, 8><<<grid, PS_NT, 0, st>>>(a);                \
-        else if (pieces <= 16) pr_ranges_kernel<KIND, 16><<<grid, PS_NT, 0, st>>>(a);              \
-        else pr_ranges_kernel<KIND, 32><<<grid, PS_NT, 0, st>>>(a);                                \
+        if (D <= 64) pr_ranges_kernel<KIND, 16><<<grid, PS_NT, 0, st>>>(a);                        \
+        else if (D <= 128) pr_ranges_kernel<KIND, 32><<<grid, PS_NT, 0, st>>>(a);                  \
+        else pr_ranges_kernel<KIND, 64><<<grid, PS_NT, 0, st>>>(a);                                \
     } while (0)
     if (cache_kind == PTA_E4M3) PTA_PR(PTA_E4M3);
     else if (cache_kind == PTA_E5M2) PTA_PR(PTA_E5M2);
