@@ -42,26 +42,44 @@ struct PSArgs {
 };
 
 
-// The token's sequence by bisection, and its place in it; b < 0: it has none.
+// A token's sequence and its place in it; b < 0: it has none.
 struct PSToken {
     int b, pos, len, n, i;
 };
-__device__ __forceinline__ PSToken ps_token(const int32_t *cu, const int32_t *lens, int B, int T, int t, int64_t most) {
-    PSToken s = {-1, -1, 0, 0, 0};
-    int     lo = 0, hi = B; // the last b with cu[b] <= t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (cu[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const int tok0 = min(max(cu[lo], 0), T), end = min(max(cu[lo + 1], tok0), T);
-    if (B <= 0 || t < tok0 || t >= end) return s;
+__device__ __forceinline__ PSToken ps_place(const PSArgs &a, int t, int lo) {
+    PSToken   s = {-1, -1, 0, 0, 0};
+    const int tok0 = min(max(a.cu[lo], 0), a.T), end = min(max(a.cu[lo + 1], tok0), a.T);
+    if (t < tok0 || t >= end) return s;
     s.b   = lo;
     s.n   = end - tok0;
     s.i   = t - tok0;
-    s.len = static_cast<int>(min(static_cast<int64_t>(max(lens[lo], 0)), most));
+    s.len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[lo], 0)), static_cast<int64_t>(a.M) * a.page));
     s.pos = s.len - s.n + s.i;
     return s;
+}
+// The last sequence that begins at or before t, 64 of them looked at together: all lanes
+// of a wave ask for the same token, and get it into scalar registers
+__device__ __forceinline__ PSToken ps_token(const PSArgs &a, int t) {
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, at = lo + lane_id() * step;
+        const int n    = __popcll(__ballot(at < hi && a.cu[min(at, hi - 1)] <= t));
+        lo += max(n - 1, 0) * step;
+        hi = min(lo + step, hi);
+    }
+    PSToken s = ps_place(a, t, __builtin_amdgcn_readfirstlane(lo));
+    for (int *f : {&s.b, &s.pos, &s.len, &s.n, &s.i}) *f = __builtin_amdgcn_readfirstlane(*f);
+    return s;
+}
+// The same by bisection, for lanes with tokens of their own
+__device__ __forceinline__ PSToken ps_token_of_lane(const PSArgs &a, int t) {
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return ps_place(a, t, lo);
 }
 
 // ---- ranges ------------------------------------------------------------------------
@@ -178,31 +196,44 @@ __device__ __forceinline__ uint64_t ps_key(double s) {
     return (u >> 63) ? ~u : u | (1ull << 63);
 }
 
-// Pages [c per, (c + 1) per) of token t for head h; 8 channels a lane
+// A query's channel to the sums of the positive and of the negative parts; to both if it is
+// NaN, which has to reach the score
+__device__ __forceinline__ void ps_add(float v, double &up, double &down) {
+    up += v < 0.0f ? 0.0f : v;
+    down += v > 0.0f ? 0.0f : v;
+}
+template <int QT> __device__ __forceinline__ void ps_channel(const PSArgs &a, int t, int h, int d, double &up, double &down) {
+    const uint16_t *q = a.q + t * a.q_st + static_cast<int64_t>(h) * a.G * a.q_sh + d;
+    up = down = 0.0;
+#pragma unroll 8
+    for (int i = 0; i < a.G; ++i) {
+        const uint32_t x = q[i * a.q_sh];
+        ps_add(QT == PTA_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x), up, down);
+    }
+}
+
+// Few tokens: pages [c per, (c + 1) per) of token t for head h, a page's range to LPR
+// lanes, 8 channels each, four pages of a lane's loads together.  Bound by the chain of
+// reads: the token's place, page numbers, ranges.
 template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_kernel(PSArgs a, int per, int parts) {
     constexpr int  GROUPS = PS_NT / LPR, PAGES = 4;
     const uint32_t w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, ti = w1 / parts;
     const int      t = a.t0 + static_cast<int>(ti);
-    const PSToken  s = ps_token(a.cu, a.lens, a.B, a.T, t, static_cast<int64_t>(a.M) * a.page);
+    const PSToken  s = ps_token(a, t);
     if (s.b < 0 || s.pos < 0) return;
     const int own = s.pos / a.page, n = own + 1, j0 = c * per, j1 = min(j0 + per, n);
     if (j0 >= j1 || n <= a.take) return;
+    __shared__ double sums[2][8 * LPR];
+    if (static_cast<int>(threadIdx.x) < a.D) ps_channel<QT>(a, t, h, threadIdx.x, sums[0][threadIdx.x], sums[1][threadIdx.x]);
+    __syncthreads();
     const int  l = threadIdx.x % LPR, g = threadIdx.x / LPR, d = l * 8;
     const bool in = d < a.D;
     double     up[8], down[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
-    if (in)
-        for (int i = 0; i < a.G; ++i) {
-            float v[8];
-            load8<QT>(a.q, t * a.q_st + (h * a.G + i) * a.q_sh + d, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // both for a NaN: it has to reach the score
-                up[e] += v[e] > 0.0f || v[e] != v[e] ? v[e] : 0.0f;
-                down[e] += v[e] < 0.0f || v[e] != v[e] ? v[e] : 0.0f;
-            }
-        }
+    for (int e = 0; e < 8; ++e) {
+        up[e]   = in ? sums[0][d + e] : 0.0;
+        down[e] = in ? sums[1][d + e] : 0.0;
+    }
     uint64_t      *out = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
     const int32_t *row = a.table + s.b * a.table_st;
     for (int p0 = j0 + g; p0 < j1; p0 += GROUPS * PAGES) {
@@ -231,26 +262,135 @@ template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_ker
             }
             if (!there[i]) x = 0.0; // also where a query is not finite
             x = ps_sum<LPR>(x);
-            if (l == 0 && j < j1) out[j] = j < a.first || own - j < a.last ? ~0ull : ps_key(x);
+            if (l == 0 && j < j1) out[j] = ps_key(x);
+        }
+    }
+}
+
+// Chunks: 16 tokens by 16 pages on the 64-bit matrix instruction, D = R B with a page's
+// range as a row of R (2 D channels, the smallest keys, then the largest) and a token's
+// sums as a column of B, which all pages read from LDS.  Which channel is which step of
+// the contraction is free: quarter k of the lanes has channels [k D / 2, (k + 1) D / 2),
+// one run of its page's range.  Tokens of several sequences are gone through sequence by
+// sequence, with the other tokens' columns unused.
+typedef double ps_d4 __attribute__((ext_vector_type(4)));
+constexpr int  PS_TILE = 16;
+
+template <int QT, int DP> __global__ __launch_bounds__(PS_NT) void ps_score_tile_kernel(PSArgs a, int per, int parts) {
+    __shared__ double sums[2 * DP * PS_TILE]; // [channel][token]
+    __shared__ int    sb[PS_TILE], spos[PS_TILE];
+    const uint32_t    w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, tile = w1 / parts;
+    const int         ti0 = static_cast<int>(tile) * PS_TILE, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid < PS_TILE) {
+        PSToken s = {-1, -1, 0, 0, 0};
+        if (ti0 + tid < a.n) s = ps_token_of_lane(a, a.t0 + ti0 + tid);
+        sb[tid]   = s.pos < 0 ? -1 : s.b;
+        spos[tid] = s.pos;
+    }
+    for (int x = tid; x < PS_TILE * (a.D / 8); x += PS_NT) {
+        const int i = x % PS_TILE, d = x / PS_TILE * 8;
+        double    up[8], down[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
+        if (ti0 + i < a.n) {
+            const uint16_t *q = a.q + (a.t0 + ti0 + i) * a.q_st + static_cast<int64_t>(h) * a.G * a.q_sh + d;
+#pragma unroll 4
+            for (int g = 0; g < a.G; ++g) {
+                float v[8];
+                load8<QT>(q, g * a.q_sh, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ps_add(v[e], up[e], down[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sums[(d + e) * PS_TILE + i]       = down[e];
+            sums[(a.D + d + e) * PS_TILE + i] = up[e];
+        }
+    }
+    __syncthreads();
+    const int r = lane & 15, quarter = lane >> 4, half = a.D / 2;
+    const int b_me = sb[r], own_me = spos[r] / a.page; // of the lane's token
+    uint64_t *out  = a.keys + (static_cast<int64_t>(ti0 + r) * a.Hkv + h) * a.M;
+    for (int i0 = 0; i0 < PS_TILE;) {
+        const int b = sb[i0];
+        int       i1 = i0 + 1;
+        while (i1 < PS_TILE && sb[i1] == b) ++i1;
+        const int n = b < 0 ? 0 : spos[i1 - 1] / a.page + 1, j0 = static_cast<int>(c) * per, j1 = min(j0 + per, n);
+        i0 = i1;
+        if (n <= a.take) continue;
+        const int32_t *row = a.table + b * a.table_st;
+        for (int p0 = j0 + wave * 16; p0 < j1; p0 += PS_NT / 64 * 16) {
+            const int       u = p0 + r < j1 ? row[p0 + r] : -1;
+            const bool      there = u >= 0 && u < a.P; // a page outside the pool holds zeros
+            const uint16_t *x = a.ranges + (static_cast<int64_t>(there ? u : 0) * a.Hkv + h) * 2 * a.D + quarter * half;
+            const double   *y = sums + quarter * half * PS_TILE + r;
+            uint4           v[DP / 16];
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) v[s] = there && s * 8 < half ? *reinterpret_cast<const uint4 *>(x + s * 8) : make_uint4(0, 0, 0, 0);
+            ps_d4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+                if (s * 8 >= half) break;
+                const uint32_t z[4] = {v[s].x, v[s].y, v[s].z, v[s].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(
+                        static_cast<double>(__uint_as_float(e % 2 ? z[e / 2] & 0xffff0000u : z[e / 2] << 16)), y[(s * 8 + e) * PS_TILE], acc, 0, 0, 0);
+            }
+            const uint64_t is = __ballot(there); // pages in its low 16 bits
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int g = quarter + 4 * i, j = p0 + g; // the lane's i-th score is of this page
+                if (b_me != b || j >= j1 || j > own_me) continue;
+                out[j] = ps_key(is >> g & 1 ? acc[i] : 0.0);
+            }
         }
     }
 }
 
 // ---- choice ------------------------------------------------------------------------
+// and, or of a wave's lanes
+__device__ __forceinline__ uint32_t ps_dpp_u32(uint32_t v, int step) {
+    switch (step) {
+    case 0: return __builtin_amdgcn_mov_dpp(v, PTA_DPP_QUAD_XOR1, 0xf, 0xf, false);
+    case 1: return __builtin_amdgcn_mov_dpp(v, PTA_DPP_QUAD_XOR2, 0xf, 0xf, false);
+    case 2: return __builtin_amdgcn_mov_dpp(v, PTA_DPP_ROW_HALF_MIRROR, 0xf, 0xf, false);
+    default: return __builtin_amdgcn_mov_dpp(v, PTA_DPP_ROW_MIRROR, 0xf, 0xf, false);
+    }
+}
+__device__ __forceinline__ void ps_common(uint32_t &all, uint32_t &any) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        all &= ps_dpp_u32(all, i);
+        any |= ps_dpp_u32(any, i);
+    }
+    auto x = __builtin_amdgcn_permlane16_swap(all, all, false, false);
+    auto y = __builtin_amdgcn_permlane16_swap(any, any, false, false);
+    all = x[0] & x[1];
+    any = y[0] | y[1];
+    x   = __builtin_amdgcn_permlane32_swap(all, all, false, false);
+    y   = __builtin_amdgcn_permlane32_swap(any, any, false, false);
+    all = __builtin_amdgcn_readfirstlane(x[0] & x[1]);
+    any = __builtin_amdgcn_readfirstlane(y[0] | y[1]);
+}
+
 // NW waves for (token, head), wave w with keys [64 w E, 64 (w + 1) E), E a lane; what
-// does not fit is read again for every step.  The bits of the least key that is taken
-// are found from the highest on: a bit is set if at least `take` keys have it.
+// does not fit is read again for every step.  The bits of the least key that is taken are
+// found from the highest that differs on: a bit is set if enough keys have it; the search
+// ends when exactly as many are left.  Bound by its steps, about 3 E instructions each (and
+// for more than one wave a barrier).
 template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_kernel(PSArgs a) {
     constexpr int  CAP = 64 * NW * E;
     __shared__ int cnt[2][2][NW];
     const int      ti = blockIdx.x / a.Hkv, h = blockIdx.x - ti * a.Hkv, t = a.t0 + ti;
     const int      lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const PSToken  s = ps_token(a.cu, a.lens, a.B, a.T, t, static_cast<int64_t>(a.M) * a.page);
+    const PSToken  s = ps_token(a, t);
     const bool     some = s.b >= 0 && s.pos >= 0;
-    const int      n = some ? s.pos / a.page + 1 : 0, take = min(n, a.take);
+    const int      own = some ? s.pos / a.page : -1, n = own + 1, take = min(n, a.take);
     int32_t       *sel = a.sel + (static_cast<int64_t>(t) * a.Hkv + h) * a.K;
     if (h == 0 && threadIdx.x == 0) {
-        a.sel_lens[t] = some ? (take - 1) * a.page + s.pos % a.page + 1 : 0;
+        a.sel_lens[t] = some ? (take - 1) * a.page + (s.pos - own * a.page) + 1 : 0;
         if (a.sel_cu != nullptr) {
             a.sel_cu[t] = t;
             if (t == a.T - 1) a.sel_cu[a.T] = a.T;
@@ -263,14 +403,20 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
         for (int j = threadIdx.x; j < n; j += 64 * NW) sel[j] = row[j];
         return;
     }
+    // the `first` and `last` pages are above all scores
     const uint64_t *in = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
+    auto            at = [&](int j) { return j < a.first || own - j < a.last ? ~0ull : in[j]; };
     uint64_t        key[E];
+    uint32_t        common = ~0u, any = 0; // bits that all scores have, or any
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int j = (wave * E + e) * 64 + lane;
-        key[e]      = j < n ? in[j] : 0; // below every score: `least` is at least 1
+        key[e]      = j < n ? at(j) : 0; // below every score
+        const uint32_t x = static_cast<uint32_t>(key[e] >> 32);
+        common &= key[e] + 1 > 1 ? x : ~0u;
+        any |= key[e] + 1 > 1 ? x : 0u;
     }
-    // keys of the workgroup for which f holds, and g
+    // sums of x and of y over the workgroup, and over the waves before
     int  buf = 0;
     auto all = [&](int x, int y, int &sx, int &sy, int &bx, int &by) {
         sx = x;
@@ -294,20 +440,53 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
             buf ^= 1;
         }
     };
+    // of the high halves first, whose comparisons are cheaper: all but ties differ there
     uint64_t least = 0;
-    for (int bit = 63; bit >= 0; --bit) {
+    bool     done  = false;
+    int      top   = 31; // highest bit in which scores differ
+    if (n <= CAP) {
+        ps_common(common, any);
+        if constexpr (NW > 1) {
+            if (lane == 0) {
+                cnt[1][0][wave] = static_cast<int>(common);
+                cnt[1][1][wave] = static_cast<int>(any);
+            }
+            __syncthreads();
+            for (int w = 0; w < NW; ++w) {
+                common &= static_cast<uint32_t>(cnt[1][0][w]);
+                any |= static_cast<uint32_t>(cnt[1][1][w]);
+            }
+        }
+        top   = 31 - __clz(common ^ any); // -1: in none
+        least = static_cast<uint64_t>(top < 0 ? any : any & ~((2u << top) - 1)) << 32;
+    }
+    for (int bit = top; bit >= 0 && !done; --bit) {
+        const uint32_t cand = static_cast<uint32_t>(least >> 32) | (1u << bit);
+        int            c = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(static_cast<uint32_t>(key[e] >> 32) >= cand));
+        for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
+            const int j = j0 + static_cast<int>(threadIdx.x);
+            c += __popcll(__ballot(j < n && static_cast<uint32_t>(at(min(j, n - 1)) >> 32) >= cand));
+        }
+        int total, none, b0, b1;
+        all(c, 0, total, none, b0, b1);
+        if (total >= take) least = static_cast<uint64_t>(cand) << 32;
+        done = total == take; // all of these and no others
+    }
+    for (int bit = 31; bit >= 0 && !done; --bit) {
         const uint64_t cand = least | (1ull << bit);
         int            c = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) c += __popcll(__ballot(key[e] >= cand));
         for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
             const int j = j0 + static_cast<int>(threadIdx.x);
-            c += __popcll(__ballot(j < n && in[min(j, n - 1)] >= cand));
+            c += __popcll(__ballot(j < n && at(min(j, n - 1)) >= cand));
         }
         int total, none, b0, b1;
         all(c, 0, total, none, b0, b1);
         if (total >= take) least = cand;
-        if (total == take) break; // all of these and no others
+        done = total == take;
     }
     // all above the least, and of those equal to it the first ones
     int above = 0, equal = 0, sa, se, ba, be;
@@ -320,7 +499,7 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     int more = 0; // above, beyond what fits
     for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
         const int j = j0 + static_cast<int>(threadIdx.x);
-        more += __popcll(__ballot(j < n && in[min(j, n - 1)] > least));
+        more += __popcll(__ballot(j < n && at(min(j, n - 1)) > least));
     }
     int sm, s0, b0, b1;
     all(more, 0, sm, s0, b0, b1);
@@ -336,13 +515,12 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     int g = ba, q = be;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int j = (wave * E + e) * 64 + lane;
-        put(j < n && key[e] > least, j < n && key[e] == least, j, g, q);
+        put(key[e] > least, key[e] == least, (wave * E + e) * 64 + lane, g, q);
     }
     int g0 = sa, q0 = se;
     for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
         const int      j = j0 + static_cast<int>(threadIdx.x);
-        const uint64_t x = in[min(j, n - 1)];
+        const uint64_t x = at(min(j, n - 1));
         const bool     gt = j < n && x > least, eq = j < n && x == least;
         int            tg, tq, wg, wq;
         all(__popcll(__ballot(gt)), __popcll(__ballot(eq)), tg, tq, wg, wq);
@@ -376,14 +554,23 @@ int ps_check(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D, in
     return PTA_OK;
 }
 
+// Chunks from two tokens a sequence on go by tiles of tokens
 template <int QT> static void ps_score(const PSArgs &a, hipStream_t st) {
-    // pages in as many parts as give every CU four workgroups, 32 of them at least
-    const int64_t want = cdiv(4 * device_cu_count(), static_cast<int64_t>(a.n) * a.Hkv);
-    const int     per = static_cast<int>(std::max<int64_t>(32, cdiv(cdiv(a.M, want), 32) * 32)), parts = static_cast<int>(cdiv(a.M, per));
-    const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.n) * a.Hkv * parts);
-    if (a.D <= 64) ps_score_kernel<QT, 8><<<grid, PS_NT, 0, st>>>(a, per, parts);
-    else if (a.D <= 128) ps_score_kernel<QT, 16><<<grid, PS_NT, 0, st>>>(a, per, parts);
-    else ps_score_kernel<QT, 32><<<grid, PS_NT, 0, st>>>(a, per, parts);
+    const bool    tiles = a.T >= 2 * a.B && a.n > 1;
+    const int64_t items = (tiles ? cdiv(a.n, PS_TILE) : a.n) * a.Hkv;
+    // pages in as many parts as give every CU four workgroups, one round of a workgroup at least
+    const int64_t least = tiles ? 64 : 32, want = cdiv(4 * device_cu_count(), items);
+    const int     per = static_cast<int>(std::max<int64_t>(least, cdiv(cdiv(a.M, want), least) * least)), parts = static_cast<int>(cdiv(a.M, per));
+    const unsigned grid = static_cast<unsigned>(items * parts);
+    if (tiles) {
+        if (a.D <= 64) ps_score_tile_kernel<QT, 64><<<grid, PS_NT, 0, st>>>(a, per, parts);
+        else if (a.D <= 128) ps_score_tile_kernel<QT, 128><<<grid, PS_NT, 0, st>>>(a, per, parts);
+        else ps_score_tile_kernel<QT, 256><<<grid, PS_NT, 0, st>>>(a, per, parts);
+    } else {
+        if (a.D <= 64) ps_score_kernel<QT, 8><<<grid, PS_NT, 0, st>>>(a, per, parts);
+        else if (a.D <= 128) ps_score_kernel<QT, 16><<<grid, PS_NT, 0, st>>>(a, per, parts);
+        else ps_score_kernel<QT, 32><<<grid, PS_NT, 0, st>>>(a, per, parts);
+    }
 }
 
 static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
@@ -397,8 +584,9 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
             PTA_CHECK_LAUNCH();
         }
         const unsigned grid = static_cast<unsigned>(a.n) * a.Hkv;
-        if (a.M <= 512) ps_choose_kernel<1, 8><<<grid, 64, 0, st>>>(a);
-        else if (a.M <= 2048) ps_choose_kernel<4, 8><<<grid, 256, 0, st>>>(a);
+        if (a.M <= 256) ps_choose_kernel<1, 4><<<grid, 64, 0, st>>>(a);
+        else if (a.M <= 512) ps_choose_kernel<1, 8><<<grid, 64, 0, st>>>(a);
+        else if (a.M <= 2048) ps_choose_kernel<8, 4><<<grid, 512, 0, st>>>(a);
         else ps_choose_kernel<16, 8><<<grid, 1024, 0, st>>>(a);
         PTA_CHECK_LAUNCH();
     }
