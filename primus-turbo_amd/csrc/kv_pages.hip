@@ -14,8 +14,10 @@
 namespace pta {
 namespace {
 
-constexpr int KP_NT = 256, KP_DEPTH = 4, KP_RUNS = 5;
-constexpr int KP_CHUNK = KP_NT * KP_DEPTH * 16; // bytes of a workgroup
+constexpr int KP_NT = 256, KP_RUNS = 5;
+// 16-byte pieces of a thread: four where that gives every CU work, else one
+constexpr int KP_DEPTH = 4;
+constexpr int64_t kp_chunk(int depth) { return static_cast<int64_t>(KP_NT) * depth * 16; } // bytes of a workgroup
 
 struct KPPool {
     uint8_t *p[KP_RUNS];
@@ -28,26 +30,34 @@ struct KPPool {
 };
 
 // Chunk c (of layer and run) of page `to` becomes that of page `from`
-__device__ __forceinline__ void kp_copy(const KPPool &a, int64_t from, int64_t to, int layer, int c) {
-    int r = 0;
+template <int DEPTH> __device__ __forceinline__ void kp_copy(const KPPool &a, int64_t from, int64_t to, int layer, int c) {
+    // by comparisons: an index that the compiler does not know would put the arguments into memory
+    uint8_t *p = a.p[0];
+    int64_t  bytes = a.bytes[0], per_layer = a.layer[0];
+    int      first = 0, wide = a.wide[0];
 #pragma unroll
     for (int i = 1; i < KP_RUNS; ++i)
-        if (i < a.runs && c >= a.first[i]) r = i;
-    const int64_t at = static_cast<int64_t>(c - a.first[r]) * KP_CHUNK;
-    const int64_t n  = min(a.bytes[r] - at, static_cast<int64_t>(KP_CHUNK));
-    const uint8_t *src = a.p[r] + layer * a.layer[r] + from * a.bytes[r] + at;
-    uint8_t       *dst = a.p[r] + layer * a.layer[r] + to * a.bytes[r] + at;
-    if (a.wide[r]) {
-        uint4 v[KP_DEPTH];
+        if (i < a.runs && c >= a.first[i]) {
+            p = a.p[i];
+            bytes = a.bytes[i]; per_layer = a.layer[i];
+            first = a.first[i]; wide = a.wide[i];
+        }
+    const int64_t at = (c - first) * kp_chunk(DEPTH), n = min(bytes - at, kp_chunk(DEPTH));
+    p += layer * per_layer + at;
+    const uint8_t *src = p + from * bytes;
+    uint8_t       *dst = p + to * bytes;
+    if (wide) {
+        typedef uint32_t piece __attribute__((ext_vector_type(4)));
+        piece v[DEPTH];
 #pragma unroll
-        for (int i = 0; i < KP_DEPTH; ++i) {
+        for (int i = 0; i < DEPTH; ++i) {
             const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
-            if (o < n) v[i] = *reinterpret_cast<const uint4 *>(src + o);
+            if (o < n) v[i] = *reinterpret_cast<const piece *>(src + o);
         }
 #pragma unroll
-        for (int i = 0; i < KP_DEPTH; ++i) {
+        for (int i = 0; i < DEPTH; ++i) {
             const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
-            if (o < n) *reinterpret_cast<uint4 *>(dst + o) = v[i];
+            if (o < n) *reinterpret_cast<piece *>(dst + o) = v[i];
         }
     } else {
         for (int64_t o = threadIdx.x * 4; o < n; o += KP_NT * 4)
@@ -59,14 +69,14 @@ __device__ __forceinline__ int64_t kp_index(const void *p, int i64, int64_t i) {
     return i64 ? reinterpret_cast<const int64_t *>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t *>(p)[i]);
 }
 
-__global__ __launch_bounds__(KP_NT) void kp_copy_kernel(KPPool a, const void *src, const void *dst, int i64, int64_t total) {
+template <int DEPTH> __global__ __launch_bounds__(KP_NT) void kp_copy_kernel(KPPool a, const void *src, const void *dst, int i64, int64_t total) {
     const int per = a.chunks * a.layers;
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
         const int64_t pair = w / per;
         const int     rest = static_cast<int>(w - pair * per), layer = rest / a.chunks;
         const int64_t s = kp_index(src, i64, pair), d = kp_index(dst, i64, pair);
         if (s < 0 || s >= a.pages || d < 0 || d >= a.pages || s == d) continue;
-        kp_copy(a, s, d, layer, rest - layer * a.chunks);
+        kp_copy<DEPTH>(a, s, d, layer, rest - layer * a.chunks);
     }
 }
 
@@ -85,7 +95,7 @@ struct KFArgs {
     int32_t *owner;      // [P] who has the page: N nobody, -1 everybody (it is full), else the sequence whose last page it is
     int32_t *free_pages; // [P] in rising order, as many as are taken
     int32_t *moved;      // [P] where pages at or past `bound` go (compact)
-    int32_t *seq;        // [N] place of its first fresh page among the free ones; -1: it came too late
+    int2    *seq;        // [N] place of its first fresh page among the free ones, -1: it came too late; 1 if that is a copy
     int2    *pairs;      // copies: from, to
     int32_t *count;      // pairs; bound
 };
@@ -129,111 +139,139 @@ __global__ __launch_bounds__(KP_NT) void kf_mark_kernel(KFArgs a) {
 constexpr int KF_NT = 1024;
 
 // exclusive sums over the workgroup's threads, and the totals
-__device__ __forceinline__ int2 kf_scan(int2 v, int2 *tmp, int2 &total) {
+struct KFSums {
+    int x, y, z;
+};
+__device__ __forceinline__ KFSums kf_scan(KFSums v, int4 *tmp, KFSums &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int2      x = v;
+    KFSums    s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int ax = __shfl_up(x.x, o), ay = __shfl_up(x.y, o);
+        const int x = __shfl_up(s.x, o), y = __shfl_up(s.y, o), z = __shfl_up(s.z, o);
         if (lane >= o) {
-            x.x += ax;
-            x.y += ay;
+            s.x += x;
+            s.y += y;
+            s.z += z;
         }
     }
     __syncthreads();
-    if (lane == 63) tmp[wave] = x;
+    if (lane == 63) tmp[wave] = make_int4(s.x, s.y, s.z, 0);
     __syncthreads();
-    int2 before = make_int2(0, 0);
-    total       = make_int2(0, 0);
+    KFSums before = {0, 0, 0};
+    total         = {0, 0, 0};
+#pragma unroll
     for (int w = 0; w < KF_NT / 64; ++w) {
-        if (w < wave) {
-            before.x += tmp[w].x;
-            before.y += tmp[w].y;
-        }
-        total.x += tmp[w].x;
-        total.y += tmp[w].y;
+        const int4 t = tmp[w];
+        const int  m = w < wave ? -1 : 0;
+        before.x += t.x & m;
+        before.y += t.y & m;
+        before.z += t.z & m;
+        total.x += t.x;
+        total.y += t.y;
+        total.z += t.z;
     }
-    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+    return {before.x + s.x - v.x, before.y + s.y - v.y, before.z + s.z - v.z};
 }
 
-// Fresh pages of a sequence (x), and whether one of them is a copy (y)
-__device__ __forceinline__ int2 kf_fresh(const KFArgs &a, int i, const KFSeq &s) {
-    const int copy = s.last >= 0 && a.owner[s.last] != i;
-    return make_int2(s.want - s.has + copy, copy);
-}
+// One workgroup: a thread has a run of pages, and of sequences.  Where LDS holds the pages'
+// owners and the table's entries are few, they are found here, else by the two kernels
+// above (64 sequences of 66 pages over 4300: 8.5 us, the three kernels 13).
+constexpr int     KF_LDS_PAGES = 12 * 1024;
+constexpr int64_t KF_LDS_ENTRIES = 128 * KF_NT;
 
-// One workgroup: a thread has a run of pages, and of sequences
-__global__ __launch_bounds__(KF_NT) void kf_plan_kernel(KFArgs a) {
-    __shared__ int2 tmp[KF_NT / 64];
+template <bool LDS> __global__ __launch_bounds__(KF_NT) void kf_plan_kernel(KFArgs a) {
+    __shared__ int4 tmp[KF_NT / 64];
+    __shared__ int  own[LDS ? KF_LDS_PAGES : 1];
+    __shared__ int  row[LDS ? KF_NT : 1], full[LDS ? KF_NT : 1], has[LDS ? KF_NT : 1];
+    int            *owner = LDS ? own : a.owner;
     const int tid = threadIdx.x;
     const int pr = (a.P + KF_NT - 1) / KF_NT, p0 = min(tid * pr, a.P), p1 = min(p0 + pr, a.P);
-    const int nr = (a.N + KF_NT - 1) / KF_NT, n0 = min(tid * nr, a.N), n1 = min(n0 + nr, a.N);
-    int2      v = make_int2(0, 0), used, fresh, total;
-    for (int u = p0; u < p1; ++u) v.x += a.owner[u] < a.N;
-    kf_scan(v, tmp, used);
-    v = make_int2(0, 0);
-    for (int i = n0; i < n1; ++i) {
-        const int2 f = kf_fresh(a, i, kf_seq(a, i));
-        v.x += f.x;
-        v.y += f.y;
+    const int nr = LDS ? 1 : (a.N + KF_NT - 1) / KF_NT, n0 = min(tid * nr, a.N), n1 = min(n0 + nr, a.N);
+    // the thread's first sequence, mostly its only one, is looked up once
+    const KFSeq mine = n0 < n1 ? kf_seq(a, n0) : KFSeq{-1, 0, 0, 0, 0, -1};
+    if constexpr (LDS) { // a sequence a thread
+        row[tid]  = max(mine.parent, 0);
+        full[tid] = mine.full;
+        has[tid]  = mine.has;
+        for (int u = tid; u < a.P; u += KF_NT) own[u] = a.N;
+        __syncthreads();
+        const int entries = a.N * a.M;
+#pragma unroll 4
+        for (int x = tid; x < entries; x += KF_NT) {
+            const int i = x / a.M, j = x - i * a.M;
+            const int u = j < has[i] ? a.table[row[i] * a.table_st + j] : -1;
+            if (u >= 0 && u < a.P) atomicMin(&own[u], j < full[i] ? -1 : i);
+        }
+        __syncthreads();
     }
-    int2      at    = kf_scan(v, tmp, fresh);
-    const int nfree = a.P - used.x;
+    auto seq = [&](int i) __attribute__((always_inline)) { return i == n0 ? mine : kf_seq(a, i); };
+    // whether the sequence's last page is another's too
+    auto copied = [&](int i, const KFSeq &s) __attribute__((always_inline)) { return s.last >= 0 && owner[s.last] != i ? 1 : 0; };
+    KFSums v = {0, 0, 0}, need, total; // pages in use, fresh ones, copies among these
+    for (int u = p0; u < p1; ++u) v.x += owner[u] < a.N;
+    for (int i = n0; i < n1; ++i) {
+        const KFSeq s = seq(i);
+        const int   c = copied(i, s);
+        v.y += s.want - s.has + c;
+        v.z += c;
+    }
+    KFSums    at    = kf_scan(v, tmp, need);
+    const int nfree = a.P - need.x;
     // pages at or past `bound` move to the first free ones
-    const int bound = a.compact ? used.x + min(fresh.x, nfree) : a.P;
-    v               = make_int2(0, 0);
+    const int bound = a.compact ? need.x + min(need.y, nfree) : a.P;
+    v               = {0, 0, 0}; // free pages, pages that move
     for (int u = p0; u < p1; ++u) {
-        if (a.owner[u] >= a.N) ++v.x;
+        if (owner[u] >= a.N) ++v.x;
         else if (u >= bound) ++v.y;
     }
-    const int2 rank = kf_scan(v, tmp, total);
-    const int  moves = total.y, taken = moves + min(fresh.x, nfree);
+    const KFSums rank = kf_scan(v, tmp, total);
+    const int    moves = total.y, taken = moves + min(need.y, nfree);
     for (int u = p0, f = rank.x; u < p1 && f < taken; ++u)
-        if (a.owner[u] >= a.N) a.free_pages[f++] = u;
+        if (owner[u] >= a.N) a.free_pages[f++] = u;
     __syncthreads(); // the free pages are in place
     if (moves > 0)
         for (int u = max(p0, bound), m = rank.y; u < p1; ++u)
-            if (a.owner[u] < a.N) {
+            if (owner[u] < a.N) {
                 const int to = a.free_pages[m];
                 a.moved[u]   = to;
                 a.pairs[m++] = make_int2(u, to);
             }
     for (int i = n0; i < n1; ++i) {
-        const KFSeq s = kf_seq(a, i);
-        const int2  f = kf_fresh(a, i, s);
+        const KFSeq s = seq(i);
+        const int   c = copied(i, s), f = s.want - s.has + c;
         // sequences take their pages in order; those that come too late get none
-        const bool none = f.x > 0 && at.x + f.x > nfree;
-        a.seq[i]        = none ? -1 : moves + at.x;
-        if (f.y) a.pairs[moves + at.y] = none ? make_int2(-1, -1) : make_int2(s.last, a.free_pages[moves + at.x]);
-        at.x += f.x;
-        at.y += f.y;
+        const bool none = f > 0 && at.y + f > nfree;
+        a.seq[i]        = make_int2(none ? -1 : moves + at.y, c);
+        if (c) a.pairs[moves + at.z] = none ? make_int2(-1, -1) : make_int2(s.last, a.free_pages[moves + at.y]);
+        at.y += f;
+        at.z += c;
     }
     if (tid == 0) {
-        a.count[0] = moves + fresh.y;
+        a.count[0] = moves + need.z;
         a.count[1] = bound;
     }
 }
 
 // The first N workgroups write the sequences' rows, the others copy pages
-__global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) {
+template <int DEPTH> __global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) {
     const int i = blockIdx.x;
     if (i < a.N) {
         const KFSeq s = kf_seq(a, i);
-        const int   place = a.seq[i], bound = a.count[1];
-        const int   copy = s.last >= 0 && a.owner[s.last] != i;
+        const int2  plan = a.seq[i];
+        const int   bound = a.count[1], kept = s.has - plan.y;
         for (int j = threadIdx.x; j < a.M; j += KP_NT) {
             int u = -1;
-            if (place >= 0 && j < s.want) {
-                if (j < s.has - copy) {
+            if (plan.x >= 0 && j < s.want) {
+                if (j < kept) {
                     u = a.table[s.parent * a.table_st + j];
                     if (u >= bound && u < a.P) u = a.moved[u];
                 } else {
-                    u = a.free_pages[place + j - (s.has - copy)];
+                    u = a.free_pages[plan.x + j - kept];
                 }
             }
             a.new_table[static_cast<int64_t>(i) * a.M + j] = u;
         }
-        if (threadIdx.x == 0) a.new_lens[i] = place < 0 ? -1 : s.parent < 0 ? 0 : a.lens[s.parent];
+        if (threadIdx.x == 0) a.new_lens[i] = plan.x < 0 ? -1 : s.parent < 0 ? 0 : a.lens[s.parent];
         return;
     }
     const int     per   = pool.chunks * pool.layers;
@@ -242,12 +280,13 @@ __global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) 
         const int64_t pair = w / per;
         const int     rest = static_cast<int>(w - pair * per), layer = rest / pool.chunks;
         const int2    p = a.pairs[pair];
-        if (p.x >= 0) kp_copy(pool, p.x, p.y, layer, rest - layer * pool.chunks);
+        if (p.x >= 0) kp_copy<DEPTH>(pool, p.x, p.y, layer, rest - layer * pool.chunks);
     }
 }
 
-int kp_pool(KPPool &a, void *k_cache, void *v_cache, int kind, int64_t layers, int64_t num_pages, int64_t Hkv, int64_t page_size, int64_t D,
-            float *k_scale, float *v_scale, void *ranges) {
+// `pairs`: of pages to copy at most; sets the pieces of a thread
+int kp_pool(KPPool &a, int &depth, int64_t pairs, void *k_cache, void *v_cache, int kind, int64_t layers, int64_t num_pages, int64_t Hkv,
+            int64_t page_size, int64_t D, float *k_scale, float *v_scale, void *ranges) {
     PTA_CHECK_ARG(kind == PTA_E4M3 || kind == PTA_E5M2 || kind == PTA_CACHE_16BIT, "unknown cache kind %d", kind);
     PTA_CHECK_ARG(layers >= 0 && num_pages >= 0 && page_size > 0 && Hkv > 0, "bad cache sizes");
     PTA_CHECK_ARG(D >= 16 && D <= 256 && D % 16 == 0, "head_dim must be a multiple of 16 in [16, 256] (got %lld)", static_cast<long long>(D));
@@ -263,7 +302,10 @@ int kp_pool(KPPool &a, void *k_cache, void *v_cache, int kind, int64_t layers, i
     const int64_t data = Hkv * page_size * D * (fp8 ? 1 : 2), scale = Hkv * page_size * 4;
     void   *const p[KP_RUNS] = {k_cache, v_cache, fp8 ? k_scale : nullptr, fp8 ? v_scale : nullptr, ranges};
     const int64_t bytes[KP_RUNS] = {data, data, scale, scale, Hkv * D * 4};
-    int64_t       chunks = 0;
+    int64_t       all = 0;
+    for (int i = 0; i < KP_RUNS; ++i) all += p[i] == nullptr ? 0 : bytes[i];
+    depth = static_cast<double>(all) * layers * pairs < static_cast<double>(kp_chunk(KP_DEPTH)) * 2 * device_cu_count() ? 1 : KP_DEPTH;
+    int64_t chunks = 0;
     for (int i = 0; i < KP_RUNS; ++i) {
         if (p[i] == nullptr) continue;
         const int r = a.runs++;
@@ -272,7 +314,7 @@ int kp_pool(KPPool &a, void *k_cache, void *v_cache, int kind, int64_t layers, i
         a.layer[r] = bytes[i] * num_pages;
         a.first[r] = static_cast<int>(chunks);
         a.wide[r]  = aligned16(p[i]) && bytes[i] % 16 == 0;
-        chunks += cdiv(bytes[i], KP_CHUNK);
+        chunks += cdiv(bytes[i], kp_chunk(depth));
     }
     PTA_CHECK_ARG(layers <= INT_MAX / chunks, "too many layers");
     a.chunks = static_cast<int>(chunks);
@@ -294,7 +336,7 @@ KFPlan kf_plan(int64_t N, int64_t M, int64_t P, int compact) {
     p.owner      = kf_round(P * 4);
     p.free_pages = kf_round(P * 4);
     p.moved      = compact ? kf_round(P * 4) : 0;
-    p.seq        = kf_round(N * 4);
+    p.seq        = kf_round(N * 8);
     p.count      = 16;
     p.pair_bytes = kf_round(p.pairs * 8);
     return p;
@@ -310,12 +352,14 @@ extern "C" int pta_kv_cache_copy(void *k_cache, void *v_cache, int cache_kind, i
                                  const void *src_pages, const void *dst_pages, int pages_i64, int64_t num_pairs, pta_stream_t stream) {
     clear_error();
     KPPool a = {};
-    if (int rc = kp_pool(a, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    int    depth = 1;
+    if (int rc = kp_pool(a, depth, num_pairs, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
     PTA_CHECK_ARG(num_pairs >= 0 && num_pairs <= INT_MAX, "bad number of pages");
     if (num_pairs == 0 || num_layers == 0 || num_pages == 0) return PTA_OK;
     PTA_CHECK_ARG(src_pages && dst_pages, "null page list");
     const int64_t total = num_pairs * a.chunks * a.layers;
-    kp_copy_kernel<<<kp_blocks(total), KP_NT, 0, as_stream(stream)>>>(a, src_pages, dst_pages, pages_i64, total);
+    const auto    kernel = depth == 1 ? kp_copy_kernel<1> : kp_copy_kernel<KP_DEPTH>;
+    kernel<<<kp_blocks(total), KP_NT, 0, as_stream(stream)>>>(a, src_pages, dst_pages, pages_i64, total);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
 }
@@ -333,7 +377,8 @@ extern "C" int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, i
                                  pta_stream_t stream) {
     clear_error();
     KPPool pool = {};
-    if (int rc = kp_pool(pool, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    int    depth = 1;
+    if (int rc = kp_pool(pool, depth, num_new_seqs + (compact ? num_pages : 0), k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
     PTA_CHECK_ARG(num_seqs >= 0 && num_new_seqs >= 0 && max_pages >= 0 && reserve >= 0, "bad sizes");
     PTA_CHECK_ARG(num_seqs < (1 << 24) && num_new_seqs < (1 << 24) && max_pages <= (INT_MAX - 1024) / page_size &&
                       max_pages <= INT_MAX / 2 / std::max<int64_t>(1, num_new_seqs) - 1,
@@ -356,20 +401,25 @@ extern "C" int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, i
     a.owner      = reinterpret_cast<int32_t *>(w);
     a.free_pages = reinterpret_cast<int32_t *>(w += p.owner);
     a.moved      = reinterpret_cast<int32_t *>(w += p.free_pages);
-    a.seq        = reinterpret_cast<int32_t *>(w += p.moved);
+    a.seq        = reinterpret_cast<int2 *>(w += p.moved);
     a.count      = reinterpret_cast<int32_t *>(w += p.seq);
     a.pairs      = reinterpret_cast<int2 *>(w += p.count);
     const hipStream_t st = as_stream(stream);
-    if (num_pages > 0) {
-        kf_init_kernel<<<static_cast<unsigned>(std::min<int64_t>(cdiv(num_pages, KP_NT), 4 * device_cu_count())), KP_NT, 0, st>>>(a);
+    if (num_pages <= KF_LDS_PAGES && num_new_seqs <= KF_NT && num_new_seqs * max_pages <= KF_LDS_ENTRIES) {
+        kf_plan_kernel<true><<<1, KF_NT, 0, st>>>(a);
+    } else {
+        if (num_pages > 0) {
+            kf_init_kernel<<<static_cast<unsigned>(std::min<int64_t>(cdiv(num_pages, KP_NT), 4 * device_cu_count())), KP_NT, 0, st>>>(a);
+            PTA_CHECK_LAUNCH();
+        }
+        kf_mark_kernel<<<static_cast<unsigned>(a.N), KP_NT, 0, st>>>(a);
         PTA_CHECK_LAUNCH();
+        kf_plan_kernel<false><<<1, KF_NT, 0, st>>>(a);
     }
-    kf_mark_kernel<<<static_cast<unsigned>(a.N), KP_NT, 0, st>>>(a);
-    PTA_CHECK_LAUNCH();
-    kf_plan_kernel<<<1, KF_NT, 0, st>>>(a);
     PTA_CHECK_LAUNCH();
     const int64_t total = num_pages > 0 ? p.pairs * pool.chunks * pool.layers : 0;
-    kf_apply_kernel<<<static_cast<unsigned>(a.N) + kp_blocks(total), KP_NT, 0, st>>>(a, pool);
+    const auto    apply = depth == 1 ? kf_apply_kernel<1> : kf_apply_kernel<KP_DEPTH>;
+    apply<<<static_cast<unsigned>(a.N) + kp_blocks(total), KP_NT, 0, st>>>(a, pool);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
 }

@@ -13,30 +13,29 @@ from primus_turbo.pytorch import _C
 from primus_turbo.pytorch.core.inference import check_tensors
 from primus_turbo.pytorch.kernels.attention.paged_attention_impl import _IN, _check_cache, _check_slots, _increment_version
 
-_INT = (torch.int32, torch.int64)
+_INT, _F32 = (torch.int32, torch.int64), torch.float32
 
 
 def _check_rotation(cos, sin, positions, lead, D) -> int:
     """Rotated elements of a head."""
     shape = cos.shape
     assert len(shape) == 2 and sin.shape == shape, f"cos and sin must be [positions, rot_dim / 2], both alike: got {tuple(shape)}, {tuple(sin.shape)}"
-    for t in (cos, sin):
-        assert t.dtype == torch.float32 and t.is_contiguous(), "cos and sin must be contiguous float32"
+    assert cos.dtype == _F32 and sin.dtype == _F32 and cos.is_contiguous() and sin.is_contiguous(), "cos and sin must be contiguous float32"
     rot = 2 * shape[1]
     assert 2 <= rot <= D, f"cos and sin turn {rot} elements of a head of {D}"
     assert positions.dtype in _INT and positions.shape == lead, f"positions must be int32 / int64 {tuple(lead)}, got {positions.dtype} {tuple(positions.shape)}"
     return rot
 
 
-def _check_weight(w: Optional[torch.Tensor], D: int) -> Tuple[Optional[int], int]:
-    """(address, type code)"""
+def _check_weight(w: Optional[torch.Tensor], D: int) -> int:
+    """Type code."""
     if w is None:
-        return None, 0
+        return 0
     assert w.shape == (D,) and w.is_contiguous(), f"a weight must be contiguous [{D}], got {tuple(w.shape)}"
     dt = _IN.get(w.dtype)
     if dt is None:
         raise TypeError(f"unsupported weight type {w.dtype}")
-    return w.data_ptr(), dt
+    return dt
 
 
 def _check_eps(eps) -> float:
@@ -49,50 +48,67 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     """[..., H, D] as [T, H, D], in place where the strides allow; D contiguous."""
     if x.dim() != 3:
         x = x.reshape(x.shape[:-2].numel(), *x.shape[-2:])
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+    return x if x.stride(2) == 1 else x.contiguous()
 
 
-def check_qk(q, k, cos, sin, positions, q_weight, k_weight, eps):
-    """(type code, D, rotated elements, eps) after checking all that both directions take."""
-    dtype = q.dtype
-    dt = _IN.get(dtype)
-    if dt is None:
+def check_qk(q, k, cos, sin, positions, q_weight, k_weight, eps) -> float:
+    """eps, after checking all that both directions take."""
+    shape, kshape, dtype = q.shape, k.shape, q.dtype
+    if dtype not in _IN:
         raise TypeError(f"unsupported type of queries and keys {dtype}")
     assert k.dtype == dtype, "q and k must have one type"
-    assert q.dim() >= 2 and k.dim() == q.dim() and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1], (
-        f"q and k must be [..., heads, D] with the same tokens and D, got {tuple(q.shape)}, {tuple(k.shape)}"
+    lead = shape[:-2]
+    assert len(shape) >= 2 and len(kshape) == len(shape) and lead == kshape[:-2] and shape[-1] == kshape[-1], (
+        f"q and k must be [..., heads, D] with the same tokens and D, got {tuple(shape)}, {tuple(kshape)}"
     )
-    D = q.shape[-1]
+    D = shape[-1]
     assert D % 2 == 0 and 2 <= D <= 256, f"head_dim must be even and at most 256, got {D}"
-    rot = _check_rotation(cos, sin, positions, q.shape[:-2], D)
+    _check_rotation(cos, sin, positions, lead, D)
     _check_weight(q_weight, D)
     _check_weight(k_weight, D)
     eps = _check_eps(eps)
     assert not cos.requires_grad and not sin.requires_grad, "cos and sin get no gradients"
-    tensors = [t for t in (q, k, cos, sin, positions, q_weight, k_weight) if t is not None]
-    assert not any(isinstance(t, FakeTensor) for t in tensors), "qk_norm_rope runs on memory: fake tensors have none"
-    first = q.device
-    assert all(t.device == first for t in tensors), f"all tensors must be on {first}"
-    assert first.type == "cuda" or not torch.cuda.is_available(), f"all tensors must be GPU tensors, got {first}"
-    return dt, D, rot, eps
+    # one is enough: they do not go together with tensors that have memory
+    assert not isinstance(q, FakeTensor), "qk_norm_rope runs on memory: fake tensors have none"
+    dev = q.get_device()
+    for t in (k, cos, sin, positions, q_weight, k_weight):
+        assert t is None or (t.get_device() == dev and t.device == q.device), f"all tensors must be on {q.device}"
+    assert dev >= 0 or not torch.cuda.is_available(), f"all tensors must be GPU tensors, got {q.device}"
+    return eps
 
 
 def qk_norm_rope_impl(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved) -> Tuple[torch.Tensor, torch.Tensor]:
     """Arguments as check_qk has passed them."""
-    dt, D = _IN[q.dtype], q.shape[-1]
-    qr, kr = _rows(q), _rows(k)
+    dtype, dev = q.dtype, q.device
+    q_out = torch.empty(q.shape, dtype=dtype, device=dev)
+    k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+    q, k = _rows(q), _rows(k)
     positions = positions.contiguous()
-    T, Hq, _ = qr.shape
-    Hkv, dev = kr.shape[1], q.device
-    (qs, ks), (qw, qwd), (kw, kwd) = (qr.stride(), kr.stride()), _check_weight(q_weight, D), _check_weight(k_weight, D)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    (T, Hq, D), Hkv, (P, half) = q.shape, k.shape[1], cos.shape
+    qs, ks = q.stride(), k.stride()
     _C.call_on(
-        dev, "pta_qk_norm_rope", qr.data_ptr(), kr.data_ptr(), dt, T, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], cos.data_ptr(),
-        sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], positions.data_ptr(), positions.dtype == torch.int64, qw, qwd, kw, kwd,
-        eps, bool(interleaved), q_out.data_ptr(), k_out.data_ptr(), _C.stream(dev),
+        dev, "pta_qk_norm_rope", q.data_ptr(), k.data_ptr(), _IN[dtype], T, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], cos.data_ptr(),
+        sin.data_ptr(), P, 2 * half, positions.data_ptr(), positions.dtype == torch.int64,
+        None if q_weight is None else q_weight.data_ptr(), 0 if q_weight is None else _IN[q_weight.dtype],
+        None if k_weight is None else k_weight.data_ptr(), 0 if k_weight is None else _IN[k_weight.dtype], eps, interleaved,
+        q_out.data_ptr(), k_out.data_ptr(), _C.stream(dev),
     )
     return q_out, k_out
+
+
+_NONE = None, 0, (0, 0), None, (0, 0), None, None, None, 0
+
+
+def _side(g, x, w, want):
+    """What the backward pass takes of the queries or of the keys."""
+    if g is None:
+        return _NONE
+    dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    g = _rows(g)
+    if w is None:
+        return g, g.shape[1], g.stride(), None, (0, 0), dx, None, None, 0
+    x = _rows(x)
+    return g, g.shape[1], g.stride(), x, x.stride(), dx, torch.empty_like(w) if want else None, w.data_ptr(), _IN[w.dtype]
 
 
 def qk_norm_rope_backward_impl(
@@ -100,27 +116,18 @@ def qk_norm_rope_backward_impl(
 ):
     """Gradients of (q, k, q_weight, k_weight); None for gq or gk leaves that side out.
     q and k may be None where they have no weight."""
-    like = gq if gq is not None else gk
+    like = gk if gq is None else gq
     dev, dtype, D = like.device, like.dtype, like.shape[-1]
     positions = positions.contiguous()
-    side = []
-    for g, x, w, want in ((gq, q, q_weight, want_qw), (gk, k, k_weight, want_kw)):
-        if g is None:
-            side.append((None, 0, (0, 0, 0), None, (0, 0, 0), None, None))
-            continue
-        gr, xr = _rows(g), None if w is None else _rows(x)
-        dx = torch.empty(g.shape, dtype=dtype, device=dev)
-        dw = torch.empty_like(w) if want else None
-        side.append((gr, g.shape[-2], gr.stride(), xr, (0, 0, 0) if xr is None else xr.stride(), dx, dw))
-    (gqr, Hq, gqs, qr, qs, dq, dqw), (gkr, Hkv, gks, kr, ks, dk, dkw) = side
-    T = positions.numel()
-    (qw, qwd), (kw, kwd) = _check_weight(q_weight, D), _check_weight(k_weight, D)
+    gq, Hq, gqs, q, qs, dq, dqw, qw, qwd = _side(gq, q, q_weight, want_qw)
+    gk, Hkv, gks, k, ks, dk, dkw, kw, kwd = _side(gk, k, k_weight, want_kw)
+    T, (P, half) = positions.numel(), cos.shape
     nbytes = _C.query("pta_qk_norm_rope_backward_workspace_size", T, Hq, Hkv, D) if want_qw or want_kw else 0
     ws = _C.workspace(nbytes, dev)
     _C.call_on(
-        dev, "pta_qk_norm_rope_backward", _C.ptr(gqr), _C.ptr(gkr), gqs[0], gqs[1], gks[0], gks[1], _C.ptr(qr), _C.ptr(kr),
-        _IN[dtype], T, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
-        positions.data_ptr(), positions.dtype == torch.int64, qw, qwd, kw, kwd, eps, bool(interleaved), _C.ptr(dq), _C.ptr(dk),
+        dev, "pta_qk_norm_rope_backward", _C.ptr(gq), _C.ptr(gk), gqs[0], gqs[1], gks[0], gks[1], _C.ptr(q), _C.ptr(k),
+        _IN[dtype], T, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], cos.data_ptr(), sin.data_ptr(), P, 2 * half,
+        positions.data_ptr(), positions.dtype == torch.int64, qw, qwd, kw, kwd, eps, interleaved, _C.ptr(dq), _C.ptr(dk),
         _C.ptr(dqw), _C.ptr(dkw), _C.ptr(ws), nbytes, _C.stream(dev),
     )
     return dq, dk, dqw, dkw
@@ -142,8 +149,7 @@ def qk_norm_rope_cache_write_impl(
     assert n == T, f"one slot for each of the {T} tokens, got {n}"
     rot = _check_rotation(cos, sin, positions, shape[:1], D)
     assert positions.is_contiguous(), "positions must be contiguous"
-    qw, qwd = _check_weight(q_weight, D)
-    kw, kwd = _check_weight(k_weight, D)
+    qwd, kwd = _check_weight(q_weight, D), _check_weight(k_weight, D)
     eps = _check_eps(eps)
     check_tensors("qk_norm_rope_cache_write", (q, k, v, cos, sin, k_cache, v_cache, k_scale_inv, v_scale_inv, q_weight, k_weight),
                   slots, positions)
@@ -158,7 +164,8 @@ def qk_norm_rope_cache_write_impl(
     _C.call_on(
         dev, "pta_qk_norm_rope_cache_write", q.data_ptr(), k.data_ptr(), v.data_ptr(), _IN[dtype], T, Hq, Hkv, D, qs[0], qs[1],
         ks[0], ks[1], vs[0], vs[1], cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot, positions.data_ptr(),
-        positions.dtype == torch.int64, qw, qwd, kw, kwd, eps, bool(interleaved), slots.data_ptr(), slots.dtype == torch.int64,
+        positions.dtype == torch.int64, None if q_weight is None else q_weight.data_ptr(), qwd,
+        None if k_weight is None else k_weight.data_ptr(), kwd, eps, bool(interleaved), slots.data_ptr(), slots.dtype == torch.int64,
         k_cache.data_ptr(), v_cache.data_ptr(), kind, P, page, k_scale_inv.data_ptr() if fp8 else None,
         v_scale_inv.data_ptr() if fp8 else None, out.data_ptr(), _C.stream(dev),
     )

@@ -72,7 +72,7 @@ def qk_norm_rope(
     no norm.  Gradients go to q, k and the weights; the weights' are summed over all
     tokens and heads in fp32, in a fixed order.  There is no second derivative.
     """
-    _, _, _, eps = check_qk(q, k, cos, sin, positions, q_weight, k_weight, eps)
+    eps = check_qk(q, k, cos, sin, positions, q_weight, k_weight, eps)
     return _QKNormRope.apply(q, k, cos, sin, positions, q_weight, k_weight, eps, bool(interleaved))
 
 
