@@ -15,10 +15,12 @@ namespace pta {
 namespace {
 
 constexpr int KP_NT = 256, KP_RUNS = 5;
-// 16-byte pieces of a thread: four, past the caches, where that gives every CU two workgroups
-// (1000 pages of 8 KB in 16 layers: 102 us, 108 through the caches, 102 with two pieces, 218 with
-// eight), else one, through them (8 pages of 136 KB: 3.1 us, 9.7 with four).
-constexpr int KP_DEPTH = 4;
+// 16-byte pieces of a thread: four where that gives every CU two workgroups (1000 pages of 8 KB in
+// 16 layers: 102 us, 102 with two, 218 with eight), else one (8 pages of 136 KB: 3.1 us, 9.7 with
+// four).  More bytes than the last cache holds go past it (102 us, 108 through it; 48 pages of
+// 139 KB in 8 layers, which the next attention reads: 10.5 and 7.3).
+constexpr int    KP_DEPTH = 4;
+constexpr double KP_CACHED = 256e6;
 constexpr int64_t kp_chunk(int depth) { return static_cast<int64_t>(KP_NT) * depth * 16; } // bytes of a workgroup
 
 struct KPPool {
@@ -32,7 +34,7 @@ struct KPPool {
 };
 
 // Chunk c (of layer and run) of page `to` becomes that of page `from`
-template <int DEPTH> __device__ __forceinline__ void kp_copy(const KPPool &a, int64_t from, int64_t to, int layer, int c) {
+template <int DEPTH, bool PAST> __device__ __forceinline__ void kp_copy(const KPPool &a, int64_t from, int64_t to, int layer, int c) {
     // by comparisons: an index that the compiler does not know would put the arguments into memory
     uint8_t *p = a.p[0];
     int64_t  bytes = a.bytes[0], per_layer = a.layer[0];
@@ -54,13 +56,13 @@ template <int DEPTH> __device__ __forceinline__ void kp_copy(const KPPool &a, in
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) {
             const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
-            if (o < n) v[i] = DEPTH > 1 ? __builtin_nontemporal_load(reinterpret_cast<const piece *>(src + o)) : *reinterpret_cast<const piece *>(src + o);
+            if (o < n) v[i] = PAST ? __builtin_nontemporal_load(reinterpret_cast<const piece *>(src + o)) : *reinterpret_cast<const piece *>(src + o);
         }
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) {
             const int64_t o = (i * KP_NT + static_cast<int>(threadIdx.x)) * 16;
             if (o >= n) continue;
-            if constexpr (DEPTH > 1) __builtin_nontemporal_store(v[i], reinterpret_cast<piece *>(dst + o));
+            if constexpr (PAST) __builtin_nontemporal_store(v[i], reinterpret_cast<piece *>(dst + o));
             else *reinterpret_cast<piece *>(dst + o) = v[i];
         }
     } else {
@@ -73,14 +75,14 @@ __device__ __forceinline__ int64_t kp_index(const void *p, int i64, int64_t i) {
     return i64 ? reinterpret_cast<const int64_t *>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t *>(p)[i]);
 }
 
-template <int DEPTH> __global__ __launch_bounds__(KP_NT) void kp_copy_kernel(KPPool a, const void *src, const void *dst, int i64, int64_t total) {
+template <int DEPTH, bool PAST> __global__ __launch_bounds__(KP_NT) void kp_copy_kernel(KPPool a, const void *src, const void *dst, int i64, int64_t total) {
     const int per = a.chunks * a.layers;
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
         const int64_t pair = w / per;
         const int     rest = static_cast<int>(w - pair * per), layer = rest / a.chunks;
         const int64_t s = kp_index(src, i64, pair), d = kp_index(dst, i64, pair);
         if (s < 0 || s >= a.pages || d < 0 || d >= a.pages || s == d) continue;
-        kp_copy<DEPTH>(a, s, d, layer, rest - layer * a.chunks);
+        kp_copy<DEPTH, PAST>(a, s, d, layer, rest - layer * a.chunks);
     }
 }
 
@@ -257,7 +259,7 @@ template <bool LDS> __global__ __launch_bounds__(KF_NT) void kf_plan_kernel(KFAr
 }
 
 // The first N workgroups write the sequences' rows, the others copy pages
-template <int DEPTH> __global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) {
+template <int DEPTH, bool PAST> __global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KFArgs a, KPPool pool) {
     const int i = blockIdx.x;
     if (i < a.N) {
         const KFSeq s = kf_seq(a, i);
@@ -284,12 +286,18 @@ template <int DEPTH> __global__ __launch_bounds__(KP_NT) void kf_apply_kernel(KF
         const int64_t pair = w / per;
         const int     rest = static_cast<int>(w - pair * per), layer = rest / pool.chunks;
         const int2    p = a.pairs[pair];
-        if (p.x >= 0) kp_copy<DEPTH>(pool, p.x, p.y, layer, rest - layer * pool.chunks);
+        if (p.x >= 0) kp_copy<DEPTH, PAST>(pool, p.x, p.y, layer, rest - layer * pool.chunks);
     }
 }
 
-// `pairs`: of pages to copy at most; sets the pieces of a thread
-int kp_pool(KPPool &a, int &depth, int64_t pairs, void *k_cache, void *v_cache, int kind, int64_t layers, int64_t num_pages, int64_t Hkv,
+// How a copy goes
+struct KPForm {
+    int  depth; // pieces of a thread
+    bool past;  // the caches
+};
+
+// `pairs`: of pages to copy at most
+int kp_pool(KPPool &a, KPForm &form, int64_t pairs, void *k_cache, void *v_cache, int kind, int64_t layers, int64_t num_pages, int64_t Hkv,
             int64_t page_size, int64_t D, float *k_scale, float *v_scale, void *ranges) {
     PTA_CHECK_ARG(kind == PTA_E4M3 || kind == PTA_E5M2 || kind == PTA_CACHE_16BIT, "unknown cache kind %d", kind);
     PTA_CHECK_ARG(layers >= 0 && num_pages >= 0 && page_size > 0 && Hkv > 0, "bad cache sizes");
@@ -308,7 +316,9 @@ int kp_pool(KPPool &a, int &depth, int64_t pairs, void *k_cache, void *v_cache, 
     const int64_t bytes[KP_RUNS] = {data, data, scale, scale, Hkv * D * 4};
     int64_t       all = 0;
     for (int i = 0; i < KP_RUNS; ++i) all += p[i] == nullptr ? 0 : bytes[i];
-    depth = static_cast<double>(all) * layers * pairs < static_cast<double>(kp_chunk(KP_DEPTH)) * 2 * device_cu_count() ? 1 : KP_DEPTH;
+    const double moved = static_cast<double>(all) * layers * pairs;
+    form.depth = moved < static_cast<double>(kp_chunk(KP_DEPTH)) * 2 * device_cu_count() ? 1 : KP_DEPTH;
+    form.past  = form.depth > 1 && 2 * moved > KP_CACHED;
     int64_t chunks = 0;
     for (int i = 0; i < KP_RUNS; ++i) {
         if (p[i] == nullptr) continue;
@@ -318,7 +328,7 @@ int kp_pool(KPPool &a, int &depth, int64_t pairs, void *k_cache, void *v_cache, 
         a.layer[r] = bytes[i] * num_pages;
         a.first[r] = static_cast<int>(chunks);
         a.wide[r]  = aligned16(p[i]) && bytes[i] % 16 == 0;
-        chunks += cdiv(bytes[i], kp_chunk(depth));
+        chunks += cdiv(bytes[i], kp_chunk(form.depth));
     }
     PTA_CHECK_ARG(layers <= INT_MAX / chunks, "too many layers");
     a.chunks = static_cast<int>(chunks);
@@ -356,13 +366,13 @@ extern "C" int pta_kv_cache_copy(void *k_cache, void *v_cache, int cache_kind, i
                                  const void *src_pages, const void *dst_pages, int pages_i64, int64_t num_pairs, pta_stream_t stream) {
     clear_error();
     KPPool a = {};
-    int    depth = 1;
-    if (int rc = kp_pool(a, depth, num_pairs, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    KPForm form = {1, false};
+    if (int rc = kp_pool(a, form, num_pairs, k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
     PTA_CHECK_ARG(num_pairs >= 0 && num_pairs <= INT_MAX, "bad number of pages");
     if (num_pairs == 0 || num_layers == 0 || num_pages == 0) return PTA_OK;
     PTA_CHECK_ARG(src_pages && dst_pages, "null page list");
     const int64_t total = num_pairs * a.chunks * a.layers;
-    const auto    kernel = depth == 1 ? kp_copy_kernel<1> : kp_copy_kernel<KP_DEPTH>;
+    const auto    kernel = form.depth == 1 ? kp_copy_kernel<1, false> : form.past ? kp_copy_kernel<KP_DEPTH, true> : kp_copy_kernel<KP_DEPTH, false>;
     kernel<<<kp_blocks(total), KP_NT, 0, as_stream(stream)>>>(a, src_pages, dst_pages, pages_i64, total);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
@@ -381,8 +391,8 @@ extern "C" int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, i
                                  pta_stream_t stream) {
     clear_error();
     KPPool pool = {};
-    int    depth = 1;
-    if (int rc = kp_pool(pool, depth, num_new_seqs + (compact ? num_pages : 0), k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
+    KPForm form = {1, false};
+    if (int rc = kp_pool(pool, form, num_new_seqs + (compact ? num_pages : 0), k_cache, v_cache, cache_kind, num_layers, num_pages, Hkv, page_size, D, k_scale_inv, v_scale_inv, key_ranges)) return rc;
     PTA_CHECK_ARG(num_seqs >= 0 && num_new_seqs >= 0 && max_pages >= 0 && reserve >= 0, "bad sizes");
     PTA_CHECK_ARG(num_seqs < (1 << 24) && num_new_seqs < (1 << 24) && max_pages <= (INT_MAX - 1024) / page_size &&
                       max_pages <= INT_MAX / 2 / std::max<int64_t>(1, num_new_seqs) - 1,
@@ -422,7 +432,7 @@ extern "C" int pta_kv_cache_fork(void *k_cache, void *v_cache, int cache_kind, i
     }
     PTA_CHECK_LAUNCH();
     const int64_t total = num_pages > 0 ? p.pairs * pool.chunks * pool.layers : 0;
-    const auto    apply = depth == 1 ? kf_apply_kernel<1> : kf_apply_kernel<KP_DEPTH>;
+    const auto    apply = form.depth == 1 ? kf_apply_kernel<1, false> : form.past ? kf_apply_kernel<KP_DEPTH, true> : kf_apply_kernel<KP_DEPTH, false>;
     apply<<<static_cast<unsigned>(a.N) + kp_blocks(total), KP_NT, 0, st>>>(a, pool);
     PTA_CHECK_LAUNCH();
     return PTA_OK;
