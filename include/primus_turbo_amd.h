@@ -670,8 +670,8 @@ int pta_select_pages(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq,
                      size_t workspace_bytes, pta_stream_t stream);
 
 /* pta_paged_attention over the pages that pta_select_pages takes, without a window. */
-size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
-                                                 int64_t page_size, int64_t num_selected);
+size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D,
+                                                 int64_t max_pages, int64_t page_size, int64_t num_selected);
 int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t,
                                int64_t q_stride_h, const void *k_cache, const void *v_cache, int cache_kind,
                                int64_t num_pages, int64_t page_size, int64_t Hkv, const float *k_scale_inv,

@@ -33,7 +33,8 @@ struct PSArgs {
     int64_t         table_st;
     const int32_t  *cu, *lens;
     uint64_t       *keys;    // workspace: [tokens of a slice, Hkv, M] scores as ordered whole numbers
-    int32_t        *sel;     // [T, Hkv, K] pages of the pool, rising in the sequence; -1 behind the last
+    int32_t        *sel;      // [T, Hkv, K] pages of the pool, rising in the sequence; -1 behind the last
+    PSTiles         tiles;    // tokens > 0: lists for tiles instead
     int32_t        *sel_lens; // [T] keys of them that the token sees
     int32_t        *sel_cu;  // [T + 1] 0, 1, 2, ... (may be null)
     int             T, B, Hq, Hkv, G, D, M, P, page;
@@ -375,11 +376,54 @@ __device__ __forceinline__ void ps_common(uint32_t &all, uint32_t &any) {
     any = __builtin_amdgcn_readfirstlane(y[0] | y[1]);
 }
 
-// NW waves for (token, head), wave w with keys [64 w E, 64 (w + 1) E), E a lane; what
-// does not fit is read again for every step.  The bits of the least key that is taken are
-// found from the highest that differs on: a bit is set if enough keys have it; the search
-// ends when exactly as many are left.  Bound by its steps, about 3 E instructions each (and
-// for more than one wave a barrier).
+// Bits of the high halves that all scores of a wave have, or any; not of pages taken always
+template <int E> __device__ __forceinline__ void ps_bits(const uint64_t (&key)[E], uint32_t &common, uint32_t &any) {
+    common = ~0u;
+    any    = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t x = static_cast<uint32_t>(key[e] >> 32);
+        common &= key[e] + 1 > 1 ? x : ~0u;
+        any |= key[e] + 1 > 1 ? x : 0u;
+    }
+    ps_common(common, any);
+}
+
+// The least of the `take` largest of a wave's keys (0: none): its bits from the highest that
+// differs on; a bit is set if enough keys have it.  The search ends when exactly as many are
+// left.  The high halves come first, whose comparisons are cheaper: all but ties differ there.
+template <int E> __device__ __forceinline__ uint64_t ps_least(const uint64_t (&key)[E], int take) {
+    uint32_t common, any;
+    ps_bits<E>(key, common, any);
+    const int top   = 31 - __clz(common ^ any); // -1: they differ in none
+    uint64_t  least = static_cast<uint64_t>(top < 0 ? any : any & ~((2u << top) - 1)) << 32;
+    for (int bit = top; bit >= 0; --bit) {
+        const uint32_t cand = static_cast<uint32_t>(least >> 32) | (1u << bit);
+        int            c = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(static_cast<uint32_t>(key[e] >> 32) >= cand));
+        if (c >= take) least = static_cast<uint64_t>(cand) << 32;
+        if (c == take) return least; // all of these and no others
+    }
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint64_t cand = least | (1ull << bit);
+        int            c = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(key[e] >= cand));
+        if (c >= take) least = cand;
+        if (c == take) return least;
+    }
+    return least;
+}
+
+// A page's key in the choice: that of its score, above all of them for the first and last pages
+__device__ __forceinline__ uint64_t ps_at(const PSArgs &a, const uint64_t *keys, int own, int j) {
+    return j < a.first || own - j < a.last ? ~0ull : keys[j];
+}
+
+// NW waves for (token, head), wave w with keys [64 w E, 64 (w + 1) E), E a lane; what does
+// not fit is read again for every step of the search.  Bound by its steps, about 3 E
+// instructions each, and for more than one wave a barrier.
 template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_kernel(PSArgs a) {
     constexpr int  CAP = 64 * NW * E;
     __shared__ int cnt[2][2][NW];
@@ -403,18 +447,12 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
         for (int j = threadIdx.x; j < n; j += 64 * NW) sel[j] = row[j];
         return;
     }
-    // the `first` and `last` pages are above all scores
     const uint64_t *in = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
-    auto            at = [&](int j) { return j < a.first || own - j < a.last ? ~0ull : in[j]; };
     uint64_t        key[E];
-    uint32_t        common = ~0u, any = 0; // bits that all scores have, or any
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int j = (wave * E + e) * 64 + lane;
-        key[e]      = j < n ? at(j) : 0; // below every score
-        const uint32_t x = static_cast<uint32_t>(key[e] >> 32);
-        common &= key[e] + 1 > 1 ? x : ~0u;
-        any |= key[e] + 1 > 1 ? x : 0u;
+        key[e]      = j < n ? ps_at(a, in, own, j) : 0; // below every score
     }
     // sums of x and of y over the workgroup, and over the waves before
     int  buf = 0;
@@ -440,53 +478,42 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
             buf ^= 1;
         }
     };
-    // of the high halves first, whose comparisons are cheaper: all but ties differ there
     uint64_t least = 0;
-    bool     done  = false;
-    int      top   = 31; // highest bit in which scores differ
-    if (n <= CAP) {
-        ps_common(common, any);
-        if constexpr (NW > 1) {
+    if constexpr (NW == 1) { // all keys fit
+        least = ps_least<E>(key, take);
+    } else {
+        bool done = false;
+        int  top  = 63;
+        if (n <= CAP) {
+            uint32_t common, any;
+            ps_bits<E>(key, common, any);
             if (lane == 0) {
                 cnt[1][0][wave] = static_cast<int>(common);
                 cnt[1][1][wave] = static_cast<int>(any);
             }
-            __syncthreads();
+            __syncthreads(); // the next to write there comes behind the next barrier but one
             for (int w = 0; w < NW; ++w) {
                 common &= static_cast<uint32_t>(cnt[1][0][w]);
                 any |= static_cast<uint32_t>(cnt[1][1][w]);
             }
+            top   = 63 - __clz(common ^ any); // 31: they differ in none
+            least = static_cast<uint64_t>(top < 32 ? any : any & ~((2u << (top - 32)) - 1)) << 32;
         }
-        top   = 31 - __clz(common ^ any); // -1: in none
-        least = static_cast<uint64_t>(top < 0 ? any : any & ~((2u << top) - 1)) << 32;
-    }
-    for (int bit = top; bit >= 0 && !done; --bit) {
-        const uint32_t cand = static_cast<uint32_t>(least >> 32) | (1u << bit);
-        int            c = 0;
+        for (int bit = top; bit >= 0 && !done; --bit) {
+            const uint64_t cand = least | (1ull << bit);
+            int            c = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) c += __popcll(__ballot(static_cast<uint32_t>(key[e] >> 32) >= cand));
-        for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
-            const int j = j0 + static_cast<int>(threadIdx.x);
-            c += __popcll(__ballot(j < n && static_cast<uint32_t>(at(min(j, n - 1)) >> 32) >= cand));
+            for (int e = 0; e < E; ++e)
+                c += __popcll(__ballot(bit >= 32 ? static_cast<uint32_t>(key[e] >> 32) >= static_cast<uint32_t>(cand >> 32) : key[e] >= cand));
+            for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
+                const int j = j0 + static_cast<int>(threadIdx.x);
+                c += __popcll(__ballot(j < n && ps_at(a, in, own, min(j, n - 1)) >= cand));
+            }
+            int total, none, b0, b1;
+            all(c, 0, total, none, b0, b1);
+            if (total >= take) least = cand;
+            done = total == take;
         }
-        int total, none, b0, b1;
-        all(c, 0, total, none, b0, b1);
-        if (total >= take) least = static_cast<uint64_t>(cand) << 32;
-        done = total == take; // all of these and no others
-    }
-    for (int bit = 31; bit >= 0 && !done; --bit) {
-        const uint64_t cand = least | (1ull << bit);
-        int            c = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) c += __popcll(__ballot(key[e] >= cand));
-        for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
-            const int j = j0 + static_cast<int>(threadIdx.x);
-            c += __popcll(__ballot(j < n && at(min(j, n - 1)) >= cand));
-        }
-        int total, none, b0, b1;
-        all(c, 0, total, none, b0, b1);
-        if (total >= take) least = cand;
-        done = total == take;
     }
     // all above the least, and of those equal to it the first ones
     int above = 0, equal = 0, sa, se, ba, be;
@@ -499,7 +526,7 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     int more = 0; // above, beyond what fits
     for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
         const int j = j0 + static_cast<int>(threadIdx.x);
-        more += __popcll(__ballot(j < n && at(min(j, n - 1)) > least));
+        more += __popcll(__ballot(j < n && ps_at(a, in, own, min(j, n - 1)) > least));
     }
     int sm, s0, b0, b1;
     all(more, 0, sm, s0, b0, b1);
@@ -520,7 +547,7 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     int g0 = sa, q0 = se;
     for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
         const int      j = j0 + static_cast<int>(threadIdx.x);
-        const uint64_t x = at(min(j, n - 1));
+        const uint64_t x = ps_at(a, in, own, min(j, n - 1));
         const bool     gt = j < n && x > least, eq = j < n && x == least;
         int            tg, tq, wg, wq;
         all(__popcll(__ballot(gt)), __popcll(__ballot(eq)), tg, tq, wg, wq);
@@ -531,13 +558,95 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     }
 }
 
+// Chunks: a workgroup for (tile of tokens, head), a wave a token.  The pages that any of the
+// tile's tokens takes become one list in the order of the sequence, with a bit for each token
+// that takes the page; sequence after sequence where the tile has tokens of several.
+template <int E> __global__ __launch_bounds__(1024) void ps_choose_tile_kernel(PSArgs a) {
+    __shared__ uint64_t bits[16][E]; // by token: pages 64 e + lane
+    __shared__ int      seq[16], pages[16], sum[16];
+    const int           tile = a.t0 / a.tiles.tokens + blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv, tt = a.tiles.tokens;
+    const int           lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = tile * tt + wave;
+    PSToken             s = {-1, -1, 0, 0, 0};
+    if (t < a.T) s = ps_token(a, t);
+    const bool some = s.b >= 0 && s.pos >= 0;
+    const int  own = some ? s.pos / a.page : -1, n = own + 1, take = min(n, a.take);
+    if (h == 0 && lane == 0 && t < a.T) {
+        a.sel_lens[t]  = some ? (take - 1) * a.page + (s.pos - own * a.page) + 1 : 0;
+        a.tiles.pos[t] = some ? s.pos : -1;
+        a.sel_cu[t]    = t;
+        if (t == a.T - 1) a.sel_cu[a.T] = a.T;
+    }
+    if (lane == 0) {
+        seq[wave]   = some ? s.b : -1;
+        pages[wave] = n;
+    }
+    uint64_t key[E];
+    if (n > a.take) {
+        const uint64_t *in = a.keys + (static_cast<int64_t>(t - a.t0) * a.Hkv + h) * a.M;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = e * 64 + lane;
+            key[e]      = j < n ? ps_at(a, in, own, j) : 0;
+        }
+        const uint64_t least = ps_least<E>(key, take);
+        int            above = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) above += __popcll(__ballot(key[e] > least));
+        int room = take - above; // of the equal ones
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint64_t eq = __ballot(key[e] == least);
+            const uint64_t m  = __ballot(key[e] > least || (key[e] == least && __popcll(eq & ((1ull << lane) - 1)) < room));
+            room -= min(room, static_cast<int>(__popcll(eq)));
+            if (lane == 0) bits[wave][e] = m;
+        }
+    } else {
+        for (int e = lane; e < E; e += 64) bits[wave][e] = n >= 64 * (e + 1) ? ~0ull : n > 64 * e ? (1ull << (n - 64 * e)) - 1 : 0;
+    }
+    __syncthreads();
+    const int64_t at = (static_cast<int64_t>(tile) * a.Hkv + h) * a.tiles.cap;
+    int           count = 0;
+    for (int i0 = 0; i0 < tt;) {
+        const int b = seq[i0];
+        int       i1 = i0 + 1;
+        while (i1 < tt && seq[i1] == b) ++i1;
+        if (b >= 0) {
+            const int32_t *row = a.table + b * a.table_st;
+            for (int j0 = 0; j0 < pages[i1 - 1]; j0 += 64 * tt) {
+                const int j = j0 + static_cast<int>(threadIdx.x);
+                uint32_t  mask = 0;
+                if (j < 64 * E)
+                    for (int i = i0; i < i1; ++i) mask |= static_cast<uint32_t>(bits[i][j >> 6] >> (j & 63) & 1) << i;
+                const uint64_t m = __ballot(mask != 0);
+                if (lane == 0) sum[wave] = __popcll(m);
+                __syncthreads();
+                int before = count + __popcll(m & ((1ull << lane) - 1));
+                for (int w = 0; w < tt; ++w) {
+                    if (w < wave) before += sum[w];
+                    count += sum[w];
+                }
+                if (mask != 0) {
+                    a.tiles.list[at + before]  = make_int2(row[j], j * a.page);
+                    a.tiles.masks[at + before] = static_cast<uint16_t>(mask);
+                }
+                __syncthreads(); // the sums are read
+            }
+        }
+        i0 = i1;
+    }
+    if (threadIdx.x == 0) a.tiles.counts[tile * a.Hkv + h] = count;
+}
+
 // Keys of a slice of tokens at most: 256 MB, or one token's
 constexpr int64_t PS_SLICE = 256 << 20;
-int64_t ps_slice(int64_t T, int64_t Hkv, int64_t M) { return std::max<int64_t>(1, std::min<int64_t>(T, PS_SLICE / std::max<int64_t>(1, Hkv * M * 8))); }
+// a multiple of `tile` tokens
+int64_t ps_slice(int64_t T, int64_t Hkv, int64_t M, int64_t tile) {
+    return std::min<int64_t>(T, std::max<int64_t>(1, PS_SLICE / std::max<int64_t>(1, Hkv * M * 8) / tile) * tile);
+}
 
 } // namespace
 
-size_t ps_workspace(int64_t T, int64_t Hkv, int64_t M) { return static_cast<size_t>(ps_slice(T, Hkv, M) * Hkv * M * 8); }
+size_t ps_workspace(int64_t T, int64_t Hkv, int64_t M, int64_t tile) { return static_cast<size_t>(ps_slice(T, Hkv, M, tile) * Hkv * M * 8); }
 
 int ps_check(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size, int64_t max_pages,
              int64_t take, int64_t first, int64_t last) {
@@ -575,7 +684,7 @@ template <int QT> static void ps_score(const PSArgs &a, hipStream_t st) {
 
 static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
     a.keys = static_cast<uint64_t *>(workspace);
-    const int step = static_cast<int>(ps_slice(a.T, a.Hkv, a.M));
+    const int tile = a.tiles.tokens, step = static_cast<int>(ps_slice(a.T, a.Hkv, a.M, std::max(1, tile)));
     for (a.t0 = 0; a.t0 < a.T; a.t0 += step) {
         a.n = std::min(step, a.T - a.t0);
         if (a.M > a.take) {
@@ -583,8 +692,12 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
             else ps_score<PTA_F16>(a, st);
             PTA_CHECK_LAUNCH();
         }
-        const unsigned grid = static_cast<unsigned>(a.n) * a.Hkv;
-        if (a.M <= 256) ps_choose_kernel<1, 4><<<grid, 64, 0, st>>>(a);
+        const unsigned grid = static_cast<unsigned>(tile > 0 ? cdiv(a.n, tile) : a.n) * a.Hkv, threads = 64 * tile;
+        if (tile > 0) {
+            if (a.M <= 256) ps_choose_tile_kernel<4><<<grid, threads, 0, st>>>(a);
+            else if (a.M <= 512) ps_choose_tile_kernel<8><<<grid, threads, 0, st>>>(a);
+            else ps_choose_tile_kernel<16><<<grid, threads, 0, st>>>(a);
+        } else if (a.M <= 256) ps_choose_kernel<1, 4><<<grid, 64, 0, st>>>(a);
         else if (a.M <= 512) ps_choose_kernel<1, 8><<<grid, 64, 0, st>>>(a);
         else if (a.M <= 2048) ps_choose_kernel<8, 4><<<grid, 512, 0, st>>>(a);
         else ps_choose_kernel<16, 8><<<grid, 1024, 0, st>>>(a);
@@ -636,20 +749,20 @@ extern "C" int pta_kv_page_ranges(const void *k_cache, int cache_kind, int is_f1
 
 extern "C" size_t pta_select_pages_workspace_size(int64_t num_tokens, int64_t Hkv, int64_t max_pages) {
     if (num_tokens <= 0 || Hkv <= 0 || max_pages <= 0) return 0;
-    return ps_workspace(num_tokens, Hkv, max_pages);
+    return ps_workspace(num_tokens, Hkv, max_pages, 1);
 }
 
 namespace pta {
 int ps_select(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
               const void *key_ranges, int64_t num_pages, int64_t page_size, int64_t Hkv, const int32_t *page_table, int64_t table_stride,
               int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs, int64_t num_selected,
-              int64_t num_first, int64_t num_last, int32_t *selected, int32_t *selected_lens, int32_t *selected_cu, void *workspace,
-              hipStream_t st) {
+              int64_t num_first, int64_t num_last, int32_t *selected, const PSTiles *tiles, int32_t *selected_lens, int32_t *selected_cu,
+              void *workspace, hipStream_t st) {
     PTA_CHECK_ARG(q_dtype == PTA_BF16 || q_dtype == PTA_F16, "queries must be bfloat16 or float16 (type %d)", q_dtype);
     if (int rc = ps_check(num_tokens, num_seqs, Hq, Hkv, D, num_pages, page_size, max_pages, num_selected, num_first, num_last)) return rc;
     if (num_tokens == 0) return PTA_OK;
     PTA_CHECK_ARG(num_seqs > 0, "tokens without a sequence");
-    PTA_CHECK_ARG(q && cu_seqlens_q && seq_lens && selected_lens && (max_pages == 0 || (page_table && selected)) && (num_pages == 0 || key_ranges),
+    PTA_CHECK_ARG(q && cu_seqlens_q && seq_lens && selected_lens && (max_pages == 0 || (page_table && (selected || tiles))) && (num_pages == 0 || key_ranges),
                   "null pointer");
     PTA_CHECK_ARG(aligned16(q) && aligned16(key_ranges) && q_stride_t % 8 == 0 && q_stride_h % 8 == 0,
                   "queries and ranges must be 16-byte aligned, with strides of multiples of 8 elements");
@@ -657,6 +770,7 @@ int ps_select(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_
     a.q = static_cast<const uint16_t *>(q); a.q_st = q_stride_t; a.q_sh = q_stride_h;
     a.ranges = static_cast<const uint16_t *>(key_ranges);
     a.table = page_table; a.table_st = table_stride; a.cu = cu_seqlens_q; a.lens = seq_lens;
+    if (tiles != nullptr) a.tiles = *tiles;
     a.sel = selected; a.sel_lens = selected_lens; a.sel_cu = selected_cu;
     a.T = static_cast<int>(num_tokens); a.B = static_cast<int>(num_seqs); a.Hq = static_cast<int>(Hq); a.Hkv = static_cast<int>(Hkv);
     a.G = static_cast<int>(Hq / Hkv); a.D = static_cast<int>(D); a.M = static_cast<int>(max_pages); a.P = static_cast<int>(num_pages);
@@ -677,6 +791,6 @@ extern "C" int pta_select_pages(const void *q, int q_dtype, int64_t num_tokens, 
     PTA_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), "workspace too small: %zu bytes needed, %zu given",
                   need, workspace_bytes);
     return ps_select(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, key_ranges, num_pages, page_size, Hkv, page_table, table_stride,
-                     max_pages, cu_seqlens_q, seq_lens, num_seqs, num_selected, num_first, num_last, selected, selected_lens, nullptr,
+                     max_pages, cu_seqlens_q, seq_lens, num_seqs, num_selected, num_first, num_last, selected, nullptr, selected_lens, nullptr,
                      workspace, as_stream(stream));
 }

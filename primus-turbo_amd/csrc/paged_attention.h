@@ -38,6 +38,7 @@
 #include <utility>
 
 #include "common.h"
+#include "page_select.h"
 
 namespace pta {
 
@@ -69,6 +70,7 @@ struct AttnArgs {
     int             split;      // narrow: chunks of a sequence
     int             part_seq, part_step; // narrow: parts go by sequence, not by token; rows of a chunk's parts
     int             rows_min, rows_max; // sequences of this launch: rows_min < n G <= rows_max
+    PSTiles         tiles;      // narrow, tiles of tokens: the B "sequences" are tiles
 };
 
 typedef float    att_f4 __attribute__((ext_vector_type(4)));
@@ -1022,14 +1024,20 @@ template <int DP> struct AttnNarrowLds {
     alignas(16) float ssc[4][3][WK];
     float2 sml[4][BQ];
 };
+// With the keys' positions, and which tokens of the tile see them
+template <int DP> struct AttnTileLds : AttnNarrowLds<DP> {
+    alignas(16) int skey[4][2][32];
+};
 
-template <int QT, int KIND, int DP>
-__device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNarrowLds<DP> &lds) {
+// TILE: the rows are a tile of tokens', whatever their sequences, the keys those of the tile's
+// list of pages, each with its position and the tokens that take its page.
+template <int QT, int KIND, int DP, bool TILE, class Lds>
+__device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &lds) {
     constexpr int  KT = ATT_NARROW_KEYS, BQ = ATT_NARROW_ROWS, WK = 32;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
     constexpr int  ES  = FP8 ? 1 : 2;
     constexpr int  EC  = 16 / ES;
-    constexpr int  ST  = DP * ES <= 128 ? 2 : 1;
+    constexpr int  ST  = TILE ? 1 : DP * ES <= 128 ? 2 : 1; // TILE: a third workgroup a CU instead (see attn_tile_kernel)
     constexpr int  KP  = DP / 4 / EC;       // 16-byte pieces of a lane's quarter of a key row
     constexpr int  CPR = DP / EC;           // pieces of a value row
     constexpr int  VP  = WK * CPR / 64;     // value pieces of a lane
@@ -1039,19 +1047,29 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
 
     const int     tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int     h = block % a.Hkv, w0 = block / a.Hkv, chunk = w0 % a.split, b = w0 / a.split;
-    const AttnSeq sq   = attn_seq(a, b);
+    AttnSeq       sq;
+    const int64_t tile_head = static_cast<int64_t>(b) * a.Hkv + h;
+    if constexpr (TILE) {
+        sq.tok0 = b * a.tiles.tokens;
+        sq.n    = min(a.tiles.tokens, a.Tq - sq.tok0);
+        sq.len  = a.tiles.counts[tile_head] * a.page; // keys of the list
+    } else {
+        sq = attn_seq(a, b);
+    }
     const int     n    = __builtin_amdgcn_readfirstlane(sq.n), len = __builtin_amdgcn_readfirstlane(sq.len);
     const int     tok0 = __builtin_amdgcn_readfirstlane(sq.tok0);
     const int     c = lane & 15, qd = lane >> 4;
     uint16_t     *V = reinterpret_cast<uint16_t *>(smem) + wave * WK * VS;
-    const int32_t *pages = a.table + b * a.table_st + h * a.table_sh;
+    const int32_t  *pages = TILE ? nullptr : a.table + b * a.table_st + h * a.table_sh;
+    const int2     *list  = TILE ? a.tiles.list + tile_head * a.tiles.cap : nullptr;
+    const uint16_t *masks = TILE ? a.tiles.masks + tile_head * a.tiles.cap : nullptr;
 
     for (int row0 = 0; row0 < n * a.G; row0 += BQ) {
         AttnItem it;
         it.b    = b;
         it.row0 = row0;
         it.rows = min(BQ, n * a.G - it.row0);
-        it.pos0 = len - n;
+        it.pos0 = TILE ? len - 1 : len - n; // TILE: no row is what ends the keys
         const int total = attn_keys<KT>(a, it, len);
         const int per   = (total + a.split - 1) / a.split;
         it.t0           = min(chunk * per, total);
@@ -1061,19 +1079,37 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
         const bool rin  = c < it.rows;
         const int  rtok = rin ? r / a.G : 0;
         const int  hq   = h * a.G + (rin ? r - rtok * a.G : 0);
-        const int  pos  = rin ? it.pos0 + rtok : -1;
+        // position of a row's token, below 0 where it sees nothing
+        auto       place = [&](int rt) PTA_INLINE { return TILE ? a.tiles.pos[tok0 + rt] : it.pos0 + rt; };
+        const int  pos  = rin ? place(rtok) : -1;
         const int  wlo  = a.window > 0 ? pos - a.window + 1 : INT_MIN;
-        const bool mixed = a.window > 0 || it.row0 / a.G != (it.row0 + it.rows - 1) / a.G; // rows may see different keys
+        const bool mixed = TILE || a.window > 0 || it.row0 / a.G != (it.row0 + it.rows - 1) / a.G; // rows may see different keys
 
         uint4    kreg[ST][2][KP], vreg[ST][VP];
         float    scl[ST][2];
         int      krow[ST], page_id = -1;
+        int2     kinfo[TILE ? ST : 1], page_info = make_int2(0, 0); // position of the lane's key, its page's tokens
         uint64_t hole[ST];
         auto     key = [&](int t) PTA_INLINE { return attn_key0(it, t, KT) + wave * WK + (lane & 31); };
-        auto     fetch_page = [&](int t) PTA_INLINE { page_id = t < it.t1 ? attn_key_page(a, it, pages, key(t)) : -1; };
+        auto     fetch_page = [&](int t) PTA_INLINE {
+            if constexpr (TILE) {
+                page_id   = -1;
+                page_info = make_int2(0, 0);
+                const int j = t < it.t1 ? key(t) : it.kend;
+                if (j < it.kend) {
+                    const int  e = attn_page_of(a, j);
+                    const int2 x = list[e];
+                    page_id      = x.x;
+                    page_info    = make_int2(x.y + (j - e * a.page), masks[e]);
+                }
+            } else {
+                page_id = t < it.t1 ? attn_key_page(a, it, pages, key(t)) : -1;
+            }
+        };
         // loads tile t, whose pages were fetched before; keys without a row read row 0
         // and become zeros when they are used
-        auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no) PTA_INLINE {
+        auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no, int2 &info) PTA_INLINE {
+            if constexpr (TILE) info = page_info;
             row = t < it.t1 ? attn_page_row(a, h, key(t), page_id) : -1;
             no  = __ballot(row < 0);
             const int at = max(row, 0);
@@ -1116,7 +1152,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
 
         att_each<ST>([&](auto u_c) PTA_INLINE {
             constexpr int u = decltype(u_c)::value;
-            load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u]);
+            load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
             fetch_page(it.t0 + u + 1);
         });
         for (int tt = it.t0; tt < it.t1; tt += ST)
@@ -1178,7 +1214,13 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
                             kf[k][s] = kreg[u][k][s];
                         }
                     }
-                load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u]);
+                if constexpr (TILE) {
+                    if (lane < WK) {
+                        lds.skey[wave][0][lane] = kinfo[u].x;
+                        lds.skey[wave][1][lane] = kinfo[u].y;
+                    }
+                }
+                load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
                 fetch_page(t + ST + 1);
                 att_f4 s[2];
 #pragma unroll
@@ -1208,10 +1250,17 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
 #pragma unroll
                         for (int j = 0; j < 4; ++j) s[k][j] *= a.scale_log2;
                     }
+                    int4 kp, km;
+                    if constexpr (TILE) {
+                        kp = *reinterpret_cast<const int4 *>(&lds.skey[wave][0][kk]);
+                        km = *reinterpret_cast<const int4 *>(&lds.skey[wave][1][kk]);
+                    }
+                    const int kpos[4] = {kp.x, kp.y, kp.z, kp.w}, kmask[4] = {km.x, km.y, km.z, km.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int  ky  = key0 + kk + j;
-                        const bool see = (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
+                        const bool see = TILE ? (kpos[j] <= pos) & ((kmask[j] >> rtok & 1) != 0)
+                                              : (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
                         s[k][j]        = see ? s[k][j] : -INFINITY;
                         mx             = fmaxf(mx, s[k][j]);
                     }
@@ -1291,7 +1340,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
             const int     rr = it.row0 + jr, rt = rr / a.G;
             const int64_t orow = static_cast<int64_t>(tok0 + rt) * a.Hq + h * a.G + (rr - rt * a.G);
             if (a.split == 1) {
-                const float inv = att_inverse(ll, it.pos0 + rt < 0);
+                const float inv = att_inverse(ll, place(rt) < 0);
 #pragma unroll
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
@@ -1304,7 +1353,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, AttnNa
                 for (int e = 0; e < DPT; e += 4)
                     if (jd + e < a.D)
                         *reinterpret_cast<float4 *>(a.part_o + at * a.D + jd + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                if (jd == 0) a.part_ml[at] = make_float2(att_part_max(mm, it.pos0 + rt < 0), ll);
+                if (jd == 0) a.part_ml[at] = make_float2(att_part_max(mm, place(rt) < 0), ll);
             }
         }
         __syncthreads(); // the outputs' LDS becomes the values' of the next row tile
@@ -1341,8 +1390,17 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
 template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_narrow_kernel(AttnArgs a, int pads) {
     __shared__ AttnNarrowLds<DP> lds;
     const int block = blockIdx.x, work = gridDim.x - pads;
-    if (block < work) attn_narrow<QT, KIND, DP>(a, block, lds);
+    if (block < work) attn_narrow<QT, KIND, DP, false>(a, block, lds);
     else attn_pad(a, block - work, pads);
+}
+// Bound by the vector instructions of a tile of 32 keys a wave, 380, and their waits: the keys
+// come from the L2 (97% of the reads hit).  Three workgroups a CU with one tile in flight:
+// 1024 tokens, 37 pages of 64 in a tile's list of 32 / 8 heads of 128, ATT_TILE_3 us; two with two in
+// flight ATT_TILE_2.
+template <int QT, int KIND, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 && KIND == PTA_CACHE_16BIT ? 2 : 3) void attn_tile_kernel(AttnArgs a) {
+    __shared__ AttnTileLds<DP> lds;
+    attn_narrow<QT, KIND, DP, true>(a, blockIdx.x, lds);
 }
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnArgs w, AttnArgs n, int w_blocks, int pads) {
@@ -1353,7 +1411,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnA
     } lds;
     const int block = blockIdx.x, work = gridDim.x - pads;
     if (block < w_blocks) attn_wide<QT, KIND, DP>(w, block, lds.w);
-    else if (block < work) attn_narrow<QT, KIND, DP>(n, block - w_blocks, lds.n);
+    else if (block < work) attn_narrow<QT, KIND, DP, false>(n, block - w_blocks, lds.n);
     else attn_pad(n, block - work, pads);
 }
 
@@ -1451,6 +1509,10 @@ struct AttnCall {
     int      pads;              // workgroups for the tokens of no sequence
 };
 template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st);
+// Tiles of tokens (a.tiles; a.B tiles), and the join of their chunks, token by token
+template <int QT> void attn_launch_tiles(const AttnArgs &a, int kind, hipStream_t st);
+extern template void attn_launch_tiles<PTA_BF16>(const AttnArgs &, int, hipStream_t);
+extern template void attn_launch_tiles<PTA_F16>(const AttnArgs &, int, hipStream_t);
 extern template void attn_launch<PTA_BF16>(const AttnCall &, int, hipStream_t);
 extern template void attn_launch<PTA_F16>(const AttnCall &, int, hipStream_t);
 

@@ -116,14 +116,14 @@ extern "C" size_t pta_paged_attention_workspace_size(int64_t num_tokens, int64_t
     return attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size).bytes();
 }
 
+// Checks the arguments that every form takes, and fills the kernels'.
 // table_stride_h: of a page table with a row for each cache head, whose sequences are single
 // tokens (so that the narrow form alone runs) of about the same length; 0: one row for all
-static int attn_call(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
-                     const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
-                     const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table, int64_t table_stride,
-                     int64_t table_stride_h, int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs,
-                     float softmax_scale, int64_t window_size, int64_t num_sinks, void *out, float *lse, void *workspace,
-                     size_t workspace_bytes, pta_stream_t stream) {
+static int attn_arguments(AttnArgs &a, const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
+                          const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                          const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table, int64_t table_stride,
+                          int64_t table_stride_h, int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs,
+                          float softmax_scale, int64_t window_size, int64_t num_sinks, void *out, float *lse) {
     PTA_CHECK_ARG(q_dtype == PTA_BF16 || q_dtype == PTA_F16, "queries must be bfloat16 or float16 (type %d)", q_dtype);
     PTA_CHECK_ARG(cache_kind == PTA_E4M3 || cache_kind == PTA_E5M2 || cache_kind == PTA_CACHE_16BIT,
                   "unknown cache kind %d", cache_kind);
@@ -150,11 +150,7 @@ static int attn_call(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq,
         PTA_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "cache pools must be 16-byte aligned");
         PTA_CHECK_ARG(cache_kind == PTA_CACHE_16BIT || (k_scale_inv && v_scale_inv), "an fp8 cache needs its scales");
     }
-    const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, table_stride_h != 0);
-    PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
-                  "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
-    AttnArgs a = {};
+    a = {};
     a.q = static_cast<const uint16_t *>(q);
     a.q_st = q_stride_t; a.q_sh = q_stride_h;
     a.kc = static_cast<const uint8_t *>(k_cache); a.vc = static_cast<const uint8_t *>(v_cache);
@@ -174,6 +170,25 @@ static int attn_call(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq,
         a.kc = a.vc = static_cast<const uint8_t *>(q);
         a.ks = a.vs = static_cast<const float *>(q);
     }
+    return PTA_OK;
+}
+
+static int attn_call(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t, int64_t q_stride_h,
+                     const void *k_cache, const void *v_cache, int cache_kind, int64_t num_pages, int64_t page_size, int64_t Hkv,
+                     const float *k_scale_inv, const float *v_scale_inv, const int32_t *page_table, int64_t table_stride,
+                     int64_t table_stride_h, int64_t max_pages, const int32_t *cu_seqlens_q, const int32_t *seq_lens, int64_t num_seqs,
+                     float softmax_scale, int64_t window_size, int64_t num_sinks, void *out, float *lse, void *workspace,
+                     size_t workspace_bytes, pta_stream_t stream) {
+    AttnArgs a;
+    if (int rc = attn_arguments(a, q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size,
+                                Hkv, k_scale_inv, v_scale_inv, page_table, table_stride, table_stride_h, max_pages, cu_seqlens_q, seq_lens,
+                                num_seqs, softmax_scale, window_size, num_sinks, out, lse))
+        return rc;
+    if (num_tokens == 0) return PTA_OK;
+    const AttnPlan p = attn_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, table_stride_h != 0);
+    PTA_CHECK_ARG(p.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes()),
+                  "workspace too small: %zu bytes needed, %zu given", p.bytes(), workspace_bytes);
+    PTA_CHECK_ARG((std::max<int64_t>(p.part[0].split, ATT_JOIN_PARTS) * num_seqs + ATT_JOIN_PARTS * p.part[1].slots) * Hkv <= INT_MAX / 4, "too many row tiles for one call");
     AttnCall c = {};
     c.has_narrow = p.part[0].rows > 0;
     c.has_wide   = p.part[1].rows > 0;
@@ -221,30 +236,51 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
                      window_size, num_sinks, out, lse, workspace, workspace_bytes, stream);
 }
 
-// The workspace of attention through selected pages: their numbers, how many keys of them
-// each token sees, 0, 1, 2, ... for its tokens as sequences, then what the choice and
-// (over the same bytes: it begins when the choice has ended) the attention need.
+// The workspace of attention through selected pages: what was chosen (pages for each token,
+// or lists for tiles of tokens), how many keys of its pages each token sees, 0, 1, 2, ... for
+// its tokens as sequences, then what the choice and, over the same bytes (it begins when the
+// choice has ended), the attention need.
+//
+// Tokens go by tiles of 16 rows where a sequence has two or more of them on average: their
+// pages overlap, and a tile's page is read and converted once for all its rows (1024 tokens
+// over 16384, 32 / 8 heads of 128, 16 of 256 pages: SPARSE_TILES us, token by token
+// SPARSE_TOKENS).  Tables of more than PS_TILE_PAGES pages go token by token: a wave has its
+// token's scores in registers.
 namespace {
 struct SparsePlan {
-    int64_t K;
-    size_t  sel, lens, cu, rest;
-    size_t  bytes() const { return sel + lens + cu + rest; }
+    int64_t  K, tile, tiles, cap; // tile: tokens of a tile, 0: none
+    size_t   sel, masks, counts, pos, lens, cu, rest;
+    AttnPart part; // of tiles
+    size_t   bytes() const { return sel + masks + counts + pos + lens + cu + rest; }
 };
-SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page, int64_t take) {
+SparsePlan sparse_plan(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages, int64_t page, int64_t take) {
     SparsePlan p = {};
     p.K    = std::min(take, max_pages);
-    p.sel  = round256(T * Hkv * p.K * 4);
     p.lens = round256(T * 4);
     p.cu   = round256((T + 1) * 4);
-    p.rest = std::max(pta::ps_workspace(T, Hkv, max_pages), attn_plan(T, T, Hq, Hkv, D, p.K, page, true).bytes());
+    const int64_t G = Hq / Hkv;
+    if (G <= ATT_NARROW_ROWS / 2 && T >= 2 * num_seqs && max_pages > 0 && max_pages <= pta::PS_TILE_PAGES) {
+        p.tile   = ATT_NARROW_ROWS / G;
+        p.tiles  = cdiv(T, p.tile);
+        p.cap    = p.tile * p.K;
+        p.sel    = round256(p.tiles * Hkv * p.cap * 8);
+        p.masks  = round256(p.tiles * Hkv * p.cap * 2);
+        p.counts = round256(p.tiles * Hkv * 4);
+        p.pos    = round256(T * 4);
+        p.part   = attn_narrow_part(T, p.tiles, Hq, Hkv, D, p.K * page, false, true);
+        p.rest   = std::max(pta::ps_workspace(T, Hkv, max_pages, p.tile), p.part.bytes());
+    } else {
+        p.sel  = round256(T * Hkv * p.K * 4);
+        p.rest = std::max(pta::ps_workspace(T, Hkv, max_pages, 1), attn_plan(T, T, Hq, Hkv, D, p.K, page, true).bytes());
+    }
     return p;
 }
 } // namespace
 
-extern "C" size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
-                                                            int64_t page_size, int64_t num_selected) {
-    if (num_tokens <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_pages < 0 || page_size <= 0 || num_selected <= 0) return 0;
-    return sparse_plan(num_tokens, Hq, Hkv, D, max_pages, page_size, num_selected).bytes();
+extern "C" size_t pta_sparse_paged_attention_workspace_size(int64_t num_tokens, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D,
+                                                            int64_t max_pages, int64_t page_size, int64_t num_selected) {
+    if (num_tokens <= 0 || num_seqs <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0 || max_pages < 0 || page_size <= 0 || num_selected <= 0) return 0;
+    return sparse_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, num_selected).bytes();
 }
 
 extern "C" int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t num_tokens, int64_t Hq, int64_t D, int64_t q_stride_t,
@@ -258,18 +294,48 @@ extern "C" int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t nu
     if (int rc = ps_check(num_tokens, num_seqs, Hq, Hkv, D, num_pages, page_size, max_pages, num_selected, num_first, num_last)) return rc;
     PTA_CHECK_ARG(softmax_scale > 0.0f && softmax_scale - softmax_scale == 0.0f, "softmax_scale must be positive and finite");
     if (num_tokens == 0) return PTA_OK;
-    const SparsePlan p = sparse_plan(num_tokens, Hq, Hkv, D, max_pages, page_size, num_selected);
+    PTA_CHECK_ARG(num_seqs > 0, "tokens without a sequence");
+    const SparsePlan p = sparse_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, num_selected);
     PTA_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= p.bytes(), "workspace too small: %zu bytes needed, %zu given",
                   p.bytes(), workspace_bytes);
+    PTA_CHECK_ARG(p.cap <= (INT_MAX - 1024) / page_size, "num_selected spans too many tokens");
     uint8_t *w    = static_cast<uint8_t *>(workspace);
-    int32_t *sel  = reinterpret_cast<int32_t *>(w), *lens = reinterpret_cast<int32_t *>(w + p.sel);
-    int32_t *cu   = reinterpret_cast<int32_t *>(w + p.sel + p.lens);
-    uint8_t *rest = w + p.sel + p.lens + p.cu;
-    if (int rc = ps_select(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, key_ranges, num_pages, page_size, Hkv, page_table,
-                           table_stride, max_pages, cu_seqlens_q, seq_lens, num_seqs, num_selected, num_first, num_last, sel, lens, cu,
-                           rest, as_stream(stream)))
+    uint8_t *sel  = w;
+    uint8_t *masks = w += p.sel, *counts = w += p.masks, *pos = w += p.counts;
+    int32_t *lens = reinterpret_cast<int32_t *>(w += p.pos), *cu = reinterpret_cast<int32_t *>(w += p.lens);
+    uint8_t *rest = w += p.cu;
+    PSTiles  tiles = {};
+    tiles.tokens = static_cast<int>(p.tile);
+    tiles.cap    = static_cast<int>(p.cap);
+    tiles.list   = reinterpret_cast<int2 *>(sel);
+    tiles.masks  = reinterpret_cast<uint16_t *>(masks);
+    tiles.counts = reinterpret_cast<int32_t *>(counts);
+    tiles.pos    = reinterpret_cast<int32_t *>(pos);
+    // all arguments are checked before the first launch
+    const int32_t *table = p.tile > 0 ? page_table : reinterpret_cast<const int32_t *>(sel);
+    AttnArgs       a;
+    if (int rc = attn_arguments(a, q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size,
+                                Hkv, k_scale_inv, v_scale_inv, table, Hkv * p.K, std::max<int64_t>(p.K, 1), p.K, cu, lens, num_tokens,
+                                softmax_scale, 0, 0, out, lse))
         return rc;
-    return attn_call(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size, Hkv,
-                     k_scale_inv, v_scale_inv, sel, Hkv * p.K, std::max<int64_t>(p.K, 1), p.K, cu, lens, num_tokens, softmax_scale, 0, 0,
-                     out, lse, rest, p.rest, stream);
+    const hipStream_t st = as_stream(stream);
+    if (int rc = ps_select(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, key_ranges, num_pages, page_size, Hkv, page_table,
+                           table_stride, max_pages, cu_seqlens_q, seq_lens, num_seqs, num_selected, num_first, num_last,
+                           reinterpret_cast<int32_t *>(sel), p.tile > 0 ? &tiles : nullptr, lens, cu, rest, st))
+        return rc;
+    if (p.tile == 0)
+        return attn_call(q, q_dtype, num_tokens, Hq, D, q_stride_t, q_stride_h, k_cache, v_cache, cache_kind, num_pages, page_size, Hkv,
+                         k_scale_inv, v_scale_inv, table, Hkv * p.K, std::max<int64_t>(p.K, 1), p.K, cu, lens, num_tokens, softmax_scale, 0, 0,
+                         out, lse, rest, p.rest, stream);
+    a.tiles     = tiles;
+    a.B         = static_cast<int>(p.tiles);
+    a.rows_max  = INT_MAX;
+    a.split     = static_cast<int>(p.part.split);
+    a.part_step = static_cast<int>(p.part.part_step);
+    a.part_ml   = reinterpret_cast<float2 *>(rest);
+    a.part_o    = reinterpret_cast<float *>(rest + p.part.ml_bytes);
+    if (q_dtype == PTA_BF16) attn_launch_tiles<PTA_BF16>(a, cache_kind, st);
+    else attn_launch_tiles<PTA_F16>(a, cache_kind, st);
+    PTA_CHECK_LAUNCH();
+    return PTA_OK;
 }

@@ -1,6 +1,8 @@
 // Kernel choice by cache kind and head dimension (instantiated per query type).
 #pragma once
 
+#include <algorithm>
+
 #include "paged_attention.h"
 
 namespace pta {
@@ -30,6 +32,28 @@ template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st) 
     if (n + w == 0) return;
     auto join = c.narrow.split > 4 ? attn_join_kernel<QT, 4> : attn_join_kernel<QT, 1>;
     join<<<static_cast<unsigned>(n + w), 256, 0, st>>>(c.narrow, c.wide, n, c.narrow_join_parts);
+}
+
+template <int QT, int KIND> void attn_launch_tiles_k(const AttnArgs &a, hipStream_t st) {
+    const unsigned grid = static_cast<unsigned>(a.B) * a.split * a.Hkv;
+    if (a.D <= 64) attn_tile_kernel<QT, KIND, 64><<<grid, 256, 0, st>>>(a);
+    else if (a.D <= 128) attn_tile_kernel<QT, KIND, 128><<<grid, 256, 0, st>>>(a);
+    else attn_tile_kernel<QT, KIND, 256><<<grid, 256, 0, st>>>(a);
+}
+
+template <int QT> void attn_launch_tiles(const AttnArgs &a, int kind, hipStream_t st) {
+    if (kind == PTA_E4M3) attn_launch_tiles_k<QT, PTA_E4M3>(a, st);
+    else if (kind == PTA_E5M2) attn_launch_tiles_k<QT, PTA_E5M2>(a, st);
+    else attn_launch_tiles_k<QT, PTA_CACHE_16BIT>(a, st);
+    if (a.split == 1) return;
+    // the parts are the tokens': each is a sequence of its own here, whose length says
+    // whether it sees a key
+    AttnArgs  x = a;
+    const int parts = static_cast<int>(std::min<int64_t>(ATT_JOIN_PARTS, cdiv(static_cast<int64_t>(a.G) * (a.D / 4), 64)));
+    x.B         = a.Tq;
+    const int n = a.Tq * a.Hkv * parts;
+    auto join   = a.split > 4 ? attn_join_kernel<QT, 4> : attn_join_kernel<QT, 1>;
+    join<<<static_cast<unsigned>(n), 256, 0, st>>>(x, x, n, parts);
 }
 
 } // namespace pta

@@ -1,0 +1,6 @@
+// Attention of tiles of tokens through their pages, bf16 queries.
+#include "paged_attention_launch.h"
+
+namespace pta {
+template void attn_launch_tiles<PTA_BF16>(const AttnArgs &, int, hipStream_t);
+}

@@ -158,7 +158,7 @@ SIGNATURES = {
         [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
          _i64, _vp, _vp, _vp, _sz, _vp],
     ),
-    "pta_sparse_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "pta_sparse_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "pta_sparse_paged_attention": (
         _i32,
         [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64,

@@ -116,7 +116,7 @@ def sparse_paged_attention_impl(
     out = torch.empty(shape, dtype=dtype, device=dev)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if T > 0:
-        nbytes = _C.query("pta_sparse_paged_attention_workspace_size", T, Hq, Hkv, D, M, page, take)
+        nbytes = _C.query("pta_sparse_paged_attention_workspace_size", T, B, Hq, Hkv, D, M, page, take)
         ws = _C.workspace(nbytes, dev)
         qs = q.stride()
         _C.call_on(

@@ -83,6 +83,20 @@ def test_copy(L, P, H, page, D, dtype, ranges, idx):
     assert _same(pools, want)
 
 
+@pytest.mark.parametrize("L,P,H,page,D,n", [(2, 300, 8, 64, 128, 100), (3, 90, 5, 33, 80, 40), (2, 2600, 8, 64, 128, 1100)])
+def test_copy_much(L, P, H, page, D, n):
+    """More than one piece a thread; more than the last cache holds."""
+    pools = _pools(L, P, H, page, D, E4, ranges=True)
+    start = [t.clone() for t in pools]
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(P)).cuda()
+    src, dst = order[:n].contiguous(), order[n:2 * n].contiguous()
+    _ops().kv_cache_copy(pools[0], pools[1], src, dst, pools[2], pools[3], key_ranges=pools[4])
+    for x, y in zip(pools, start):
+        x, y = _bytes(x), _bytes(y)
+        y[:, dst] = y[:, src]
+        assert torch.equal(x, y)
+
+
 def test_copy_nothing():
     ops = _ops()
     pools = _pools(0, 4, 2, 8, 32, E4)
