@@ -9,7 +9,7 @@ import torch
 
 from primus_turbo.pytorch import _C
 from primus_turbo.pytorch.core.inference import check_tensors
-from primus_turbo.pytorch.kernels.attention.paged_attention_impl import _check_cache, _increment_version
+from primus_turbo.pytorch.kernels.attention.paged_attention_impl import _KIND, _check_cache, _increment_version
 
 _INT = (torch.int32, torch.int64)
 
@@ -24,21 +24,36 @@ def check_ranges(key_ranges: torch.Tensor, shape: torch.Size) -> None:
 
 def _check_pools(k_cache, v_cache, k_scale_inv, v_scale_inv, key_ranges):
     """(kind, layers, pages, heads, page size, D, the tensors) of pools with or without a dimension of layers."""
-    layers, shape = 1, k_cache.shape
-    if len(shape) == 5:
-        layers = shape[0]
-        assert v_cache.shape == shape, f"caches must be both alike: got {tuple(shape)}, {tuple(v_cache.shape)}"
-        assert k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous"
-        for s in (k_scale_inv, v_scale_inv):
-            assert s is None or (s.shape == shape[:4] and s.is_contiguous()), f"scale_inv must be contiguous float32 {tuple(shape[:4])}"
-        flat = [None if t is None else t.flatten(0, 1) for t in (k_cache, v_cache, k_scale_inv, v_scale_inv)]
-        kind, _ = _check_cache(*flat)
+    shape = k_cache.shape
+    if len(shape) == 4:
+        kind, (P, Hkv, page, D) = _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv)
+        L = 1
     else:
-        kind, _ = _check_cache(k_cache, v_cache, k_scale_inv, v_scale_inv)
+        dtype = k_cache.dtype
+        assert len(shape) == 5 and v_cache.shape == shape, (
+            f"caches must be [(layers,) num_pages, Hkv, page_size, D], both alike: got {tuple(shape)}, {tuple(v_cache.shape)}"
+        )
+        assert v_cache.dtype == dtype, "k_cache and v_cache must have one type"
+        kind = _KIND.get(dtype)
+        assert kind is not None, f"unsupported cache type {dtype}"
+        assert k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous"
+        L, P, Hkv, page, D = shape
+        assert D % 16 == 0 and 16 <= D <= 256, f"head_dim must be a multiple of 16 in [16, 256], got {D}"
+        assert page > 0 and Hkv > 0, "page_size and the number of heads must not be 0"
+        if kind == _C.CACHE_16BIT:
+            assert k_scale_inv is None and v_scale_inv is None, "a 16-bit cache has no scales"
+        else:
+            assert k_scale_inv is not None and v_scale_inv is not None, "an fp8 cache needs k_scale_inv and v_scale_inv"
+            want = shape[:4]
+            for s in (k_scale_inv, v_scale_inv):
+                assert s.shape == want and s.dtype == torch.float32 and s.is_contiguous(), (
+                    f"scale_inv must be contiguous float32 {tuple(want)}, got {s.dtype} {tuple(s.shape)}"
+                )
+    tensors = (k_cache, v_cache) if k_scale_inv is None else (k_cache, v_cache, k_scale_inv, v_scale_inv)
     if key_ranges is not None:
         check_ranges(key_ranges, shape)
-    tensors = tuple(t for t in (k_cache, v_cache, k_scale_inv, v_scale_inv, key_ranges) if t is not None)
-    return kind, layers, *shape[-4:], tensors
+        tensors += (key_ranges,)
+    return kind, L, P, Hkv, page, D, tensors
 
 
 def kv_cache_copy_impl(k_cache, v_cache, src_pages, dst_pages, k_scale_inv, v_scale_inv, key_ranges) -> None:

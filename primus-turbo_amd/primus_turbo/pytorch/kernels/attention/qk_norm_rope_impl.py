@@ -13,7 +13,7 @@ from primus_turbo.pytorch import _C
 from primus_turbo.pytorch.core.inference import check_tensors
 from primus_turbo.pytorch.kernels.attention.paged_attention_impl import _IN, _check_cache, _check_slots, _increment_version
 
-_INT, _F32 = (torch.int32, torch.int64), torch.float32
+_INT, _F32, _DENSE = (torch.int32, torch.int64), torch.float32, torch.contiguous_format
 
 
 def _check_rotation(cos, sin, positions, lead, D) -> int:
@@ -80,10 +80,10 @@ def check_qk(q, k, cos, sin, positions, q_weight, k_weight, eps) -> float:
 def qk_norm_rope_impl(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved) -> Tuple[torch.Tensor, torch.Tensor]:
     """Arguments as check_qk has passed them."""
     dtype, dev = q.dtype, q.device
-    q_out = torch.empty(q.shape, dtype=dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+    q_out, k_out = torch.empty_like(q, memory_format=_DENSE), torch.empty_like(k, memory_format=_DENSE)
     q, k = _rows(q), _rows(k)
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     (T, Hq, D), Hkv, (P, half) = q.shape, k.shape[1], cos.shape
     qs, ks = q.stride(), k.stride()
     _C.call_on(
@@ -103,7 +103,7 @@ def _side(g, x, w, want):
     """What the backward pass takes of the queries or of the keys."""
     if g is None:
         return _NONE
-    dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    dx = torch.empty_like(g, memory_format=_DENSE)
     g = _rows(g)
     if w is None:
         return g, g.shape[1], g.stride(), None, (0, 0), dx, None, None, 0
@@ -118,17 +118,18 @@ def qk_norm_rope_backward_impl(
     q and k may be None where they have no weight."""
     like = gk if gq is None else gq
     dev, dtype, D = like.device, like.dtype, like.shape[-1]
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     gq, Hq, gqs, q, qs, dq, dqw, qw, qwd = _side(gq, q, q_weight, want_qw)
     gk, Hkv, gks, k, ks, dk, dkw, kw, kwd = _side(gk, k, k_weight, want_kw)
     T, (P, half) = positions.numel(), cos.shape
     nbytes = _C.query("pta_qk_norm_rope_backward_workspace_size", T, Hq, Hkv, D) if want_qw or want_kw else 0
-    ws = _C.workspace(nbytes, dev)
+    ws, ptr = _C.workspace(nbytes, dev), _C.ptr
     _C.call_on(
-        dev, "pta_qk_norm_rope_backward", _C.ptr(gq), _C.ptr(gk), gqs[0], gqs[1], gks[0], gks[1], _C.ptr(q), _C.ptr(k),
+        dev, "pta_qk_norm_rope_backward", ptr(gq), ptr(gk), gqs[0], gqs[1], gks[0], gks[1], ptr(q), ptr(k),
         _IN[dtype], T, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], cos.data_ptr(), sin.data_ptr(), P, 2 * half,
-        positions.data_ptr(), positions.dtype == torch.int64, qw, qwd, kw, kwd, eps, interleaved, _C.ptr(dq), _C.ptr(dk),
-        _C.ptr(dqw), _C.ptr(dkw), _C.ptr(ws), nbytes, _C.stream(dev),
+        positions.data_ptr(), positions.dtype == torch.int64, qw, qwd, kw, kwd, eps, interleaved, ptr(dq), ptr(dk),
+        ptr(dqw), ptr(dkw), ptr(ws), nbytes, _C.stream(dev),
     )
     return dq, dk, dqw, dkw
 
@@ -154,7 +155,7 @@ def qk_norm_rope_cache_write_impl(
     check_tensors("qk_norm_rope_cache_write", (q, k, v, cos, sin, k_cache, v_cache, k_scale_inv, v_scale_inv, q_weight, k_weight),
                   slots, positions)
     dev = q.device
-    out = torch.empty(shape, dtype=dtype, device=dev)
+    out = torch.empty_like(q, memory_format=_DENSE)
     if T == 0:
         return out
     qs, ks, vs = q.stride(), k.stride(), v.stride()

@@ -33,6 +33,18 @@ from primus_turbo.pytorch.kernels.attention.qk_norm_rope_impl import (
 __all__ = ["qk_norm_rope", "qk_norm_rope_cache_write"]
 
 
+def _backward(ctx, gq, gk):
+    q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
+    need_q, need_k, _, _, _, need_qw, need_kw, _, _ = ctx.needs_input_grad
+    eps, interleaved = ctx.how
+    dq, dk, dqw, dkw = qk_norm_rope_backward_impl(gq if need_q or need_qw else None, gk if need_k or need_kw else None, q, k, cos, sin,
+                                                  positions, q_weight, k_weight, eps, interleaved, need_qw, need_kw)
+    return dq if need_q else None, dk if need_k else None, None, None, None, dqw, dkw, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _QKNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved):
@@ -42,13 +54,9 @@ class _QKNormRope(torch.autograd.Function):
         return qk_norm_rope_impl(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
-        need_q, need_k, need_qw, need_kw = (ctx.needs_input_grad[i] for i in (0, 1, 5, 6))
-        gq, gk = gq if need_q or need_qw else None, gk if need_k or need_kw else None
-        dq, dk, dqw, dkw = qk_norm_rope_backward_impl(gq, gk, q, k, cos, sin, positions, q_weight, k_weight, *ctx.how, need_qw, need_kw)
-        return dq if need_q else None, dk if need_k else None, None, None, None, dqw, dkw, None, None
+        # with gradients enabled (create_graph) a second derivative has to fail, not to be missing
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, gq, gk)
 
 
 @torch._dynamo.disable

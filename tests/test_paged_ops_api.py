@@ -129,6 +129,12 @@ def test_cache_write_refuses(over, match):
     (dict(k_cache=z(2, 4, 2, 8, 32, dtype=E4)), "both alike"),
     (dict(k_cache=z(2, 4, 2, 8, 32, dtype=E4), v_cache=z(2, 4, 2, 8, 32, dtype=E4)), "scale_inv must be"),
     (dict(k_cache=z(4, 3, 2, 8, 32, dtype=E4).transpose(0, 1), v_cache=z(4, 3, 2, 8, 32, dtype=E4).transpose(0, 1)), "contiguous"),
+    (dict(k_cache=z(2, 4, 2, 8, 24, dtype=E4), v_cache=z(2, 4, 2, 8, 24, dtype=E4)), "multiple of 16"),
+    (dict(k_cache=z(2, 4, 2, 8, 32), v_cache=z(2, 4, 2, 8, 32)), "has no scales"),
+    (dict(k_cache=z(2, 4, 2, 8, 32, dtype=FF), v_cache=z(2, 4, 2, 8, 32, dtype=FF)), "unsupported cache type"),
+    (dict(k_cache=z(2, 4, 2, 8, 32), v_cache=z(2, 4, 2, 8, 32, dtype=FH)), "one type"),
+    (dict(k_cache=z(2, 4, 2, 8, 32, dtype=E4), v_cache=z(2, 4, 2, 8, 32, dtype=E4), v_scale_inv=None), "needs k_scale_inv"),
+    (dict(k_cache=z(8, 32, dtype=E4), v_cache=z(8, 32, dtype=E4)), "both alike"),
     (dict(key_ranges=z(4, 2, 2, 16)), "key_ranges must be"),
     (dict(key_ranges=z(4, 2, 2, 32, dtype=FH)), "key_ranges must be"),
     (dict(k_scale_inv=z(4, 2, 8, dtype=FF).requires_grad_()), "no backward"),
