@@ -213,30 +213,19 @@ template <int QT> __device__ __forceinline__ void ps_channel(const PSArgs &a, in
     }
 }
 
-// Few tokens: pages [c per, (c + 1) per) of token t for head h, a page's range to LPR
-// lanes, 8 channels each, four pages of a lane's loads together.  Bound by the chain of
-// reads: the token's place, page numbers, ranges.
-template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_kernel(PSArgs a, int per, int parts) {
-    constexpr int  GROUPS = PS_NT / LPR, PAGES = 4;
-    const uint32_t w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, ti = w1 / parts;
-    const int      t = a.t0 + static_cast<int>(ti);
-    const PSToken  s = ps_token(a, t);
-    if (s.b < 0 || s.pos < 0) return;
-    const int own = s.pos / a.page, n = own + 1, j0 = c * per, j1 = min(j0 + per, n);
-    if (j0 >= j1 || n <= a.take) return;
-    __shared__ double sums[2][8 * LPR];
-    if (static_cast<int>(threadIdx.x) < a.D) ps_channel<QT>(a, t, h, threadIdx.x, sums[0][threadIdx.x], sums[1][threadIdx.x]);
-    __syncthreads();
-    const int  l = threadIdx.x % LPR, g = threadIdx.x / LPR, d = l * 8;
-    const bool in = d < a.D;
-    double     up[8], down[8];
+// Keys of pages [j0, j1) of the token's sequence to out: a page's range to LPR of the NT
+// threads, 8 channels each, four pages of a thread's loads together.
+template <int LPR, int NT>
+__device__ __forceinline__ void ps_scores(const PSArgs &a, const double (&sums)[2][8 * LPR], const int32_t *row, int h, int j0, int j1, uint64_t *out) {
+    constexpr int GROUPS = NT / LPR, PAGES = 4;
+    const int     l = threadIdx.x % LPR, g = threadIdx.x / LPR, d = l * 8;
+    const bool    in = d < a.D;
+    double        up[8], down[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         up[e]   = in ? sums[0][d + e] : 0.0;
         down[e] = in ? sums[1][d + e] : 0.0;
     }
-    uint64_t      *out = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
-    const int32_t *row = a.table + s.b * a.table_st;
     for (int p0 = j0 + g; p0 < j1; p0 += GROUPS * PAGES) {
         uint4 lo[PAGES], hi[PAGES];
         bool  there[PAGES];
@@ -266,6 +255,21 @@ template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_ker
             if (l == 0 && j < j1) out[j] = ps_key(x);
         }
     }
+}
+
+// Few tokens with many pages: pages [c per, (c + 1) per) of token t for head h.  Bound by the
+// chain of reads: the token's place, queries and page numbers, ranges.
+template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_kernel(PSArgs a, int per, int parts) {
+    __shared__ double sums[2][8 * LPR];
+    const uint32_t w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, ti = w1 / parts;
+    const int      t = a.t0 + static_cast<int>(ti);
+    const PSToken  s = ps_token(a, t);
+    if (s.b < 0 || s.pos < 0) return;
+    const int n = s.pos / a.page + 1, j0 = c * per, j1 = min(j0 + per, n);
+    if (j0 >= j1 || n <= a.take) return;
+    if (static_cast<int>(threadIdx.x) < a.D) ps_channel<QT>(a, t, h, threadIdx.x, sums[0][threadIdx.x], sums[1][threadIdx.x]);
+    __syncthreads();
+    ps_scores<LPR, PS_NT>(a, sums, a.table + s.b * a.table_st, h, j0, j1, a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M);
 }
 
 // Chunks: 16 tokens by 16 pages on the 64-bit matrix instruction, D = R B with a page's
@@ -421,32 +425,86 @@ __device__ __forceinline__ uint64_t ps_at(const PSArgs &a, const uint64_t *keys,
     return j < a.first || own - j < a.last ? ~0ull : keys[j];
 }
 
-// NW waves for (token, head), wave w with keys [64 w E, 64 (w + 1) E), E a lane; what does
-// not fit is read again for every step of the search.  Bound by its steps, about 3 E
-// instructions each, and for more than one wave a barrier.
-template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_kernel(PSArgs a) {
-    constexpr int  CAP = 64 * NW * E;
-    __shared__ int cnt[2][2][NW];
-    const int      ti = blockIdx.x / a.Hkv, h = blockIdx.x - ti * a.Hkv, t = a.t0 + ti;
-    const int      lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const PSToken  s = ps_token(a, t);
-    const bool     some = s.b >= 0 && s.pos >= 0;
-    const int      own = some ? s.pos / a.page : -1, n = own + 1, take = min(n, a.take);
-    int32_t       *sel = a.sel + (static_cast<int64_t>(t) * a.Hkv + h) * a.K;
+// What a token gets without a choice; true if it needs one.  All threads call it.
+__device__ __forceinline__ bool ps_begin(const PSArgs &a, const PSToken &s, int t, int h, int own, int take, int32_t *sel) {
     if (h == 0 && threadIdx.x == 0) {
-        a.sel_lens[t] = some ? (take - 1) * a.page + (s.pos - own * a.page) + 1 : 0;
+        a.sel_lens[t] = own >= 0 ? (take - 1) * a.page + (s.pos - own * a.page) + 1 : 0;
         if (a.sel_cu != nullptr) {
             a.sel_cu[t] = t;
             if (t == a.T - 1) a.sel_cu[a.T] = a.T;
         }
     }
-    for (int j = take + static_cast<int>(threadIdx.x); j < a.K; j += 64 * NW) sel[j] = -1;
-    if (!some) return;
+    for (int j = take + static_cast<int>(threadIdx.x); j < a.K; j += blockDim.x) sel[j] = -1;
+    if (own < 0) return false;
+    if (own + 1 > a.take) return true;
     const int32_t *row = a.table + s.b * a.table_st;
-    if (n <= a.take) {
-        for (int j = threadIdx.x; j < n; j += 64 * NW) sel[j] = row[j];
-        return;
+    for (int j = threadIdx.x; j <= own; j += blockDim.x) sel[j] = row[j];
+    return false;
+}
+
+// One wave's choice among up to 64 E pages: the keys above the least, and of those equal to it
+// the first ones, in the pages' order.
+template <int E> __device__ __forceinline__ void ps_take(const PSArgs &a, const uint64_t *keys, int own, int take, const int32_t *row, int32_t *sel) {
+    const int lane = lane_id(), n = own + 1;
+    uint64_t  key[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = e * 64 + lane < n ? ps_at(a, keys, own, e * 64 + lane) : 0; // below every score
+    const uint64_t least = ps_least<E>(key, take), below = (1ull << lane) - 1;
+    int            above = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) above += __popcll(__ballot(key[e] > least));
+    int at = 0, room = take - above; // of the equal ones
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint64_t eq = __ballot(key[e] == least);
+        const uint64_t m  = __ballot(key[e] > least || (key[e] == least && __popcll(eq & below) < room));
+        if (m >> lane & 1) sel[at + __popcll(m & below)] = row[e * 64 + lane];
+        at += __popcll(m);
+        room -= min(room, static_cast<int>(__popcll(eq)));
     }
+}
+
+// Up to 256 or 512 pages, a wave for (token, head)
+template <int E> __global__ __launch_bounds__(64) void ps_choose_kernel(PSArgs a) {
+    const int      ti = blockIdx.x / a.Hkv, h = blockIdx.x - ti * a.Hkv, t = a.t0 + ti;
+    const PSToken  s = ps_token(a, t);
+    const int      own = s.b >= 0 && s.pos >= 0 ? s.pos / a.page : -1, take = min(own + 1, a.take);
+    int32_t       *sel = a.sel + (static_cast<int64_t>(t) * a.Hkv + h) * a.K;
+    if (!ps_begin(a, s, t, h, own, take, sel)) return;
+    ps_take<E>(a, a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M, own, take, a.table + s.b * a.table_st, sel);
+}
+
+// Few tokens with up to 512 pages: scores and choice in one workgroup for (token, head)
+constexpr int PS_ONE = 512;
+template <int QT, int LPR> __global__ __launch_bounds__(1024) void ps_select_kernel(PSArgs a) {
+    __shared__ double   sums[2][8 * LPR];
+    __shared__ uint64_t keys[PS_ONE];
+    const int      ti = blockIdx.x / a.Hkv, h = blockIdx.x - ti * a.Hkv, t = a.t0 + ti;
+    const PSToken  s = ps_token(a, t);
+    const int      own = s.b >= 0 && s.pos >= 0 ? s.pos / a.page : -1, take = min(own + 1, a.take);
+    int32_t       *sel = a.sel + (static_cast<int64_t>(t) * a.Hkv + h) * a.K;
+    if (!ps_begin(a, s, t, h, own, take, sel)) return;
+    const int32_t *row = a.table + s.b * a.table_st;
+    if (static_cast<int>(threadIdx.x) < a.D) ps_channel<QT>(a, t, h, threadIdx.x, sums[0][threadIdx.x], sums[1][threadIdx.x]);
+    __syncthreads();
+    ps_scores<LPR, 1024>(a, sums, row, h, 0, own + 1, keys);
+    __syncthreads();
+    if (threadIdx.x < 64) ps_take<PS_ONE / 64>(a, keys, own, take, row, sel);
+}
+
+// More pages: NW waves for (token, head), wave w with keys [64 w E, 64 (w + 1) E), E a lane;
+// what does not fit is read again for every step of the search.  The search is ps_least's, with
+// a barrier a step.
+template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_many_kernel(PSArgs a) {
+    constexpr int  CAP = 64 * NW * E;
+    __shared__ int cnt[2][2][NW];
+    const int      ti = blockIdx.x / a.Hkv, h = blockIdx.x - ti * a.Hkv, t = a.t0 + ti;
+    const int      lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const PSToken  s = ps_token(a, t);
+    const int      own = s.b >= 0 && s.pos >= 0 ? s.pos / a.page : -1, n = own + 1, take = min(n, a.take);
+    int32_t       *sel = a.sel + (static_cast<int64_t>(t) * a.Hkv + h) * a.K;
+    if (!ps_begin(a, s, t, h, own, take, sel)) return;
+    const int32_t  *row = a.table + s.b * a.table_st;
     const uint64_t *in = a.keys + (static_cast<int64_t>(ti) * a.Hkv + h) * a.M;
     uint64_t        key[E];
 #pragma unroll
@@ -457,63 +515,54 @@ template <int NW, int E> __global__ __launch_bounds__(64 * NW) void ps_choose_ke
     // sums of x and of y over the workgroup, and over the waves before
     int  buf = 0;
     auto all = [&](int x, int y, int &sx, int &sy, int &bx, int &by) {
-        sx = x;
-        sy = y;
-        bx = by = 0;
-        if constexpr (NW > 1) {
-            if (lane == 0) {
-                cnt[buf][0][wave] = x;
-                cnt[buf][1][wave] = y;
-            }
-            __syncthreads();
-            sx = sy = 0;
-            for (int w = 0; w < NW; ++w) {
-                if (w < wave) {
-                    bx += cnt[buf][0][w];
-                    by += cnt[buf][1][w];
-                }
-                sx += cnt[buf][0][w];
-                sy += cnt[buf][1][w];
-            }
-            buf ^= 1;
+        if (lane == 0) {
+            cnt[buf][0][wave] = x;
+            cnt[buf][1][wave] = y;
         }
+        __syncthreads();
+        sx = sy = bx = by = 0;
+        for (int w = 0; w < NW; ++w) {
+            if (w < wave) {
+                bx += cnt[buf][0][w];
+                by += cnt[buf][1][w];
+            }
+            sx += cnt[buf][0][w];
+            sy += cnt[buf][1][w];
+        }
+        buf ^= 1;
     };
     uint64_t least = 0;
-    if constexpr (NW == 1) { // all keys fit
-        least = ps_least<E>(key, take);
-    } else {
-        bool done = false;
-        int  top  = 63;
-        if (n <= CAP) {
-            uint32_t common, any;
-            ps_bits<E>(key, common, any);
-            if (lane == 0) {
-                cnt[1][0][wave] = static_cast<int>(common);
-                cnt[1][1][wave] = static_cast<int>(any);
-            }
-            __syncthreads(); // the next to write there comes behind the next barrier but one
-            for (int w = 0; w < NW; ++w) {
-                common &= static_cast<uint32_t>(cnt[1][0][w]);
-                any |= static_cast<uint32_t>(cnt[1][1][w]);
-            }
-            top   = 63 - __clz(common ^ any); // 31: they differ in none
-            least = static_cast<uint64_t>(top < 32 ? any : any & ~((2u << (top - 32)) - 1)) << 32;
+    bool done = false;
+    int  top  = 63;
+    if (n <= CAP) {
+        uint32_t common, any;
+        ps_bits<E>(key, common, any);
+        if (lane == 0) {
+            cnt[1][0][wave] = static_cast<int>(common);
+            cnt[1][1][wave] = static_cast<int>(any);
         }
-        for (int bit = top; bit >= 0 && !done; --bit) {
-            const uint64_t cand = least | (1ull << bit);
-            int            c = 0;
+        __syncthreads(); // the next to write there comes behind the next barrier but one
+        for (int w = 0; w < NW; ++w) {
+            common &= static_cast<uint32_t>(cnt[1][0][w]);
+            any |= static_cast<uint32_t>(cnt[1][1][w]);
+        }
+        top   = 63 - __clz(common ^ any); // 31: they differ in none
+        least = static_cast<uint64_t>(top < 32 ? any : any & ~((2u << (top - 32)) - 1)) << 32;
+    }
+    for (int bit = top; bit >= 0 && !done; --bit) {
+        const uint64_t cand = least | (1ull << bit);
+        int            c = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                c += __popcll(__ballot(bit >= 32 ? static_cast<uint32_t>(key[e] >> 32) >= static_cast<uint32_t>(cand >> 32) : key[e] >= cand));
-            for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
-                const int j = j0 + static_cast<int>(threadIdx.x);
-                c += __popcll(__ballot(j < n && ps_at(a, in, own, min(j, n - 1)) >= cand));
-            }
-            int total, none, b0, b1;
-            all(c, 0, total, none, b0, b1);
-            if (total >= take) least = cand;
-            done = total == take;
+        for (int e = 0; e < E; ++e)
+            c += __popcll(__ballot(bit >= 32 ? static_cast<uint32_t>(key[e] >> 32) >= static_cast<uint32_t>(cand >> 32) : key[e] >= cand));
+        for (int j0 = CAP; j0 < n; j0 += 64 * NW) {
+            const int j = j0 + static_cast<int>(threadIdx.x);
+            c += __popcll(__ballot(j < n && ps_at(a, in, own, min(j, n - 1)) >= cand));
         }
+        int total, none, b0, b1;
+        all(c, 0, total, none, b0, b1);
+        if (total >= take) least = cand;
+        done = total == take;
     }
     // all above the least, and of those equal to it the first ones
     int above = 0, equal = 0, sa, se, ba, be;
@@ -663,9 +712,18 @@ int ps_check(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int64_t D, in
     return PTA_OK;
 }
 
-// Chunks from two tokens a sequence on go by tiles of tokens
+// Scores go by tiles of tokens from two tokens a sequence on
+static bool ps_tiles(const PSArgs &a) { return a.T >= 2 * a.B; }
+
+template <int QT> static void ps_select_one(const PSArgs &a, hipStream_t st) {
+    const unsigned grid = static_cast<unsigned>(a.n) * a.Hkv;
+    if (a.D <= 64) ps_select_kernel<QT, 8><<<grid, 1024, 0, st>>>(a);
+    else if (a.D <= 128) ps_select_kernel<QT, 16><<<grid, 1024, 0, st>>>(a);
+    else ps_select_kernel<QT, 32><<<grid, 1024, 0, st>>>(a);
+}
+
 template <int QT> static void ps_score(const PSArgs &a, hipStream_t st) {
-    const bool    tiles = a.T >= 2 * a.B && a.n > 1;
+    const bool    tiles = ps_tiles(a);
     const int64_t items = (tiles ? cdiv(a.n, PS_TILE) : a.n) * a.Hkv;
     // pages in as many parts as give every CU four workgroups, one round of a workgroup at least
     const int64_t least = tiles ? 64 : 32, want = cdiv(4 * device_cu_count(), items);
@@ -687,6 +745,12 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
     const int tile = a.tiles.tokens, step = static_cast<int>(ps_slice(a.T, a.Hkv, a.M, std::max(1, tile)));
     for (a.t0 = 0; a.t0 < a.T; a.t0 += step) {
         a.n = std::min(step, a.T - a.t0);
+        if (!ps_tiles(a) && a.M <= PS_ONE) {
+            if (q_dtype == PTA_BF16) ps_select_one<PTA_BF16>(a, st);
+            else ps_select_one<PTA_F16>(a, st);
+            PTA_CHECK_LAUNCH();
+            continue;
+        }
         if (a.M > a.take) {
             if (q_dtype == PTA_BF16) ps_score<PTA_BF16>(a, st);
             else ps_score<PTA_F16>(a, st);
@@ -697,10 +761,10 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
             if (a.M <= 256) ps_choose_tile_kernel<4><<<grid, threads, 0, st>>>(a);
             else if (a.M <= 512) ps_choose_tile_kernel<8><<<grid, threads, 0, st>>>(a);
             else ps_choose_tile_kernel<16><<<grid, threads, 0, st>>>(a);
-        } else if (a.M <= 256) ps_choose_kernel<1, 4><<<grid, 64, 0, st>>>(a);
-        else if (a.M <= 512) ps_choose_kernel<1, 8><<<grid, 64, 0, st>>>(a);
-        else if (a.M <= 2048) ps_choose_kernel<8, 4><<<grid, 512, 0, st>>>(a);
-        else ps_choose_kernel<16, 8><<<grid, 1024, 0, st>>>(a);
+        } else if (a.M <= 256) ps_choose_kernel<4><<<grid, 64, 0, st>>>(a);
+        else if (a.M <= 512) ps_choose_kernel<8><<<grid, 64, 0, st>>>(a);
+        else if (a.M <= 2048) ps_choose_many_kernel<8, 4><<<grid, 512, 0, st>>>(a);
+        else ps_choose_many_kernel<16, 8><<<grid, 1024, 0, st>>>(a);
         PTA_CHECK_LAUNCH();
     }
     return PTA_OK;
