@@ -259,7 +259,8 @@ SparsePlan sparse_plan(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int
     p.lens = round256(T * 4);
     p.cu   = round256((T + 1) * 4);
     const int64_t G = Hq / Hkv;
-    if (G <= ATT_NARROW_ROWS / 2 && T >= 2 * num_seqs && max_pages > 0 && max_pages <= pta::PS_TILE_PAGES) {
+    if (G <= ATT_NARROW_ROWS / 2 && T >= 2 * num_seqs && max_pages > 0 && max_pages <= pta::PS_TILE_PAGES &&
+        ATT_NARROW_ROWS * p.K <= (INT_MAX - 1024) / page) { // a list's keys are counted in 32 bits
         p.tile   = ATT_NARROW_ROWS / G;
         p.tiles  = cdiv(T, p.tile);
         p.cap    = p.tile * p.K;
@@ -298,7 +299,6 @@ extern "C" int pta_sparse_paged_attention(const void *q, int q_dtype, int64_t nu
     const SparsePlan p = sparse_plan(num_tokens, num_seqs, Hq, Hkv, D, max_pages, page_size, num_selected);
     PTA_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= p.bytes(), "workspace too small: %zu bytes needed, %zu given",
                   p.bytes(), workspace_bytes);
-    PTA_CHECK_ARG(p.cap <= (INT_MAX - 1024) / page_size, "num_selected spans too many tokens");
     uint8_t *w    = static_cast<uint8_t *>(workspace);
     uint8_t *sel  = w;
     uint8_t *masks = w += p.sel, *counts = w += p.masks, *pos = w += p.counts;

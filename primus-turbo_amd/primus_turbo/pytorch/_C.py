@@ -229,6 +229,14 @@ def call_on(device, name: str, *args) -> None:
             call(name, *args)
 
 
+def query_on(device, name: str, *args) -> int:
+    """``query`` likewise: some sizes depend on the device."""
+    if device.type != "cuda" or device.index == _cur_device():
+        return query(name, *args)
+    with torch.cuda.device(device):
+        return query(name, *args)
+
+
 # Debug mode (PRIMUS_TURBO_CHECK_WAITS=1): after each call that launched a
 # bounded cross-workgroup wait, synchronize and raise if the wait gave up.
 CHECK_WAITS = os.environ.get("PRIMUS_TURBO_CHECK_WAITS", "0") not in ("", "0")

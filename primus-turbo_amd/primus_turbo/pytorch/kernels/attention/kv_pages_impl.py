@@ -99,7 +99,7 @@ def kv_cache_fork_impl(
     lens = torch.empty((N,), dtype=i32, device=dev)
     if N == 0:
         return table, lens
-    nbytes = _C.query("pta_kv_cache_fork_workspace_size", N, M, P, bool(compact))
+    nbytes = _C.query_on(dev, "pta_kv_cache_fork_workspace_size", N, M, P, bool(compact))
     ws = _C.workspace(nbytes, dev)
     _C.call_on(
         dev, "pta_kv_cache_fork", k_cache.data_ptr(), v_cache.data_ptr(), kind, L, P, Hkv, page, D, _C.ptr(k_scale_inv),

@@ -123,7 +123,7 @@ def qk_norm_rope_backward_impl(
     gq, Hq, gqs, q, qs, dq, dqw, qw, qwd = _side(gq, q, q_weight, want_qw)
     gk, Hkv, gks, k, ks, dk, dkw, kw, kwd = _side(gk, k, k_weight, want_kw)
     T, (P, half) = positions.numel(), cos.shape
-    nbytes = _C.query("pta_qk_norm_rope_backward_workspace_size", T, Hq, Hkv, D) if want_qw or want_kw else 0
+    nbytes = _C.query_on(dev, "pta_qk_norm_rope_backward_workspace_size", T, Hq, Hkv, D) if want_qw or want_kw else 0
     ws, ptr = _C.workspace(nbytes, dev), _C.ptr
     _C.call_on(
         dev, "pta_qk_norm_rope_backward", ptr(gq), ptr(gk), gqs[0], gqs[1], gks[0], gks[1], ptr(q), ptr(k),

@@ -79,7 +79,7 @@ def select_pages_impl(
     sel = torch.empty((T, Hkv, min(take, M)), dtype=torch.int32, device=dev)
     lens = torch.empty((T,), dtype=torch.int32, device=dev)
     if T > 0:
-        nbytes = _C.query("pta_select_pages_workspace_size", T, Hkv, M)
+        nbytes = _C.query_on(dev, "pta_select_pages_workspace_size", T, Hkv, M)
         ws = _C.workspace(nbytes, dev)
         _C.call_on(
             dev, "pta_select_pages", q.data_ptr(), _IN[q.dtype], T, Hq, D, q.stride(0), q.stride(1), key_ranges.data_ptr(), P, page,
@@ -116,7 +116,7 @@ def sparse_paged_attention_impl(
     out = torch.empty(shape, dtype=dtype, device=dev)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if T > 0:
-        nbytes = _C.query("pta_sparse_paged_attention_workspace_size", T, B, Hq, Hkv, D, M, page, take)
+        nbytes = _C.query_on(dev, "pta_sparse_paged_attention_workspace_size", T, B, Hq, Hkv, D, M, page, take)
         ws = _C.workspace(nbytes, dev)
         qs = q.stride()
         _C.call_on(

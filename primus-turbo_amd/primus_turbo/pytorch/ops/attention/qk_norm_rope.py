@@ -13,7 +13,9 @@ For a row x, the D elements of one token and head:
 angles of position p (scaled in whatever way the model asks for); R, even, is D or
 less.  Pairs are (i, i + R / 2), with ``interleaved`` (2 i, 2 i + 1).  A token whose
 position lies outside the tables, -1 for padding, gets zeros and gives no gradient.
-Everything is fp32 up to the one rounding of the result.
+Everything is fp32 up to the one rounding of the result, the sums of squares too: a row
+whose squares leave its range (elements beyond about 1e18) becomes zeros.  Under
+torch.compile the calls run between its graphs; fake tensors are refused.
 """
 
 from __future__ import annotations

@@ -208,6 +208,27 @@ def test_infinities_and_nan_stay_in_their_rows():
     assert not bool(ops.qk_norm_rope(zero, k, cos, sin, pos, wq, wk)[0].any())
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes of queries, forward and backward: the last tokens' rows are where they belong."""
+    ops = _ops()
+    T, Hq, D = 540000, 32, 128  # 4.4e9 bytes
+    _, k, _, wq, wk, cos, sin, _ = _inputs(6, Hq, 1, D, 128, BF)
+    q, g = (torch.empty(T, Hq, D, dtype=BF, device="cuda") for _ in range(2))
+    for t in (q, g):
+        for i in range(0, T, 90000):
+            t[i:i + 90000].normal_()
+    k = k[:1].expand(T, 1, D).contiguous()
+    pos = torch.arange(T, device="cuda") % 97
+    q.requires_grad_()
+    y, _ = ops.qk_norm_rope(q, k, cos, sin, pos, wq, wk)
+    (dq,) = torch.autograd.grad(y, q, g)
+    at = torch.tensor([0, T // 2, T - 3, T - 1], device="cuda")
+    x = q.detach()[at].requires_grad_()
+    y2, _ = ops.qk_norm_rope(x, k[at], cos, sin, pos[at], wq, wk)
+    (dx,) = torch.autograd.grad(y2, x, g[at])
+    assert torch.equal(y[at], y2) and torch.equal(dq[at], dx)
+
+
 def test_no_second_derivative_and_changed_inputs():
     ops = _ops()
     q, k, _, wq, wk, cos, sin, pos = _inputs(3, 2, 1, 32, 32, FF)

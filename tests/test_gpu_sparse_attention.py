@@ -213,6 +213,41 @@ def test_pages_outside_the_pool_lengths_past_the_table():
     _check(case, 4, 1, 1)
 
 
+def test_chunks_over_bad_pages_and_lengths():
+    """The same of tiles of tokens: pages outside the pool are zeros that every token sees."""
+    case = list(_batch([6, 5, 4], [16 * 9 + 3, 16 * 7, 16 * 8], 4, 2, 64, 16, BF, E4))
+    table = case[5]
+    table[0, 2], table[0, 5], table[1, 6], table[2, 0], table[2, 7] = -1, case[1].shape[0], 10 ** 9, -5, -1
+    _check(case, 4, 1, 1)
+    case[7] = _i32([10 ** 9, -4, 2])  # past the table, below 0, fewer than the new tokens
+    _check(case, 4, 1, 1)
+
+
+def test_ranges_and_attention_past_32_bits():
+    """Pools of more than 2^32 bytes: the last pages are where they belong."""
+    ops = _ops()
+    P, H, page, D = 4200, 8, 512, 256  # 4.4e9 bytes a pool
+    g = torch.Generator().manual_seed(1)
+    kc, vc = (torch.zeros((P, H, page, D), dtype=torch.uint8, device="cuda").view(E4) for _ in range(2))
+    ks, vs = (torch.ones((P, H, page), device="cuda") for _ in range(2))
+    ids = [P - 1, 7, P - 2, P // 2, P - 5]
+    small = [torch.randn(5, H, page, D, generator=g).to(E4) for _ in range(2)]
+    for t, x in zip((kc, vc), small):
+        t.view(torch.uint8)[ids] = x.view(torch.uint8).cuda()
+    q = torch.randn(2, 8, D, generator=g).to(BF).cuda()
+    ranges = torch.zeros((P, H, 2, D), dtype=BF, device="cuda")
+    table, cu, lens = _i32([ids]), _i32([0, 2]), _i32([5 * page - 3])
+    ops.kv_page_ranges(kc, table, _i32([0, 5 * page - 3]), lens, ranges, ks)
+    near = [x.cuda() for x in small] + [torch.ones((5, H, page), device="cuda") for _ in range(2)]
+    r2 = torch.zeros((5, H, 2, D), dtype=BF, device="cuda")
+    t2 = _i32([[0, 1, 2, 3, 4]])
+    ops.kv_page_ranges(near[0], t2, _i32([0, 5 * page - 3]), lens, r2, near[2])
+    assert torch.equal(ranges[ids], r2)
+    a = ops.sparse_paged_attention(q, kc, vc, ranges, table, cu, lens, ks, vs, num_selected=3)
+    b = ops.sparse_paged_attention(q, near[0], near[1], r2, t2, cu, lens, near[2], near[3], num_selected=3)
+    assert torch.equal(a, b) and bool(a.any())
+
+
 def test_no_tokens_no_pages():
     ops = _ops()
     q, kc, vc, ks, vs, table, cu, lens = _batch([1, 1], [40, 3], 4, 2, 64, 16, BF, E4)

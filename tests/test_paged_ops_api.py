@@ -255,6 +255,33 @@ def test_changed_tensors_count_as_changed(monkeypatch):
         assert all(args[n]._version > b for n, b in zip(names, before)), fn
 
 
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    """The current device is the tensors' while a size is asked for and a kernel launched."""
+    from primus_turbo.pytorch import _C
+
+    class Device:
+        current = 0
+
+        def __init__(self, device):
+            self.device, self.before = device, Device.current
+
+        def __enter__(self):
+            Device.current = self.device.index
+
+        def __exit__(self, *_):
+            Device.current = self.before
+
+    seen = []
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_C, "_cur_device", lambda: Device.current)
+    monkeypatch.setattr(_C, "call", lambda name, *args: seen.append((name, Device.current)))
+    monkeypatch.setattr(_C, "query", lambda name, *args: seen.append((name, Device.current)))
+    for i in (1, 0):
+        _C.call_on(torch.device("cuda", i), "launch")
+        _C.query_on(torch.device("cuda", i), "size")
+    assert seen == [("launch", 1), ("size", 1), ("launch", 0), ("size", 0)] and Device.current == 0
+
+
 def test_c_entries_refuse():
     from primus_turbo.pytorch import _C
 
@@ -335,6 +362,12 @@ def test_workspaces_stay_small():
     assert _C.query("pta_select_pages_workspace_size", 100000, 8, 4096) <= 256 << 20
     assert _C.query("pta_select_pages_workspace_size", 1, 64, 1 << 20) == 64 * 8 << 20  # one token's
     assert _C.query("pta_select_pages_workspace_size", 0, 8, 64) == 0
+    # lists of a tile's tokens: 10 bytes for each page that a token takes, 12 a token; parts of tiles
+    # that do not fill the chip
+    q = lambda *a: _C.query("pta_sparse_paged_attention_workspace_size", *a)  # noqa: E731
+    assert q(8192, 1, 32, 8, 128, 256, 64, 16) <= 8192 * 8 * 16 * 10 + 12 * 8192 + (256 << 20) + 4096
+    assert q(64, 64, 32, 4, 64, 512, 32, 48) <= 64 * 4 * 48 * 4 + 12 * 64 + max(64 * 4 * 512 * 8, 8 * 64 * 32 * (4 * 64 + 8)) + 4096
+    assert q(0, 1, 32, 8, 128, 256, 64, 16) == 0
     # a row for each workgroup that sums
     assert _C.query("pta_qk_norm_rope_backward_workspace_size", 1 << 20, 32, 8, 128) <= (8 * 256 + 2) * 128 * 4
     assert _C.query("pta_qk_norm_rope_backward_workspace_size", 0, 32, 8, 128) == 0
