@@ -1394,9 +1394,10 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
     else attn_pad(a, block - work, pads);
 }
 // Bound by the vector instructions of a tile of 32 keys a wave, 380, and their waits: the keys
-// come from the L2 (97% of the reads hit).  Three workgroups a CU with one tile in flight:
-// 1024 tokens, 37 pages of 64 in a tile's list of 32 / 8 heads of 128, ATT_TILE_3 us; two with two in
-// flight ATT_TILE_2.
+// come from the L2 (97% of the reads hit).  Three workgroups a CU with one tile in flight, at the
+// price of 11 spilled registers: 1024 tokens, 37 pages of 64 in a tile's list, 32 / 8 heads of
+// 128, e4m3, 173 us; two with two in flight 206, two with one 204.  The 16-bit cache at 128
+// elements would spill 56: two.
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 && KIND == PTA_CACHE_16BIT ? 2 : 3) void attn_tile_kernel(AttnArgs a) {
     __shared__ AttnTileLds<DP> lds;

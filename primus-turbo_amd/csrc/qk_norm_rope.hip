@@ -18,6 +18,13 @@
 // sizes allow, that is 8 elements of either half, 16 bytes each.
 //
 // All of it is fp32 between the loads and the one rounding of what is stored.
+//
+// Bound by memory: each row is read once and written once, the angles' tables come from the
+// caches.  8192 tokens of 32 and 8 heads of 128, bf16, inputs and outputs not in the caches:
+// forward 34 us (4.9 TB/s; a large copy 5.2), backward 52 (4.8) and 3 for the joined sums,
+// cache write to e4m3 37 (5.1).  A row a group of lanes, no loop over rows in the forward
+// pass: with two or four heads a lane, whose loads are in flight together, 36 and 37 us (the
+// chip has enough rows in flight, and more small workgroups spread loads and stores better).
 #include <algorithm>
 #include <climits>
 
@@ -583,7 +590,8 @@ template <int KIND, int DT, bool NB> void qr_forward(QRArgs &a, QRShape s, hipSt
 }
 
 // Workgroups of the backward pass for the queries and the keys, each with the same
-// number of runs of rows: at most QR_BACK a CU of both.
+// number of runs of rows: at most QR_BACK a CU of both (8192 tokens of 32 and 8 heads of 128
+// with the sums: 54.7 us with three or four, 58 with two or eight, 63 with 16).
 constexpr int QR_BACK = 4;
 void qr_back_blocks(int64_t T, int64_t Hq, int64_t Hkv, int64_t (&blocks)[2]) {
     const int64_t H[2] = {Hq, Hkv}, most = QR_BACK * device_cu_count();
