@@ -91,7 +91,7 @@ def kv_cache_fork_impl(
         assert parents.dim() == 1 and parents.dtype in _INT and parents.is_contiguous(), "parents must be contiguous one-dimensional int32 / int64"
         N = parents.shape[0]
         others.append(parents)
-    reserve = int(reserve)
+    reserve = min(int(reserve), 2**31 - 1)  # more than any length
     assert reserve >= 0, "reserve must not be negative"
     check_tensors("kv_cache_fork", tensors, *others)
     dev = k_cache.device
