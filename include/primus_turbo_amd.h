@@ -629,9 +629,9 @@ int pta_kv_cache_copy(void *k_cache, void *v_cache, int cache_kind, int64_t num_
  * one fills it); the others get copies.  Every new sequence gets pages for `reserve`
  * further tokens, as far as max_pages reach.  Copies and fresh pages are the lowest
  * pages that no new sequence has, taken in the sequences' order; where they run out a
- * sequence gets length -1 and no pages.  Other sequences' pages are free afterwards,
- * and so are pages past a sequence's length.  compact: the new sequences' pages, n of
- * them, move to pages below n.
+ * sequence gets length -1 and no pages, and so do those that go on from it.  Other
+ * sequences' pages are free afterwards, and so are pages past a sequence's length.
+ * compact: the new sequences' pages, n of them, move to pages below n, unless pages run out.
  *   new_page_table [num_new_seqs, max_pages], -1 behind a sequence's pages
  *   new_seq_lens   [num_new_seqs]: its parent's; 0 for a parent that does not exist
  * Entries of page_table outside the pool stay as they are.  The old table is left as it

@@ -116,8 +116,9 @@ __device__ __forceinline__ KFSeq kf_seq(const KFArgs &a, int i) {
     const int64_t p = a.parents ? kp_index(a.parents, a.parents_i64, i) : i;
     if (p < 0 || p >= a.B) return s;
     s.parent        = static_cast<int>(p);
+    if (a.lens[p] < 0) return s; // pages had run out for it
     const int64_t most = static_cast<int64_t>(a.M) * a.page;
-    const int64_t len  = min(static_cast<int64_t>(max(a.lens[p], 0)), most);
+    const int64_t len  = min(static_cast<int64_t>(a.lens[p]), most);
     s.full = static_cast<int>(len / a.page);
     s.part = len - static_cast<int64_t>(s.full) * a.page > 0;
     s.has  = s.full + s.part;

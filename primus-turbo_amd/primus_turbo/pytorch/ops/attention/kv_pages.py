@@ -68,10 +68,11 @@ def kv_cache_fork(
     many further tokens, as far as ``max_pages`` reach.  Copies and fresh pages go to the
     lowest pages that no new sequence has, in the order of the sequences.  Pages of
     sequences that nobody goes on from, and pages past a length, are free.  ``compact``:
-    the n pages that the new sequences have become pages 0 to n - 1.
+    the n pages that the new sequences have become pages 0 to n - 1, unless pages run out.
 
     New rows end in -1.  A sequence for which the pages run out gets length -1 and no
-    pages, one whose parent does not exist length 0.  Table entries outside the pool
-    (pages that read as zeros) stay as they are.
+    pages, and so does one that goes on from it (a parent's length below 0 is handed on);
+    one whose parent does not exist gets length 0.  Table entries outside the pool (pages
+    that read as zeros) stay as they are.
     """
     return kv_cache_fork_impl(k_cache, v_cache, page_table, seq_lens, parents, k_scale_inv, v_scale_inv, key_ranges, reserve, compact)

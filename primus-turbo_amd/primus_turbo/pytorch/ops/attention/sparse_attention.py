@@ -46,7 +46,8 @@ def kv_page_ranges(
 
     The other arguments are ``paged_attention``'s.  A page's range is that of its tokens
     below the sequence's length, rounded outward to bfloat16 (a channel in which a key is
-    NaN has NaN); other pages' ranges stay as they are.
+    NaN has NaN); other pages' ranges stay as they are.  A page with new tokens is one
+    sequence's alone, as ``kv_cache_fork`` leaves it.
     """
     kv_page_ranges_impl(k_cache, page_table, cu_seqlens_q, seq_lens, key_ranges, k_scale_inv)
 

@@ -114,7 +114,7 @@ def fork_books(table, lens, parents, page, P, reserve, compact):
             seqs.append(None)
             continue
         n = min(max(lens[p], 0), M * page)
-        seqs.append((p, n // page, -(-n // page), min(M, -(-(n + reserve) // page))))
+        seqs.append((p, n // page, -(-n // page), min(M, -(-(n + reserve) // page)) if lens[p] >= 0 else 0))
     inside = lambda u: 0 <= u < P  # noqa: E731
     full = {u for s in seqs if s for u in table[s[0]][:s[1]] if inside(u)}
     keeper = {}

@@ -227,6 +227,18 @@ def test_fork_without_parents_sequences_or_pages():
     assert got[0].shape == (2, 0) and got[1].tolist() == [6, 3]
 
 
+def test_fork_of_a_sequence_without_pages():
+    """Pages run out for one sequence; what goes on from it gets none either, and takes none from the others."""
+    ops = _ops()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    pools = _pools(0, 3, 2, 4, 16, BF)
+    table, lens = ops.kv_cache_fork(pools[0], pools[1], i32([0, -1], [1, -1]), i32(2, 2), i32(0, 0, 1, 1))
+    assert table.tolist() == [[0, -1], [2, -1], [1, -1], [-1, -1]] and lens.tolist() == [2, 2, 2, -1]
+    for compact in (False, True):
+        got = ops.kv_cache_fork(pools[0], pools[1], table, lens, i32(3, 0), reserve=6, compact=compact)
+        assert got[0].tolist() == [[-1, -1], [0, 1]] and got[1].tolist() == [-1, 2]
+
+
 def test_fork_other_stream_and_captured():
     ops = _ops()
     r = random.Random(8)

@@ -385,3 +385,5 @@ def test_books_by_hand():
     assert fork_books([[5, 6], [5, -1]], [8, 3], [0, 1], 4, 8, 0, False) == ([[5, 6], [0, -1]], [8, 3], [(5, 0)])
     # too few pages: the first in order get theirs
     assert fork_books([[0, -1], [1, -1]], [2, 2], [0, 0, 1, 1], 4, 3, 0, False) == ([[0, -1], [2, -1], [1, -1], [-1, -1]], [2, 2, 2, -1], [(0, 2)])
+    # and one that had none gets none, whatever it is to reserve
+    assert fork_books([[0, -1], [-1, -1]], [2, -1], [1, 0, 1], 4, 3, 9, False) == ([[-1, -1], [0, 1], [-1, -1]], [-1, 2, -1], [])
