@@ -1031,7 +1031,9 @@ template <int DP> struct AttnTileLds : AttnNarrowLds<DP> {
 
 // TILE: the rows are a tile of tokens', whatever their sequences, the keys those of the tile's
 // list of pages, each with its position and the tokens that take its page.
-template <int QT, int KIND, int DP, bool TILE, class Lds>
+// RUN: a wave's 32 keys of a tile are one run of a page (pages of whole runs, a pool that has
+// some): its address, its page's tokens and whether it is there are the wave's, not a key's.
+template <int QT, int KIND, int DP, bool TILE, bool RUN, class Lds>
 __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &lds) {
     constexpr int  KT = ATT_NARROW_KEYS, BQ = ATT_NARROW_ROWS, WK = 32;
     constexpr bool FP8 = KIND != PTA_CACHE_16BIT;
@@ -1088,11 +1090,22 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
         uint4    kreg[ST][2][KP], vreg[ST][VP];
         float    scl[ST][2];
         int      krow[ST], page_id = -1;
-        int2     kinfo[TILE ? ST : 1], page_info = make_int2(0, 0); // position of the lane's key, its page's tokens
+        // position of the lane's key, or of the run's first, and its page's tokens; RUN: the list's position, the page's tokens
+        int2     kinfo[TILE ? ST : 1], page_info = make_int2(0, 0);
         uint64_t hole[ST];
         auto     key = [&](int t) PTA_INLINE { return attn_key0(it, t, KT) + wave * WK + (lane & 31); };
         auto     fetch_page = [&](int t) PTA_INLINE {
-            if constexpr (TILE) {
+            if constexpr (RUN) { // as loaded: nothing waits for it here
+                page_id     = -1;
+                page_info.y = 0;
+                const int j = attn_key0(it, t, KT) + wave * WK;
+                if (t < it.t1 && j < it.kend) {
+                    const int  e = attn_page_of(a, j);
+                    const int2 x = list[e];
+                    page_id      = x.x;
+                    page_info    = make_int2(x.y, masks[e]);
+                }
+            } else if constexpr (TILE) {
                 page_id   = -1;
                 page_info = make_int2(0, 0);
                 const int j = t < it.t1 ? key(t) : it.kend;
@@ -1109,6 +1122,33 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
         // loads tile t, whose pages were fetched before; keys without a row read row 0
         // and become zeros when they are used
         auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no, int2 &info) PTA_INLINE {
+            if constexpr (RUN) {
+                const int  id = __builtin_amdgcn_readfirstlane(page_id), j = attn_key0(it, t, KT) + wave * WK;
+                const int  off = j - attn_page_of(a, j) * a.page;
+                const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.num_pages);
+                info = make_int2(__builtin_amdgcn_readfirstlane(page_info.x) + off, __builtin_amdgcn_readfirstlane(page_info.y));
+                no   = !there;
+                const int      at = there ? (id * a.Hkv + h) * a.page + off : 0; // the run, and so its 32 rows, are the pool's
+                const int64_t  byte = static_cast<int64_t>(at) * a.D * ES;
+                const uint8_t *kp = a.kc + byte, *vp = a.vc + byte;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < KP; ++i) {
+                        const int e = qd * (DP / 4) + i * EC;
+                        kr[k][i]    = *reinterpret_cast<const uint4 *>(kp + k * 16 * a.D * ES + static_cast<uint32_t>((c * a.D + (e < a.D ? e : 0)) * ES));
+                    }
+#pragma unroll
+                for (int i = 0; i < VP; ++i) {
+                    const int e = (lane % CPR) * EC;
+                    vr[i]       = *reinterpret_cast<const uint4 *>(vp + i * (64 / CPR) * a.D * ES + static_cast<uint32_t>((lane / CPR * a.D + (e < a.D ? e : 0)) * ES));
+                }
+                if constexpr (FP8) {
+                    sc[0] = a.ks[at + (lane & 31)];
+                    sc[1] = a.vs[at + (lane & 31)];
+                }
+                return;
+            }
             if constexpr (TILE) info = page_info;
             row = t < it.t1 ? attn_page_row(a, h, key(t), page_id) : -1;
             no  = __ballot(row < 0);
@@ -1163,7 +1203,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 if (a.D != DP || hole[u] != 0) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const bool no = __shfl(krow[u], k * 16 + c) < 0;
+                        const bool no = RUN ? hole[u] != 0 : __shfl(krow[u], k * 16 + c) < 0;
 #pragma unroll
                         for (int i = 0; i < KP; ++i)
                             if (no || qd * (DP / 4) + i * EC >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
@@ -1171,9 +1211,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
 #pragma unroll
                     for (int i = 0; i < VP; ++i) {
                         const int p = i * 64 + lane;
-                        if (__shfl(krow[u], p / CPR) < 0 || (p % CPR) * EC >= a.D) vreg[u][i] = make_uint4(0, 0, 0, 0);
+                        if ((RUN ? hole[u] != 0 : __shfl(krow[u], p / CPR) < 0) || (p % CPR) * EC >= a.D) vreg[u][i] = make_uint4(0, 0, 0, 0);
                     }
-                    if (krow[u] < 0) {
+                    if (RUN ? hole[u] != 0 : krow[u] < 0) {
                         scl[u][0] = 0.0f;
                         scl[u][1] = 1.0f;
                     }
@@ -1214,7 +1254,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                             kf[k][s] = kreg[u][k][s];
                         }
                     }
-                if constexpr (TILE) {
+                // the last of the run's keys that the lane's row sees
+                const int upto = RUN && rin && (kinfo[TILE ? u : 0].y >> rtok & 1) ? pos - kinfo[TILE ? u : 0].x : -1;
+                if constexpr (TILE && !RUN) {
                     if (lane < WK) {
                         lds.skey[wave][0][lane] = kinfo[u].x;
                         lds.skey[wave][1][lane] = kinfo[u].y;
@@ -1251,7 +1293,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                         for (int j = 0; j < 4; ++j) s[k][j] *= a.scale_log2;
                     }
                     int4 kp, km;
-                    if constexpr (TILE) {
+                    if constexpr (TILE && !RUN) {
                         kp = *reinterpret_cast<const int4 *>(&lds.skey[wave][0][kk]);
                         km = *reinterpret_cast<const int4 *>(&lds.skey[wave][1][kk]);
                     }
@@ -1259,8 +1301,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int  ky  = key0 + kk + j;
-                        const bool see = TILE ? (kpos[j] <= pos) & ((kmask[j] >> rtok & 1) != 0)
-                                              : (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
+                        const bool see = RUN    ? kk + j <= upto
+                                         : TILE ? (kpos[j] <= pos) & ((kmask[j] >> rtok & 1) != 0)
+                                                : (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
                         s[k][j]        = see ? s[k][j] : -INFINITY;
                         mx             = fmaxf(mx, s[k][j]);
                     }
@@ -1390,7 +1433,7 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
 template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_narrow_kernel(AttnArgs a, int pads) {
     __shared__ AttnNarrowLds<DP> lds;
     const int block = blockIdx.x, work = gridDim.x - pads;
-    if (block < work) attn_narrow<QT, KIND, DP, false>(a, block, lds);
+    if (block < work) attn_narrow<QT, KIND, DP, false, false>(a, block, lds);
     else attn_pad(a, block - work, pads);
 }
 // Bound by the vector instructions of a tile of 32 keys a wave, 380, and their waits: the keys
@@ -1398,10 +1441,10 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
 // price of 11 spilled registers: 1024 tokens, 37 pages of 64 in a tile's list, 32 / 8 heads of
 // 128, e4m3, 173 us; two with two in flight 206, two with one 204.  The 16-bit cache at 128
 // elements would spill 56: two.
-template <int QT, int KIND, int DP>
+template <int QT, int KIND, int DP, bool RUN>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 && KIND == PTA_CACHE_16BIT ? 2 : 3) void attn_tile_kernel(AttnArgs a) {
     __shared__ AttnTileLds<DP> lds;
-    attn_narrow<QT, KIND, DP, true>(a, blockIdx.x, lds);
+    attn_narrow<QT, KIND, DP, true, RUN>(a, blockIdx.x, lds);
 }
 template <int QT, int KIND, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnArgs w, AttnArgs n, int w_blocks, int pads) {
@@ -1412,7 +1455,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_both_kernel(AttnA
     } lds;
     const int block = blockIdx.x, work = gridDim.x - pads;
     if (block < w_blocks) attn_wide<QT, KIND, DP>(w, block, lds.w);
-    else if (block < work) attn_narrow<QT, KIND, DP, false>(n, block - w_blocks, lds.n);
+    else if (block < work) attn_narrow<QT, KIND, DP, false, false>(n, block - w_blocks, lds.n);
     else attn_pad(n, block - work, pads);
 }
 

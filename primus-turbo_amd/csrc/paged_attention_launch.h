@@ -34,11 +34,16 @@ template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st) 
     join<<<static_cast<unsigned>(n + w), 256, 0, st>>>(c.narrow, c.wide, n, c.narrow_join_parts);
 }
 
-template <int QT, int KIND> void attn_launch_tiles_k(const AttnArgs &a, hipStream_t st) {
+template <int QT, int KIND, int DP> void attn_launch_tiles_d(const AttnArgs &a, hipStream_t st) {
     const unsigned grid = static_cast<unsigned>(a.B) * a.split * a.Hkv;
-    if (a.D <= 64) attn_tile_kernel<QT, KIND, 64><<<grid, 256, 0, st>>>(a);
-    else if (a.D <= 128) attn_tile_kernel<QT, KIND, 128><<<grid, 256, 0, st>>>(a);
-    else attn_tile_kernel<QT, KIND, 256><<<grid, 256, 0, st>>>(a);
+    if (a.page % 32 == 0 && a.num_pages > 0) attn_tile_kernel<QT, KIND, DP, true><<<grid, 256, 0, st>>>(a);
+    else attn_tile_kernel<QT, KIND, DP, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <int QT, int KIND> void attn_launch_tiles_k(const AttnArgs &a, hipStream_t st) {
+    if (a.D <= 64) attn_launch_tiles_d<QT, KIND, 64>(a, st);
+    else if (a.D <= 128) attn_launch_tiles_d<QT, KIND, 128>(a, st);
+    else attn_launch_tiles_d<QT, KIND, 256>(a, st);
 }
 
 template <int QT> void attn_launch_tiles(const AttnArgs &a, int kind, hipStream_t st) {
