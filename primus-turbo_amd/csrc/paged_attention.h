@@ -1119,36 +1119,40 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 page_id = t < it.t1 ? attn_key_page(a, it, pages, key(t)) : -1;
             }
         };
+        // RUN: row of tile t's first key, whose page was fetched before, or row 0 (the pool has a
+        // run of rows there too) if it is none of the pool's
+        auto run_at = [&](int t, uint64_t &no, int2 &info) PTA_INLINE {
+            const int  id = __builtin_amdgcn_readfirstlane(page_id), j = attn_key0(it, t, KT) + wave * WK;
+            const int  off = j - attn_page_of(a, j) * a.page;
+            const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.num_pages);
+            info = make_int2(__builtin_amdgcn_readfirstlane(page_info.x) + off, __builtin_amdgcn_readfirstlane(page_info.y));
+            no   = !there;
+            return there ? (id * a.Hkv + h) * a.page + off : 0;
+        };
+        auto run_keys = [&](int at, uint4(&kr)[2][KP], float(&sc)[2]) PTA_INLINE {
+            const uint8_t *p = a.kc + static_cast<int64_t>(at) * a.D * ES;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+                    const int e = qd * (DP / 4) + i * EC;
+                    kr[k][i]    = *reinterpret_cast<const uint4 *>(p + k * 16 * a.D * ES + static_cast<uint32_t>((c * a.D + (e < a.D ? e : 0)) * ES));
+                }
+            if constexpr (FP8) {
+                sc[0] = a.ks[at + (lane & 31)];
+                sc[1] = a.vs[at + (lane & 31)];
+            }
+        };
+        auto run_values = [&](int at, uint4(&vr)[VP]) PTA_INLINE {
+            const uint8_t *p = a.vc + static_cast<int64_t>(at) * a.D * ES;
+            const int      e = (lane % CPR) * EC;
+#pragma unroll
+            for (int i = 0; i < VP; ++i)
+                vr[i] = *reinterpret_cast<const uint4 *>(p + i * (64 / CPR) * a.D * ES + static_cast<uint32_t>((lane / CPR * a.D + (e < a.D ? e : 0)) * ES));
+        };
         // loads tile t, whose pages were fetched before; keys without a row read row 0
         // and become zeros when they are used
         auto     load = [&](int t, uint4(&kr)[2][KP], uint4(&vr)[VP], float(&sc)[2], int &row, uint64_t &no, int2 &info) PTA_INLINE {
-            if constexpr (RUN) {
-                const int  id = __builtin_amdgcn_readfirstlane(page_id), j = attn_key0(it, t, KT) + wave * WK;
-                const int  off = j - attn_page_of(a, j) * a.page;
-                const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.num_pages);
-                info = make_int2(__builtin_amdgcn_readfirstlane(page_info.x) + off, __builtin_amdgcn_readfirstlane(page_info.y));
-                no   = !there;
-                const int      at = there ? (id * a.Hkv + h) * a.page + off : 0; // the run, and so its 32 rows, are the pool's
-                const int64_t  byte = static_cast<int64_t>(at) * a.D * ES;
-                const uint8_t *kp = a.kc + byte, *vp = a.vc + byte;
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int i = 0; i < KP; ++i) {
-                        const int e = qd * (DP / 4) + i * EC;
-                        kr[k][i]    = *reinterpret_cast<const uint4 *>(kp + k * 16 * a.D * ES + static_cast<uint32_t>((c * a.D + (e < a.D ? e : 0)) * ES));
-                    }
-#pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    const int e = (lane % CPR) * EC;
-                    vr[i]       = *reinterpret_cast<const uint4 *>(vp + i * (64 / CPR) * a.D * ES + static_cast<uint32_t>((lane / CPR * a.D + (e < a.D ? e : 0)) * ES));
-                }
-                if constexpr (FP8) {
-                    sc[0] = a.ks[at + (lane & 31)];
-                    sc[1] = a.vs[at + (lane & 31)];
-                }
-                return;
-            }
             if constexpr (TILE) info = page_info;
             row = t < it.t1 ? attn_page_row(a, h, key(t), page_id) : -1;
             no  = __ballot(row < 0);
@@ -1172,7 +1176,6 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 sc[1] = a.vs[at];
             }
         };
-        fetch_page(it.t0);
         // k-step s of the products over the head dimension takes elements
         // qd * DP / 4 + 8 s .. + 7 from quarter qd of the lanes: a lane's part of a
         // key row is one run of bytes
@@ -1184,15 +1187,28 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                                          : make_uint4(0, 0, 0, 0);
         }
         att_f4 o[DP / 16];
+        float  m, l;
+        // Infinities and NaN among the values that only some rows see take a product of their own.
+        // TILE goes without and looks at the sums, which are not finite then: all is done again
+        // with care.  Else each tile of values is looked at.
+        auto keys = [&](auto careful_c) PTA_INLINE {
+        constexpr bool careful = decltype(careful_c)::value != 0;
+        fetch_page(it.t0);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
-
+        m = -INFINITY;
+        l = 0.0f;
         att_each<ST>([&](auto u_c) PTA_INLINE {
             constexpr int u = decltype(u_c)::value;
-            load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+            if constexpr (RUN) {
+                const int at = run_at(it.t0 + u, hole[u], kinfo[u]);
+                run_keys(at, kreg[u], scl[u]);
+                run_values(at, vreg[u]);
+            } else {
+                load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+            }
             fetch_page(it.t0 + u + 1);
         });
         for (int tt = it.t0; tt < it.t1; tt += ST)
@@ -1218,8 +1234,8 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                         scl[u][1] = 1.0f;
                     }
                 }
-                bool special = false;
-                if (mixed) {
+                bool special = careful;
+                if (!TILE && mixed) {
 #pragma unroll
                     for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[u][i]);
                     special = __any(special);
@@ -1242,36 +1258,49 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                         ssc[wave][2][lane] = 1.0f / att_clamp_scale(scl[u][1]);
                     }
                 }
-                uint4 kf[2][DP / 32];
+                auto key_of = [&](int k, int i) PTA_INLINE { // operand of k-step i
+                    if constexpr (FP8) {
+                        const uint4 w = kreg[u][k][i / 2];
+                        return i % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
+                    } else {
+                        return kreg[u][k][i];
+                    }
+                };
+                // the last of the run's keys that the lane's row sees
+                const int upto = RUN && rin && (kinfo[TILE ? u : 0].y >> rtok & 1) ? pos - kinfo[TILE ? u : 0].x : -1;
+                att_f4    s[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int s = 0; s < DP / 32; ++s) {
-                        if constexpr (FP8) {
-                            const uint4 w = kreg[u][k][s / 2];
-                            kf[k][s] = s % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
-                        } else {
-                            kf[k][s] = kreg[u][k][s];
+                    for (int j = 0; j < 4; ++j) s[k][j] = 0.0f;
+                if constexpr (RUN) {
+                    // the keys as they are until the products take them: fewer registers, another workgroup
+                    const int at = run_at(t + ST, hole[u], kinfo[u]);
+                    run_values(at, vreg[u]);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) s[k] = AttT<QT>::mfma16(key_of(k, i), qf[i], s[k]);
+                    run_keys(at, kreg[u], scl[u]);
+                } else {
+                    uint4 kf[2][DP / 32];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) kf[k][i] = key_of(k, i);
+                    if constexpr (TILE) {
+                        if (lane < WK) {
+                            lds.skey[wave][0][lane] = kinfo[u].x;
+                            lds.skey[wave][1][lane] = kinfo[u].y;
                         }
                     }
-                // the last of the run's keys that the lane's row sees
-                const int upto = RUN && rin && (kinfo[TILE ? u : 0].y >> rtok & 1) ? pos - kinfo[TILE ? u : 0].x : -1;
-                if constexpr (TILE && !RUN) {
-                    if (lane < WK) {
-                        lds.skey[wave][0][lane] = kinfo[u].x;
-                        lds.skey[wave][1][lane] = kinfo[u].y;
-                    }
+                    load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) s[k] = AttT<QT>::mfma16(kf[k][i], qf[i], s[k]);
                 }
-                load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
                 fetch_page(t + ST + 1);
-                att_f4 s[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[k][j] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) s[k] = AttT<QT>::mfma16(kf[k][i], qf[i], s[k]);
-                }
                 // the wave's own LDS writes are seen by its later reads once they are done
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
@@ -1308,11 +1337,20 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                         mx             = fmaxf(mx, s[k][j]);
                     }
                 }
-                mx                = max_xor32(max_xor16(mx));
-                const float base  = mx == -INFINITY ? 0.0f : mx;
-                const float alpha = att_exp2(m - base);
-                m                 = mx;
-                l *= alpha;
+                mx = max_xor32(max_xor16(mx));
+                // TILE: the sums stay as they are while no row's maximum has grown by more than 8 (P to 2^8)
+                float alpha = 1.0f;
+                if (!TILE || __any(mx > m + 8.0f)) {
+                    alpha = att_exp2(m - (mx == -INFINITY ? 0.0f : mx));
+                    m     = mx;
+                    l *= alpha;
+                    if constexpr (TILE)
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -1326,8 +1364,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 const int   kr = 4 * qd + c / 4, dc = 4 * (c & 3);
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) {
+                    if constexpr (!TILE)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+                        for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
                     const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
                     const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
                     if (!special) {
@@ -1354,6 +1393,16 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             });
+        };
+        keys(std::integral_constant<int, 0>{});
+        if constexpr (TILE) {
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) finite &= fabsf(o[i][j]) < INFINITY;
+            if (!__all(finite)) keys(std::integral_constant<int, 1>{});
+        }
         l = add_xor32(add_xor16(l));
         // the four waves' parts join in LDS
         __syncthreads(); // the values' LDS becomes the outputs'
