@@ -1045,6 +1045,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
     constexpr int  VP  = WK * CPR / 64;     // value pieces of a lane
     constexpr int  VS = AttnNarrowLds<DP>::VS, OS = AttnNarrowLds<DP>::OS;
     static_assert(KP >= 1, "a quarter row is a piece at least");
+    constexpr bool QUAD = RUN && KP >= 2; // keys are read by quads of lanes, and change places (run_keys)
     auto &smem = lds.smem; auto &ssc = lds.ssc; auto &sml = lds.sml;
 
     const int     tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1129,26 +1130,72 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
             no   = !there;
             return there ? (id * a.Hkv + h) * a.page + off : 0;
         };
+        // The base is opaque, so that it stays in scalar registers and the lane's part is 32 bits
+        auto run_load = [&](const uint8_t *pool, int64_t base, uint32_t part) PTA_INLINE {
+            typedef uint32_t piece __attribute__((ext_vector_type(4)));
+            typedef const __attribute__((address_space(1))) uint8_t byte;
+            uint64_t p = reinterpret_cast<uint64_t>(pool) + base;
+            asm volatile("" : "+s"(p));
+            return __builtin_bit_cast(uint4, *reinterpret_cast<const __attribute__((address_space(1))) piece *>(reinterpret_cast<byte *>(p) + part));
+        };
+        // Element at which piece i of the lane's keys begins.  QUAD: eight pieces of a row, 128 bytes, are
+        // the four quarters' in the order 0, 2, 1, 3.
+        auto piece_at = [&](int i) PTA_INLINE {
+            return QUAD ? (i / 2 * 8 + 4 * (qd & 1) + 2 * (qd >> 1) + i % 2) * EC : qd * (DP / 4) + i * EC;
+        };
+        // As they are loaded, QUAD: piece i of 128 bytes of key 4 (c / 4) + i, of the first or second 16
+        // keys by the lane's half, whose four lanes read 64 bytes of one key.  (A lane a row takes the
+        // memory pipe a cycle a lane, 64 where these take 16.)
+        auto loaded_at = [&](int i) PTA_INLINE { return QUAD ? (i / 2 * 8 + 4 * (qd & 1) + (lane & 3)) * EC : piece_at(i); };
         auto run_keys = [&](int at, uint4(&kr)[2][KP], float(&sc)[2]) PTA_INLINE {
-            const uint8_t *p = a.kc + static_cast<int64_t>(at) * a.D * ES;
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < KP; ++i) {
-                    const int e = qd * (DP / 4) + i * EC;
-                    kr[k][i]    = *reinterpret_cast<const uint4 *>(p + k * 16 * a.D * ES + static_cast<uint32_t>((c * a.D + (e < a.D ? e : 0)) * ES));
+                    const int e = loaded_at(i), row = QUAD ? (lane >> 5) * 16 + (c & ~3) : c;
+                    kr[k][i]    = run_load(a.kc, (static_cast<int64_t>(at) + (QUAD ? 2 * k + i % 2 : 16 * k)) * a.D * ES,
+                                           (row * a.D + (e < a.D ? e : 0)) * ES);
                 }
             if constexpr (FP8) {
                 sc[0] = a.ks[at + (lane & 31)];
                 sc[1] = a.vs[at + (lane & 31)];
             }
         };
+        // QUAD: to the places of an operand.  Lane p of four gets piece i of key p for key i's piece p,
+        // then the halves exchange, so that a register has the same 16 keys in all quarters.
+        auto run_turn = [&](uint4(&kr)[2][KP]) PTA_INLINE {
+            const bool odd = lane & 1, high = lane & 2;
+            auto       swap = [&](uint32_t &x, uint32_t &y, bool second, auto step) PTA_INLINE {
+                const uint32_t u = __builtin_amdgcn_mov_dpp(y, decltype(step)::value, 0xf, 0xf, true);
+                const uint32_t v = __builtin_amdgcn_mov_dpp(x, decltype(step)::value, 0xf, 0xf, true);
+                x = second ? u : x;
+                y = second ? y : v;
+            };
+            auto word = [](uint4 &v, int w) PTA_INLINE -> uint32_t & { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; };
+#pragma unroll
+            for (int i = 0; i < KP; i += 2)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t x[4] = {word(kr[0][i], w), word(kr[0][i + 1], w), word(kr[1][i], w), word(kr[1][i + 1], w)};
+                    using one = std::integral_constant<int, PTA_DPP_QUAD_XOR1>;
+                    using two = std::integral_constant<int, PTA_DPP_QUAD_XOR2>;
+                    swap(x[0], x[1], odd, one{});
+                    swap(x[2], x[3], odd, one{});
+                    swap(x[0], x[2], high, two{});
+                    swap(x[1], x[3], high, two{});
+                    const auto y = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+                    const auto z = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+                    word(kr[0][i], w)     = y[0];
+                    word(kr[1][i], w)     = y[1];
+                    word(kr[0][i + 1], w) = z[0];
+                    word(kr[1][i + 1], w) = z[1];
+                }
+        };
         auto run_values = [&](int at, uint4(&vr)[VP]) PTA_INLINE {
-            const uint8_t *p = a.vc + static_cast<int64_t>(at) * a.D * ES;
-            const int      e = (lane % CPR) * EC;
+            const int e = (lane % CPR) * EC;
 #pragma unroll
             for (int i = 0; i < VP; ++i)
-                vr[i] = *reinterpret_cast<const uint4 *>(p + i * (64 / CPR) * a.D * ES + static_cast<uint32_t>((lane / CPR * a.D + (e < a.D ? e : 0)) * ES));
+                vr[i] = run_load(a.vc, (static_cast<int64_t>(at) + i * (64 / CPR)) * a.D * ES, (lane / CPR * a.D + (e < a.D ? e : 0)) * ES);
         };
         // loads tile t, whose pages were fetched before; keys without a row read row 0
         // and become zeros when they are used
@@ -1182,7 +1229,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
         uint4 qf[DP / 32];
 #pragma unroll
         for (int s = 0; s < DP / 32; ++s) {
-            const int d = qd * (DP / 4) + s * 8;
+            const int d = FP8 ? piece_at(s / 2) + s % 2 * 8 : piece_at(s);
             qf[s]       = rin && d < a.D ? *reinterpret_cast<const uint4 *>(a.q + (tok0 + rtok) * a.q_st + hq * a.q_sh + d)
                                          : make_uint4(0, 0, 0, 0);
         }
@@ -1222,7 +1269,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                         const bool no = RUN ? hole[u] != 0 : __shfl(krow[u], k * 16 + c) < 0;
 #pragma unroll
                         for (int i = 0; i < KP; ++i)
-                            if (no || qd * (DP / 4) + i * EC >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
+                            if (no || loaded_at(i) >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
                     }
 #pragma unroll
                     for (int i = 0; i < VP; ++i) {
@@ -1277,6 +1324,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                     // the keys as they are until the products take them: fewer registers, another workgroup
                     const int at = run_at(t + ST, hole[u], kinfo[u]);
                     run_values(at, vreg[u]);
+                    if constexpr (QUAD) run_turn(kreg[u]);
 #pragma unroll
                     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -1305,15 +1353,29 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                // values as operands: element block i of the wave's keys
+                const int kr = 4 * qd + c / 4, dc = 4 * (c & 3);
+                auto      value_of = [&](int i) PTA_INLINE {
+                    const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
+                    return make_uint4(v0.x, v0.y, v1.x, v1.y);
+                };
+                // RUN: half of them are read before the exponentials and half behind, all before the products
+                uint4 vf[DP / 16];
+                if constexpr (RUN && !careful) {
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) vf[i] = value_of(i);
+                }
                 const int key0 = attn_key0(it, t, KT) + wave * WK;
                 float     mx = m, iv[2][4];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int kk = k * 16 + 4 * qd;
                     if constexpr (FP8) {
-                        const float4 x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
-                        const float4 y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
+                        float4       x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
+                        float4       y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
                         const float4 z = *reinterpret_cast<const float4 *>(&ssc[wave][2][kk]);
+                        // opaque: else they are read behind a branch, where a key is seen
+                        if constexpr (TILE) asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w), "+v"(y.x), "+v"(y.y), "+v"(y.z), "+v"(y.w));
                         s[k][0] = fmaf(s[k][0], x.x, y.x); s[k][1] = fmaf(s[k][1], x.y, y.y);
                         s[k][2] = fmaf(s[k][2], x.z, y.z); s[k][3] = fmaf(s[k][3], x.w, y.w);
                         iv[k][0] = z.x; iv[k][1] = z.y; iv[k][2] = z.z; iv[k][3] = z.w;
@@ -1361,23 +1423,26 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
                     }
                 const uint4 pf = make_uint4(AttT<QT>::pack(s[0][0], s[0][1]), AttT<QT>::pack(s[0][2], s[0][3]),
                                             AttT<QT>::pack(s[1][0], s[1][1]), AttT<QT>::pack(s[1][2], s[1][3]));
-                const int   kr = 4 * qd + c / 4, dc = 4 * (c & 3);
+                if constexpr (RUN && !careful) {
+#pragma unroll
+                    for (int i = DP / 32; i < DP / 16; ++i) vf[i] = value_of(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) {
                     if constexpr (!TILE)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
-                    const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
-                    const uint4 vf = make_uint4(v0.x, v0.y, v1.x, v1.y);
+                    if constexpr (!RUN || careful) vf[i] = value_of(i);
                     if (!special) {
-                        o[i] = AttT<QT>::mfma16(vf, pf, o[i]);
+                        o[i] = AttT<QT>::mfma16(vf[i], pf, o[i]);
                     } else {
                         // infinities and NaN that only some rows see: 0 * inf must not reach the
                         // others.  Finite values go as ever; then a count of the special ones that
                         // a row sees decides.
                         uint4  fin, plus, minus;
                         att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
-                        att_split_special<QT>(vf, fin, plus, minus);
+                        att_split_special<QT>(vf[i], fin, plus, minus);
                         const uint4 seen = att_nonzero<QT>(pf);
                         o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
                         np   = AttT<QT>::mfma16(plus, seen, np);
