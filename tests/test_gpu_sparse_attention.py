@@ -174,6 +174,47 @@ def test_chunk_with_special_values():
     assert torch.equal(got[:7], want[:7]) and bool(got[7].isnan().all())
 
 
+@pytest.mark.parametrize("cache,dtype", [(E4, BF), (E5, FH), (BF, BF), (FH, FH)])
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(4, 1, 64, 64), (8, 2, 128, 32), (4, 2, 256, 96), (2, 2, 16, 32), (12, 4, 112, 64), (6, 1, 48, 32)])
+def test_chunks_over_pages_of_whole_runs(cache, dtype, Hq, Hkv, D, page):
+    """Pages of 32 tokens or a multiple, some of them none of the pool's, lengths that end anywhere in a page."""
+    case = list(_batch([19, 1, 4], [page * 9 + 5, page * 4, page * 6 - 31], Hq, Hkv, D, page, dtype, cache, seed=page))
+    _check(case, 5, 1, 2)
+    table = case[5]
+    table[0, 3], table[0, 8], table[1, 0], table[2, 2] = -1, case[1].shape[0], 10 ** 9, -7
+    _check(case, 5, 1, 2)
+    case[7] = _i32([10 ** 9, -4, 3])
+    _check(case, 4, 0, 1)
+
+
+@pytest.mark.parametrize("cache,dtype", [(E4, BF), (E5, FH), (BF, BF), (FH, FH)])
+@pytest.mark.parametrize("D,page", [(128, 32), (64, 64), (128, 16)])
+def test_chunk_over_special_values(cache, dtype, D, page):
+    """Special values of a page that a part of a tile's tokens takes reach those alone, whose other elements hold."""
+    ops = _ops()
+    q, kc, vc, ks, vs, table, cu, lens = _batch([12], [page * 20], 4, 1, D, page, dtype, cache, seed=5)
+    ranges = _all_ranges(kc, ks, table, lens, page).cuda()
+    call = lambda: ops.sparse_paged_attention(q, kc, vc, ranges, table, cu, lens, ks, vs, num_selected=5)  # noqa: E731
+    sel, _ = ops.select_pages(q, ranges, table, cu, lens, page, num_selected=5)
+    want = call()
+    count = {int(p): [int(p) in sel[t, 0].tolist() for t in range(12)] for p in table[0].tolist()}
+    p, takers = next((p, x) for p, x in count.items() if 0 < sum(x[:4]) < 4)
+    for bad in (float("nan"),) if cache == E4 else (float("nan"), float("inf"), -float("inf")):
+        x = vc[p, 0, 3].float().cpu()
+        keep = x.clone()
+        x[7] = bad
+        vc[p, 0, 3] = x.to(cache).cuda()
+        got = call()
+        vc[p, 0, 3] = keep.to(cache).cuda()
+        other = [d for d in range(D) if d != 7]
+        for t in range(12):
+            if not takers[t]:
+                assert torch.equal(got[t], want[t])
+            else:
+                assert torch.equal(got[t, :, other], want[t, :, other])
+                assert bool(got[t, :, 7].isnan().all()) if math.isnan(bad) else bool((got[t, :, 7] == bad).all())
+
+
 def test_no_more_pages_than_selected_is_paged_attention():
     ops = _ops()
     q, kc, vc, ks, vs, table, cu, lens = _batch([1, 5, 1], [100, 90, 1], 8, 4, 128, 32, BF, E4)
