@@ -259,8 +259,8 @@ __device__ __forceinline__ void ps_scores(const PSArgs &a, const double (&sums)[
     }
 }
 
-// Few tokens with many pages (1 token, 2048 pages, 8 heads of 128: 5.4 us): pages [c per, (c + 1) per) of token t for head h.  Bound by the
-// chain of reads: the token's place, queries and page numbers, ranges.
+// Few tokens with many pages (1 token, 2048 pages, 8 heads of 128: 5.4 us): pages [c per, (c + 1) per)
+// of token t for head h.  Bound by the chain of reads: the token's place, queries and page numbers, ranges.
 template <int QT, int LPR> __global__ __launch_bounds__(PS_NT) void ps_score_kernel(PSArgs a, int per, int parts) {
     __shared__ double sums[2][8 * LPR];
     const uint32_t w = blockIdx.x, h = w % a.Hkv, w1 = w / a.Hkv, c = w1 % parts, ti = w1 / parts;

@@ -1239,225 +1239,227 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs &a, int block, Lds &l
         // TILE goes without and looks at the sums, which are not finite then: all is done again
         // with care.  Else each tile of values is looked at.
         auto keys = [&](auto careful_c) PTA_INLINE {
-        constexpr bool careful = decltype(careful_c)::value != 0;
-        fetch_page(it.t0);
+            constexpr bool careful = decltype(careful_c)::value != 0;
+            fetch_page(it.t0);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i)
+            for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-        m = -INFINITY;
-        l = 0.0f;
-        att_each<ST>([&](auto u_c) PTA_INLINE {
-            constexpr int u = decltype(u_c)::value;
-            if constexpr (RUN) {
-                const int at = run_at(it.t0 + u, hole[u], kinfo[u]);
-                run_keys(at, kreg[u], scl[u]);
-                run_values(at, vreg[u]);
-            } else {
-                load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
-            }
-            fetch_page(it.t0 + u + 1);
-        });
-        for (int tt = it.t0; tt < it.t1; tt += ST)
+                for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+            m = -INFINITY;
+            l = 0.0f;
             att_each<ST>([&](auto u_c) PTA_INLINE {
                 constexpr int u = decltype(u_c)::value;
-                const int     t = tt + u;
-                if (u > 0 && t >= it.t1) return;
-                if (a.D != DP || hole[u] != 0) {
+                if constexpr (RUN) {
+                    const int at = run_at(it.t0 + u, hole[u], kinfo[u]);
+                    run_keys(at, kreg[u], scl[u]);
+                    run_values(at, vreg[u]);
+                } else {
+                    load(it.t0 + u, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+                }
+                fetch_page(it.t0 + u + 1);
+            });
+            for (int tt = it.t0; tt < it.t1; tt += ST)
+                att_each<ST>([&](auto u_c) PTA_INLINE {
+                    constexpr int u = decltype(u_c)::value;
+                    const int     t = tt + u;
+                    if (u > 0 && t >= it.t1) return;
+                    if (a.D != DP || hole[u] != 0) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const bool no = RUN ? hole[u] != 0 : __shfl(krow[u], k * 16 + c) < 0;
+                        for (int k = 0; k < 2; ++k) {
+                            const bool no = RUN ? hole[u] != 0 : __shfl(krow[u], k * 16 + c) < 0;
 #pragma unroll
-                        for (int i = 0; i < KP; ++i)
-                            if (no || loaded_at(i) >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
+                            for (int i = 0; i < KP; ++i)
+                                if (no || loaded_at(i) >= a.D) kreg[u][k][i] = make_uint4(0, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < VP; ++i) {
+                            const int p = i * 64 + lane;
+                            if ((RUN ? hole[u] != 0 : __shfl(krow[u], p / CPR) < 0) || (p % CPR) * EC >= a.D) vreg[u][i] = make_uint4(0, 0, 0, 0);
+                        }
+                        if (RUN ? hole[u] != 0 : krow[u] < 0) {
+                            scl[u][0] = 0.0f;
+                            scl[u][1] = 1.0f;
+                        }
                     }
+                    bool special = careful;
+                    if (!TILE && mixed) {
+#pragma unroll
+                        for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[u][i]);
+                        special = __any(special);
+                    }
+                    // this tile's values to LDS, its keys as operands; then the loads of the tile after next
 #pragma unroll
                     for (int i = 0; i < VP; ++i) {
-                        const int p = i * 64 + lane;
-                        if ((RUN ? hole[u] != 0 : __shfl(krow[u], p / CPR) < 0) || (p % CPR) * EC >= a.D) vreg[u][i] = make_uint4(0, 0, 0, 0);
-                    }
-                    if (RUN ? hole[u] != 0 : krow[u] < 0) {
-                        scl[u][0] = 0.0f;
-                        scl[u][1] = 1.0f;
-                    }
-                }
-                bool special = careful;
-                if (!TILE && mixed) {
-#pragma unroll
-                    for (int i = 0; i < VP; ++i) special |= att_has_special<QT, KIND>(vreg[u][i]);
-                    special = __any(special);
-                }
-                // this tile's values to LDS, its keys as operands; then the loads of the tile after next
-#pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    const int p = i * 64 + lane, ky = p / CPR, e = (p % CPR) * EC;
-                    if constexpr (FP8) {
-                        *reinterpret_cast<uint4 *>(V + ky * VS + e)     = att_cvt8<QT, KIND>(vreg[u][i].x, vreg[u][i].y);
-                        *reinterpret_cast<uint4 *>(V + ky * VS + e + 8) = att_cvt8<QT, KIND>(vreg[u][i].z, vreg[u][i].w);
-                    } else {
-                        *reinterpret_cast<uint4 *>(V + ky * VS + e) = vreg[u][i];
-                    }
-                }
-                if constexpr (FP8) {
-                    if (lane < WK) {
-                        ssc[wave][0][lane] = scl[u][0] * a.scale_log2;
-                        ssc[wave][1][lane] = att_log2_scale(scl[u][1]);
-                        ssc[wave][2][lane] = 1.0f / att_clamp_scale(scl[u][1]);
-                    }
-                }
-                auto key_of = [&](int k, int i) PTA_INLINE { // operand of k-step i
-                    if constexpr (FP8) {
-                        const uint4 w = kreg[u][k][i / 2];
-                        return i % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
-                    } else {
-                        return kreg[u][k][i];
-                    }
-                };
-                // the last of the run's keys that the lane's row sees
-                const int upto = RUN && rin && (kinfo[TILE ? u : 0].y >> rtok & 1) ? pos - kinfo[TILE ? u : 0].x : -1;
-                att_f4    s[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[k][j] = 0.0f;
-                if constexpr (RUN) {
-                    // the keys as they are until the products take them: fewer registers, another workgroup
-                    const int at = run_at(t + ST, hole[u], kinfo[u]);
-                    run_values(at, vreg[u]);
-                    if constexpr (QUAD) run_turn(kreg[u]);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) s[k] = AttT<QT>::mfma16(key_of(k, i), qf[i], s[k]);
-                    run_keys(at, kreg[u], scl[u]);
-                } else {
-                    uint4 kf[2][DP / 32];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < DP / 32; ++i) kf[k][i] = key_of(k, i);
-                    if constexpr (TILE) {
-                        if (lane < WK) {
-                            lds.skey[wave][0][lane] = kinfo[u].x;
-                            lds.skey[wave][1][lane] = kinfo[u].y;
+                        const int p = i * 64 + lane, ky = p / CPR, e = (p % CPR) * EC;
+                        if constexpr (FP8) {
+                            *reinterpret_cast<uint4 *>(V + ky * VS + e)     = att_cvt8<QT, KIND>(vreg[u][i].x, vreg[u][i].y);
+                            *reinterpret_cast<uint4 *>(V + ky * VS + e + 8) = att_cvt8<QT, KIND>(vreg[u][i].z, vreg[u][i].w);
+                        } else {
+                            *reinterpret_cast<uint4 *>(V + ky * VS + e) = vreg[u][i];
                         }
                     }
-                    load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+                    if constexpr (FP8) {
+                        if (lane < WK) {
+                            ssc[wave][0][lane] = scl[u][0] * a.scale_log2;
+                            ssc[wave][1][lane] = att_log2_scale(scl[u][1]);
+                            ssc[wave][2][lane] = 1.0f / att_clamp_scale(scl[u][1]);
+                        }
+                    }
+                    auto key_of = [&](int k, int i) PTA_INLINE { // operand of k-step i
+                        if constexpr (FP8) {
+                            const uint4 w = kreg[u][k][i / 2];
+                            return i % 2 == 0 ? att_cvt8<QT, KIND>(w.x, w.y) : att_cvt8<QT, KIND>(w.z, w.w);
+                        } else {
+                            return kreg[u][k][i];
+                        }
+                    };
+                    // the last of the run's keys that the lane's row sees
+                    const int upto = RUN && rin && (kinfo[TILE ? u : 0].y >> rtok & 1) ? pos - kinfo[TILE ? u : 0].x : -1;
+                    att_f4    s[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int i = 0; i < DP / 32; ++i) s[k] = AttT<QT>::mfma16(kf[k][i], qf[i], s[k]);
-                }
-                fetch_page(t + ST + 1);
-                // the wave's own LDS writes are seen by its later reads once they are done
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-                // values as operands: element block i of the wave's keys
-                const int kr = 4 * qd + c / 4, dc = 4 * (c & 3);
-                auto      value_of = [&](int i) PTA_INLINE {
-                    const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
-                    return make_uint4(v0.x, v0.y, v1.x, v1.y);
-                };
-                // RUN: half of them are read before the exponentials and half behind, all before the products
-                uint4 vf[DP / 16];
-                if constexpr (RUN && !careful) {
+                        for (int j = 0; j < 4; ++j) s[k][j] = 0.0f;
+                    if constexpr (RUN) {
+                        // the keys as they are until the products take them: fewer registers, another workgroup
+                        const int at = run_at(t + ST, hole[u], kinfo[u]);
+                        run_values(at, vreg[u]);
+                        if constexpr (QUAD) run_turn(kreg[u]);
 #pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) vf[i] = value_of(i);
-                }
-                const int key0 = attn_key0(it, t, KT) + wave * WK;
-                float     mx = m, iv[2][4];
+                        for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int kk = k * 16 + 4 * qd;
-                    if constexpr (FP8) {
-                        float4       x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
-                        float4       y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
-                        const float4 z = *reinterpret_cast<const float4 *>(&ssc[wave][2][kk]);
-                        // opaque: else they are read behind a branch, where a key is seen
-                        if constexpr (TILE) asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w), "+v"(y.x), "+v"(y.y), "+v"(y.z), "+v"(y.w));
-                        s[k][0] = fmaf(s[k][0], x.x, y.x); s[k][1] = fmaf(s[k][1], x.y, y.y);
-                        s[k][2] = fmaf(s[k][2], x.z, y.z); s[k][3] = fmaf(s[k][3], x.w, y.w);
-                        iv[k][0] = z.x; iv[k][1] = z.y; iv[k][2] = z.z; iv[k][3] = z.w;
+                            for (int k = 0; k < 2; ++k) s[k] = AttT<QT>::mfma16(key_of(k, i), qf[i], s[k]);
+                        run_keys(at, kreg[u], scl[u]);
                     } else {
+                        uint4 kf[2][DP / 32];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[k][j] *= a.scale_log2;
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int i = 0; i < DP / 32; ++i) kf[k][i] = key_of(k, i);
+                        if constexpr (TILE) {
+                            if (lane < WK) {
+                                lds.skey[wave][0][lane] = kinfo[u].x;
+                                lds.skey[wave][1][lane] = kinfo[u].y;
+                            }
+                        }
+                        load(t + ST, kreg[u], vreg[u], scl[u], krow[u], hole[u], kinfo[TILE ? u : 0]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int i = 0; i < DP / 32; ++i) s[k] = AttT<QT>::mfma16(kf[k][i], qf[i], s[k]);
                     }
-                    int4 kp, km;
-                    if constexpr (TILE && !RUN) {
-                        kp = *reinterpret_cast<const int4 *>(&lds.skey[wave][0][kk]);
-                        km = *reinterpret_cast<const int4 *>(&lds.skey[wave][1][kk]);
+                    fetch_page(t + ST + 1);
+                    // the wave's own LDS writes are seen by its later reads once they are done
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                    // values as operands: element block i of the wave's keys
+                    const int kr = 4 * qd + c / 4, dc = 4 * (c & 3);
+                    auto      value_of = [&](int i) PTA_INLINE {
+                        const uint2 v0 = att_tr16(V + kr * VS + i * 16 + dc), v1 = att_tr16(V + (kr + 16) * VS + i * 16 + dc);
+                        return make_uint4(v0.x, v0.y, v1.x, v1.y);
+                    };
+                    // RUN: half of them are read before the exponentials and half behind, all before the products
+                    uint4 vf[DP / 16];
+                    if constexpr (RUN && !careful) {
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) vf[i] = value_of(i);
                     }
-                    const int kpos[4] = {kp.x, kp.y, kp.z, kp.w}, kmask[4] = {km.x, km.y, km.z, km.w};
+                    const int key0 = attn_key0(it, t, KT) + wave * WK;
+                    float     mx = m, iv[2][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int  ky  = key0 + kk + j;
-                        const bool see = RUN    ? kk + j <= upto
-                                         : TILE ? (kpos[j] <= pos) & ((kmask[j] >> rtok & 1) != 0)
-                                                : (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
-                        s[k][j]        = see ? s[k][j] : -INFINITY;
-                        mx             = fmaxf(mx, s[k][j]);
-                    }
-                }
-                mx = max_xor32(max_xor16(mx));
-                // TILE: the sums stay as they are while no row's maximum has grown by more than 8 (P to 2^8)
-                float alpha = 1.0f;
-                if (!TILE || __any(mx > m + 8.0f)) {
-                    alpha = att_exp2(m - (mx == -INFINITY ? 0.0f : mx));
-                    m     = mx;
-                    l *= alpha;
-                    if constexpr (TILE)
+                    for (int k = 0; k < 2; ++k) {
+                        const int kk = k * 16 + 4 * qd;
+                        if constexpr (FP8) {
+                            float4       x = *reinterpret_cast<const float4 *>(&ssc[wave][0][kk]);
+                            float4       y = *reinterpret_cast<const float4 *>(&ssc[wave][1][kk]);
+                            const float4 z = *reinterpret_cast<const float4 *>(&ssc[wave][2][kk]);
+                            // opaque: else they are read behind a branch, where a key is seen
+                            if constexpr (TILE) asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w), "+v"(y.x), "+v"(y.y), "+v"(y.z), "+v"(y.w));
+                            s[k][0] = fmaf(s[k][0], x.x, y.x); s[k][1] = fmaf(s[k][1], x.y, y.y);
+                            s[k][2] = fmaf(s[k][2], x.z, y.z); s[k][3] = fmaf(s[k][3], x.w, y.w);
+                            iv[k][0] = z.x; iv[k][1] = z.y; iv[k][2] = z.z; iv[k][3] = z.w;
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
-                }
-                const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[k][j] = att_exp2(s[k][j] - base);
-                        if constexpr (FP8) l = fmaf(s[k][j], iv[k][j], l);
-                        else l += s[k][j];
-                    }
-                const uint4 pf = make_uint4(AttT<QT>::pack(s[0][0], s[0][1]), AttT<QT>::pack(s[0][2], s[0][3]),
-                                            AttT<QT>::pack(s[1][0], s[1][1]), AttT<QT>::pack(s[1][2], s[1][3]));
-                if constexpr (RUN && !careful) {
-#pragma unroll
-                    for (int i = DP / 32; i < DP / 16; ++i) vf[i] = value_of(i);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    if constexpr (!TILE)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
-                    if constexpr (!RUN || careful) vf[i] = value_of(i);
-                    if (!special) {
-                        o[i] = AttT<QT>::mfma16(vf[i], pf, o[i]);
-                    } else {
-                        // infinities and NaN that only some rows see: 0 * inf must not reach the
-                        // others.  Finite values go as ever; then a count of the special ones that
-                        // a row sees decides.
-                        uint4  fin, plus, minus;
-                        att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
-                        att_split_special<QT>(vf[i], fin, plus, minus);
-                        const uint4 seen = att_nonzero<QT>(pf);
-                        o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
-                        np   = AttT<QT>::mfma16(plus, seen, np);
-                        nm   = AttT<QT>::mfma16(minus, seen, nm);
+                            for (int j = 0; j < 4; ++j) s[k][j] *= a.scale_log2;
+                        }
+                        int4 kp, km;
+                        if constexpr (TILE && !RUN) {
+                            kp = *reinterpret_cast<const int4 *>(&lds.skey[wave][0][kk]);
+                            km = *reinterpret_cast<const int4 *>(&lds.skey[wave][1][kk]);
+                        }
+                        const int kpos[4] = {kp.x, kp.y, kp.z, kp.w}, kmask[4] = {km.x, km.y, km.z, km.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            if (np[j] > 0.0f) o[i][j] += INFINITY;
-                            if (nm[j] > 0.0f) o[i][j] -= INFINITY;
+                            const int  ky  = key0 + kk + j;
+                            const bool see = RUN    ? kk + j <= upto
+                                             : TILE ? (kpos[j] <= pos) & ((kmask[j] >> rtok & 1) != 0)
+                                                    : (ky <= pos) & ((ky >= wlo) | (ky < a.sinks));
+                            s[k][j]        = see ? s[k][j] : -INFINITY;
+                            mx             = fmaxf(mx, s[k][j]);
                         }
                     }
-                }
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            });
+                    mx = max_xor32(max_xor16(mx));
+                    // TILE: the sums stay as they are while no row's maximum has grown by more than 8, P by
+                    // 2^8, as in the wide kernel: 126 us, with every growth 133 (the error against 64 bits
+                    // 0.0023 and 0.0020: the largest P is no longer 1, which its 16 bits hold exactly)
+                    float alpha = 1.0f;
+                    if (!TILE || __any(mx > m + 8.0f)) {
+                        alpha = att_exp2(m - (mx == -INFINITY ? 0.0f : mx));
+                        m     = mx;
+                        l *= alpha;
+                        if constexpr (TILE)
+#pragma unroll
+                            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            s[k][j] = att_exp2(s[k][j] - base);
+                            if constexpr (FP8) l = fmaf(s[k][j], iv[k][j], l);
+                            else l += s[k][j];
+                        }
+                    const uint4 pf = make_uint4(AttT<QT>::pack(s[0][0], s[0][1]), AttT<QT>::pack(s[0][2], s[0][3]),
+                                                AttT<QT>::pack(s[1][0], s[1][1]), AttT<QT>::pack(s[1][2], s[1][3]));
+                    if constexpr (RUN && !careful) {
+#pragma unroll
+                        for (int i = DP / 32; i < DP / 16; ++i) vf[i] = value_of(i);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        if constexpr (!TILE)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) o[i][j] *= alpha;
+                        if constexpr (!RUN || careful) vf[i] = value_of(i);
+                        if (!special) {
+                            o[i] = AttT<QT>::mfma16(vf[i], pf, o[i]);
+                        } else {
+                            // infinities and NaN that only some rows see: 0 * inf must not reach the
+                            // others.  Finite values go as ever; then a count of the special ones that
+                            // a row sees decides.
+                            uint4  fin, plus, minus;
+                            att_f4 np = {0.f, 0.f, 0.f, 0.f}, nm = {0.f, 0.f, 0.f, 0.f};
+                            att_split_special<QT>(vf[i], fin, plus, minus);
+                            const uint4 seen = att_nonzero<QT>(pf);
+                            o[i] = AttT<QT>::mfma16(fin, pf, o[i]);
+                            np   = AttT<QT>::mfma16(plus, seen, np);
+                            nm   = AttT<QT>::mfma16(minus, seen, nm);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (np[j] > 0.0f) o[i][j] += INFINITY;
+                                if (nm[j] > 0.0f) o[i][j] -= INFINITY;
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                });
         };
         keys(std::integral_constant<int, 0>{});
         if constexpr (TILE) {
@@ -1550,11 +1552,14 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
     if (block < work) attn_narrow<QT, KIND, DP, false, false>(a, block, lds);
     else attn_pad(a, block - work, pads);
 }
-// Bound by the vector instructions of a tile of 32 keys a wave, 380, and their waits: the keys
-// come from the L2 (97% of the reads hit).  Three workgroups a CU with one tile in flight, at the
-// price of 11 spilled registers: 1024 tokens, 37 pages of 64 in a tile's list, 32 / 8 heads of
-// 128, e4m3, 173 us; two with two in flight 206, two with one 204.  The 16-bit cache at 128
-// elements would spill 56: two.
+// The keys come from the L2 (97% of the reads hit, after 100 cycles).  RUN: bound by the vector
+// instructions of a tile of 32 keys a wave, 285 beside 16 matrix instructions, 55% of the time of
+// the units.  1024 tokens, 37 pages of 64 in a tile's list, 32 / 8 heads of 128, e4m3: 128 us, with
+// three workgroups a CU as with four (of fewer registers).  Its steps: a wave's addresses, masks and
+// positions once for its keys 150 (else 169), special values and rescaling out of the way 133, values'
+// operands read ahead 130, keys by quads 128.
+// Else one tile in flight, not two, for a third workgroup, at the price of spilled registers; the
+// 16-bit cache at 128 elements would spill 56: two.
 template <int QT, int KIND, int DP, bool RUN>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 && KIND == PTA_CACHE_16BIT ? 2 : 3) void attn_tile_kernel(AttnArgs a) {
     __shared__ AttnTileLds<DP> lds;
