@@ -6,7 +6,7 @@
 namespace pta {
 
 // Tiles of tokens: the pages that any token of a tile takes, as one list for each cache head
-constexpr int64_t PS_TILE_PAGES = 1024; // of a sequence at most
+constexpr int64_t PS_TILE_PAGES = 2048; // of a sequence at most
 struct PSTiles {
     int       tokens; // of a tile, 16 at most
     int       cap;    // pages of a list at most

@@ -767,7 +767,8 @@ static int ps_launch(PSArgs a, int q_dtype, void *workspace, hipStream_t st) {
         if (tile > 0) {
             if (a.M <= 256) ps_choose_tile_kernel<4><<<grid, threads, 0, st>>>(a);
             else if (a.M <= 512) ps_choose_tile_kernel<8><<<grid, threads, 0, st>>>(a);
-            else ps_choose_tile_kernel<16><<<grid, threads, 0, st>>>(a);
+            else if (a.M <= 1024) ps_choose_tile_kernel<16><<<grid, threads, 0, st>>>(a);
+            else ps_choose_tile_kernel<32><<<grid, threads, 0, st>>>(a);
         } else if (a.M <= 256) ps_choose_kernel<4><<<grid, 64, 0, st>>>(a);
         else if (a.M <= 512) ps_choose_kernel<8><<<grid, 64, 0, st>>>(a);
         else if (a.M <= 2048) ps_choose_many_kernel<8, 4><<<grid, 512, 0, st>>>(a);

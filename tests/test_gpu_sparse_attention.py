@@ -138,6 +138,8 @@ def test_long_contexts(L):
     (3, 3, 80, 16, 5, [33], [16 * 40 + 7]),                   # a head of its own for each query, sixteen tokens
     (6, 2, 128, 33, 6, [3, 3, 3, 3, 11], [700, 5, 33 * 12, 34, 400]),  # several sequences in a tile, three query heads: a row too few
     (8, 1, 256, 8, 12, [9, 2], [8 * 60, 8 * 70 + 3]),         # two tokens
+    (2, 1, 64, 1, 50, [3, 17], [1999, 2048]),                 # more pages than a lane has sixteen scores for
+    (1, 1, 16, 1, 9, [18], [2048]), (2, 2, 16, 1, 9, [18], [2049]),  # the most pages of a tile, and one more
     (16, 2, 64, 1, 3, [5, 40], [5, 64])])
 def test_chunks(Hq, Hkv, D, page, take, new, lens):
     """Tokens that share their pages' reads, each with its own pages and position."""
