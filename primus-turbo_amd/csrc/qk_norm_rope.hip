@@ -155,8 +155,8 @@ template <int LPR> __device__ __forceinline__ float qr_max(float v) {
 // two neighbouring runs (pairs (2 i, 2 i + 1)); beyond the rotated elements any two.
 template <int V, int P> struct QRLane {
     int   at[P][2];
-    bool  in[P];
-    float c[P][V], s[P][V]; // of pair j; (1, 0) beyond the rotated elements
+    bool  in[P], turned[P];
+    float c[P][V], s[P][V]; // of pair j; (1, 0) where the token has no angles
 };
 
 template <int V, int LPR> constexpr int qr_pieces() { return V == 8 ? 1 : 128 / (V * LPR); }
@@ -169,6 +169,7 @@ __device__ __forceinline__ QRLane<V, qr_pieces<V, LPR>()> qr_lane(const QRArgs &
     for (int p = 0; p < P; ++p) {
         const int e = (p * LPR + l) * V; // number of its first pair
         k.in[p]     = 2 * e < a.D;
+        k.turned[p] = e < a.half; // all of the piece's pairs or none
         if constexpr (NB) {
             k.at[p][0] = 2 * e;
             k.at[p][1] = 2 * e + V;
@@ -224,9 +225,12 @@ template <int V, int LPR, int P> __device__ __forceinline__ bool qr_angles(const
 
 // Turns the lane's pairs by the angles, BACK: by their negatives.  The products are fused
 // here and not left to the compiler, so that every form of the kernels gives the same bits.
+// Beyond the rotated elements two that are not a pair would meet here: they are left alone,
+// since an angle of 0 would make a NaN of one beside an infinity.
 template <bool NB, bool BACK, int V, int P> __device__ __forceinline__ void qr_turn(const QRLane<V, P> &k, float (&v)[P][2][V]) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
+        if (!k.turned[p]) continue;
         if constexpr (V > 1 && NB) {
             // the 2 V elements are V pairs of neighbours
 #pragma unroll

@@ -208,6 +208,91 @@ def test_infinities_and_nan_stay_in_their_rows():
     assert not bool(ops.qk_norm_rope(zero, k, cos, sin, pos, wq, wk)[0].any())
 
 
+def _bits(x):
+    return x.contiguous().view(torch.int32 if x.element_size() == 4 else torch.int16)
+
+
+# runs of 8, 4, 2 and 1 elements
+PARTLY = [(128, 64), (256, 128), (80, 24), (64, 4), (10, 6)]
+
+
+def _partner(j, rot, interleaved):
+    """The element that is turned with element j; j itself beyond the turned ones."""
+    if j >= rot:
+        return j
+    return j ^ 1 if interleaved else (j + rot // 2) % rot
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FH, FF])
+@pytest.mark.parametrize("D,rot", PARTLY)
+def test_special_values_reach_their_pair_alone(D, rot, dtype, interleaved):
+    """Without a norm an element depends on its pair, and beyond the turned ones on nothing else:
+    outputs, gradients, and keys in a cache."""
+    ops = _ops()
+    q, k, v, _, _, cos, sin, pos = _inputs(6, 3, 2, D, rot, dtype, norm=False)
+    gs = [torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(dtype).cuda() for x in (q, k)]
+    cached = dtype != FF and D % 16 == 0
+    slots = torch.arange(6, device="cuda")
+
+    def run(k, gk):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k)]
+        out = ops.qk_norm_rope(leaves[0], leaves[1], cos, sin, pos, interleaved=interleaved)
+        res = [out[1].detach(), torch.autograd.grad(out, leaves, (gs[0], gk))[1]]
+        if cached:
+            kc, vc, _, _ = _cache(2, 2, 4, D, dtype)
+            ops.qk_norm_rope_cache_write(q, k, v, cos, sin, pos, kc, vc, slots, interleaved=interleaved)
+            res.append(_rows(kc, slots, 4))
+        return res
+
+    want = run(k, gs[1])
+    for j in sorted({0, rot - 1, rot, (rot + D) // 2, D - 1}):
+        p = _partner(j, rot, interleaved)
+        other = [d for d in range(D) if d not in (j, p)]
+        for bad in (float("inf"), -float("inf"), float("nan")):
+            k2, g2 = k.clone(), gs[1].clone()
+            k2[2, 1, j] = g2[2, 1, j] = bad
+            for got, ref in zip(run(k2, g2), want):
+                rows = torch.ones(6, 2, dtype=torch.bool, device="cuda")
+                rows[2, 1] = False
+                assert torch.equal(_bits(got[rows]), _bits(ref[rows]))
+                assert torch.equal(_bits(got[2, 1, other]), _bits(ref[2, 1, other])), f"element {j} is {bad}"
+                if j >= rot:
+                    assert bool(got[2, 1, j].isnan()) if bad != bad else got[2, 1, j].item() == bad
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FH, FF])
+@pytest.mark.parametrize("D,rot", PARTLY)
+def test_special_values_of_normed_rows(D, rot, dtype, interleaved):
+    """A norm joins a row's elements: an infinity makes zeros of the others, as the formula does.
+    One of a gradient's reaches its own channel of the weight's gradient, and no unrelated one."""
+    ops = _ops()
+    q, k, _, wq, wk, cos, sin, pos = _inputs(6, 3, 2, D, rot, dtype)
+    gs = [torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(dtype).cuda() for x in (q, k)]
+
+    def run(k, gk):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
+        out = ops.qk_norm_rope(leaves[0], leaves[1], cos, sin, pos, leaves[2], leaves[3], eps=EPS, interleaved=interleaved)
+        return [out[1].detach(), *torch.autograd.grad(out, leaves, (gs[0], gk))]
+
+    want = run(k, gs[1])
+    for j in sorted({rot, (rot + D) // 2, D - 1}):
+        other = [d for d in range(D) if d != j]
+        for bad in (float("inf"), -float("inf")):
+            k2 = k.clone()
+            k2[2, 1, j] = bad
+            y = run(k2, gs[1])[0]
+            assert bool(y[2, 1, j].isnan()) and not bool(y[2, 1, other].any()), f"element {j} is {bad}"
+            g2 = gs[1].clone()
+            g2[2, 1, j] = bad
+            _, _, dk, _, dw = run(k, g2)
+            assert torch.equal(_bits(dw[other]), _bits(want[4][other])) and not bool(dw[j].isfinite()), f"gradient {j} is {bad}"
+            ref = norm_rope_grads(k, wk, cos, sin, pos, EPS, interleaved, g2)[0][0]
+            assert torch.equal(dk.isnan(), ref.isnan())
+            assert torch.equal(dk.isinf(), ref.isinf()) and bool((dk.sign() == ref.sign())[ref.isinf()].all())
+
+
 def test_offsets_past_32_bits():
     """More than 2^32 bytes of queries, forward and backward: the last tokens' rows are where they belong."""
     ops = _ops()
@@ -349,6 +434,20 @@ def test_cache_write_without_norm_or_angle_is_kv_cache_write(cache):
     out = ops.qk_norm_rope_cache_write(q, k, v, cos, sin, pos.to(torch.int32), a[0], a[1], slots, a[2], a[3])
     ops.kv_cache_write(k, v, b[0], b[1], slots, b[2], b[3])
     assert torch.equal(out, q) and all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("cache", [E4, E5])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_cache_write_of_special_values_that_are_not_turned(cache, interleaved):
+    ops = _ops()
+    q, k, v, _, _, cos, sin, pos = _inputs(6, 4, 2, 128, 64, BF, norm=False)
+    k = k.clone()
+    k[0, 0, 64], k[1, 1, 127], k[2, 0, 100], k[3, 1, 96] = float("inf"), -float("inf"), float("nan"), float("inf")
+    cos, sin, slots = torch.ones_like(cos), torch.zeros_like(sin), torch.arange(6, device="cuda")
+    a, b = _cache(1, 2, 16, 128, cache), _cache(1, 2, 16, 128, cache)
+    ops.qk_norm_rope_cache_write(q, k, v, cos, sin, pos, a[0], a[1], slots, a[2], a[3], interleaved=interleaved)
+    ops.kv_cache_write(k, v, b[0], b[1], slots, b[2], b[3])
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
 
 
 def test_cache_write_offsets_past_32_bits_and_no_pages():
