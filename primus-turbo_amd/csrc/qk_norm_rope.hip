@@ -393,8 +393,8 @@ template <int KIND, int DT, bool NB, int V, int LPR> __global__ __launch_bounds_
             for (int i = 0; i < 2; ++i) raw[p][i] = {};
     }
     qr_row<DT, V, P>(raw, v);
-    if (qr_of(a.w, which) != nullptr) {
-        const float r = in ? qr_rsqrt<LPR, V, P>(a, k, v) : 0.0f; // eps may be 0
+    if (qr_of(a.w, which) != nullptr && in) { // zeros stay zeros, whatever eps and the weights are
+        const float r = qr_rsqrt<LPR, V, P>(a, k, v);
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -446,15 +446,15 @@ template <int DT, bool NB, int V, int LPR> __global__ __launch_bounds__(QR_NT) v
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) rg[p][i] = rx[p][i] = {};
+                for (int i = 0; i < 2; ++i) rg[p][i] = {};
         }
         float g[P][2][V];
         qr_row<DT, V, P>(rg, g);
         qr_turn<NB, true, V, P>(k, g);
-        if (norm) {
+        if (norm && in) {
             float v[P][2][V], dot = 0.0f;
             qr_row<DT, V, P>(rx, v);
-            const float r = in ? qr_rsqrt<LPR, V, P>(a, k, v) : 0.0f;
+            const float r = qr_rsqrt<LPR, V, P>(a, k, v);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 float x = 0.0f;

@@ -130,6 +130,38 @@ def test_positions_outside_the_tables():
     assert torch.equal(g2[0], grads[0][keep])
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("D,rot,dtype", [(128, 128, BF), (80, 32, FH), (10, 6, FF)])
+def test_positions_outside_the_tables_beside_weights_that_are_not_finite(D, rot, dtype, bad):
+    """Zeros and no gradient are what padding gets, whatever the weights hold."""
+    ops = _ops()
+    q, k, v, wq, wk, cos, sin, pos = _inputs(9, 4, 2, D, rot, dtype)
+    pos[1], pos[4], pos[8] = -1, 97, -7
+    pad = torch.tensor([1, 4, 8], device="cuda")
+    gs = [torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(dtype).cuda() for x in (q, k)]
+
+    def run(wq, wk):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
+        out = ops.qk_norm_rope(leaves[0], leaves[1], cos, sin, pos, leaves[2], leaves[3])
+        return [o.detach() for o in out] + list(torch.autograd.grad(out, leaves, gs))
+
+    w2 = [w.clone() for w in (wq, wk)]
+    w2[0][0] = w2[1][D - 1] = bad
+    want, got = run(wq, wk), run(*w2)
+    for t in got[:4]:
+        assert not bool(t[pad].any()) and bool(t[0].isnan().any() or t[0].isinf().any())
+    for a, b in zip(got[4:], want[4:]):  # the weights' gradients do not depend on the weights
+        assert torch.equal(a, b)
+    if D % 16 or dtype == FF:
+        return
+    slots = torch.arange(9, device="cuda")
+    for kind in (E4, dtype):
+        kc, vc, ks, vs = _cache(1, 2, 16, D, kind)
+        o = ops.qk_norm_rope_cache_write(q, k, v, cos, sin, pos, kc, vc, slots, ks, vs, q_weight=w2[0], k_weight=w2[1])
+        assert not bool(o[pad].any()) and not bool(_rows(kc, pad, 16).any())
+        assert ks is None or bool(ks.isfinite().all(0).all(0)[pad].all())
+
+
 def test_gradient_against_differences():
     ops = _ops()
     q, k, _, wq, wk, cos, sin, pos = _inputs(6, 3, 2, 32, 16, FF)
