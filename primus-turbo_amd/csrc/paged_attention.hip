@@ -264,7 +264,8 @@ SparsePlan sparse_plan(int64_t T, int64_t num_seqs, int64_t Hq, int64_t Hkv, int
         ATT_NARROW_ROWS * p.K <= (INT_MAX - 1024) / page) { // a list's keys are counted in 32 bits
         p.tile   = ATT_NARROW_ROWS / G;
         p.tiles  = cdiv(T, p.tile);
-        p.cap    = p.tile * p.K;
+        // a tile's sequences are at most one run of its tokens each, and a run has a page of its row once
+        p.cap    = std::min(p.tile * p.K, std::min(p.tile, num_seqs) * max_pages);
         p.sel    = round256(p.tiles * Hkv * p.cap * 8);
         p.masks  = round256(p.tiles * Hkv * p.cap * 2);
         p.counts = round256(p.tiles * Hkv * 4);

@@ -147,6 +147,13 @@ def test_chunks(Hq, Hkv, D, page, take, new, lens):
         _check(_batch(new, lens, Hq, Hkv, D, page, dtype, cache, seed=3), take, 1, 2)
 
 
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("Hq,Hkv,new,pages", [(2, 2, [40], [30]), (4, 2, [3, 2, 35], [30, 30, 30]), (3, 3, [7, 20, 9], [30, 29, 30])])
+def test_chunks_whose_lists_are_full(Hq, Hkv, new, pages, page):
+    """Every token takes all of its sequence's pages: lists as long as their sequences' rows of the table."""
+    _check(_batch(new, [page * n for n in pages], Hq, Hkv, 64, page, BF, E4, seed=6), 30, 1, 2)
+
+
 def test_chunk_with_special_values():
     """Infinities and NaN of keys that only some of a tile's tokens take or see."""
     ops = _ops()

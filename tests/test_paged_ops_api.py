@@ -373,6 +373,20 @@ def test_workspaces_stay_small():
     assert _C.query("pta_qk_norm_rope_backward_workspace_size", 0, 32, 8, 128) == 0
 
 
+def test_lists_of_tiles_hold_no_page_twice():
+    """A list of a tile's pages is no longer than its sequences' rows of the table: sixteen tokens of one
+    sequence that take all of its pages have them once (10 bytes each), not sixteen times."""
+    from primus_turbo.pytorch import _C
+
+    q = lambda *a: _C.query("pta_sparse_paged_attention_workspace_size", *a)  # noqa: E731
+    T, H, M = 8192, 8, 2048  # a query head to each cache head: sixteen tokens a tile
+    rest = (256 << 20) + 12 * T + 4 * (T // 16 * H) + 4096  # the scores, the tokens' lengths and positions, the lists' lengths
+    assert q(T, 1, H, H, 128, M, 16, M) <= T // 16 * H * M * 10 + rest
+    assert q(T, 3, H, H, 128, M, 16, M) <= T // 16 * H * 3 * M * 10 + rest
+    # many sequences, or few pages a token: as many as the tokens take
+    assert q(T, 4096, H, H, 128, M, 16, 16) <= T // 16 * H * 16 * 16 * 10 + rest
+
+
 def test_books_by_hand():
     """The oracle's own check: what the documentation says, on cases small enough to follow."""
     # two answers to one prompt of 6 tokens in pages of 4: the full page is shared, the second answer's last page is a copy
