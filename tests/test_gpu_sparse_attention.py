@@ -224,6 +224,27 @@ def test_chunk_over_special_values(cache, dtype, D, page):
                 assert bool(got[t, :, 7].isnan().all()) if math.isnan(bad) else bool((got[t, :, 7] == bad).all())
 
 
+def test_chunks_of_several_slices():
+    """More scores than are held at once: tiles of five tokens on both sides of where a slice ends,
+    against the same tokens by themselves."""
+    ops = _ops()
+    Hkv, M, take, n = 8, 2048, 12, 1100
+    q, kc, vc, ks, vs, table, cu, lens = _batch([n, n], [M, M], 3 * Hkv, Hkv, 16, 1, BF, E4, seed=9)
+    lo, hi = torch.sort(torch.randn(2, kc.shape[0], Hkv, 16, generator=torch.Generator().manual_seed(3)), dim=0)[0]
+    ranges = torch.stack((lo, hi), dim=2).to(BF).cuda()
+    step = (256 << 20) // (Hkv * M * 8) // 5 * 5
+    assert n < step < 2 * n
+    o, l = ops.sparse_paged_attention(q, kc, vc, ranges, table, cu, lens, ks, vs, num_selected=take, return_lse=True)
+    at = [0, n - 1, n, *range(step - 6, step + 6), 2 * n - 1]
+    rows = _i32([t // n for t in at]).long()
+    one = (q[at], kc, vc, ks, vs, ranges, table[rows], _i32(list(range(len(at) + 1))), _i32([M - n + t % n + 1 for t in at]), 0.25, take, 1, 2)
+    out, lse, b_out, b_lse, pages, _ = _attention(*one)
+    within(o[at], out, b_out, "out")
+    within(l[at], lse, b_lse, "lse")
+    sel, _ = ops.select_pages(q, ranges, table, cu, lens, 1, num_selected=take)
+    assert torch.equal(sel[at].cpu(), pages)
+
+
 def test_no_more_pages_than_selected_is_paged_attention():
     ops = _ops()
     q, kc, vc, ks, vs, table, cu, lens = _batch([1, 5, 1], [100, 90, 1], 8, 4, 128, 32, BF, E4)
