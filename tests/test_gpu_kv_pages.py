@@ -179,6 +179,23 @@ def test_fork(B, N, M, page, P, reserve, wild, compact):
 
 
 @pytest.mark.parametrize("compact", [False, True])
+@pytest.mark.parametrize("B,N,M,page,P,reserve", [(40, 60, 300, 2, 12 * 1024, 3), (40, 60, 300, 2, 12 * 1024 + 1, 3), (70, 70, 900, 1, 50021, 0),
+                                                  (300, 900, 160, 2, 9000, 5)])
+def test_fork_of_large_pools(B, N, M, page, P, reserve, compact):
+    """As many pages as one workgroup's LDS has owners for, and more; more entries than it goes through."""
+    r = random.Random(P + N)
+    table, lens, parents = _case(r, B, N, M, page, P, False)
+    rows, new_lens, pairs = fork_books(table, lens, parents, page, P, reserve, compact)
+    pools = _pools(0, P, 1, page, 16, E4, seed=P)
+    want = _moved(pools, pairs, 0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = _ops().kv_cache_fork(pools[0], pools[1], i32(table), i32(lens), i32(parents), pools[2], pools[3], reserve=reserve, compact=compact)
+    assert torch.equal(got[0].cpu(), torch.tensor(rows, dtype=torch.int32)) and got[1].tolist() == new_lens
+    # fresh pages hold whatever they held: all pages are compared, since copies alone write
+    assert _same(pools, want)
+
+
+@pytest.mark.parametrize("compact", [False, True])
 def test_fork_of_many(compact):
     """More sequences and pages than one workgroup has threads."""
     ops = _ops()

@@ -210,6 +210,29 @@ def test_only_what_is_asked_for():
     close(leaves[0].grad, *norm_rope_grads(q, wq, cos, sin, pos, 1e-6, False, ones(q))[0], "expanded")
 
 
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("wdtype", [BF, FF])
+def test_a_norm_of_one_side(which, wdtype):
+    """A weight for the queries or for the keys alone: the other side is only turned."""
+    ops = _ops()
+    q, k, v, wq, wk, cos, sin, pos = _inputs(21, 6, 2, 64, 32, BF, wdtype=wdtype)
+    w = [wq, None] if which == 0 else [None, wk]
+    leaves = [None if t is None else t.detach().clone().requires_grad_() for t in (q, k, *w)]
+    out = ops.qk_norm_rope(leaves[0], leaves[1], cos, sin, pos, leaves[2], leaves[3], eps=EPS)
+    gs = [torch.randn(o.shape, generator=torch.Generator().manual_seed(5)).to(BF).cuda() for o in out]
+    torch.autograd.backward(out, gs)
+    for n, x, y, g, lx, lw, wx in zip("qk", (q, k), out, gs, leaves[:2], leaves[2:], w):
+        close(y.detach(), *norm_rope(x, wx, cos, sin, pos, EPS, False), n)
+        dx, dw = norm_rope_grads(x, wx, cos, sin, pos, EPS, False, g)
+        close(lx.grad, *dx, "d" + n)
+        if wx is not None:
+            close(lw.grad, *dw, "dw")
+    kc, vc, _, _ = _cache(2, 2, 16, 64, BF)
+    slots = torch.arange(21, device="cuda")
+    o = ops.qk_norm_rope_cache_write(q, k, v, cos, sin, pos, kc, vc, slots, q_weight=w[0], k_weight=w[1], eps=EPS)
+    assert torch.equal(o, out[0]) and torch.equal(_rows(kc, slots, 16), out[1])
+
+
 def test_no_tokens_no_heads():
     ops = _ops()
     q, k, v, wq, wk, cos, sin, pos = _inputs(4, 2, 1, 32, 32, BF)
