@@ -5,7 +5,8 @@
 //
 // A page is up to five runs of bytes: keys, values, their scales and the keys'
 // ranges, in each of the layers.  Copies are bound by memory: a workgroup moves 16 KB
-// of one run, 4 x 16 bytes a thread in flight: 5.1 TB/s, what a large copy reaches.
+// of one run at a time, 4 x 16 bytes a thread in flight (4 KB where there is little to
+// copy): 5.1 TB/s, what a large copy reaches.
 #include <algorithm>
 #include <climits>
 
@@ -182,7 +183,9 @@ __device__ __forceinline__ KFSums kf_scan(KFSums v, int4 *tmp, KFSums &total) {
 
 // One workgroup: a thread has a run of pages, and of sequences.  Where LDS holds the pages'
 // owners and the table's entries are few, they are found here, else by the two kernels
-// above (64 sequences of 66 pages over 4300: 8.5 us, the three kernels 13).
+// above (64 sequences of 66 pages over 4300: 8.5 us, the three kernels 13).  Past that the runs
+// are strided reads of memory by one workgroup: calls of 64 sequences over 12289 pages 26 us (over
+// 12288 in LDS 19), over 65536 73, over 200000 225; compacting 35 (25), 128 and 364.
 constexpr int     KF_LDS_PAGES = 12 * 1024;
 constexpr int64_t KF_LDS_ENTRIES = 128 * KF_NT;
 

@@ -10,10 +10,11 @@
 //   score = sum_d hi_d P_d - lo_d N_d,   P_d = sum_i max(q_id, 0),  N_d = sum_i max(-q_id, 0)
 //
 // the largest that sum_i q_i . k can be for a key k within the ranges.  The heads'
-// sum turns G products of 2 D into one.  It is computed in 64 bits, where the order of
-// the sum does not show: the choice is the same whatever the launch's shape, and ties
-// are what the formula says they are.  A NaN counts as +inf: pages with NaN are
-// attended, and show.  The first `first` and the last `last` pages of those that a
+// sum turns G products of 2 D into one.  It is computed in 64 bits.  The forms below sum in
+// orders of their own, so that scores closer than a few roundings (2^-53 of the sum of the
+// terms' magnitudes each) may rank otherwise in another form; within a form a score depends
+// on its query and range alone, and equal ranges tie.  A NaN counts as +inf: pages with NaN
+// are attended, and show.  The first `first` and the last `last` pages of those that a
 // token sees are taken always, the rest by score, ties to the lower page.
 #include <algorithm>
 #include <climits>

@@ -1558,8 +1558,9 @@ template <int QT, int KIND, int DP> __global__ __launch_bounds__(256, DP <= 128 
 // three workgroups a CU as with four (of fewer registers).  Its steps: a wave's addresses, masks and
 // positions once for its keys 150 (else 169), special values and rescaling out of the way 133, values'
 // operands read ahead 130, keys by quads 128.
-// Else one tile in flight, not two, for a third workgroup, at the price of spilled registers; the
-// 16-bit cache at 128 elements would spill 56: two.
+// Else one tile in flight, not two, for a third workgroup.  No vector registers are spilled (scalar
+// ones go to lanes of them); three workgroups of the 16-bit cache at 128 elements would spill 28
+// (39 key by key): two.
 template <int QT, int KIND, int DP, bool RUN>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 && KIND == PTA_CACHE_16BIT ? 2 : 3) void attn_tile_kernel(AttnArgs a) {
     __shared__ AttnTileLds<DP> lds;

@@ -244,9 +244,9 @@ extern "C" int pta_paged_attention(const void *q, int q_dtype, int64_t num_token
 // Tokens go by tiles of 16 rows where a sequence has two or more of them on average: their
 // pages overlap, and a tile's page is read and converted once for all its rows (1024 tokens
 // over 16384, 32 / 8 heads of 128, 16 of 256 pages, of which four tokens take 37: attention
-// 128 us, token by token 320; 64 of 2048 pages, the call 786 us, token by token 1293).
-// Tables of more than PS_TILE_PAGES pages go token by token: a wave has its token's scores in
-// registers.
+// 128 us, token by token 320; 64 of 2048 pages, with the ranges 680 us, token by token 1217).
+// Tables of more than PS_TILE_PAGES pages go token by token: the choice that makes lists has a
+// token's scores in one wave's registers, and the one of several waves a token makes none.
 namespace {
 struct SparsePlan {
     int64_t  K, tile, tiles, cap; // tile: tokens of a tile, 0: none

@@ -34,8 +34,9 @@ template <int QT> void attn_launch(const AttnCall &c, int kind, hipStream_t st) 
     join<<<static_cast<unsigned>(n + w), 256, 0, st>>>(c.narrow, c.wide, n, c.narrow_join_parts);
 }
 
-// Pages of whole runs of 32 keys: calls of 1024 tokens over 16384, 16 of 256 pages of 64, 32 / 8 heads
-// of 64, 128 and 256, e4m3, take 116, 171 and 451 us, by a key at a time 158, 210 and 709.
+// Pages of whole runs of 32 keys: ranges and attention of 1024 tokens over 16384, 16 of 256 pages of 64,
+// 32 / 8 heads of 64, 128 and 256, e4m3, take 105, 157 and 453 us, by a key at a time 118, 179 and 574
+// (bf16 caches 111, 178 and 468; 155, 251 and 668).
 template <int QT, int KIND, int DP> void attn_launch_tiles_d(const AttnArgs &a, hipStream_t st) {
     const unsigned grid = static_cast<unsigned>(a.B) * a.split * a.Hkv;
     if (a.page % 32 == 0 && a.num_pages > 0) attn_tile_kernel<QT, KIND, DP, true><<<grid, 256, 0, st>>>(a);

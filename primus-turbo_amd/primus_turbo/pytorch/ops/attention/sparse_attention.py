@@ -11,11 +11,12 @@ head the score of a page is
 
   sum_d (sum_i max(q_id, 0)) hi_d + (sum_i min(q_id, 0)) lo_d
 
-the largest that sum_i q_i . k can be for a key k of the page.  A token attends through
-the first ``num_first`` and the last ``num_last`` of the pages that it sees, the last
-being its own, and the best of the others up to ``num_selected`` in all (ties to the
-earlier page; a NaN counts as the largest).  With no more pages than that the result is
-``paged_attention``'s.  Lengths and tables stay on the device; the calls may be captured.
+the largest that sum_i q_i . k can be for a key k of the page, in 64 bits.  A token
+attends through the first ``num_first`` and the last ``num_last`` of the pages that it
+sees, the last being its own, and the best of the others up to ``num_selected`` in all
+(ties to the earlier page; a NaN counts as the largest).  With no more pages than that
+the result is ``paged_attention``'s.  Lengths and tables stay on the device; the calls
+may be captured.
 """
 
 from __future__ import annotations
@@ -92,7 +93,8 @@ def sparse_paged_attention(
     """``paged_attention`` of every token over the pages selected for it (without a window).
 
     A token of a chunk has pages of its own, whose ranges have to be up to date for the
-    whole chunk.  ``softmax_scale`` is positive.  What a token that sees no key gets, what
+    whole chunk.  A chunk's tokens go over their pages together: where they take more than
+    about a quarter of the table, ``paged_attention`` of all of it is faster.  ``softmax_scale`` is positive.  What a token that sees no key gets, what
     is rounded and what the cache may hold is as in ``paged_attention``.
     """
     out, lse = sparse_paged_attention_impl(q, k_cache, v_cache, key_ranges, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv,
