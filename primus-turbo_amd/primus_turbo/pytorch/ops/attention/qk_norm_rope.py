@@ -16,7 +16,8 @@ position lies outside the tables, -1 for padding, gets zeros and gives no gradie
 Everything is fp32 up to the one rounding of the result, the sums of squares too: a row
 whose squares leave its range becomes zeros (elements beyond about 1e18) or, where eps is
 0, inaccurate and at last infinite (all below about 1e-19).  Elements beyond the first R
-depend on the others through the norm alone.  Under torch.compile the calls run between its graphs; fake tensors are refused.
+depend on the others through the norm alone.  Under torch.compile the calls run between
+its graphs; fake tensors are refused.
 """
 
 from __future__ import annotations

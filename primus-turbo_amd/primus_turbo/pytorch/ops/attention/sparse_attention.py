@@ -93,9 +93,10 @@ def sparse_paged_attention(
     """``paged_attention`` of every token over the pages selected for it (without a window).
 
     A token of a chunk has pages of its own, whose ranges have to be up to date for the
-    whole chunk.  A chunk's tokens go over their pages together: where they take more than
-    about a quarter of the table, ``paged_attention`` of all of it is faster.  ``softmax_scale`` is positive.  What a token that sees no key gets, what
-    is rounded and what the cache may hold is as in ``paged_attention``.
+    whole chunk.  A chunk's tokens go over their pages together: where they take more
+    than about a quarter of the table, ``paged_attention`` of all of it is faster.
+    ``softmax_scale`` is positive.  What a token that sees no key gets, what is rounded
+    and what the cache may hold is as in ``paged_attention``.
     """
     out, lse = sparse_paged_attention_impl(q, k_cache, v_cache, key_ranges, page_table, cu_seqlens_q, seq_lens, k_scale_inv, v_scale_inv,
                                            num_selected, num_first, num_last, softmax_scale, return_lse)
